@@ -25,6 +25,19 @@ c_size = ctypes.c_size_t
 c_f32 = ctypes.c_float
 c_i32 = ctypes.c_int32
 
+
+
+class WindowAttentionArgs(ctypes.Structure):
+    """geo_window_attention_t of include/geo_api.h."""
+
+    _fields_ = [(n, c_vp) for n in ("q", "k", "v")] + \
+        [(n, c_i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head")] + \
+        [(n, c_vp) for n in ("ptr", "mask", "bias", "bias_lut")] + \
+        [(n, c_i64) for n in ("tokens", "sequences", "left", "right", "sinks")] + \
+        [(n, c_i32) for n in ("dtype", "bias_dtype", "heads", "kv_heads", "head_dim", "buckets", "max_distance")] + \
+        [("scale", c_f32)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "geo_last_error": (ctypes.c_char_p, []),
@@ -128,11 +141,18 @@ _SIGNATURES = {
                                       c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32,
                                       c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp,
                                       c_vp]),
+    "geo_window_attention_fwd": (c_int, [ctypes.POINTER(WindowAttentionArgs), c_vp, c_vp, c_vp]),
+    "geo_window_attention_bwd_workspace_bytes": (c_size, [ctypes.POINTER(WindowAttentionArgs)]),
+    "geo_window_attention_bwd": (c_int, [ctypes.POINTER(WindowAttentionArgs), c_vp, c_vp, c_vp, c_vp, c_vp,
+                                         c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
 
 GEO_F32, GEO_BF16, GEO_F64 = 0, 1, 2
+GEO_F16 = 3
+# element types of the sequence operators
+SEQUENCE_DTYPES = {torch.float32: GEO_F32, torch.bfloat16: GEO_BF16, torch.float16: GEO_F16}
 REDUCE_CODES = {"sum": 0, "mean": 1, "max": 2}
 DTYPE_CODES = {torch.float32: GEO_F32, torch.bfloat16: GEO_BF16, torch.float64: GEO_F64}
 

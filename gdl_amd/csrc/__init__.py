@@ -501,6 +501,93 @@ def segment_softmax_backward_hip(
     return grad
 
 
+def _sequence_code(name: str, *tensors: Tensor) -> int:
+    """Type code of a sequence operator's tensors, which have one type."""
+    code = _nat.SEQUENCE_DTYPES.get(tensors[0].dtype)
+    if code is None or any(t.dtype is not tensors[0].dtype for t in tensors):
+        raise TypeError(f"{name}: float32, bfloat16 or float16 tensors of one type, got "
+                        f"{', '.join(str(t.dtype) for t in tensors)}")
+    return code
+
+
+def _same_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
+    dev = tensors[0].device
+    if any(t is not None and t.device != dev for t in tensors):
+        raise ValueError(f"{name}: tensors on different devices")
+    return dev
+
+
+def _in_pieces(t: Tensor) -> Tensor:
+    """t [T, H, D] itself where its rows are contiguous and begin on multiples of 16 bytes."""
+    size = t.element_size()
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * size % 16 == 0 and t.stride(1) * size % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
+    """geo_window_attention_t of the call, and the tensors that it points into."""
+    _require_gpu(name, q, k, v, ptr, mask, bias)
+    code = _sequence_code(name, q, k, v)
+    dev = _same_device(name, q, k, v, ptr, mask, bias)
+    q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
+    T, H, D = q.shape
+    if k.shape[1] < 1 or H < 1 or H % k.shape[1]:
+        raise ValueError(f"{name}: {H} heads are no multiple of {k.shape[1]} key heads")
+    if ptr is not None:
+        ptr = _i64(ptr, dev)
+        if ptr.dim() != 1 or ptr.numel() < 2:
+            raise ValueError(f"{name}: ptr must be [B + 1] with at least one sequence, got {tuple(ptr.shape)}")
+    if mask is not None:
+        if mask.dtype is not torch.bool or mask.shape != (T,):
+            raise ValueError(f"{name}: mask must be bool [{T}], got {mask.dtype} {tuple(mask.shape)}")
+        mask = mask.contiguous()
+    bias_code = maxd = buckets = 0
+    lut = None
+    if bias is not None:
+        bias_code = _sequence_code(f"{name} bias", bias)
+        bias = bias.contiguous()
+        lut, _, maxd = plan
+        buckets = bias.shape[0]
+    args = _nat.WindowAttentionArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+        v.stride(1), _nat.ptr(ptr), _nat.ptr(mask), _nat.ptr(bias), _nat.ptr(lut), T,
+        1 if ptr is None else ptr.numel() - 1, left, right, sinks, code, bias_code, H, k.shape[1], D, buckets, maxd, scale)
+    return args, (q, k, v, ptr, mask, bias, lut), dev
+
+
+def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, with_lse):
+    """(out [T, H, D], log-sums float32 [H, T] or None); ``plan``: (bucket of each distance, spans,
+    max_distance) of the bias."""
+    args, _held, dev = _attention_args("window_attention", q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=dev) if with_lse else None
+    with _nat.on_device(dev):
+        _nat.check(_nat.lib().geo_window_attention_fwd(args, out.data_ptr(), _nat.ptr(lse), _nat.stream_of(dev)),
+                   "geo_window_attention_fwd")
+    return out, lse
+
+
+def window_attention_backward_hip(grad, out, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
+    """(dq, dk, dv, dbias or None), contiguous and of the inputs' types."""
+    name = "window_attention backward"
+    args, _held, dev = _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
+    grad = _in_pieces(grad.to(out.dtype).contiguous())
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dbias = None if bias is None else torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+    L = _nat.lib()
+    with _nat.on_device(dev):
+        ws_bytes = L.geo_window_attention_bwd_workspace_bytes(args)
+        ws = _nat.workspace(ws_bytes, dev)
+        _nat.check(L.geo_window_attention_bwd(
+            args, out.data_ptr(), grad.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            None if bias is None else plan[1].data_ptr(), _nat.ptr(dbias), ws.data_ptr(), ws_bytes,
+            _nat.stream_of(dev)), "geo_window_attention_bwd")
+    if dbias is not None and q.shape[0] == 0:
+        dbias.zero_()
+    return dq, dk, dv, dbias
+
+
 def gather_weighted_sum_forward_hip(feat: Tensor, idx: Tensor, w: Tensor) -> Tensor:
     """out[n] = sum_k w[n, k] * feat[idx[n, k]] (idx < 0 or >= N_src contributes nothing)."""
     _require_gpu("gather_weighted_sum", feat, idx, w)
@@ -872,6 +959,7 @@ __all__ = [
     "edge_geometry_backward_hip", "spherical_harmonics_hip", "spherical_harmonics_backward_hip",
     "graph_avg_degree_hip",
     "segment_reduce_forward_hip", "segment_reduce_backward_hip",
+    "window_attention_forward_hip", "window_attention_backward_hip",
     "knn_available", "knn_cuda", "knn_self_cuda",
     "fps_available", "fps_cuda", "fps_uniform_hip",
 ]

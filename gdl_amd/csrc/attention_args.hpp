@@ -1,0 +1,66 @@
+// attention_args.hpp — the attention kernels' arguments, and their checks on the host.
+#pragma once
+
+#include "attention_tile.hpp"
+
+namespace geo {
+namespace attn {
+
+struct Attend {
+  const void *q, *k, *v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // elements from token to token and from head to head
+  Packing seq;
+  const uint8_t* mask;
+  Bias bias;
+  int Hq, Hk, D, left, right, sinks;
+  float scale;
+};
+
+// Reads of 16 bytes begin at any token and head: pointer and strides are multiples of that.
+inline bool in_pieces(const void* p, int64_t st, int64_t sh, int size) {
+  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+}
+
+inline int attend_args(const geo_window_attention_t* g, Attend* a) {
+  GEO_REQUIRE(g, "window attention: null arguments");
+  GEO_REQUIRE(g->dtype == GEO_F32 || g->dtype == GEO_BF16 || g->dtype == GEO_F16, "window attention: dtype code %d",
+              static_cast<int>(g->dtype));
+  GEO_REQUIRE(g->tokens >= 0 && g->tokens < (int64_t(1) << 30), "window attention: %lld tokens (at most 2^30 - 1)",
+              static_cast<long long>(g->tokens));
+  GEO_REQUIRE(g->kv_heads >= 1 && g->heads >= 1 && g->heads % g->kv_heads == 0,
+              "window attention: %d heads are no multiple of %d key heads", g->heads, g->kv_heads);
+  GEO_REQUIRE(g->head_dim >= 8 && g->head_dim <= 128 && g->head_dim % 8 == 0,
+              "window attention: head size %d (a multiple of 8 up to 128)", g->head_dim);
+  GEO_REQUIRE(g->left >= 0 && g->right >= 0 && g->sinks >= 0 && g->sinks <= 256,
+              "window attention: window of %lld and %lld, %lld first tokens (none negative, at most 256 of these)",
+              static_cast<long long>(g->left), static_cast<long long>(g->right), static_cast<long long>(g->sinks));
+  GEO_REQUIRE(!g->ptr || (g->sequences >= 1 && g->sequences < (int64_t(1) << 30)), "window attention: %lld sequences",
+              static_cast<long long>(g->sequences));
+  if (g->bias) {
+    GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16,
+                "window attention: bias dtype code %d", static_cast<int>(g->bias_dtype));
+    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->buckets <= 256 && g->max_distance >= 1 && g->max_distance <= 1024,
+                "window attention: bias of %d buckets up to distance %d (at most 256 and 1024)", g->buckets, g->max_distance);
+  }
+  if (g->tokens == 0) return GEO_OK;
+  const int size = g->dtype == GEO_F32 ? 4 : 2;
+  GEO_REQUIRE(in_pieces(g->q, g->q_token, g->q_head, size) && in_pieces(g->k, g->k_token, g->k_head, size) &&
+                  in_pieces(g->v, g->v_token, g->v_head, size),
+              "window attention: null q, k or v, or their rows not on multiples of 16 bytes");
+  const int T = static_cast<int>(g->tokens);
+  auto up_to = [T](int64_t x) { return static_cast<int>(x < T ? x : T); };
+  *a = Attend{g->q, g->k, g->v, g->q_token, g->q_head, g->k_token, g->k_head, g->v_token, g->v_head,
+              {g->ptr, static_cast<int>(g->ptr ? g->sequences : 1), T}, g->mask,
+              {g->bias, g->bias_lut, g->bias_dtype, g->buckets, g->max_distance},
+              g->heads, g->kv_heads, g->head_dim, up_to(g->left), up_to(g->right), up_to(g->sinks), g->scale};
+  return GEO_OK;
+}
+
+// Dynamic LDS beyond 64 KB has to be asked for.
+inline hipError_t allow_lds(const void* kernel, size_t bytes) {
+  return bytes <= 60 * 1024 ? hipSuccess
+                            : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
+}  // namespace attn
+}  // namespace geo

@@ -1,0 +1,215 @@
+// window_attention.hip — softmax attention within a window over packed sequences, forward.
+//
+// Token i of the sequence [first, end) sees key j iff first <= j < end, j <= i + right,
+// (j >= i - left or j < first + sinks) and mask[j].  With s_ij = scale q_i.k_j + bias(j - i):
+// o_i = sum_j exp(s_ij) v_j / sum_j exp(s_ij) over the keys it sees, 0 where it sees none.
+#include "attention_args.hpp"
+#include "attention_tile.hpp"
+
+namespace geo {
+namespace attn {
+
+// One workgroup holds 32 NW queries of one head, 32 a wave, one a lane (twice, once in each half),
+// and walks the keys that any of them sees in tiles of BN: first the leading tokens of the sequence
+// that the first query belongs to, as far as they lie before its window, then all from the first
+// query's first key to the last query's last.  Products are transposed, S^T = K Q^T and
+// O^T = V^T P^T, so that a query's weights, running maximum and sum stay in one lane.
+//
+// Which of a tile's keys a query sees is a 64-bit word per lane: the tile is skipped by a wave
+// whose words are all zero, and takes no select where all bits are set.
+template <typename T, int DP, int NW, int BN, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restrict__ out, float* __restrict__ lse) {
+  using Tl = Tile<T, DP, BN, 64 * NW>;
+  using Frag = typename Type<T>::Frag;
+  constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBm = 32 * NW;
+  extern __shared__ __align__(16) unsigned char lds[];
+  T* const ks = reinterpret_cast<T*>(lds);
+  T* const vs = reinterpret_cast<T*>(lds + Tl::kBytes);
+  float* const near = reinterpret_cast<float*>(lds + 2 * Tl::kBytes);  // the tile's biases by distance
+  float* const base = near + (BIAS ? kBm + BN : 0);                    // the head's, -maxd..maxd
+  __shared__ int sptr[kStagedPtr];
+  __shared__ unsigned long long wild[2];
+
+  const int64_t w = xcd_block();
+  const int h = static_cast<int>(w % a.Hq), q0 = static_cast<int>(w / a.Hq) * kBm;
+  const int hk = h / (a.Hq / a.Hk);
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const T* const kbase = static_cast<const T*>(a.k) + hk * a.k_sh;
+  const T* const vbase = static_cast<const T*>(a.v) + hk * a.v_sh;
+
+  stage_ptr(a.seq, sptr);
+  if (BIAS) stage_bias(a.bias, a.Hq, h, base);
+  if (threadIdx.x < 2) wild[threadIdx.x] = 0;
+  __syncthreads();
+
+  // what this lane's query sees: keys lo..hi, and first..far
+  const int i = q0 + 32 * wave + (lane & 31);
+  const bool real = i < a.seq.T;
+  int first, end;
+  seq_of(a.seq, sptr, real ? i : a.seq.T - 1, first, end);
+  const int lo = max(first, i - a.left), hi = real ? min(end - 1, i + a.right) : -1;
+  const int far = min(first + a.sinks - 1, hi);
+  // the workgroup's keys: those of its first and last queries bound them, both grow with the query
+  int first0, end0, first1, end1;
+  seq_of(a.seq, sptr, q0, first0, end0);
+  const int q1 = min(q0 + kBm, a.seq.T) - 1;
+  seq_of(a.seq, sptr, q1, first1, end1);
+  const int jlo = max(first0, q0 - a.left), jend = min(end1, q1 + a.right + 1);
+  const int sink_end = min(min(first0 + a.sinks, jlo), end0);
+  const int sink_tiles = sink_end > first0 ? (sink_end - first0 + BN - 1) / BN : 0;
+  const int tiles = sink_tiles + (jend > jlo ? (jend - jlo + BN - 1) / BN : 0);
+
+  Frag qf[kKc];
+  {
+    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(real ? i : 0) * a.q_st + h * a.q_sh;
+#pragma unroll
+    for (int kc = 0; kc < kKc; ++kc) qf[kc] = frag_global(q, kc, a.D, real);
+  }
+  f32x16 o[kMt] = {};
+  float m = -kInf, l = 0.f;
+  const float scale2 = a.scale * kLog2e;
+
+  auto tile_at = [&](int t, int& j0, int& jlim) {
+    const bool s = t < sink_tiles;
+    j0 = s ? first0 + t * BN : jlo + (t - sink_tiles) * BN;
+    jlim = s ? sink_end : jend;
+  };
+  Tl kt, vt;
+  uint32_t seen_byte = 1;
+  auto fetch = [&](int t) {
+    int j0, jlim;
+    tile_at(t, j0, jlim);
+    kt.load(kbase, a.k_st, j0, jlim, a.D);
+    vt.load(vbase, a.v_st, j0, jlim, a.D);
+    if (a.mask) seen_byte = a.mask[min(j0 + lane, jlim - 1)];
+  };
+  if (tiles > 0) fetch(0);
+  for (int t = 0; t < tiles; ++t) {
+    int j0, jlim;
+    tile_at(t, j0, jlim);
+    uint64_t rows = bit_range(0, min(jlim - j0, BN) - 1);
+    if (a.mask) rows &= __ballot(seen_byte != 0);
+    __syncthreads();
+    kt.store(ks, rows, a.D);
+    vt.store_finite(vs, rows, a.D, &wild[t & 1]);
+    if (threadIdx.x == 0) wild[(t + 1) & 1] = 0;
+    if (BIAS)
+      for (int x = threadIdx.x; x < kBm + BN - 1; x += 64 * NW)
+        near[x] = base[min(max(j0 - q0 + x - (kBm - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1);
+
+    uint64_t vis = bit_range(lo - j0, hi - j0);
+    if (a.sinks) vis |= bit_range(first - j0, far - j0);
+    vis &= rows;
+    const uint64_t bits = vis >> (4 * half);
+    const uint32_t word[2] = {static_cast<uint32_t>(bits) & 0x0f0f0f0fu, static_cast<uint32_t>(bits >> 32) & 0x0f0f0f0fu};
+    if (__ballot((word[0] | (kSub > 1 ? word[1] : 0u)) != 0) == 0) continue;
+    const bool whole = __ballot(word[0] == 0x0f0f0f0fu && (kSub == 1 || word[1] == 0x0f0f0f0fu)) == ~0ull;
+
+    f32x16 s[kSub];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      s[u] = f32x16{};
+#pragma unroll
+      for (int kc = 0; kc < kKc; ++kc) s[u] = Type<T>::mma(Tl::frag_along(ks, 32 * u, kc), qf[kc], s[u]);
+    }
+    const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31);
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kk = 8 * (r >> 2) + (r & 3);
+        s[u][r] = BIAS ? fmaf(s[u][r], scale2, bias[32 * u + kk]) : s[u][r] * scale2;
+      }
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((word[u] >> (8 * (r >> 2) + (r & 3))) & 1)) s[u][r] = -kInf;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = fmaxf(m, halves_max(top));
+    const float shift = top == -kInf ? 0.f : top;  // no key so far: every exponential below is 0
+    const float keep = exp2_hw(m - shift);
+    m = top;
+    l *= keep;
+    if (__ballot(keep != 1.f)) {
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt) o[mt] *= keep;
+    }
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = exp2_hw(s[u][r] - shift);
+        l += s[u][r];
+      }
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const Frag p = frag_of<T>(s[u], c);
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) o[mt] = Type<T>::mma(Tl::frag_down(vs, 32 * u + 16 * c, mt), p, o[mt]);
+      }
+    if (wild[t & 1]) add_wild<T, kMt, false>(vbase, a.v_st, j0, wild[t & 1], vis, a.D, o);
+  }
+  l = halves_sum(l);
+  if (real) {
+    T* row = out + (static_cast<int64_t>(i) * a.Hq + h) * a.D;
+    store_row<T>(row, o, l == 0.f ? 0.f : 1.f / l, a.D);
+    // +inf where no key is seen: the backward's exp2(s - lse) is 0 there
+    if (lse && half == 0) lse[static_cast<int64_t>(h) * a.seq.T + i] = l == 0.f ? kInf : m + log2f(l);
+  }
+}
+
+template <typename T, int DP, int NW, int BN, bool BIAS>
+int launch_fwd(const Attend& a, void* out, float* lse, hipStream_t stream) {
+  const int64_t blocks = ceil_div(a.seq.T, 32 * NW) * a.Hq;
+  GEO_REQUIRE(blocks < (int64_t(1) << 31), "window attention: %lld workgroups", static_cast<long long>(blocks));
+  const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
+                     (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_fwd<T, DP, NW, BN, BIAS>), lds));
+  attend_fwd<T, DP, NW, BN, BIAS><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
+      a, static_cast<T*>(out), lse);
+  GEO_LAUNCH_CHECK("attend_fwd");
+  return GEO_OK;
+}
+
+template <typename T, int DP>
+int choose_fwd(const Attend& a, void* out, float* lse, hipStream_t stream) {
+  // Four waves share a tile's loads; one wave alone where that leaves less than a workgroup for
+  // each of the 256 CUs.
+  const bool few = ceil_div(a.seq.T, 128) * a.Hq < 256;
+  if (a.bias.table)
+    return few ? launch_fwd<T, DP, 1, 32, true>(a, out, lse, stream) : launch_fwd<T, DP, 4, 64, true>(a, out, lse, stream);
+  return few ? launch_fwd<T, DP, 1, 32, false>(a, out, lse, stream) : launch_fwd<T, DP, 4, 64, false>(a, out, lse, stream);
+}
+
+template <typename T>
+int choose_width(const Attend& a, void* out, float* lse, hipStream_t stream) {
+  if (a.D <= 32) return choose_fwd<T, 32>(a, out, lse, stream);
+  if (a.D <= 64) return choose_fwd<T, 64>(a, out, lse, stream);
+  if (a.D <= 96) return choose_fwd<T, 96>(a, out, lse, stream);
+  return choose_fwd<T, 128>(a, out, lse, stream);
+}
+
+}  // namespace attn
+}  // namespace geo
+
+extern "C" int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, float* lse, void* stream) {
+  geo::attn::Attend a;
+  const int rc = geo::attn::attend_args(args, &a);
+  if (rc != GEO_OK || args->tokens == 0) return rc;
+  GEO_REQUIRE(out, "window attention: null output");
+  const hipStream_t s = geo::as_stream(stream);
+  if (args->dtype == GEO_F32) return geo::attn::choose_width<float>(a, out, lse, s);
+  if (args->dtype == GEO_BF16) return geo::attn::choose_width<__bf16>(a, out, lse, s);
+  return geo::attn::choose_width<_Float16>(a, out, lse, s);
+}

@@ -1,0 +1,578 @@
+// window_attention_bwd.hip — gradients of the window attention (window_attention.hip).
+//
+// With p_ij the weights, g_i the output's gradient and delta_i = g_i.o_i:
+//   dv_j = sum_i p_ij g_i,  ds_ij = p_ij (g_i.v_j - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dbias(d) = sum of ds_ij, j - i = d.
+// The weights are formed again from the scores and the forward's log-sums, once for dq (and the
+// bias) and once for dk and dv: seven products instead of five, for sums that no two workgroups
+// share, so every gradient is the same from run to run.
+#include "attention_args.hpp"
+#include "attention_tile.hpp"
+
+namespace geo {
+namespace attn {
+
+// ------------------------------------------------------------------ dq, bias ---
+
+// As the forward, a wave's 32 queries over tiles of keys.  The bias gradient is summed by distance:
+// a lane's score of query i and key j goes to LDS slot j - i of its wave and half, where the 32
+// lanes of a half always hold 32 different distances, so no two lanes add to one word at once;
+// distances at or beyond the ends go to two registers.  The workgroup's sums leave by bucket.
+template <typename T, int DP, int NW, int BN, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T* __restrict__ out,
+                                                        const T* __restrict__ grad, const float* __restrict__ lse,
+                                                        float* __restrict__ delta, T* __restrict__ dq,
+                                                        const int32_t* __restrict__ range, float* __restrict__ part) {
+  using Tl = Tile<T, DP, BN, 64 * NW>;
+  using Frag = typename Type<T>::Frag;
+  constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBm = 32 * NW;
+  extern __shared__ __align__(16) unsigned char lds[];
+  T* const ks = reinterpret_cast<T*>(lds);
+  T* const vs = reinterpret_cast<T*>(lds + Tl::kBytes);
+  float* const near = reinterpret_cast<float*>(lds + 2 * Tl::kBytes);
+  float* const base = near + (BIAS ? kBm + BN : 0);
+  const int slots = 2 * a.bias.maxd + 1;
+  float* const sums = base + (BIAS ? slots : 0);  // [2 NW][slots]
+  __shared__ int sptr[kStagedPtr];
+  __shared__ unsigned long long wild[2];
+
+  const int64_t w = xcd_block();
+  const int h = static_cast<int>(w % a.Hq), block = static_cast<int>(w / a.Hq), q0 = block * kBm;
+  const int hk = h / (a.Hq / a.Hk);
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  const T* const kbase = static_cast<const T*>(a.k) + hk * a.k_sh;
+  const T* const vbase = static_cast<const T*>(a.v) + hk * a.v_sh;
+
+  stage_ptr(a.seq, sptr);
+  if (BIAS) {
+    stage_bias(a.bias, a.Hq, h, base);
+    for (int x = threadIdx.x; x < 2 * NW * slots; x += 64 * NW) sums[x] = 0.f;
+  }
+  if (threadIdx.x < 2) wild[threadIdx.x] = 0;
+  __syncthreads();
+
+  const int iw = q0 + 32 * wave, i = iw + (lane & 31);
+  const bool real = i < a.seq.T;
+  int first, end;
+  seq_of(a.seq, sptr, real ? i : a.seq.T - 1, first, end);
+  const int lo = max(first, i - a.left), hi = real ? min(end - 1, i + a.right) : -1;
+  const int far = min(first + a.sinks - 1, hi);
+  int first0, end0, first1, end1;
+  seq_of(a.seq, sptr, q0, first0, end0);
+  const int q1 = min(q0 + kBm, a.seq.T) - 1;
+  seq_of(a.seq, sptr, q1, first1, end1);
+  const int jlo = max(first0, q0 - a.left), jend = min(end1, q1 + a.right + 1);
+  const int sink_end = min(min(first0 + a.sinks, jlo), end0);
+  const int sink_tiles = sink_end > first0 ? (sink_end - first0 + BN - 1) / BN : 0;
+  const int tiles = sink_tiles + (jend > jlo ? (jend - jlo + BN - 1) / BN : 0);
+
+  Frag qf[kKc], gf[kKc];
+  float dl = 0.f;
+  {
+    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(real ? i : 0) * a.q_st + h * a.q_sh;
+    const int64_t row = (static_cast<int64_t>(real ? i : 0) * a.Hq + h) * a.D;
+#pragma unroll
+    for (int kc = 0; kc < kKc; ++kc) {
+      qf[kc] = frag_global(q, kc, a.D, real);
+      gf[kc] = frag_global(grad + row, kc, a.D, real);
+      const Frag of = frag_global(out + row, kc, a.D, real);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dl += static_cast<float>(gf[kc][j]) * static_cast<float>(of[j]);
+    }
+    dl = halves_sum(dl);
+    if (real && half == 0) delta[static_cast<int64_t>(h) * a.seq.T + i] = dl;
+  }
+  const float ls = real ? lse[static_cast<int64_t>(h) * a.seq.T + i] : kInf;
+  f32x16 o[kMt] = {};
+  float below = 0.f, above = 0.f;
+  const float scale2 = a.scale * kLog2e;
+
+  auto tile_at = [&](int t, int& j0, int& jlim) {
+    const bool s = t < sink_tiles;
+    j0 = s ? first0 + t * BN : jlo + (t - sink_tiles) * BN;
+    jlim = s ? sink_end : jend;
+  };
+  Tl kt, vt;
+  uint32_t seen_byte = 1;
+  auto fetch = [&](int t) {
+    int j0, jlim;
+    tile_at(t, j0, jlim);
+    kt.load(kbase, a.k_st, j0, jlim, a.D);
+    vt.load(vbase, a.v_st, j0, jlim, a.D);
+    if (a.mask) seen_byte = a.mask[min(j0 + lane, jlim - 1)];
+  };
+  if (tiles > 0) fetch(0);
+  for (int t = 0; t < tiles; ++t) {
+    int j0, jlim;
+    tile_at(t, j0, jlim);
+    uint64_t rows = bit_range(0, min(jlim - j0, BN) - 1);
+    if (a.mask) rows &= __ballot(seen_byte != 0);
+    __syncthreads();
+    kt.store_finite(ks, rows, a.D, &wild[t & 1]);
+    vt.store(vs, rows, a.D);
+    if (threadIdx.x == 0) wild[(t + 1) & 1] = 0;
+    if (BIAS)
+      for (int x = threadIdx.x; x < kBm + BN - 1; x += 64 * NW)
+        near[x] = base[min(max(j0 - q0 + x - (kBm - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1);
+
+    uint64_t vis = bit_range(lo - j0, hi - j0);
+    if (a.sinks) vis |= bit_range(first - j0, far - j0);
+    vis &= rows;
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half)) & 0x0f0f0f0fu;
+      if (__ballot(word != 0) == 0) continue;
+      const bool whole = __ballot(word == 0x0f0f0f0fu) == ~0ull;
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int kc = 0; kc < kKc; ++kc) {
+        s = Type<T>::mma(Tl::frag_along(ks, 32 * u, kc), qf[kc], s);
+        dp = Type<T>::mma(Tl::frag_along(vs, 32 * u, kc), gf[kc], dp);
+      }
+      const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31) + 32 * u;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kk = 8 * (r >> 2) + (r & 3);
+        const float x = BIAS ? fmaf(s[r], scale2, bias[kk]) : s[r] * scale2;
+        s[r] = exp2_hw(x - ls) * (dp[r] - dl);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = 0.f;
+      }
+      if (BIAS) {
+        const int d0 = j0 + 32 * u - iw;  // this sub-tile's distances: d0 - 31 .. d0 + 31
+        float* const mine = sums + (2 * wave + half) * slots + a.bias.maxd;
+        if (d0 + 31 <= -a.bias.maxd) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) below += s[r];
+        } else if (d0 - 31 >= a.bias.maxd) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) above += s[r];
+        } else {
+          const int d1 = d0 + 4 * half - (lane & 31);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = d1 + 8 * (r >> 2) + (r & 3);
+            if (d <= -a.bias.maxd) below += s[r];
+            else if (d >= a.bias.maxd) above += s[r];
+            else __hip_atomic_fetch_add(mine + d, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const Frag p = frag_of<T>(s, c);
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) o[mt] = Type<T>::mma(Tl::frag_down(ks, 32 * u + 16 * c, mt), p, o[mt]);
+      }
+    }
+    if (wild[t & 1]) add_wild<T, kMt, true>(kbase, a.k_st, j0, wild[t & 1], vis, a.D, o);
+  }
+  if (real) store_row<T>(dq + (static_cast<int64_t>(i) * a.Hq + h) * a.D, o, a.scale, a.D);
+  if (BIAS) {
+    below = wave_sum(below);
+    above = wave_sum(above);
+    if (lane == 0) {
+      sums[2 * wave * slots] = below;
+      sums[2 * wave * slots + slots - 1] = above;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.bias.buckets; b += 64 * NW) {
+      float x = 0.f;
+      const int x0 = max(range[2 * b], 0), x1 = min(range[2 * b + 1], slots);
+      for (int at = x0; at < x1; ++at)
+#pragma unroll
+        for (int n = 0; n < 2 * NW; ++n) x += sums[n * slots + at];
+      part[(static_cast<int64_t>(h) * gridDim.x / a.Hq + block) * a.bias.buckets + b] = x;
+    }
+  }
+}
+
+// The workgroups' bucket sums of one head and bucket, added in their order by one wave.
+__global__ __launch_bounds__(64) void attend_bwd_bias(const float* __restrict__ part, int64_t blocks, int buckets,
+                                                      int Hq, int dtype, void* __restrict__ dbias) {
+  const int b = blockIdx.x % buckets, h = blockIdx.x / buckets, lane = threadIdx.x;
+  double x = 0.0;
+  for (int64_t n = lane; n < blocks; n += 64) x += part[(h * blocks + n) * buckets + b];
+  x = wave_sum(x);
+  if (lane == 0) {
+    const int64_t at = static_cast<int64_t>(b) * Hq + h;
+    const float y = static_cast<float>(x);
+    if (dtype == GEO_F32) static_cast<float*>(dbias)[at] = y;
+    else if (dtype == GEO_BF16) static_cast<__bf16*>(dbias)[at] = static_cast<__bf16>(y);
+    else static_cast<_Float16*>(dbias)[at] = static_cast<_Float16>(y);
+  }
+}
+
+// -------------------------------------------------------------------- dk, dv ---
+
+// Queries far behind a leading token still see it, so such a key's gradient is a sum over the rest
+// of its sequence.  That is cut at multiples of `len` tokens: the key's own workgroup adds the
+// queries up to the first cut past its window, workgroups of their own (PART) add one piece each,
+// per query head, and attend_bwd_join adds the sums of a key in their order.
+struct Far {
+  int len;       // 0: no leading tokens beyond a window
+  float* own;    // [pieces][Hk][sinks][2][D]: by the piece that the sequence begins in
+  float* part;   // [pieces][Hq][sinks][2][D]: by the piece of the queries
+};
+__device__ __forceinline__ int own_end(const Far& f, int j, int left) { return (j + left) / f.len * f.len + f.len; }
+
+// Stores a transposed result's row as float32.
+template <int MT>
+__device__ __forceinline__ void store_sums(float* row, const f32x16 (&acc)[MT], int D) {
+  store_row<float>(row, acc, 1.f, D);
+}
+
+// One workgroup holds 32 NW keys of one key head, a lane one of them, and walks the queries of all
+// heads that share it in tiles of BN.  S = Q K^T and dP = G V^T leave a key's weights of 16 queries
+// in a lane's registers, where dV^T = G^T P and dK^T = Q^T dS take them as operands; the sums over
+// heads and queries stay in registers.
+template <typename T, int DP, int NW, int BN, bool BIAS, bool PART>
+__global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T* __restrict__ grad,
+                                                         const float* __restrict__ lse, const float* __restrict__ delta,
+                                                         T* __restrict__ dk, T* __restrict__ dv, const Far f) {
+  using Tl = Tile<T, DP, BN, 64 * NW>;
+  using Frag = typename Type<T>::Frag;
+  constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBk = 32 * NW;
+  extern __shared__ __align__(16) unsigned char lds[];
+  T* const qs = reinterpret_cast<T*>(lds);
+  T* const gs = reinterpret_cast<T*>(lds + Tl::kBytes);
+  float* const rowl = reinterpret_cast<float*>(lds + 2 * Tl::kBytes);  // the tile's log-sums and deltas
+  float* const rowd = rowl + BN;
+  float* const near = rowd + BN;
+  float* const base = near + (BIAS ? kBk + BN : 0);
+  __shared__ int sptr[kStagedPtr];
+  __shared__ unsigned long long wildq[2], wildg[2];
+  __shared__ int last;
+
+  const int group = a.Hq / a.Hk;
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+  int hk, key0, g0 = 0, heads = group, cut = 0;
+  if constexpr (PART) {  // (piece - 1, query head, 32 NW of the leading tokens)
+    const int64_t w = blockIdx.x;
+    const int h = static_cast<int>(w % a.Hq);
+    const int blocks = (a.sinks + kBk - 1) / kBk;
+    cut = static_cast<int>(w / a.Hq / blocks + 1) * f.len;
+    key0 = static_cast<int>(w / a.Hq % blocks) * kBk;
+    hk = h / group;
+    g0 = h % group;
+    heads = 1;
+  } else {
+    const int64_t w = xcd_block();
+    hk = static_cast<int>(w % a.Hk);
+    key0 = static_cast<int>(w / a.Hk) * kBk;
+  }
+
+  stage_ptr(a.seq, sptr);
+  if (threadIdx.x < 2) wildq[threadIdx.x] = wildg[threadIdx.x] = 0;
+  if (threadIdx.x == 0) last = -1;
+  __syncthreads();
+
+  int first, end;
+  if constexpr (PART) {  // the leading tokens of the sequence that holds the cut
+    seq_of(a.seq, sptr, cut, first, end);
+    if (first >= cut || end <= cut || own_end(f, first, a.left) > cut) return;
+    key0 += first;
+  }
+  const int j = key0 + 32 * wave + (lane & 31);
+  bool real = j < a.seq.T;
+  if constexpr (PART) real = j < min(end, first + a.sinks);
+  else seq_of(a.seq, sptr, real ? j : a.seq.T - 1, first, end);
+  const bool sink = real && j - first < a.sinks;
+  int ilo = max(first, j - a.right), ihi = min(end - 1, j + a.left);
+  bool more = false;  // sums of other workgroups are added to this key's
+  if constexpr (PART) {
+    ilo = cut;
+    ihi = own_end(f, j, a.left) <= cut ? min(end, cut + f.len) - 1 : -1;
+  } else if (f.len && sink) {
+    more = own_end(f, j, a.left) < end;
+    ihi = more ? own_end(f, j, a.left) - 1 : end - 1;
+  } else if (sink) {
+    ihi = end - 1;
+  }
+  const bool on = real && (!a.mask || a.mask[j]);
+  if (!on) ihi = -1;
+  // queries of the workgroup: from its first key's on (they grow with the key), to the last of any
+  int i0, ilast;
+  if constexpr (PART) {
+    i0 = cut;
+  } else {
+    int first0, end0;
+    seq_of(a.seq, sptr, key0, first0, end0);
+    i0 = max(first0, key0 - a.right);
+  }
+  atomicMax(&last, ihi);
+  __syncthreads();
+  ilast = last;
+  const int span = ilast >= i0 ? (ilast - i0) / BN + 1 : 0;
+  const int tiles = span * heads;
+
+  Frag kf[kKc], vf[kKc];
+  {
+    const T* kr = static_cast<const T*>(a.k) + static_cast<int64_t>(real ? j : 0) * a.k_st + hk * a.k_sh;
+    const T* vr = static_cast<const T*>(a.v) + static_cast<int64_t>(real ? j : 0) * a.v_st + hk * a.v_sh;
+#pragma unroll
+    for (int kc = 0; kc < kKc; ++kc) {
+      kf[kc] = frag_global(kr, kc, a.D, on);
+      vf[kc] = frag_global(vr, kc, a.D, on);
+    }
+  }
+  f32x16 dka[kMt] = {}, dva[kMt] = {};
+  const float scale2 = a.scale * kLog2e;
+
+  Tl qt, gt;
+  float row_value = 0.f;
+  auto fetch = [&](int t) {
+    const int h = hk * group + g0 + t / span, it = i0 + t % span * BN;
+    qt.load(static_cast<const T*>(a.q) + h * a.q_sh, a.q_st, it, ilast + 1, a.D);
+    gt.load(grad + static_cast<int64_t>(h) * a.D, static_cast<int64_t>(a.Hq) * a.D, it, ilast + 1, a.D);
+    const int n = threadIdx.x % (2 * BN);
+    row_value = (n < BN ? lse : delta)[static_cast<int64_t>(h) * a.seq.T + min(it + n % BN, ilast)];
+  };
+  static_assert(2 * BN <= 64 * NW, "one thread for each of a tile's log-sums and deltas");
+  if (tiles > 0) fetch(0);
+  for (int t = 0; t < tiles; ++t) {
+    const int it = i0 + t % span * BN;
+    const uint64_t rows = bit_range(0, min(ilast + 1 - it, BN) - 1);
+    if (BIAS && t % span == 0) stage_bias(a.bias, a.Hq, hk * group + g0 + t / span, base);
+    __syncthreads();
+    qt.store_finite(qs, rows, a.D, &wildq[t & 1]);
+    gt.store_finite(gs, rows, a.D, &wildg[t & 1]);
+    if (threadIdx.x < 2 * BN) rowl[threadIdx.x] = row_value;
+    if (threadIdx.x == 0) wildq[(t + 1) & 1] = wildg[(t + 1) & 1] = 0;
+    if (BIAS)
+      for (int x = threadIdx.x; x < kBk + BN - 1; x += 64 * NW)
+        near[x] = base[min(max(key0 - it + x - (BN - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1);
+
+    const uint64_t vis = bit_range(ilo - it, ihi - it) & rows;
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half)) & 0x0f0f0f0fu;
+      if (__ballot(word != 0) == 0) continue;
+      const bool whole = __ballot(word == 0x0f0f0f0fu) == ~0ull;
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int kc = 0; kc < kKc; ++kc) {
+        s = Type<T>::mma(Tl::frag_along(qs, 32 * u, kc), kf[kc], s);
+        dp = Type<T>::mma(Tl::frag_along(gs, 32 * u, kc), vf[kc], dp);
+      }
+      const float* bias = near + (lane & 31) + 32 * wave - 4 * half + (BN - 32 * u - 28);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 ls = *reinterpret_cast<const float4*>(rowl + 32 * u + 8 * g + 4 * half);
+        const float4 dl = *reinterpret_cast<const float4*>(rowd + 32 * u + 8 * g + 4 * half);
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dlv[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = 4 * g + q, kk = 8 * g + q;
+          const float x = BIAS ? fmaf(s[r], scale2, bias[27 - kk]) : s[r] * scale2;
+          s[r] = exp2_hw(x - lsv[q]);
+          dp[r] = s[r] * (dp[r] - dlv[q]);
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const Frag p = frag_of<T>(s, c), ds = frag_of<T>(dp, c);
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) {
+          dva[mt] = Type<T>::mma(Tl::frag_down(gs, 32 * u + 16 * c, mt), p, dva[mt]);
+          dka[mt] = Type<T>::mma(Tl::frag_down(qs, 32 * u + 16 * c, mt), ds, dka[mt]);
+        }
+      }
+    }
+    if (wildq[t & 1] | wildg[t & 1]) {
+      const int h = hk * group + g0 + t / span;
+      add_wild<T, kMt, false>(grad + static_cast<int64_t>(h) * a.D, static_cast<int64_t>(a.Hq) * a.D, it, wildg[t & 1], vis,
+                              a.D, dva);
+      add_wild<T, kMt, true>(static_cast<const T*>(a.q) + h * a.q_sh, a.q_st, it, wildq[t & 1], vis, a.D, dka);
+    }
+  }
+  if (!real) return;
+  if constexpr (PART) {
+    const int h = hk * group + g0;
+    float* row = f.part + ((static_cast<int64_t>(cut / f.len) * a.Hq + h) * a.sinks + (j - first)) * 2 * a.D;
+    store_sums(row, dka, a.D);
+    store_sums(row + a.D, dva, a.D);
+  } else if (more) {
+    float* row = f.own + ((static_cast<int64_t>(first / f.len) * a.Hk + hk) * a.sinks + (j - first)) * 2 * a.D;
+    store_sums(row, dka, a.D);
+    store_sums(row + a.D, dva, a.D);
+  } else {
+    const int64_t at = (static_cast<int64_t>(j) * a.Hk + hk) * a.D;
+    store_row<T>(dk + at, dka, a.scale, a.D);
+    store_row<T>(dv + at, dva, 1.f, a.D);
+  }
+}
+
+// The sums of leading token s of the one sequence that begins in piece c and reaches past its end:
+// the key's own, then each later piece's, heads in order.
+template <typename T>
+__global__ __launch_bounds__(256) void attend_bwd_join(const Attend a, T* __restrict__ dk, T* __restrict__ dv, const Far f) {
+  __shared__ int sptr[kStagedPtr];
+  const int64_t w = blockIdx.x;
+  const int s = static_cast<int>(w % a.sinks), hk = static_cast<int>(w / a.sinks % a.Hk);
+  const int64_t c = w / a.sinks / a.Hk;
+  stage_ptr(a.seq, sptr);
+  __syncthreads();
+  int first, end;
+  seq_of(a.seq, sptr, static_cast<int>((c + 1) * f.len), first, end);
+  const int j = first + s;
+  if (first / f.len != c || j >= end || own_end(f, j, a.left) >= end) return;
+  const int x = threadIdx.x;
+  if (x >= 2 * a.D) return;
+  const int group = a.Hq / a.Hk;
+  float sum = f.own[((c * a.Hk + hk) * a.sinks + s) * 2 * a.D + x];
+  const int64_t p0 = own_end(f, j, a.left) / f.len, p1 = (end - 1) / f.len;
+  const float* at = f.part + ((p0 * a.Hq + hk * group) * a.sinks + s) * 2 * a.D + x;
+  const int64_t step = static_cast<int64_t>(a.sinks) * 2 * a.D;
+  for (int64_t p = p0; p <= p1; ++p, at += a.Hq * step)
+    for (int g = 0; g < group; ++g) sum += at[g * step];
+  const int64_t row = (static_cast<int64_t>(j) * a.Hk + hk) * a.D;
+  if (x < a.D) dk[row + x] = static_cast<T>(sum * a.scale);
+  else dv[row + x - a.D] = static_cast<T>(sum);
+}
+
+// ---------------------------------------------------------------------- host ---
+
+// Workgroups of four waves share a tile; one wave alone where that leaves less than one workgroup
+// for each of the 256 CUs.
+inline bool few_blocks(int T, int heads) { return ceil_div(T, 128) * heads < 256; }
+
+// Pieces of the queries past a leading token's window: 256 tokens (64 pieces keep the sums of a
+// sequence of 16,384 small), longer where that would be more than 512 pieces.
+inline int far_len(int T, int left, int sinks) {
+  if (sinks == 0 || T - 1 <= left) return 0;
+  int len = 256;
+  while (ceil_div(T, len) > 512) len *= 2;
+  return (left / len + 1) * len < T ? len : 0;
+}
+
+struct Plan {
+  int64_t q_blocks;
+  float *delta, *part;
+  Far far;
+  int64_t pieces;
+};
+inline size_t plan(const geo_window_attention_t& g, void* workspace, Plan* p) {
+  const int T = static_cast<int>(g.tokens);
+  Carver c(workspace);
+  p->q_blocks = ceil_div(T, few_blocks(T, g.heads) ? 32 : 128);
+  p->delta = c.take<float>(static_cast<size_t>(g.heads) * T);
+  p->part = c.take<float>(g.bias ? static_cast<size_t>(p->q_blocks) * g.heads * g.buckets : 0);
+  const int sinks = static_cast<int>(g.sinks < T ? g.sinks : T);
+  p->far.len = far_len(T, static_cast<int>(g.left < T ? g.left : T), sinks);
+  p->pieces = p->far.len ? ceil_div(T, p->far.len) : 0;
+  p->far.own = c.take<float>(static_cast<size_t>(p->pieces) * g.kv_heads * sinks * 2 * g.head_dim);
+  p->far.part = c.take<float>(static_cast<size_t>(p->pieces) * g.heads * sinks * 2 * g.head_dim);
+  return c.used;
+}
+
+struct Grads {
+  const void *out, *grad;
+  const float* lse;
+  void *dq, *dk, *dv, *dbias;
+  const int32_t* range;
+};
+
+template <typename T, int DP, int NW, int BN, bool BIAS>
+int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
+  const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
+                     (BIAS ? sizeof(float) * (32 * NW + BN + (2 * NW + 1) * (2 * a.bias.maxd + 1)) : 0);
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_q<T, DP, NW, BN, BIAS>), lds));
+  attend_bwd_q<T, DP, NW, BN, BIAS><<<dim3(static_cast<uint32_t>(p.q_blocks * a.Hq)), dim3(64 * NW), lds, stream>>>(
+      a, static_cast<const T*>(g.out), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
+      p.part);
+  GEO_LAUNCH_CHECK("attend_bwd_q");
+  if (BIAS) {
+    attend_bwd_bias<<<dim3(a.bias.buckets * a.Hq), dim3(64), 0, stream>>>(p.part, p.q_blocks, a.bias.buckets, a.Hq,
+                                                                          a.bias.dtype, g.dbias);
+    GEO_LAUNCH_CHECK("attend_bwd_bias");
+  }
+  return GEO_OK;
+}
+
+template <typename T, int DP, int NW, int BN, bool BIAS, bool PART>
+int launch_kv(const Attend& a, const Grads& g, const Plan& p, int64_t blocks, hipStream_t stream) {
+  const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes + 2 * BN * sizeof(float) +
+                     (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_kv<T, DP, NW, BN, BIAS, PART>), lds));
+  attend_bwd_kv<T, DP, NW, BN, BIAS, PART><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
+      a, static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
+  GEO_LAUNCH_CHECK("attend_bwd_kv");
+  return GEO_OK;
+}
+
+template <typename T, int DP, bool BIAS>
+int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
+  int rc = few_blocks(a.seq.T, a.Hq) ? launch_q<T, DP, 1, 32, BIAS>(a, g, p, stream)
+                                     : launch_q<T, DP, 4, 64, BIAS>(a, g, p, stream);
+  if (rc == GEO_OK && p.far.len)
+    rc = launch_kv<T, DP, 1, 32, BIAS, true>(a, g, p, (p.pieces - 1) * ceil_div(a.sinks, 32) * a.Hq, stream);
+  if (rc == GEO_OK)
+    rc = few_blocks(a.seq.T, a.Hk)
+             ? launch_kv<T, DP, 1, 32, BIAS, false>(a, g, p, ceil_div(a.seq.T, 32) * a.Hk, stream)
+             : launch_kv<T, DP, 4, 64, BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
+  if (rc == GEO_OK && p.far.len) {
+    attend_bwd_join<T><<<dim3(static_cast<uint32_t>((p.pieces - 1) * a.Hk * a.sinks)), dim3(256), 0, stream>>>(
+        a, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
+    GEO_LAUNCH_CHECK("attend_bwd_join");
+  }
+  return rc;
+}
+
+template <typename T, int DP>
+int choose_bias(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
+  return a.bias.table ? all_grads<T, DP, true>(a, g, p, stream) : all_grads<T, DP, false>(a, g, p, stream);
+}
+template <typename T>
+int choose_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
+  if (a.D <= 32) return choose_bias<T, 32>(a, g, p, stream);
+  if (a.D <= 64) return choose_bias<T, 64>(a, g, p, stream);
+  if (a.D <= 96) return choose_bias<T, 96>(a, g, p, stream);
+  return choose_bias<T, 128>(a, g, p, stream);
+}
+
+}  // namespace attn
+}  // namespace geo
+
+extern "C" size_t geo_window_attention_bwd_workspace_bytes(const geo_window_attention_t* args) {
+  geo::attn::Attend a;
+  if (geo::attn::attend_args(args, &a) != GEO_OK || args->tokens == 0) return 0;
+  geo::attn::Plan p;
+  return geo::attn::plan(*args, nullptr, &p);
+}
+
+extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* grad,
+                                        const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
+                                        void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+  geo::attn::Attend a;
+  const int rc = geo::attn::attend_args(args, &a);
+  if (rc != GEO_OK || args->tokens == 0) return rc;
+  GEO_REQUIRE(out && grad && lse && dq && dk && dv, "window attention backward: null tensor");
+  GEO_REQUIRE(reinterpret_cast<uintptr_t>(grad) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+              "window attention backward: out and grad must lie on multiples of 16 bytes");
+  GEO_REQUIRE(!args->bias || (bucket_range && dbias), "window attention backward: null bucket_range or dbias");
+  geo::attn::Plan p;
+  const size_t need = geo::attn::plan(*args, workspace, &p);
+  if (!workspace || workspace_bytes < need)
+    return geo::set_error(GEO_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes, %zu needed",
+                          workspace ? workspace_bytes : size_t(0), need);
+  GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks < (int64_t(1) << 31),
+              "window attention backward: too many workgroups");
+  const geo::attn::Grads g{out, grad, lse, dq, dk, dv, dbias, bucket_range};
+  const hipStream_t s = geo::as_stream(stream);
+  if (args->dtype == GEO_F32) return geo::attn::choose_grads<float>(a, g, p, s);
+  if (args->dtype == GEO_BF16) return geo::attn::choose_grads<__bf16>(a, g, p, s);
+  return geo::attn::choose_grads<_Float16>(a, g, p, s);
+}

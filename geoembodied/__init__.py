@@ -21,10 +21,12 @@ _ALIASES = (
     "csrc",
     "functional",
     "functional.adaptive",
+    "functional.attention",
     "functional.fps",
     "functional.gather",
     "functional.knn",
     "functional.radius_graph",
+    "functional.relative_bias",
     "functional.segment_reduce",
     "functional.segment_softmax",
     "kernels",

@@ -40,6 +40,7 @@ extern "C" {
 #define GEO_F32 0
 #define GEO_BF16 1
 #define GEO_F64 2
+#define GEO_F16 3 /* the sequence operators only */
 
 /* reduction codes for segment reduce */
 #define GEO_REDUCE_SUM 0
@@ -612,6 +613,39 @@ int geo_radial_mlp_bwd(const float* dist, int64_t E, const float* freqs, int32_t
                        const float* W1, const float* b1, int32_t H, const float* W2, const float* b2,
                        int32_t P, const float* dR, float* d_dist, float* dW1, float* db1, float* dW2,
                        float* db2, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------- sequence operators --- */
+/*
+ * Attention within a window over packed sequences, softmax in float32.  Token i of the sequence
+ * [ptr[b], ptr[b+1]) sees key j of its sequence iff j <= i + right, and j >= i - left or j is one
+ * of the sequence's first `sinks` tokens, and mask[j] (if given).  Query head h reads key head
+ * h / (heads / kv_heads).  Scores are scale * q.k, plus, with a bias,
+ * bias[bias_lut[clamp(j - i, -max_distance, max_distance) + max_distance], h].  A query that sees
+ * nothing gives 0.  Values of keys that a query does not see have no effect on it, infinities and
+ * NaN included; keys whose mask is 0 are not looked at.  Tokens that lie in no sequence see nothing.
+ */
+typedef struct {
+  const void *q, *k, *v;                 /* [tokens, heads or kv_heads, head_dim], 16-byte aligned */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides in elements, rows contiguous */
+  const int64_t* ptr;                    /* [sequences + 1], or NULL: one sequence */
+  const uint8_t* mask;                   /* [tokens], 0 = no key, or NULL */
+  const void* bias;                      /* [buckets, heads], or NULL */
+  const int32_t* bias_lut;               /* [2 max_distance + 1], each in [0, buckets) */
+  int64_t tokens, sequences, left, right, sinks; /* window sizes of `tokens` or more: unbounded */
+  int32_t dtype, bias_dtype, heads, kv_heads, head_dim, buckets, max_distance; /* GEO_F32/BF16/F16 */
+  float scale;
+} geo_window_attention_t;
+
+/* out [tokens, heads, head_dim]; lse [heads, tokens] (may be NULL): log2 of the softmax's sum, for
+ * the backward. */
+int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, float* lse, void* stream);
+/* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out and
+ * lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of
+ * bias_lut that hold the bucket (each bucket's places are consecutive).  Sums have a fixed order. */
+size_t geo_window_attention_bwd_workspace_bytes(const geo_window_attention_t* args);
+int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* grad,
+                             const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
+                             void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
