@@ -38,6 +38,26 @@ class WindowAttentionArgs(ctypes.Structure):
         [("scale", c_f32)]
 
 
+class WindowStepArgs(ctypes.Structure):
+    """geo_window_step_t of include/geo_api.h."""
+
+    _fields_ = [(n, c_vp) for n in ("q", "k", "v", "k_cache", "v_cache")] + \
+        [(n, c_i64) for n in ("q_stream", "q_head", "k_stream", "k_head", "v_stream", "v_head", "k_cache_stream",
+                              "k_cache_head", "v_cache_stream", "v_cache_head")] + \
+        [(n, c_vp) for n in ("positions", "bias", "bias_lut")] + [(n, c_i64) for n in ("batch", "slots", "sinks")] + \
+        [(n, c_i32) for n in ("dtype", "bias_dtype", "heads", "kv_heads", "head_dim", "buckets", "max_distance")] + \
+        [("scale", c_f32)]
+
+
+class RecurrenceArgs(ctypes.Structure):
+    """geo_recurrence_t of include/geo_api.h."""
+
+    _fields_ = [(n, c_vp) for n in ("x", "gate_a", "gate_x")] + \
+        [(n, c_i64) for n in ("x_token", "gate_a_token", "gate_x_token")] + \
+        [(n, c_vp) for n in ("decay", "ptr", "state")] + [(n, c_i64) for n in ("tokens", "channels", "sequences")] + \
+        [("dtype", c_i32), ("reverse", c_i32), ("rate", c_f32)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "geo_last_error": (ctypes.c_char_p, []),
@@ -145,6 +165,16 @@ _SIGNATURES = {
     "geo_window_attention_bwd_workspace_bytes": (c_size, [ctypes.POINTER(WindowAttentionArgs)]),
     "geo_window_attention_bwd": (c_int, [ctypes.POINTER(WindowAttentionArgs), c_vp, c_vp, c_vp, c_vp, c_vp,
                                          c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "geo_window_attention_step_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "geo_window_attention_step": (c_int, [ctypes.POINTER(WindowStepArgs), c_vp, c_vp, c_size, c_vp]),
+    "geo_window_cache_fill": (c_int, [c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                      c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "geo_recurrence_chunks": (c_i64, [c_i64]),
+    "geo_recurrence_fwd": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "geo_recurrence_bwd_workspace_bytes": (c_size, [c_i64, c_i64]),
+    "geo_recurrence_bwd": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                   c_size, c_vp]),
+    "geo_recurrence_step": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -588,6 +588,129 @@ def window_attention_backward_hip(grad, out, lse, q, k, v, left, right, sinks, s
     return dq, dk, dv, dbias
 
 
+def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale, bias, plan, workspace):
+    """[B, H, D] of the tokens at ``positions``, whose k and v go into the caches [B, Hk, slots, D];
+    ``workspace(bytes)`` gives the scratch."""
+    name = "window_attention_step"
+    _require_gpu(name, q, k, v, k_cache, v_cache, positions, bias)
+    code = _sequence_code(name, q, k, v, k_cache, v_cache)
+    dev = _same_device(name, q, k, v, k_cache, v_cache, positions, bias)
+    q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
+    positions = _i64(positions, dev)
+    B, H, D = q.shape
+    Hk, slots = k_cache.shape[1], k_cache.shape[2]
+    bias_code = maxd = buckets = 0
+    lut = None
+    if bias is not None:
+        bias_code = _sequence_code(f"{name} bias", bias)
+        bias = bias.contiguous()
+        lut, _, maxd = plan
+        buckets = bias.shape[0]
+    args = _nat.WindowStepArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q.stride(0), q.stride(1),
+        k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
+        v_cache.stride(1), positions.data_ptr(), _nat.ptr(bias), _nat.ptr(lut), B, slots, sinks, code, bias_code, H, Hk, D,
+        buckets, maxd, scale)
+    out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
+    L = _nat.lib()
+    with _nat.on_device(dev):
+        ws = workspace(L.geo_window_attention_step_workspace_bytes(B, H, Hk, slots, D))
+        _nat.check(L.geo_window_attention_step(args, out.data_ptr(), _nat.ptr(ws), 0 if ws is None else ws.numel(),
+                                               _nat.stream_of(dev)), "geo_window_attention_step")
+    return out
+
+
+def window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start):
+    """Tokens k, v [T, Hk, D] of packed sequences into the caches [B, Hk, slots, D]."""
+    name = "WindowCache.fill"
+    _require_gpu(name, k, v, k_cache, v_cache, ptr, start)
+    code = _sequence_code(name, k, v, k_cache, v_cache)
+    dev = _same_device(name, k, v, k_cache, v_cache, ptr, start)
+    k, v = _in_pieces(k), _in_pieces(v)
+    ptr = None if ptr is None else _i64(ptr, dev)
+    start = None if start is None else _i64(start, dev)
+    with _nat.on_device(dev):
+        _nat.check(_nat.lib().geo_window_cache_fill(
+            code, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _nat.ptr(ptr),
+            _nat.ptr(start), k.shape[0], k_cache.shape[0], k.shape[1], k.shape[2], k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.stride(0), k_cache.stride(1), v_cache.stride(0), v_cache.stride(1), k_cache.shape[2], sinks,
+            _nat.stream_of(dev)), "geo_window_cache_fill")
+
+
+def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate):
+    """geo_recurrence_t of the call, and the tensors that it points into."""
+    _require_gpu(name, x, gate_a, gate_x, decay, ptr, state)
+    code = _sequence_code(name, x, gate_a, gate_x)
+    dev = _same_device(name, x, gate_a, gate_x, decay, ptr, state)
+    x, gate_a, gate_x = (t if t.stride(1) == 1 else t.contiguous() for t in (x, gate_a, gate_x))
+    decay = _nat.f32c(decay)
+    ptr = None if ptr is None else _i64(ptr, dev)
+    state = None if state is None else _nat.f32c(state)
+    T, C = x.shape
+    B = ptr.numel() - 1 if ptr is not None else 1
+    args = _nat.RecurrenceArgs(x.data_ptr(), gate_a.data_ptr(), gate_x.data_ptr(), x.stride(0), gate_a.stride(0),
+                               gate_x.stride(0), decay.data_ptr(), _nat.ptr(ptr), _nat.ptr(state), T, C, B, code,
+                               int(bool(reverse)), rate)
+    return args, (x, gate_a, gate_x, decay, ptr, state), dev, B
+
+
+def gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate):
+    """(h [T, C], last float32 [B, C], states that the scan's chunks begin with)."""
+    args, held, dev, B = _recurrence_args("gated_recurrence", x, gate_a, gate_x, decay, ptr, state, reverse, rate)
+    T, C = x.shape
+    L = _nat.lib()
+    h = torch.empty(T, C, dtype=x.dtype, device=dev)
+    if T == 0 or C == 0:
+        last = torch.zeros(B, C, dtype=torch.float32, device=dev) if state is None else held[5].clone()
+        return h, last, h.new_empty(0, C, dtype=torch.float32)
+    last = torch.empty(B, C, dtype=torch.float32, device=dev)
+    carry = torch.empty(L.geo_recurrence_chunks(T), C, dtype=torch.float32, device=dev)
+    ws = torch.empty_like(carry)
+    with _nat.on_device(dev):
+        _nat.check(L.geo_recurrence_fwd(args, h.data_ptr(), last.data_ptr(), carry.data_ptr(), ws.data_ptr(),
+                                        ws.numel() * 4, _nat.stream_of(dev)), "geo_recurrence_fwd")
+    return h, last, carry
+
+
+def gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr, state, reverse, rate):
+    """(dx, dgate_a, dgate_x, ddecay float32, dstate float32 or None)."""
+    name = "gated_recurrence backward"
+    args, held, dev, B = _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate)
+    T, C = x.shape
+    if dh is not None:
+        dh = dh.to(x.dtype).contiguous()
+        if dh.data_ptr() % 4:
+            dh = dh.clone()
+    dlast = None if dlast is None else _nat.f32c(dlast)
+    dx, dga, dgx = (torch.empty(T, C, dtype=x.dtype, device=dev) for _ in range(3))
+    if T == 0 or C == 0:
+        dstate = None if state is None else (torch.zeros_like(held[5]) if dlast is None else dlast.clone())
+        return dx, dga, dgx, torch.zeros(C, dtype=torch.float32, device=dev), dstate
+    ddecay = torch.empty(C, dtype=torch.float32, device=dev)
+    dstate = None if state is None else torch.empty(B, C, dtype=torch.float32, device=dev)
+    L = _nat.lib()
+    with _nat.on_device(dev):
+        ws_bytes = L.geo_recurrence_bwd_workspace_bytes(T, C)
+        ws = _nat.workspace(ws_bytes, dev)
+        _nat.check(L.geo_recurrence_bwd(
+            args, carry.data_ptr(), _nat.ptr(dh), _nat.ptr(dlast), dx.data_ptr(), dga.data_ptr(), dgx.data_ptr(),
+            ddecay.data_ptr(), _nat.ptr(dstate), ws.data_ptr(), ws_bytes, _nat.stream_of(dev)), "geo_recurrence_bwd")
+    return dx, dga, dgx, ddecay, dstate
+
+
+def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate):
+    """(h [B, C], new state float32 [B, C]) of one token per stream."""
+    args, held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, None, state, False, rate)
+    args.sequences = x.shape[0]
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    new = torch.empty(x.shape, dtype=torch.float32, device=dev)
+    if x.numel():
+        with _nat.on_device(dev):
+            _nat.check(_nat.lib().geo_recurrence_step(args, new.data_ptr(), h.data_ptr(), _nat.stream_of(dev)),
+                       "geo_recurrence_step")
+    return h, new
+
+
 def gather_weighted_sum_forward_hip(feat: Tensor, idx: Tensor, w: Tensor) -> Tensor:
     """out[n] = sum_k w[n, k] * feat[idx[n, k]] (idx < 0 or >= N_src contributes nothing)."""
     _require_gpu("gather_weighted_sum", feat, idx, w)
@@ -959,7 +1082,9 @@ __all__ = [
     "edge_geometry_backward_hip", "spherical_harmonics_hip", "spherical_harmonics_backward_hip",
     "graph_avg_degree_hip",
     "segment_reduce_forward_hip", "segment_reduce_backward_hip",
-    "window_attention_forward_hip", "window_attention_backward_hip",
+    "window_attention_forward_hip", "window_attention_backward_hip", "window_attention_step_hip",
+    "window_cache_fill_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
+    "gated_recurrence_step_hip",
     "knn_available", "knn_cuda", "knn_self_cuda",
     "fps_available", "fps_cuda", "fps_uniform_hip",
 ]

@@ -1,0 +1,592 @@
+// recurrence.hip — gated linear recurrence over packed sequences, forward, backward and one step.
+//
+// Per channel, with r = sigmoid(gate_a), z = sigmoid(gate_x) and log a = -rate softplus(decay) r:
+//   h_t = a_t h_{t-1} + m_t z_t x_t,   m_t = sqrt(1 - a_t^2),
+// h before a sequence's first token from `state`, or 0.  In reverse, the scan runs from each
+// sequence's last token to its first.
+//
+// A chunk of kLen tokens is one wave's, a lane V channels of it.  The chunk's map h -> A h + H is
+// formed from its inputs, the maps are composed over the chunks, and a second pass over the inputs
+// gives each chunk its outputs from the state it begins with.  All in float32, whatever the inputs.
+#include "common.hpp"
+
+namespace geo {
+namespace rec {
+
+constexpr int kLen = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T, int V> struct Pack;
+template <> struct Pack<float, 1> { using Raw = float; };
+template <> struct Pack<float, 2> { using Raw = float2; };
+template <> struct Pack<__bf16, 1> { using Raw = uint16_t; };
+template <> struct Pack<__bf16, 2> { using Raw = uint32_t; };
+template <> struct Pack<_Float16, 1> { using Raw = uint16_t; };
+template <> struct Pack<_Float16, 2> { using Raw = uint32_t; };
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(typename Pack<T, V>::Raw r, float (&f)[V]) {
+  union { typename Pack<T, V>::Raw r; T t[V]; } u;
+  u.r = r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = static_cast<float>(u.t[v]);
+}
+template <typename T, int V>
+__device__ __forceinline__ typename Pack<T, V>::Raw pack(const float (&f)[V]) {
+  union { typename Pack<T, V>::Raw r; T t[V]; } u;
+#pragma unroll
+  for (int v = 0; v < V; ++v) u.t[v] = static_cast<T>(f[v]);
+  return u.r;
+}
+
+// Relatively exact far out too: exp2's argument loses |x| log2(e) units by its rounding, which the
+// factor 1 + ln 2 err gives back.  (The median turns the NaN that err is for infinite x into a
+// finite number; exp2 is then 0 or infinite, and NaN where x is.)
+__device__ __forceinline__ float sigmoid(float x) {
+  const float t = -x * kLog2e;
+  const float err = __builtin_amdgcn_fmed3f(fmaf(-x, kLog2e, -t), -1.f, 1.f);
+  return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(t), fmaf(err, 0.6931471805599453f, 1.f), 1.f));
+}
+// 1 - exp(u) for u <= 0 to a few units in the last place: near 0 the series of -expm1, since the
+// difference would cancel.
+__device__ __forceinline__ float one_minus_exp(float u, float exp_u) {
+  float s = 1.f / 40320.f;
+  s = fmaf(s, u, 1.f / 5040.f);
+  s = fmaf(s, u, 1.f / 720.f);
+  s = fmaf(s, u, 1.f / 120.f);
+  s = fmaf(s, u, 1.f / 24.f);
+  s = fmaf(s, u, 1.f / 6.f);
+  s = fmaf(s, u, 0.5f);
+  s = fmaf(s, u, 1.f);
+  return u > -0.5f ? -u * s : 1.f - exp_u;
+}
+// A channel's log a per unit of the gate, -rate softplus(decay); softplus(x) = x for large x, where
+// exp(x) would overflow.
+__device__ __forceinline__ float log_rate(float decay, float rate) {
+  return -rate * (decay > 20.f ? decay : log1pf(expf(decay)));
+}
+
+struct Gates {
+  float a, m, r, z;
+};
+__device__ __forceinline__ Gates gates(float ga, float gx, float lr) {
+  Gates g;
+  g.r = sigmoid(ga);
+  g.z = sigmoid(gx);
+  const float la = lr * g.r;
+  g.a = __builtin_amdgcn_exp2f(la * kLog2e);
+  g.m = __builtin_amdgcn_sqrtf(one_minus_exp(2.f * la, g.a * g.a));
+  return g;
+}
+__device__ __forceinline__ float decay_of(float ga, float lr) {
+  return __builtin_amdgcn_exp2f(lr * sigmoid(ga) * kLog2e);
+}
+
+struct Scan {
+  const void *x, *ga, *gx;
+  int64_t x_st, ga_st, gx_st;  // elements from token to token
+  const float* decay;
+  const int64_t* ptr;          // [B + 1], or null: one sequence
+  const float* state;          // [B, C], or null
+  int64_t T, C;
+  int64_t B;
+  float rate;
+  int reverse;
+};
+
+// The tokens of a chunk in scan order: lane l < kLen looks at token number l of it.
+struct Chunk {
+  uint32_t begin, finish, live;  // bits: first of its sequence in scan order, last, of a sequence
+  int64_t seq;                   // this lane's token's sequence
+};
+__device__ __forceinline__ int64_t token(const Scan& s, int64_t n) { return s.reverse ? s.T - 1 - n : n; }
+__device__ __forceinline__ Chunk look(const Scan& s, int64_t chunk) {
+  const int lane = lane_id();
+  const int64_t n = chunk * kLen + (lane & (kLen - 1)), t = token(s, min(n, s.T - 1));
+  int64_t lo = 0, first = 0, end = s.T;
+  if (s.ptr) {
+    int64_t hi = s.B - 1;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi + 1) >> 1;
+      if (s.ptr[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    first = s.ptr[lo];
+    end = min(s.ptr[lo + 1], s.T);
+  }
+  const bool live = n < s.T && first <= t && t < end;
+  Chunk c;
+  c.live = static_cast<uint32_t>(__ballot(live));
+  c.begin = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? end - 1 : max(first, int64_t(0)))));
+  c.finish = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? max(first, int64_t(0)) : end - 1)));
+  c.seq = lo;
+  return c;
+}
+__device__ __forceinline__ int64_t seq_at(const Chunk& c, int l) {
+  return (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq >> 32), l)) << 32) |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq), l));
+}
+
+template <typename T, int V>
+struct Rows {
+  typename Pack<T, V>::Raw raw[kLen];
+  __device__ __forceinline__ void load(const void* base, int64_t stride, const Scan& s, int64_t chunk, int64_t at) {
+#pragma unroll
+    for (int l = 0; l < kLen; ++l) {
+      const int64_t n = min(chunk * kLen + l, s.T - 1);
+      raw[l] = *reinterpret_cast<const typename Pack<T, V>::Raw*>(static_cast<const T*>(base) + token(s, n) * stride + at);
+    }
+  }
+};
+
+// Grid of all passes: one wave per workgroup, (chunk, block of 64 V channels), channels fastest.
+struct Place {
+  int64_t chunk, at;  // this lane's first channel, in range
+  bool mine;
+};
+template <int V>
+__device__ __forceinline__ Place place(const Scan& s) {
+  const int64_t blocks = (s.C + 64 * V - 1) / (64 * V), w = xcd_block();
+  const int64_t at = (w % blocks * 64 + lane_id()) * V;
+  return {w / blocks, min(at, s.C - V), at < s.C};
+}
+
+// The factor of a map across which nothing passes, as at the beginning of a sequence: a factor of 0
+// would let the infinities and NaN of the sequence before through.  No decay is negative.
+constexpr float kCut = -1.f;
+__device__ __forceinline__ float after(float a, float add, float h) { return a == kCut ? add : fmaf(a, h, add); }
+
+// Pass 1: the chunk's map.
+template <typename T, int V>
+__global__ __launch_bounds__(64) void scan_map(const Scan s, float* __restrict__ mapa, float* __restrict__ maph) {
+  const Place p = place<V>(s);
+  Rows<T, V> x, ga, gx;
+  x.load(s.x, s.x_st, s, p.chunk, p.at);
+  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
+  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
+  const Chunk c = look(s, p.chunk);
+  float lr[V], A[V], H[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    A[v] = 1.f;
+    H[v] = 0.f;
+  }
+#pragma unroll
+  for (int l = 0; l < kLen; ++l) {
+    float xf[V], af[V], gf[V];
+    unpack<T, V>(x.raw[l], xf);
+    unpack<T, V>(ga.raw[l], af);
+    unpack<T, V>(gx.raw[l], gf);
+    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = begin ? seq_at(c, l) : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Gates g = gates(af[v], gf[v], lr[v]);
+      if (begin) {
+        A[v] = kCut;
+        H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
+      }
+      A[v] = live && A[v] != kCut ? A[v] * g.a : kCut;
+      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
+    }
+  }
+  if (p.mine) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      mapa[p.chunk * s.C + p.at + v] = A[v];
+      maph[p.chunk * s.C + p.at + v] = H[v];
+    }
+  }
+}
+
+// Between the passes: maps composed over the chunks, `maph` replaced by the state before each chunk
+// (or, `back`, after it, from the last chunk to the first).  Sixteen waves share 64 channels.
+__global__ __launch_bounds__(1024) void scan_carry(const float* __restrict__ mapa, float* __restrict__ maph, int64_t chunks,
+                                                   int64_t C, int back) {
+  __shared__ float sa[16][64], sh[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = min(static_cast<int64_t>(blockIdx.x) * 64 + lane, C - 1);
+  const bool mine = static_cast<int64_t>(blockIdx.x) * 64 + lane < C;
+  const int64_t per = (chunks + 15) / 16, c0 = min(wave * per, chunks), c1 = min(c0 + per, chunks);
+  auto index = [&](int64_t c) { return (back ? chunks - 1 - c : c) * C + at; };
+  float A = 1.f, H = 0.f;
+  for (int64_t c = c0; c < c1; c += 8) {
+    float a[8], h[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int64_t i = index(min(c + n, c1 - 1));
+      a[n] = mapa[i];
+      h[n] = maph[i];
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+      if (c + n < c1) {
+        A = a[n] == kCut || A == kCut ? kCut : A * a[n];
+        H = after(a[n], h[n], H);
+      }
+  }
+  sa[wave][lane] = A;
+  sh[wave][lane] = H;
+  __syncthreads();
+  float h0 = 0.f;
+  for (int n = 0; n < wave; ++n) h0 = after(sa[n][lane], sh[n][lane], h0);
+  for (int64_t c = c0; c < c1; c += 8) {
+    float a[8], h[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int64_t i = index(min(c + n, c1 - 1));
+      a[n] = mapa[i];
+      h[n] = maph[i];
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+      if (c + n < c1) {
+        if (mine) maph[index(c + n)] = h0;
+        h0 = after(a[n], h[n], h0);
+      }
+  }
+}
+
+// A sequence without tokens passes its state (or its state's gradient) on; chunk c sees to its share.
+__device__ __forceinline__ void pass_empty(const Scan& s, const Place& p, int64_t chunks, int V, const float* from, float* to) {
+  if (!s.ptr || !to) return;
+  const int64_t per = (s.B + chunks - 1) / chunks;
+  for (int64_t b = p.chunk * per; b < min((p.chunk + 1) * per, s.B); ++b) {
+    if (max(s.ptr[b], int64_t(0)) < min(s.ptr[b + 1], s.T) || !p.mine) continue;
+    for (int v = 0; v < V; ++v) to[b * s.C + p.at + v] = from ? from[b * s.C + p.at + v] : 0.f;
+  }
+}
+
+// Pass 2: the outputs.
+template <typename T, int V>
+__global__ __launch_bounds__(64) void scan_out(const Scan s, int64_t chunks, const float* __restrict__ carry,
+                                               T* __restrict__ h, float* __restrict__ last) {
+  const Place p = place<V>(s);
+  Rows<T, V> x, ga, gx;
+  x.load(s.x, s.x_st, s, p.chunk, p.at);
+  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
+  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
+  const Chunk c = look(s, p.chunk);
+  float lr[V], H[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    H[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
+  }
+#pragma unroll
+  for (int l = 0; l < kLen; ++l) {
+    float xf[V], af[V], gf[V];
+    unpack<T, V>(x.raw[l], xf);
+    unpack<T, V>(ga.raw[l], af);
+    unpack<T, V>(gx.raw[l], gf);
+    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = seq_at(c, l), n = p.chunk * kLen + l;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Gates g = gates(af[v], gf[v], lr[v]);
+      if (begin) H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
+      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
+    }
+    if (p.mine && n < s.T)
+      *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, n) * s.C + p.at) = pack<T, V>(H);
+    if (((c.finish >> l) & 1) && p.mine)
+#pragma unroll
+      for (int v = 0; v < V; ++v) last[b * s.C + p.at + v] = H[v];
+  }
+  pass_empty(s, p, chunks, V, s.state, last);
+}
+
+// Backward.  With e_t = a_t g_t, what token t's gradient hands to the token before:
+//   g_t = dh_t + e_{t+1} (dlast beyond a sequence's last token),  e_t = a_t g_t,
+// a scan against the order of the forward's, whose maps need gate_a and dh alone.
+struct Grad {
+  const void* dh;          // contiguous [T, C], or null
+  const float* dlast;      // [B, C], or null
+  void *dx, *dga, *dgx;    // contiguous [T, C]
+  float *dstate;           // [B, C], or null
+  float* ddecay;           // [chunks, C] sums of the chunks
+};
+
+template <typename T, int V>
+__global__ __launch_bounds__(64) void scan_bwd_map(const Scan s, const Grad d, float* __restrict__ mapa,
+                                                   float* __restrict__ mape) {
+  const Place p = place<V>(s);
+  Rows<T, V> ga, dh;
+  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
+  if (d.dh) dh.load(d.dh, s.C, s, p.chunk, p.at);
+  const Chunk c = look(s, p.chunk);
+  float lr[V], A[V], E[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    A[v] = 1.f;
+    E[v] = 0.f;
+  }
+#pragma unroll
+  for (int l = kLen - 1; l >= 0; --l) {
+    float af[V], hf[V] = {};
+    unpack<T, V>(ga.raw[l], af);
+    if (d.dh) unpack<T, V>(dh.raw[l], hf);
+    const bool finish = (c.finish >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = seq_at(c, l);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float a = decay_of(af[v], lr[v]);
+      if (finish) {
+        A[v] = kCut;
+        E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
+      }
+      A[v] = live && A[v] != kCut ? A[v] * a : kCut;
+      E[v] = live ? a * (hf[v] + E[v]) : 0.f;
+    }
+  }
+  if (p.mine) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      mapa[p.chunk * s.C + p.at + v] = A[v];
+      mape[p.chunk * s.C + p.at + v] = E[v];
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(64) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks, const float* __restrict__ carry,
+                                                   const float* __restrict__ carry_e) {
+  using Raw = typename Pack<T, V>::Raw;
+  const Place p = place<V>(s);
+  Rows<T, V> x, ga, gx, dh;
+  x.load(s.x, s.x_st, s, p.chunk, p.at);
+  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
+  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
+  if (d.dh) dh.load(d.dh, s.C, s, p.chunk, p.at);
+  const Chunk c = look(s, p.chunk);
+  float lr[V], H[V], E[V], dlr[V] = {};
+  float before[kLen][V];  // the state ahead of each token, formed again from the chunk's first
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    H[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
+    E[v] = chunks > 1 ? carry_e[p.chunk * s.C + p.at + v] : 0.f;
+  }
+#pragma unroll
+  for (int l = 0; l < kLen; ++l) {
+    float xf[V], af[V], gf[V];
+    unpack<T, V>(x.raw[l], xf);
+    unpack<T, V>(ga.raw[l], af);
+    unpack<T, V>(gx.raw[l], gf);
+    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = seq_at(c, l);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Gates g = gates(af[v], gf[v], lr[v]);
+      if (begin) H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
+      before[l][v] = H[v];
+      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int l = kLen - 1; l >= 0; --l) {
+    float xf[V], af[V], gf[V], hf[V] = {}, ox[V], oa[V], og[V];
+    unpack<T, V>(x.raw[l], xf);
+    unpack<T, V>(ga.raw[l], af);
+    unpack<T, V>(gx.raw[l], gf);
+    if (d.dh) unpack<T, V>(dh.raw[l], hf);
+    const bool finish = (c.finish >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = seq_at(c, l), n = p.chunk * kLen + l;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const Gates g = gates(af[v], gf[v], lr[v]);
+      if (finish) E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
+      const float G = live ? hf[v] + E[v] : 0.f;
+      E[v] = live ? g.a * G : 0.f;
+      const float in = g.z * xf[v];
+      ox[v] = live ? G * g.m * g.z : 0.f;
+      og[v] = live ? G * g.m * in * (1.f - g.z) : 0.f;
+      // d log a of a h + m z x: a h - a^2 / m z x.  Times d log a / d gate = log a (1 - r), whose
+      // log a / m has the limit 0 at m = 0 (no decay left in the type's range).
+      const float la = lr[v] * g.r, up = g.a * before[l][v];
+      const float lam = g.m > 0.f ? la * __builtin_amdgcn_rcpf(g.m) : 0.f;
+      const float dla = G * (up * la - g.a * g.a * in * lam);  // d log a times log a
+      oa[v] = live ? dla * (1.f - g.r) : 0.f;
+      dlr[v] += live ? dla : 0.f;
+    }
+    if (p.mine && n < s.T) {
+      const int64_t at = token(s, n) * s.C + p.at;
+      *reinterpret_cast<Raw*>(static_cast<T*>(d.dx) + at) = pack<T, V>(ox);
+      *reinterpret_cast<Raw*>(static_cast<T*>(d.dga) + at) = pack<T, V>(oa);
+      *reinterpret_cast<Raw*>(static_cast<T*>(d.dgx) + at) = pack<T, V>(og);
+    }
+    if (((c.begin >> l) & 1) && p.mine && d.dstate)
+#pragma unroll
+      for (int v = 0; v < V; ++v) d.dstate[b * s.C + p.at + v] = E[v];
+  }
+  if (p.mine)
+#pragma unroll
+    for (int v = 0; v < V; ++v) d.ddecay[p.chunk * s.C + p.at + v] = dlr[v];
+  pass_empty(s, p, chunks, V, d.dlast, d.dstate);
+}
+
+// The chunks' sums of d log a times log a, added in their order; d log a / d decay = log a times
+// sigmoid(decay) / softplus(decay).
+__global__ __launch_bounds__(1024) void scan_bwd_decay(const float* __restrict__ part, int64_t chunks, int64_t C,
+                                                       const float* __restrict__ decay, float* __restrict__ out) {
+  __shared__ float sum[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float x = 0.f;
+  for (int64_t c = wave; c < chunks; c += 16) x += part[c * C + min(at, C - 1)];
+  sum[wave][lane] = x;
+  __syncthreads();
+  if (wave || at >= C) return;
+  for (int n = 1; n < 16; ++n) x += sum[n][lane];
+  const float y = decay[at];
+  // sigmoid / softplus, near 1 where both are exp(y)
+  const float ratio = y < -15.f ? 1.f - 0.5f * expf(y) : (y > 20.f ? 1.f / y : 1.f / (1.f + expf(-y)) / log1pf(expf(y)));
+  out[at] = x * ratio;
+}
+
+// One token of each of B streams.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict__ state_out, T* __restrict__ h) {
+  const int64_t per = s.C / V, n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (n >= s.B * per) return;
+  const int64_t b = n / per, at = n % per * V;
+  using Raw = typename Pack<T, V>::Raw;
+  float xf[V], af[V], gf[V], H[V];
+  unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.x) + b * s.x_st + at), xf);
+  unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.ga) + b * s.ga_st + at), af);
+  unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.gx) + b * s.gx_st + at), gf);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const Gates g = gates(af[v], gf[v], log_rate(s.decay[at + v], s.rate));
+    H[v] = fmaf(g.a, s.state[b * s.C + at + v], g.m * g.z * xf[v]);
+    state_out[b * s.C + at + v] = H[v];
+  }
+  *reinterpret_cast<Raw*>(h + b * s.C + at) = pack<T, V>(H);
+}
+
+// ---------------------------------------------------------------------- host ---
+
+inline int64_t chunks_of(int64_t T) { return ceil_div(T, kLen); }
+
+inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
+  GEO_REQUIRE(g, "gated recurrence: null arguments");
+  GEO_REQUIRE(g->dtype == GEO_F32 || g->dtype == GEO_BF16 || g->dtype == GEO_F16, "gated recurrence: dtype code %d",
+              static_cast<int>(g->dtype));
+  GEO_REQUIRE(g->tokens >= 0 && g->channels >= 0 && g->sequences >= 1, "gated recurrence: %lld tokens, %lld channels, %lld sequences",
+              static_cast<long long>(g->tokens), static_cast<long long>(g->channels), static_cast<long long>(g->sequences));
+  *s = Scan{g->x, g->gate_a, g->gate_x, g->x_token, g->gate_a_token, g->gate_x_token, g->decay, g->ptr, g->state,
+            g->tokens, g->channels, g->sequences, g->rate, g->reverse};
+  const int size = g->dtype == GEO_F32 ? 4 : 2;
+  auto even = [size](const void* p, int64_t st) { return reinterpret_cast<uintptr_t>(p) % (2 * size) == 0 && st % 2 == 0; };
+  // two 16-bit channels to a lane where every row begins on a multiple of 4 bytes
+  *v = size == 2 && g->channels % 2 == 0 && even(g->x, g->x_token) && even(g->gate_a, g->gate_a_token) &&
+               even(g->gate_x, g->gate_x_token) ? 2 : 1;
+  GEO_REQUIRE(g->tokens == 0 || g->channels == 0 || (g->x && g->gate_a && g->gate_x && g->decay), "gated recurrence: null tensor");
+  GEO_REQUIRE(chunks_of(g->tokens) * ceil_div(g->channels, 64 * *v) < (int64_t(1) << 31), "gated recurrence: too many workgroups");
+  return GEO_OK;
+}
+
+template <typename T, int V>
+int forward(const Scan& s, void* h, float* last, float* maph, float* mapa, hipStream_t stream) {
+  const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
+  const dim3 grid(static_cast<uint32_t>(chunks * blocks));
+  if (chunks > 1) {
+    scan_map<T, V><<<grid, dim3(64), 0, stream>>>(s, mapa, maph);
+    GEO_LAUNCH_CHECK("scan_map");
+    scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, maph, chunks, s.C, 0);
+    GEO_LAUNCH_CHECK("scan_carry");
+  }
+  scan_out<T, V><<<grid, dim3(64), 0, stream>>>(s, chunks, maph, static_cast<T*>(h), last);
+  GEO_LAUNCH_CHECK("scan_out");
+  return GEO_OK;
+}
+
+template <typename T, int V>
+int backward(const Scan& s, const Grad& d, const float* carry, float* mape, float* mapa, float* ddecay, hipStream_t stream) {
+  const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
+  const dim3 grid(static_cast<uint32_t>(chunks * blocks));
+  if (chunks > 1) {
+    scan_bwd_map<T, V><<<grid, dim3(64), 0, stream>>>(s, d, mapa, mape);
+    GEO_LAUNCH_CHECK("scan_bwd_map");
+    scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, mape, chunks, s.C, 1);
+    GEO_LAUNCH_CHECK("scan_carry");
+  }
+  scan_bwd_out<T, V><<<grid, dim3(64), 0, stream>>>(s, d, chunks, carry, mape);
+  GEO_LAUNCH_CHECK("scan_bwd_out");
+  scan_bwd_decay<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(d.ddecay, chunks, s.C, s.decay, ddecay);
+  GEO_LAUNCH_CHECK("scan_bwd_decay");
+  return GEO_OK;
+}
+
+}  // namespace rec
+}  // namespace geo
+
+#define GEO_REC_CALL(F, ...)                                                                      \
+  (g->dtype == GEO_F32    ? geo::rec::F<float, 1>(__VA_ARGS__)                                    \
+   : g->dtype == GEO_BF16 ? (v == 2 ? geo::rec::F<__bf16, 2>(__VA_ARGS__) : geo::rec::F<__bf16, 1>(__VA_ARGS__)) \
+                          : (v == 2 ? geo::rec::F<_Float16, 2>(__VA_ARGS__) : geo::rec::F<_Float16, 1>(__VA_ARGS__)))
+
+extern "C" int64_t geo_recurrence_chunks(int64_t tokens) { return tokens < 0 ? 0 : geo::rec::chunks_of(tokens); }
+
+extern "C" int geo_recurrence_fwd(const geo_recurrence_t* g, void* h, float* last, float* carry, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  geo::rec::Scan s;
+  int v;
+  const int rc = geo::rec::scan_args(g, &s, &v);
+  if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
+  GEO_REQUIRE(h && last && carry, "gated recurrence: null output");
+  const size_t need = static_cast<size_t>(geo::rec::chunks_of(s.T)) * s.C * sizeof(float);
+  if (!workspace || workspace_bytes < need)
+    return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes, %zu needed",
+                          workspace ? workspace_bytes : size_t(0), need);
+  return GEO_REC_CALL(forward, s, h, last, carry, static_cast<float*>(workspace), geo::as_stream(stream));
+}
+
+extern "C" size_t geo_recurrence_bwd_workspace_bytes(int64_t tokens, int64_t channels) {
+  if (tokens < 1 || channels < 1) return 0;
+  return static_cast<size_t>(geo::rec::chunks_of(tokens)) * channels * 3 * sizeof(float);
+}
+
+extern "C" int geo_recurrence_bwd(const geo_recurrence_t* g, const float* carry, const void* dh, const float* dlast, void* dx,
+                                  void* dgate_a, void* dgate_x, float* ddecay, float* dstate, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  geo::rec::Scan s;
+  int v;
+  const int rc = geo::rec::scan_args(g, &s, &v);
+  if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
+  GEO_REQUIRE(carry && dx && dgate_a && dgate_x && ddecay, "gated recurrence backward: null tensor");
+  GEO_REQUIRE(v == 1 || reinterpret_cast<uintptr_t>(dh) % 4 == 0, "gated recurrence backward: dh must lie on a multiple of 4 bytes");
+  const size_t need = geo_recurrence_bwd_workspace_bytes(s.T, s.C);
+  if (!workspace || workspace_bytes < need)
+    return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence backward: workspace of %zu bytes, %zu needed",
+                          workspace ? workspace_bytes : size_t(0), need);
+  const int64_t n = geo::rec::chunks_of(s.T) * s.C;
+  float* w = static_cast<float*>(workspace);
+  const geo::rec::Grad d{dh, dlast, dx, dgate_a, dgate_x, dstate, w + 2 * n};
+  return GEO_REC_CALL(backward, s, d, carry, w, w + n, ddecay, geo::as_stream(stream));
+}
+
+namespace geo {
+namespace rec {
+template <typename T, int V>
+int step(const Scan& s, float* state_out, void* h, hipStream_t stream) {
+  const int64_t blocks = ceil_div(s.B * (s.C / V), 256);
+  GEO_REQUIRE(blocks < (int64_t(1) << 31), "gated recurrence step: too many workgroups");
+  scan_step<T, V><<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(s, state_out, static_cast<T*>(h));
+  GEO_LAUNCH_CHECK("scan_step");
+  return GEO_OK;
+}
+}  // namespace rec
+}  // namespace geo
+
+extern "C" int geo_recurrence_step(const geo_recurrence_t* g, float* state_out, void* h, void* stream) {
+  geo::rec::Scan s;
+  int v;
+  const int rc = geo::rec::scan_args(g, &s, &v);
+  if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
+  GEO_REQUIRE(g->sequences == g->tokens, "gated recurrence step: one token for each of %lld streams, got %lld",
+              static_cast<long long>(g->sequences), static_cast<long long>(g->tokens));
+  GEO_REQUIRE(s.state && state_out && h, "gated recurrence step: null tensor");
+  return GEO_REC_CALL(step, s, state_out, h, geo::as_stream(stream));
+}

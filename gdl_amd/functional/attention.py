@@ -7,6 +7,13 @@ token ``i`` sees the keys of its own sequence from ``i - left`` to ``i + right``
 first ``sinks`` tokens, as far as they lie at or before ``i + right``.  The softmax, the relative
 position bias and every gradient (of ``q``, ``k``, ``v`` and the bias table) are computed tile by
 tile on the matrix units; no score, weight or bias matrix is ever written.
+
+For streams that are answered token by token ``WindowCache`` keeps what a causal window
+``(left, 0)`` still reaches, and ``window_attention_step`` adds one token to it and attends:
+
+    cache = WindowCache.empty(B, Hk, D, left, sinks=4, dtype=torch.bfloat16, device="cuda")
+    cache.fill(k, v, ptr)                                     # the tokens that are there already
+    out = window_attention_step(q, k, v, cache, positions)    # [B, H, D], one token per stream
 """
 
 from __future__ import annotations
@@ -18,7 +25,13 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from gdl_amd.csrc import window_attention_backward_hip, window_attention_forward_hip
+from gdl_amd import _native as _nat
+from gdl_amd.csrc import (
+    window_attention_backward_hip,
+    window_attention_forward_hip,
+    window_attention_step_hip,
+    window_cache_fill_hip,
+)
 from gdl_amd.functional.relative_bias import bucket_plan
 
 _UNBOUNDED = 1 << 40
@@ -105,3 +118,92 @@ def window_attention(
     else:
         out, _ = window_attention_forward_hip(q, k, v, left, right, int(sinks), scale, ptr, mask, bias, plan, False)
     return out[..., :d] if d % 8 else out
+
+
+class WindowCache:
+    """Keys and values of streams that a causal window reaches: ``k, v [B, Hk, sinks + ring, D]``.
+
+    Token ``j`` of a stream lies in slot ``j`` for ``j < sinks``, else in slot
+    ``sinks + (j - sinks) % ring``, ``ring`` = left + 1 tokens of the window.  The object holds the two
+    tensors (given ones are used as they are) and the scratch of the steps; calls on it are ordered by
+    the caller's stream.
+    """
+
+    def __init__(self, k: Tensor, v: Tensor, *, sinks: int = 0):
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"WindowCache: k and v [B, Hk, sinks + ring, D], got {tuple(k.shape)}, {tuple(v.shape)}")
+        if not 0 <= sinks < k.shape[2]:
+            raise ValueError(f"WindowCache: {sinks} of {k.shape[2]} slots for first tokens (at least one is the window's)")
+        if k.shape[3] % 8 or not 8 <= k.shape[3] <= 128:
+            raise ValueError(f"WindowCache: head size {k.shape[3]} (a multiple of 8 up to 128)")
+        for t in (k, v):
+            size = t.element_size()
+            if t.stride(3) != 1 or t.stride(2) != t.shape[3] or any(x % 16 for x in (
+                    t.data_ptr(), t.stride(0) * size, t.stride(1) * size)):
+                raise ValueError("WindowCache: a head's slots must adjoin, on multiples of 16 bytes")
+        self.k, self.v, self.sinks = k, v, int(sinks)
+        self.left = k.shape[2] - self.sinks - 1
+        self._scratch: Optional[Tensor] = None
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, head_dim: int, left: int, *, sinks: int = 0,
+              dtype: torch.dtype = torch.float32, device="cuda") -> "WindowCache":
+        """A cache of no tokens for a window of ``left`` tokens and the current one."""
+        if left < 0 or sinks < 0:
+            raise ValueError(f"WindowCache: window of {left} tokens, {sinks} first tokens")
+        k, v = (torch.empty(batch, kv_heads, sinks + left + 1, head_dim, dtype=dtype, device=device) for _ in range(2))
+        return cls(k, v, sinks=sinks)
+
+    def fill(self, k: Tensor, v: Tensor, ptr: Optional[Tensor] = None, start: Optional[Tensor] = None) -> None:
+        """Tokens ``k, v [T, Hk, D]`` of packed sequences (``ptr`` int64 [B + 1]; None: one stream) into the
+        cache; sequence ``b`` begins at position ``start[b]`` (0)."""
+        batch, heads, _, d = self.k.shape
+        if k.dim() != 3 or v.shape != k.shape or k.shape[1:] != (heads, d):
+            raise ValueError(f"WindowCache.fill: k and v [T, {heads}, {d}], got {tuple(k.shape)}, {tuple(v.shape)}")
+        if (ptr is None and batch != 1) or (ptr is not None and ptr.shape != (batch + 1,)):
+            raise ValueError(f"WindowCache.fill: ptr [{batch + 1}] of {batch} streams")
+        if start is not None and start.shape != (batch,):
+            raise ValueError(f"WindowCache.fill: start [{batch}], got {tuple(start.shape)}")
+        window_cache_fill_hip(k, v, self.k, self.v, self.sinks, ptr, start)
+
+    def _workspace(self, nbytes: int) -> Optional[Tensor]:
+        if nbytes and (self._scratch is None or self._scratch.numel() < nbytes):
+            self._scratch = _nat.workspace(nbytes, self.k.device)
+        return self._scratch if nbytes else None
+
+
+def window_attention_step(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    cache: WindowCache,
+    positions: Tensor,
+    *,
+    bias: Optional[Tensor] = None,
+    max_distance: int = 128,
+    scale: Optional[float] = None,
+) -> Tensor:
+    """One token of each stream: ``k, v [B, Hk, D]`` go into the cache at ``positions`` (int64 [B], from
+    0), and ``q [B, H, D]`` attends to the tokens that the cache then holds.
+
+    The result is ``window_attention``'s for the last token of such streams with the window
+    ``(cache.left, 0)`` and ``cache.sinks`` first tokens.  A stream at a negative position is left
+    alone (its row is 0).  No gradients.  ``bias`` is one-sided.
+    """
+    batch, hk, _, d = cache.k.shape
+    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] != d or k.shape != (batch, hk, d) or v.shape != k.shape:
+        raise ValueError(f"window_attention_step: q [{batch}, H, {d}], k and v [{batch}, {hk}, {d}]; got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.shape[1] < 1 or q.shape[1] % hk:
+        raise ValueError(f"window_attention_step: {q.shape[1]} heads are no multiple of {hk} key heads")
+    if positions.shape != (batch,) or positions.dtype.is_floating_point:
+        raise ValueError(f"window_attention_step: positions int64 [{batch}], got {positions.dtype} {tuple(positions.shape)}")
+    plan = None
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] != q.shape[1]:
+            raise ValueError(f"window_attention_step: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
+        plan = bucket_plan(bias.shape[0], int(max_distance), False, q.device) + (int(max_distance),)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+        raise RuntimeError("window_attention_step has no backward: call it under torch.no_grad()")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    return window_attention_step_hip(q, k, v, cache.k, cache.v, cache.sinks, positions, scale, bias, plan, cache._workspace)

@@ -1,0 +1,116 @@
+"""Gated linear recurrence over packed point sequences.
+
+    h, last = gated_recurrence(x, gate_a, gate_x, decay, ptr=ptr)        # [T, C], float32 [B, C]
+    h, state = gated_recurrence_step(x, gate_a, gate_x, decay, state)    # one token per stream
+
+mixes a whole cloud along its order with a state per channel: with ``r = sigmoid(gate_a)``,
+``z = sigmoid(gate_x)`` and ``log a = -rate * softplus(decay) * r``,
+
+    h_t = a_t * h_{t-1} + sqrt(1 - a_t ** 2) * z_t * x_t,
+
+so a channel keeps its scale whatever it forgets.  The scan runs over all chunks of all sequences at
+once, in float32 whatever the inputs' type; the backward forms the states again from the chunks'
+first ones instead of reading the rounded outputs.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from gdl_amd.csrc import (
+    gated_recurrence_backward_hip,
+    gated_recurrence_forward_hip,
+    gated_recurrence_step_hip,
+)
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_a, gate_x, decay, state, ptr, reverse, rate):
+        h, last, carry = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate)
+        ctx.save_for_backward(x, gate_a, gate_x, decay, state, ptr, carry)
+        ctx.rest = (reverse, rate)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dlast):
+        x, gate_a, gate_x, decay, state, ptr, carry = ctx.saved_tensors
+        dx, dga, dgx, ddecay, dstate = gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr, state,
+                                                                     *ctx.rest)
+        return (dx, dga, dgx, ddecay.to(decay.dtype), None if dstate is None else dstate.to(state.dtype), None, None,
+                None)
+
+
+def _check(name: str, x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor) -> None:
+    if x.dim() != 2 or gate_a.shape != x.shape or gate_x.shape != x.shape or decay.shape != x.shape[1:]:
+        raise ValueError(f"{name}: x, gate_a and gate_x [T, C], decay [C]; got {tuple(x.shape)}, {tuple(gate_a.shape)}, "
+                         f"{tuple(gate_x.shape)}, {tuple(decay.shape)}")
+    if not decay.dtype.is_floating_point:
+        raise TypeError(f"{name}: decay must be a floating type, got {decay.dtype}")
+
+
+def gated_recurrence(
+    x: Tensor,
+    gate_a: Tensor,
+    gate_x: Tensor,
+    decay: Tensor,
+    *,
+    ptr: Optional[Tensor] = None,
+    state: Optional[Tensor] = None,
+    reverse: bool = False,
+    rate: float = 8.0,
+) -> Tuple[Tensor, Tensor]:
+    """The recurrence over packed sequences.
+
+    Args:
+        x, gate_a, gate_x: [T, C] of one type, float32, bfloat16 or float16; rows may be strided.
+        decay: [C], any floating type.
+        ptr: int64 [B + 1] ascending offsets of the sequences; None: one sequence.
+        state: [B, C] states before the first tokens; None: 0.
+        reverse: from each sequence's last token to its first.
+        rate: positive; scales the decay.
+
+    Returns:
+        (h [T, C] of x's type, last float32 [B, C]: the state after each sequence's last token in scan
+        order, its ``state`` where it has no tokens).  Tokens of no sequence give 0.
+    """
+    _check("gated_recurrence", x, gate_a, gate_x, decay)
+    batch = 1 if ptr is None else ptr.numel() - 1
+    if ptr is not None and (ptr.dim() != 1 or batch < 1):
+        raise ValueError(f"gated_recurrence: ptr must be [B + 1] with at least one sequence, got {tuple(ptr.shape)}")
+    if state is not None and (state.shape != (batch, x.shape[1]) or not state.dtype.is_floating_point):
+        raise ValueError(f"gated_recurrence: state must be [{batch}, {x.shape[1]}], got {state.dtype} {tuple(state.shape)}")
+    rate = float(rate)
+    if not rate > 0:
+        raise ValueError(f"gated_recurrence: rate {rate} must be positive")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_a, gate_x, decay, state)):
+        return _GatedRecurrence.apply(x, gate_a, gate_x, decay, state, ptr, bool(reverse), rate)
+    h, last, _ = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, bool(reverse), rate)
+    return h, last
+
+
+def gated_recurrence_step(
+    x: Tensor,
+    gate_a: Tensor,
+    gate_x: Tensor,
+    decay: Tensor,
+    state: Tensor,
+    *,
+    rate: float = 8.0,
+) -> Tuple[Tensor, Tensor]:
+    """One token of each stream: x, gates [B, C] and the streams' float32 states [B, C] to
+    (h [B, C] of x's type, new states float32 [B, C]).  No gradients."""
+    _check("gated_recurrence_step", x, gate_a, gate_x, decay)
+    if state.shape != x.shape or state.dtype is not torch.float32:
+        raise ValueError(f"gated_recurrence_step: state must be float32 {tuple(x.shape)}, got {state.dtype} {tuple(state.shape)}")
+    if not rate > 0:
+        raise ValueError(f"gated_recurrence_step: rate {rate} must be positive")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_a, gate_x, decay, state)):
+        raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad()")
+    return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, float(rate))

@@ -26,6 +26,7 @@ _ALIASES = (
     "functional.gather",
     "functional.knn",
     "functional.radius_graph",
+    "functional.recurrence",
     "functional.relative_bias",
     "functional.segment_reduce",
     "functional.segment_softmax",

@@ -647,6 +647,73 @@ int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out
                              const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
                              void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * One new token for each of `batch` streams of the attention above (right = 0), over a cache of
+ * slots rows per stream and key head: token j lies in slot j for j < sinks, else in slot
+ * sinks + (j - sinks) mod (slots - sinks).  k and v of the token at positions[b] (int64, from 0) are
+ * written to its slot; q attends to the tokens up to it that are held, which are the first `sinks`
+ * and the last slots - sinks.  A negative position leaves the stream's cache as it is and gives 0.
+ * Slots that hold no token are not read.  Rows contiguous, 16-byte aligned.
+ */
+typedef struct {
+  const void *q, *k, *v;       /* [batch, heads or kv_heads, head_dim] */
+  void *k_cache, *v_cache;     /* [batch, kv_heads, slots, head_dim], rows of a head adjoining */
+  int64_t q_stream, q_head, k_stream, k_head, v_stream, v_head; /* strides in elements */
+  int64_t k_cache_stream, k_cache_head, v_cache_stream, v_cache_head;
+  const int64_t* positions;    /* [batch] */
+  const void* bias;            /* [buckets, heads], or NULL; places of bias_lut as above */
+  const int32_t* bias_lut;
+  int64_t batch, slots, sinks;
+  int32_t dtype, bias_dtype, heads, kv_heads, head_dim, buckets, max_distance;
+  float scale;
+} geo_window_step_t;
+size_t geo_window_attention_step_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                 int64_t slots, int64_t head_dim);
+int geo_window_attention_step(const geo_window_step_t* args, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* Tokens of packed sequences into such caches: token t of sequence b, [ptr[b], ptr[b+1]), has the
+ * position start[b] + t - ptr[b] (start NULL: from 0); those that the cache still holds after the
+ * sequence's last one are written.  k, v [tokens, kv_heads, head_dim] by strides. */
+int geo_window_cache_fill(int dtype, const void* k, const void* v, int64_t k_token, int64_t k_head,
+                          int64_t v_token, int64_t v_head, const int64_t* ptr, const int64_t* start,
+                          int64_t tokens, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                          void* k_cache, void* v_cache, int64_t k_cache_stream, int64_t k_cache_head,
+                          int64_t v_cache_stream, int64_t v_cache_head, int64_t slots, int64_t sinks,
+                          void* stream);
+
+/*
+ * Gated linear recurrence over packed sequences, in float32: with r = sigmoid(gate_a),
+ * z = sigmoid(gate_x), log a = -rate softplus(decay) r, per channel
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) z_t x_t,
+ * h before a sequence's first token from state, or 0.  reverse: from each sequence's last token to
+ * its first.  Tokens in no sequence give 0.
+ */
+typedef struct {
+  const void *x, *gate_a, *gate_x;              /* [tokens, channels], rows contiguous */
+  int64_t x_token, gate_a_token, gate_x_token;  /* strides in elements */
+  const float* decay;                           /* [channels] */
+  const int64_t* ptr;                           /* [sequences + 1], or NULL: one sequence */
+  const float* state;                           /* [sequences, channels], or NULL */
+  int64_t tokens, channels, sequences;
+  int32_t dtype, reverse;
+  float rate;
+} geo_recurrence_t;
+/* Chunks of the scan: carry is [chunks, channels], the states that the chunks begin with, which the
+ * backward reads. */
+int64_t geo_recurrence_chunks(int64_t tokens);
+/* h [tokens, channels]; last float32 [sequences, channels], the states after each sequence's last
+ * token in scan order (its state where it has none).  Workspace: as large as carry. */
+int geo_recurrence_fwd(const geo_recurrence_t* args, void* h, float* last, float* carry,
+                       void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from dh [tokens, channels] and dlast (each may be NULL: zero); dstate may be NULL. */
+size_t geo_recurrence_bwd_workspace_bytes(int64_t tokens, int64_t channels);
+int geo_recurrence_bwd(const geo_recurrence_t* args, const float* carry, const void* dh,
+                       const float* dlast, void* dx, void* dgate_a, void* dgate_x, float* ddecay,
+                       float* dstate, void* workspace, size_t workspace_bytes, void* stream);
+/* One token of each of `sequences` = `tokens` streams: x, gates and h [streams, channels], state read,
+ * state_out written (they may be one tensor). */
+int geo_recurrence_step(const geo_recurrence_t* args, float* state_out, void* h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
