@@ -43,8 +43,13 @@ DEVICE_FLAGS = [
 # Per-file device flags.  fps.hip: the sampling loops end every iteration with one lane's LDS
 # atomic max; the atomic optimizer would wrap it in a single-lane election (mbcnt, compare, exec
 # mask) that lengthens the path to the barrier in every wave, every iteration.
+# window_attention*.hip: the matrix products' results are rescaled and turned operand by ordinary
+# instructions; in accumulation registers each of those would first be copied out (three copies per
+# score in the forward's loop).
 FILE_FLAGS = {
     "fps.hip": ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
+    "window_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "window_attention_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

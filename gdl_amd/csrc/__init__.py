@@ -518,9 +518,10 @@ def _same_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
 
 
 def _in_pieces(t: Tensor) -> Tensor:
-    """t [T, H, D] itself where its rows are contiguous and begin on multiples of 16 bytes."""
-    size = t.element_size()
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * size % 16 == 0 and t.stride(1) * size % 16 == 0:
+    """t [T, H, D] itself where its rows are contiguous, begin on multiples of 16 bytes and do not
+    overlap."""
+    size, (st, sh, sd) = t.element_size(), t.stride()
+    if sd == 1 and t.data_ptr() % 16 == 0 and st * size % 16 == 0 and sh * size % 16 == 0 and t.shape[2] <= st < 1 << 22:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -16,9 +16,30 @@ struct Attend {
   float scale;
 };
 
-// Reads of 16 bytes begin at any token and head: pointer and strides are multiples of that.
-inline bool in_pieces(const void* p, int64_t st, int64_t sh, int size) {
-  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+// The keys of a workgroup's queries q0 .. q0 + rows - 1: the first and last queries' bound them, for
+// both ends grow with the query; and the leading tokens of the first query's sequence, as far as
+// they lie before those.  Wave-uniform.
+struct Span {
+  int first, sink_end, jlo, jend;
+};
+__device__ __forceinline__ Span span_of(const Attend& a, const int* sptr, int q0, int rows) {
+  int first0, end0, first1, end1;
+  seq_of(a.seq, sptr, q0, first0, end0);
+  const int q1 = min(q0 + rows, a.seq.T) - 1;
+  seq_of(a.seq, sptr, q1, first1, end1);
+  Span k;
+  k.first = __builtin_amdgcn_readfirstlane(first0);
+  k.jlo = __builtin_amdgcn_readfirstlane(max(first0, q0 - a.left));
+  k.jend = __builtin_amdgcn_readfirstlane(min(end1, q1 + a.right + 1));
+  k.sink_end = __builtin_amdgcn_readfirstlane(min(min(first0 + a.sinks, k.jlo), end0));
+  return k;
+}
+
+// Reads of 16 bytes begin at any token and head: pointer and strides are multiples of that.  Tokens
+// do not overlap, and a tile's offsets stay below 2^31.
+inline bool in_pieces(const void* p, int64_t st, int64_t sh, int D, int size) {
+  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0 && st >= D &&
+         st < (int64_t(1) << 22);
 }
 
 inline int attend_args(const geo_window_attention_t* g, Attend* a) {
@@ -44,9 +65,11 @@ inline int attend_args(const geo_window_attention_t* g, Attend* a) {
   }
   if (g->tokens == 0) return GEO_OK;
   const int size = g->dtype == GEO_F32 ? 4 : 2;
-  GEO_REQUIRE(in_pieces(g->q, g->q_token, g->q_head, size) && in_pieces(g->k, g->k_token, g->k_head, size) &&
-                  in_pieces(g->v, g->v_token, g->v_head, size),
-              "window attention: null q, k or v, or their rows not on multiples of 16 bytes");
+  GEO_REQUIRE(in_pieces(g->q, g->q_token, g->q_head, g->head_dim, size) &&
+                  in_pieces(g->k, g->k_token, g->k_head, g->head_dim, size) &&
+                  in_pieces(g->v, g->v_token, g->v_head, g->head_dim, size),
+              "window attention: null q, k or v, rows not on multiples of 16 bytes, or a token stride below the head size "
+              "or from 2^22 on");
   const int T = static_cast<int>(g->tokens);
   auto up_to = [T](int64_t x) { return static_cast<int>(x < T ? x : T); };
   *a = Attend{g->q, g->k, g->v, g->q_token, g->q_head, g->k_token, g->k_head, g->v_token, g->v_head,

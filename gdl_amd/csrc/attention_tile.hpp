@@ -27,9 +27,10 @@ template <> struct Type<__bf16> {
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // nonzero iff one of the packed values is infinite or NaN
-  static __device__ __forceinline__ uint32_t wild(uint32_t w) {
-    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  // x plus 0 times the packed values: x, or NaN where one of them is infinite or NaN
+  static __device__ __forceinline__ float probe(uint32_t w, float x) {
+    using Two = __bf16 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, w), Two{}, x, false);
   }
 };
 template <> struct Type<_Float16> {
@@ -37,8 +38,9 @@ template <> struct Type<_Float16> {
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t wild(uint32_t w) {
-    return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+  static __device__ __forceinline__ float probe(uint32_t w, float x) {
+    using Two = _Float16 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(Two, w), Two{}, x, false);
   }
 };
 // float32: eight products with one k of each half, which cover the same sixteen k.
@@ -49,9 +51,7 @@ template <> struct Type<float> {
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ uint32_t wild(uint32_t w) {
-    return (w & 0x7f800000u) == 0x7f800000u;
-  }
+  static __device__ __forceinline__ float probe(uint32_t w, float x) { return fmaf(__uint_as_float(w), 0.f, x); }
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -69,93 +69,152 @@ __device__ __forceinline__ float halves_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A tile of rows in LDS: ROWS rows of DP values (a head's D, zero beyond), 16 bytes of padding per
-// row so that the rows of a column of 16-byte reads start in different banks.
+// Rows row0 .. end - 1 of a head as a buffer: reads past them give zeros.  A row's offset is a
+// multiple of the stride (at least D values), so a piece of row r lies inside iff r < end - row0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* base, int64_t stride_bytes, int row0, int end) {
+  const int64_t bytes = (end - row0) * stride_bytes;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + row0 * stride_bytes, 0,
+                                           static_cast<int>(min(bytes, int64_t(0x7fffffff))), 0x00020000);
+}
+
+// A tile of ROWS rows in LDS, DP values each (a head's D, zeros beyond), in pieces of 16 bytes.
+// Rows adjoin (their pieces rounded up to a power of two), and piece c of row r lies in the place
+// c ^ turn(r), which keeps the wave's reads out of each other's banks (64 of 4 bytes): a read along
+// the rows takes one piece of eight neighbouring rows at a time, a transposing read two to four
+// neighbouring pieces of four rows.
 template <typename T, int DP, int ROWS, int NT>
 struct Tile {
-  static constexpr int kPer = 16 / sizeof(T);            // values in 16 bytes
-  static constexpr int kStride = DP + kPer;              // values from row to row
-  static constexpr int kChunks = DP / kPer;              // 16-byte pieces of a row
-  static constexpr int kLoads = ROWS * kChunks / NT;     // per thread
-  static constexpr int kBytes = ROWS * kStride * sizeof(T);
+  static constexpr int kPer = 16 / sizeof(T);        // values in a piece
+  static constexpr int kChunks = DP / kPer;          // pieces of a row
+  static constexpr int kPlaces = kChunks <= 4 ? 4 : kChunks <= 8 ? 8 : kChunks <= 16 ? 16 : 32;
+  static constexpr int kRow = kPlaces * 16;          // bytes from row to row
+  static constexpr int kLoads = ROWS * kChunks / NT; // per thread
+  static constexpr int kBytes = ROWS * kRow;
   static_assert(ROWS * kChunks % NT == 0, "a thread loads whole pieces");
 
-  uint4 reg[kLoads];
-
-  // Rows row0.. of a head into registers; rows from `end` on and values from D on are not read
-  // (their address is the last one's, in bounds: `end` >= 1).
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int D) {
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) {
-      const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks * kPer;
-      const int r = min(row0 + row, end - 1), d = at < D ? at : 0;
-      reg[n] = *reinterpret_cast<const uint4*>(base + r * stride + d);
+  static __device__ __forceinline__ int turn(int r) {
+    if constexpr (sizeof(T) == 2) {
+      if constexpr (kPlaces == 4) return (r >> 2) & 3;
+      else if constexpr (kPlaces == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+      else return (r & 3) << 2 | ((r >> 2) & 3);
+    } else {
+      if constexpr (kPlaces == 8) return (r >> 1) & 3;
+      else return (r & 3) | ((r >> 2) & 1) << 3;
     }
   }
-  // The registers into LDS, rows whose bit is off and values from D on as zeros.
-  __device__ __forceinline__ void store(T* lds, uint64_t rows, int D) const {
+
+  uint4 reg[kLoads];
+  uint32_t off[kLoads];  // of the thread's pieces from the tile's first row, in bytes
+
+  __device__ __forceinline__ void init(int64_t stride_bytes, int D) {
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
       const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks * kPer;
-      *reinterpret_cast<uint4*>(lds + row * kStride + at) = piece(n, rows, D);
+      off[n] = at < D ? static_cast<uint32_t>(row * static_cast<uint32_t>(stride_bytes) + at * sizeof(T)) : 0x80000000u;
     }
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows) {
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n)
+      reg[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, off[n], 0, 0));
+  }
+  static __device__ __forceinline__ uint4* place(T* lds, int n) {
+    const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks;
+    return reinterpret_cast<uint4*>(reinterpret_cast<char*>(lds) + row * kRow + ((at ^ turn(row)) << 4));
+  }
+  // Rows whose bit is off as zeros (`some`: there may be such rows).
+  __device__ __forceinline__ void drop(uint64_t rows, bool some) {
+    if (!some) return;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int row = (threadIdx.x + n * NT) / kChunks;
+      if (!((rows >> row) & 1)) reg[n] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) *place(lds, n) = reg[n];
   }
   // The same with zeros in the place of infinities and NaN, whose rows' bits go to `wild` (LDS): a
   // product down the rows gives every column's query or key a weight for every row, and a weight
   // of 0 would not keep them from the ones that do not see the row.  add_wild adds them where the
   // row is seen.
-  __device__ __forceinline__ void store_finite(T* lds, uint64_t rows, int D, unsigned long long* wild) const {
+  __device__ __forceinline__ void store_finite(T* lds, unsigned long long* wild) const {
+    float x = 0.f;
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
-      const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks * kPer;
-      union { uint4 u; T t[kPer]; } v;
-      v.u = piece(n, rows, D);
-      if (Type<T>::wild(v.u.x) | Type<T>::wild(v.u.y) | Type<T>::wild(v.u.z) | Type<T>::wild(v.u.w)) {
-        atomicOr(wild, 1ull << row);
+      *place(lds, n) = reg[n];
+      x = Type<T>::probe(reg[n].x, x);
+      x = Type<T>::probe(reg[n].y, x);
+      x = Type<T>::probe(reg[n].z, x);
+      x = Type<T>::probe(reg[n].w, x);
+    }
+    if (x == 0.f) return;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e)
-          v.t[e] = fabsf(static_cast<float>(v.t[e])) < kInf ? v.t[e] : static_cast<T>(0.f);
+    for (int n = 0; n < kLoads; ++n) {
+      union { uint4 u; T t[kPer]; } v;
+      v.u = reg[n];
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (!(fabsf(static_cast<float>(v.t[e])) < kInf)) {
+          v.t[e] = static_cast<T>(0.f);
+          any = true;
+        }
+      if (any) {
+        atomicOr(wild, 1ull << ((threadIdx.x + n * NT) / kChunks));
+        *place(lds, n) = v.u;
       }
-      *reinterpret_cast<uint4*>(lds + row * kStride + at) = v.u;
     }
   }
-  __device__ __forceinline__ uint4 piece(int n, uint64_t rows, int D) const {
-    const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks * kPer;
-    const bool in = ((rows >> row) & 1) && at < D;
-    uint4 v = reg[n];
-    v.x = in ? v.x : 0; v.y = in ? v.y : 0; v.z = in ? v.z : 0; v.w = in ? v.w : 0;
-    return v;
-  }
-  // Operand with this lane's row `row0 + lane % 32`, k = 16 kc + 8 half + 0..7 along the row.
+  // Operand with this lane's row `row0 + lane % 32` (row0 a multiple of 32), k = 16 kc + 8 half + 0..7
+  // along the row.
   static __device__ __forceinline__ typename Type<T>::Frag frag_along(const T* lds, int row0, int kc) {
-    const int lane = threadIdx.x & 63;
-    const T* p = lds + (row0 + (lane & 31)) * kStride + 16 * kc + 8 * (lane >> 5);
-    return *reinterpret_cast<const typename Type<T>::Frag*>(p);
+    const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
+    const char* row = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow;
+    constexpr int kPieces = 8 / kPer;
+    union { uint4 u[kPieces]; typename Type<T>::Frag f; } x;
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n)
+      x.u[n] = *reinterpret_cast<const uint4*>(row + ((((2 * kc + half) * kPieces + n) ^ turn(r)) << 4));
+    return x.f;
   }
   // Operand with this lane's column `32 mt + lane % 32`, k down the rows in a result's order:
-  // rows row0 + 8 (j / 4) + 4 half + j % 4.  For 2-byte types by the transposing LDS read, which
-  // gives lane l of sixteen column l of the 4 x 16 values that the sixteen address, four of a row
-  // each.
+  // rows row0 + 8 (j / 4) + 4 half + j % 4 (row0 a multiple of 16).  For 2-byte types by the
+  // transposing LDS read, which gives lane l of sixteen column l of the 4 x 16 values that the
+  // sixteen address, four of a row each.
   static __device__ __forceinline__ typename Type<T>::Frag frag_down(const T* lds, int row0, int mt) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     typename Type<T>::Frag f;
     if constexpr (sizeof(T) == 2) {
-      const int l = lane & 15;
-      const T* p = lds + (row0 + 4 * half + (l >> 2)) * kStride + 32 * mt + (lane & 16) + 4 * (l & 3);
       using LdsI16x4 = __attribute__((address_space(3))) i16x4;
-      const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
-      const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + 8 * kStride));
       union { i16x4 h[2]; typename Type<T>::Frag f; } u;
-      u.h[0] = a; u.h[1] = b;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int r = 8 * n + 4 * half + ((lane & 15) >> 2);
+        const int c = (4 * mt + ((lane & 16) >> 3) + ((lane & 3) >> 1)) ^ turn(r);
+        const char* p = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow + (c << 4) + 8 * (lane & 1);
+        u.h[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
+      }
       f = u.f;
     } else {
-      const T* p = lds + (row0 + 4 * half) * kStride + 32 * mt + (lane & 31);
+      const int x = 32 * mt + (lane & 31);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = p[(8 * (j >> 2) + (j & 3)) * kStride];
+      for (int j = 0; j < 8; ++j) {
+        const int r = 8 * (j >> 2) + 4 * half + (j & 3);
+        const char* p = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow + (((x >> 2) ^ turn(r)) << 4) + 4 * (x & 3);
+        f[j] = *reinterpret_cast<const float*>(p);
+      }
     }
     return f;
   }
 };
+
+// x where bit n of `word` is set, else `other`: two instructions, with no condition mask.
+__device__ __forceinline__ float keep_bit(float x, uint32_t word, int n, float other) {
+  const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(word, n, 1));
+  return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
 
 // Registers 8 c .. 8 c + 7 of a result as an operand's chunk c.  Rounded to the inputs' type: the
 // matrix units multiply 16-bit types only by their like, and a weight's relative error of half a
@@ -168,9 +227,10 @@ __device__ __forceinline__ typename Type<T>::Frag frag_of(const f32x16& x, int c
   return f;
 }
 
-// Operand with this lane's row of global memory, as frag_along; zero where !in or beyond D.
+// Operand with this lane's row of global memory, as frag_along; zero where !in or beyond D, the
+// signs turned by `flip` (0 or the sign bit).
 template <typename T>
-__device__ __forceinline__ typename Type<T>::Frag frag_global(const T* row, int kc, int D, bool in) {
+__device__ __forceinline__ typename Type<T>::Frag frag_global(const T* row, int kc, int D, bool in, uint32_t flip = 0) {
   const int at = 16 * kc + 8 * ((threadIdx.x & 63) >> 5);
   const bool ok = in && at < D;
   union { uint4 u[sizeof(T) / 2]; typename Type<T>::Frag f; } x;
@@ -179,6 +239,10 @@ __device__ __forceinline__ typename Type<T>::Frag frag_global(const T* row, int 
   for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) {
     x.u[n] = p[n];
     if (!ok) x.u[n] = make_uint4(0, 0, 0, 0);
+    if (flip) {
+      const uint32_t m = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+      x.u[n].x ^= m; x.u[n].y ^= m; x.u[n].z ^= m; x.u[n].w ^= m;
+    }
   }
   return x.f;
 }
@@ -191,14 +255,22 @@ __device__ __forceinline__ void add_wild(const T* base, int64_t stride, int row0
   const int half = (threadIdx.x & 63) >> 5;
   for (; wild; wild &= wild - 1) {
     const int row = __builtin_ctzll(wild);
-    const T* p = base + (row0 + row) * stride;
+    const bool seen = (vis >> row) & 1;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + (row0 + row) * stride), 0,
+                                                      static_cast<int>(D * sizeof(T)), 0x00020000);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = 32 * mt + 8 * (r >> 2) + 4 * half + (r & 3);
-        const float x = d < D ? static_cast<float>(p[d]) : 0.f;
-        if (!(fabsf(x) < kInf) && ((vis >> row) & 1)) acc[mt][r] += AS_NAN ? __builtin_nanf("") : x;
+      for (int g = 0; g < 4; ++g) {
+        const int at = (32 * mt + 8 * g + 4 * half) * static_cast<int>(sizeof(T));
+        union { uint4 u; decltype(__builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0)) w; T t[4]; } x;
+        if constexpr (sizeof(T) == 2) x.w = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
+        else x.u = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float y = static_cast<float>(x.t[q]);
+          if (!(fabsf(y) < kInf) && seen) acc[mt][4 * g + q] += AS_NAN ? __builtin_nanf("") : y;
+        }
       }
   }
 }
@@ -270,6 +342,14 @@ __device__ __forceinline__ float table_value(const void* table, int dtype, int64
   if (dtype == GEO_BF16) return static_cast<float>(static_cast<const __bf16*>(table)[at]);
   return static_cast<float>(static_cast<const _Float16*>(table)[at]);
 }
+
+// Largest and least over the wave's lanes, once per workgroup.
+__device__ __forceinline__ int wave_most(int x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x = max(x, __shfl_xor(x, d, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_least(int x) { return -wave_most(-x); }
 
 // The relative bias of one head, in LDS: times log2 e, for distances -maxd..maxd (any other has the
 // bucket, and so the bias, of the nearer end).

@@ -22,6 +22,7 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
   using Tl = Tile<T, DP, BN, 64 * NW>;
   using Frag = typename Type<T>::Frag;
   constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBm = 32 * NW;
+  constexpr float kSlack = 8.f;
   extern __shared__ __align__(16) unsigned char lds[];
   T* const ks = reinterpret_cast<T*>(lds);
   T* const vs = reinterpret_cast<T*>(lds + Tl::kBytes);
@@ -43,44 +44,43 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
   __syncthreads();
 
   // what this lane's query sees: keys lo..hi, and first..far
-  const int i = q0 + 32 * wave + (lane & 31);
+  const int iw = q0 + 32 * wave, i = iw + (lane & 31);
   const bool real = i < a.seq.T;
   int first, end;
   seq_of(a.seq, sptr, real ? i : a.seq.T - 1, first, end);
   const int lo = max(first, i - a.left), hi = real ? min(end - 1, i + a.right) : -1;
   const int far = min(first + a.sinks - 1, hi);
-  // the workgroup's keys: those of its first and last queries bound them, both grow with the query
-  int first0, end0, first1, end1;
-  seq_of(a.seq, sptr, q0, first0, end0);
-  const int q1 = min(q0 + kBm, a.seq.T) - 1;
-  seq_of(a.seq, sptr, q1, first1, end1);
-  const int jlo = max(first0, q0 - a.left), jend = min(end1, q1 + a.right + 1);
-  const int sink_end = min(min(first0 + a.sinks, jlo), end0);
-  const int sink_tiles = sink_end > first0 ? (sink_end - first0 + BN - 1) / BN : 0;
-  const int tiles = sink_tiles + (jend > jlo ? (jend - jlo + BN - 1) / BN : 0);
+  // keys that all of the wave's queries see (both ends grow with the query), or none
+  const int all_lo = __builtin_amdgcn_readlane(lo, max(min(a.seq.T - 1 - iw, 31), 0)), all_hi = __builtin_amdgcn_readlane(hi, 0);
+  const Span k = span_of(a, sptr, q0, kBm);
+  const int sink_tiles = k.sink_end > k.first ? (k.sink_end - k.first + BN - 1) / BN : 0;
+  const int tiles = sink_tiles + (k.jend > k.jlo ? (k.jend - k.jlo + BN - 1) / BN : 0);
 
   Frag qf[kKc];
   {
     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(real ? i : 0) * a.q_st + h * a.q_sh;
 #pragma unroll
-    for (int kc = 0; kc < kKc; ++kc) qf[kc] = frag_global(q, kc, a.D, real);
+    for (int kc = 0; kc < kKc; ++kc) qf[kc] = frag_global(q, kc, a.D, real && a.scale != 0.f, a.scale < 0.f);
   }
   f32x16 o[kMt] = {};
   float m = -kInf, l = 0.f;
-  const float scale2 = a.scale * kLog2e;
+  // positive, so that the products' maximum is the scores': the queries carry its sign, or are zeros
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
 
   auto tile_at = [&](int t, int& j0, int& jlim) {
     const bool s = t < sink_tiles;
-    j0 = s ? first0 + t * BN : jlo + (t - sink_tiles) * BN;
-    jlim = s ? sink_end : jend;
+    j0 = s ? k.first + t * BN : k.jlo + (t - sink_tiles) * BN;
+    jlim = s ? k.sink_end : k.jend;
   };
   Tl kt, vt;
+  kt.init(a.k_st * sizeof(T), a.D);
+  vt.init(a.v_st * sizeof(T), a.D);
   uint32_t seen_byte = 1;
   auto fetch = [&](int t) {
     int j0, jlim;
     tile_at(t, j0, jlim);
-    kt.load(kbase, a.k_st, j0, jlim, a.D);
-    vt.load(vbase, a.v_st, j0, jlim, a.D);
+    kt.load(rows_at(kbase, a.k_st * sizeof(T), j0, jlim));
+    vt.load(rows_at(vbase, a.v_st * sizeof(T), j0, jlim));
     if (a.mask) seen_byte = a.mask[min(j0 + lane, jlim - 1)];
   };
   if (tiles > 0) fetch(0);
@@ -90,8 +90,10 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
     uint64_t rows = bit_range(0, min(jlim - j0, BN) - 1);
     if (a.mask) rows &= __ballot(seen_byte != 0);
     __syncthreads();
-    kt.store(ks, rows, a.D);
-    vt.store_finite(vs, rows, a.D, &wild[t & 1]);
+    kt.drop(rows, a.mask);
+    vt.drop(rows, a.mask);
+    kt.store(ks);
+    vt.store_finite(vs, &wild[t & 1]);
     if (threadIdx.x == 0) wild[(t + 1) & 1] = 0;
     if (BIAS)
       for (int x = threadIdx.x; x < kBm + BN - 1; x += 64 * NW)
@@ -99,14 +101,14 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1);
 
-    uint64_t vis = bit_range(lo - j0, hi - j0);
-    if (a.sinks) vis |= bit_range(first - j0, far - j0);
-    vis &= rows;
-    const uint64_t bits = vis >> (4 * half);
-    const uint32_t word[2] = {static_cast<uint32_t>(bits) & 0x0f0f0f0fu, static_cast<uint32_t>(bits >> 32) & 0x0f0f0f0fu};
-    if (__ballot((word[0] | (kSub > 1 ? word[1] : 0u)) != 0) == 0) continue;
-    const bool whole = __ballot(word[0] == 0x0f0f0f0fu && (kSub == 1 || word[1] == 0x0f0f0f0fu)) == ~0ull;
-
+    const bool whole = rows == (~0ull >> (64 - BN)) && j0 >= all_lo && j0 + BN - 1 <= all_hi;
+    uint64_t vis = ~0ull;
+    if (!whole) {
+      vis = bit_range(lo - j0, hi - j0);
+      if (a.sinks) vis |= bit_range(first - j0, far - j0);
+      vis &= rows;
+      if (__ballot(vis != 0) == 0) continue;
+    }
     f32x16 s[kSub];
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
@@ -114,40 +116,43 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
 #pragma unroll
       for (int kc = 0; kc < kKc; ++kc) s[u] = Type<T>::mma(Tl::frag_along(ks, 32 * u, kc), qf[kc], s[u]);
     }
-    const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31);
+    if (BIAS) {
+      const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31);
 #pragma unroll
-    for (int u = 0; u < kSub; ++u)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int kk = 8 * (r >> 2) + (r & 3);
-        s[u][r] = BIAS ? fmaf(s[u][r], scale2, bias[32 * u + kk]) : s[u][r] * scale2;
-      }
+        for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], scale2, bias[32 * u + 8 * (r >> 2) + (r & 3)]);
+    }
     if (!whole) {
+      const uint64_t bits = vis >> (4 * half);
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!((word[u] >> (8 * (r >> 2) + (r & 3))) & 1)) s[u][r] = -kInf;
+          s[u][r] = keep_bit(s[u][r], static_cast<uint32_t>(bits >> (32 * u)), 8 * (r >> 2) + (r & 3), -kInf);
     }
     float top = s[0][0];
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = fmaxf(m, halves_max(top));
-    const float shift = top == -kInf ? 0.f : top;  // no key so far: every exponential below is 0
-    const float keep = exp2_hw(m - shift);
-    m = top;
-    l *= keep;
-    if (__ballot(keep != 1.f)) {
+    top = halves_max(top) * (BIAS ? 1.f : scale2);
+    // The exponentials' reference moves only when a score passes it by more than kSlack: they stay
+    // below 2^kSlack, which loses nothing in any of the types, and most tiles leave the sums alone.
+    const bool up = top > m + kSlack;
+    if (__ballot(up)) {
+      const float keep = up ? exp2_hw(m - top) : 1.f;
+      m = up ? top : m;
+      l *= keep;
 #pragma unroll
       for (int mt = 0; mt < kMt; ++mt) o[mt] *= keep;
     }
+    const float shift = m == -kInf ? 0.f : m;  // no key so far: every exponential below is 0
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[u][r] = exp2_hw(s[u][r] - shift);
+        s[u][r] = exp2_hw(BIAS ? s[u][r] - shift : fmaf(s[u][r], scale2, -shift));
         l += s[u][r];
       }
 #pragma unroll

@@ -14,10 +14,39 @@ namespace attn {
 
 // ------------------------------------------------------------------ dq, bias ---
 
-// As the forward, a wave's 32 queries over tiles of keys.  The bias gradient is summed by distance:
-// a lane's score of query i and key j goes to LDS slot j - i of its wave and half, where the 32
-// lanes of a half always hold 32 different distances, so no two lanes add to one word at once;
-// distances at or beyond the ends go to two registers.  The workgroup's sums leave by bucket.
+// Slots of a bias gradient's sums by distance: -maxd..maxd and, at both ends, the distances of a
+// 32 x 32 tile that reaches inside.
+constexpr int kPast = 64;
+__host__ __device__ inline int bias_slots(int maxd) { return 2 * maxd + 1 + 2 * kPast; }
+
+// A result's sums along its diagonals: lane l < 63 gets the sum over key c and query n (row and
+// column) with c - n = 31 - l.  The sums move up a lane from key to key while each key's values are
+// added, so a value of key c ends 31 - c lanes above its query; a key's values of the 32 queries are
+// first moved to the lower half, the upper one left empty for them to move into.  Three
+// instructions per 64 values; an LDS atomic for each took as long as forty.
+__device__ __forceinline__ float sum_by_distance(const f32x16& x) {
+  float sum = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    float low[4], high[4];  // keys 8 g + 0..3 (of the lower half), 8 g + 4..7 (of the upper)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[4 * g + r]), 0u, false, false);
+      low[r] = __uint_as_float(p[0]);
+      high[r] = __uint_as_float(p[1]);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int up = __builtin_amdgcn_update_dpp(0, __float_as_int(sum), 0x138, 0xF, 0xF, true);  // from the lane below
+      sum = __int_as_float(up) + (c < 4 ? low[c & 3] : high[c & 3]);
+    }
+  }
+  return sum;
+}
+
+// As the forward, a wave's 32 queries over tiles of keys.  The bias gradient is summed by distance,
+// each wave into its own places; sub-tiles with no distance inside the ends go to two registers.  The
+// workgroup's sums leave by bucket.
 template <typename T, int DP, int NW, int BN, bool BIAS>
 __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T* __restrict__ out,
                                                         const T* __restrict__ grad, const float* __restrict__ lse,
@@ -31,8 +60,8 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
   T* const vs = reinterpret_cast<T*>(lds + Tl::kBytes);
   float* const near = reinterpret_cast<float*>(lds + 2 * Tl::kBytes);
   float* const base = near + (BIAS ? kBm + BN : 0);
-  const int slots = 2 * a.bias.maxd + 1;
-  float* const sums = base + (BIAS ? slots : 0);  // [2 NW][slots]
+  const int slots = bias_slots(a.bias.maxd);
+  float* const sums = base + (BIAS ? 2 * a.bias.maxd + 1 : 0);  // [NW][slots]
   __shared__ int sptr[kStagedPtr];
   __shared__ unsigned long long wild[2];
 
@@ -46,7 +75,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
   stage_ptr(a.seq, sptr);
   if (BIAS) {
     stage_bias(a.bias, a.Hq, h, base);
-    for (int x = threadIdx.x; x < 2 * NW * slots; x += 64 * NW) sums[x] = 0.f;
+    for (int x = threadIdx.x; x < NW * slots; x += 64 * NW) sums[x] = 0.f;
   }
   if (threadIdx.x < 2) wild[threadIdx.x] = 0;
   __syncthreads();
@@ -57,14 +86,10 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
   seq_of(a.seq, sptr, real ? i : a.seq.T - 1, first, end);
   const int lo = max(first, i - a.left), hi = real ? min(end - 1, i + a.right) : -1;
   const int far = min(first + a.sinks - 1, hi);
-  int first0, end0, first1, end1;
-  seq_of(a.seq, sptr, q0, first0, end0);
-  const int q1 = min(q0 + kBm, a.seq.T) - 1;
-  seq_of(a.seq, sptr, q1, first1, end1);
-  const int jlo = max(first0, q0 - a.left), jend = min(end1, q1 + a.right + 1);
-  const int sink_end = min(min(first0 + a.sinks, jlo), end0);
-  const int sink_tiles = sink_end > first0 ? (sink_end - first0 + BN - 1) / BN : 0;
-  const int tiles = sink_tiles + (jend > jlo ? (jend - jlo + BN - 1) / BN : 0);
+  const int all_lo = __builtin_amdgcn_readlane(lo, max(min(a.seq.T - 1 - iw, 31), 0)), all_hi = __builtin_amdgcn_readlane(hi, 0);
+  const Span k = span_of(a, sptr, q0, kBm);
+  const int sink_tiles = k.sink_end > k.first ? (k.sink_end - k.first + BN - 1) / BN : 0;
+  const int tiles = sink_tiles + (k.jend > k.jlo ? (k.jend - k.jlo + BN - 1) / BN : 0);
 
   Frag qf[kKc], gf[kKc];
   float dl = 0.f;
@@ -89,16 +114,18 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
 
   auto tile_at = [&](int t, int& j0, int& jlim) {
     const bool s = t < sink_tiles;
-    j0 = s ? first0 + t * BN : jlo + (t - sink_tiles) * BN;
-    jlim = s ? sink_end : jend;
+    j0 = s ? k.first + t * BN : k.jlo + (t - sink_tiles) * BN;
+    jlim = s ? k.sink_end : k.jend;
   };
   Tl kt, vt;
+  kt.init(a.k_st * sizeof(T), a.D);
+  vt.init(a.v_st * sizeof(T), a.D);
   uint32_t seen_byte = 1;
   auto fetch = [&](int t) {
     int j0, jlim;
     tile_at(t, j0, jlim);
-    kt.load(kbase, a.k_st, j0, jlim, a.D);
-    vt.load(vbase, a.v_st, j0, jlim, a.D);
+    kt.load(rows_at(kbase, a.k_st * sizeof(T), j0, jlim));
+    vt.load(rows_at(vbase, a.v_st * sizeof(T), j0, jlim));
     if (a.mask) seen_byte = a.mask[min(j0 + lane, jlim - 1)];
   };
   if (tiles > 0) fetch(0);
@@ -108,8 +135,10 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
     uint64_t rows = bit_range(0, min(jlim - j0, BN) - 1);
     if (a.mask) rows &= __ballot(seen_byte != 0);
     __syncthreads();
-    kt.store_finite(ks, rows, a.D, &wild[t & 1]);
-    vt.store(vs, rows, a.D);
+    kt.drop(rows, a.mask);
+    vt.drop(rows, a.mask);
+    kt.store_finite(ks, &wild[t & 1]);
+    vt.store(vs);
     if (threadIdx.x == 0) wild[(t + 1) & 1] = 0;
     if (BIAS)
       for (int x = threadIdx.x; x < kBm + BN - 1; x += 64 * NW)
@@ -117,14 +146,18 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1);
 
-    uint64_t vis = bit_range(lo - j0, hi - j0);
-    if (a.sinks) vis |= bit_range(first - j0, far - j0);
-    vis &= rows;
+    const bool whole = rows == (~0ull >> (64 - BN)) && j0 >= all_lo && j0 + BN - 1 <= all_hi;
+    uint64_t vis = ~0ull;
+    if (!whole) {
+      vis = bit_range(lo - j0, hi - j0);
+      if (a.sinks) vis |= bit_range(first - j0, far - j0);
+      vis &= rows;
+      if (__ballot(vis != 0) == 0) continue;
+    }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half)) & 0x0f0f0f0fu;
-      if (__ballot(word != 0) == 0) continue;
-      const bool whole = __ballot(word == 0x0f0f0f0fu) == ~0ull;
+      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
+      if (!whole && __ballot((word & 0x0f0f0f0fu) != 0) == 0) continue;
       f32x16 s{}, dp{};
 #pragma unroll
       for (int kc = 0; kc < kKc; ++kc) {
@@ -135,17 +168,15 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int kk = 8 * (r >> 2) + (r & 3);
-        const float x = BIAS ? fmaf(s[r], scale2, bias[kk]) : s[r] * scale2;
-        s[r] = exp2_hw(x - ls) * (dp[r] - dl);
+        s[r] = exp2_hw(BIAS ? fmaf(s[r], scale2, bias[kk]) - ls : fmaf(s[r], scale2, -ls)) * (dp[r] - dl);
       }
       if (!whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = 0.f;
+          s[r] = keep_bit(s[r], word, 8 * (r >> 2) + (r & 3), 0.f);
       }
       if (BIAS) {
         const int d0 = j0 + 32 * u - iw;  // this sub-tile's distances: d0 - 31 .. d0 + 31
-        float* const mine = sums + (2 * wave + half) * slots + a.bias.maxd;
         if (d0 + 31 <= -a.bias.maxd) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) below += s[r];
@@ -153,14 +184,10 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
 #pragma unroll
           for (int r = 0; r < 16; ++r) above += s[r];
         } else {
-          const int d1 = d0 + 4 * half - (lane & 31);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int d = d1 + 8 * (r >> 2) + (r & 3);
-            if (d <= -a.bias.maxd) below += s[r];
-            else if (d >= a.bias.maxd) above += s[r];
-            else __hip_atomic_fetch_add(mine + d, s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          }
+          const float x = sum_by_distance(s);
+          if (lane < 63)
+            __hip_atomic_fetch_add(sums + wave * slots + a.bias.maxd + kPast + d0 + 31 - lane, x, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_WORKGROUP);
         }
       }
 #pragma unroll
@@ -177,16 +204,22 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
     below = wave_sum(below);
     above = wave_sum(above);
     if (lane == 0) {
-      sums[2 * wave * slots] = below;
-      sums[2 * wave * slots + slots - 1] = above;
+      sums[wave * slots] += below;
+      sums[wave * slots + slots - 1] += above;
     }
     __syncthreads();
     for (int b = threadIdx.x; b < a.bias.buckets; b += 64 * NW) {
       float x = 0.f;
-      const int x0 = max(range[2 * b], 0), x1 = min(range[2 * b + 1], slots);
+      // the bucket's places among the distances; the first and the last extend past the ends
+      const int n = 2 * a.bias.maxd + 1, r0 = max(range[2 * b], 0), r1 = min(range[2 * b + 1], n);
+      const int x0 = r0 == 0 ? 0 : r0 + kPast, x1 = r1 == n ? slots : r1 + kPast;
+      if (r0 >= r1) {
+        part[(static_cast<int64_t>(h) * gridDim.x / a.Hq + block) * a.bias.buckets + b] = 0.f;
+        continue;
+      }
       for (int at = x0; at < x1; ++at)
 #pragma unroll
-        for (int n = 0; n < 2 * NW; ++n) x += sums[n * slots + at];
+        for (int q = 0; q < NW; ++q) x += sums[q * slots + at];
       part[(static_cast<int64_t>(h) * gridDim.x / a.Hq + block) * a.bias.buckets + b] = x;
     }
   }
@@ -307,7 +340,10 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
   }
   atomicMax(&last, ihi);
   __syncthreads();
-  ilast = last;
+  ilast = __builtin_amdgcn_readfirstlane(last);
+  i0 = __builtin_amdgcn_readfirstlane(i0);
+  // queries that see all of the wave's keys
+  const int all_lo = wave_most(real ? ilo : 0), all_hi = wave_least(real ? ihi : a.seq.T);
   const int span = ilast >= i0 ? (ilast - i0) / BN + 1 : 0;
   const int tiles = span * heads;
 
@@ -325,37 +361,48 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
   const float scale2 = a.scale * kLog2e;
 
   Tl qt, gt;
+  qt.init(a.q_st * sizeof(T), a.D);
+  gt.init(static_cast<int64_t>(a.Hq) * a.D * sizeof(T), a.D);
   float row_value = 0.f;
-  auto fetch = [&](int t) {
-    const int h = hk * group + g0 + t / span, it = i0 + t % span * BN;
-    qt.load(static_cast<const T*>(a.q) + h * a.q_sh, a.q_st, it, ilast + 1, a.D);
-    gt.load(grad + static_cast<int64_t>(h) * a.D, static_cast<int64_t>(a.Hq) * a.D, it, ilast + 1, a.D);
+  auto fetch = [&](int h, int it) {
+    qt.load(rows_at(static_cast<const T*>(a.q) + h * a.q_sh, a.q_st * sizeof(T), it, ilast + 1));
+    gt.load(rows_at(grad + static_cast<int64_t>(h) * a.D, static_cast<int64_t>(a.Hq) * a.D * sizeof(T), it, ilast + 1));
     const int n = threadIdx.x % (2 * BN);
     row_value = (n < BN ? lse : delta)[static_cast<int64_t>(h) * a.seq.T + min(it + n % BN, ilast)];
   };
   static_assert(2 * BN <= 64 * NW, "one thread for each of a tile's log-sums and deltas");
-  if (tiles > 0) fetch(0);
+  int h = hk * group + g0, it = i0;
+  if (tiles > 0) fetch(h, it);
   for (int t = 0; t < tiles; ++t) {
-    const int it = i0 + t % span * BN;
-    const uint64_t rows = bit_range(0, min(ilast + 1 - it, BN) - 1);
-    if (BIAS && t % span == 0) stage_bias(a.bias, a.Hq, hk * group + g0 + t / span, base);
+    const int now = it, head = h;
+    const uint64_t rows = bit_range(0, min(ilast + 1 - now, BN) - 1);
+    if (BIAS && now == i0) stage_bias(a.bias, a.Hq, head, base);
     __syncthreads();
-    qt.store_finite(qs, rows, a.D, &wildq[t & 1]);
-    gt.store_finite(gs, rows, a.D, &wildg[t & 1]);
+    qt.store_finite(qs, &wildq[t & 1]);
+    gt.store_finite(gs, &wildg[t & 1]);
     if (threadIdx.x < 2 * BN) rowl[threadIdx.x] = row_value;
     if (threadIdx.x == 0) wildq[(t + 1) & 1] = wildg[(t + 1) & 1] = 0;
     if (BIAS)
       for (int x = threadIdx.x; x < kBk + BN - 1; x += 64 * NW)
-        near[x] = base[min(max(key0 - it + x - (BN - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
+        near[x] = base[min(max(key0 - now + x - (BN - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
     __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1);
+    it += BN;
+    if (it > ilast) {
+      it = i0;
+      ++h;
+    }
+    if (t + 1 < tiles) fetch(h, it);
 
-    const uint64_t vis = bit_range(ilo - it, ihi - it) & rows;
+    const bool whole = rows == (~0ull >> (64 - BN)) && now >= all_lo && now + BN - 1 <= all_hi;
+    uint64_t vis = ~0ull;
+    if (!whole) {
+      vis = bit_range(ilo - now, ihi - now) & rows;
+      if (__ballot(vis != 0) == 0) continue;
+    }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half)) & 0x0f0f0f0fu;
-      if (__ballot(word != 0) == 0) continue;
-      const bool whole = __ballot(word == 0x0f0f0f0fu) == ~0ull;
+      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
+      if (!whole && __ballot((word & 0x0f0f0f0fu) != 0) == 0) continue;
       f32x16 s{}, dp{};
 #pragma unroll
       for (int kc = 0; kc < kKc; ++kc) {
@@ -371,15 +418,16 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r = 4 * g + q, kk = 8 * g + q;
-          const float x = BIAS ? fmaf(s[r], scale2, bias[27 - kk]) : s[r] * scale2;
-          s[r] = exp2_hw(x - lsv[q]);
+          s[r] = exp2_hw(BIAS ? fmaf(s[r], scale2, bias[27 - kk]) - lsv[q] : fmaf(s[r], scale2, -lsv[q]));
           dp[r] = s[r] * (dp[r] - dlv[q]);
         }
       }
       if (!whole) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((word >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = dp[r] = 0.f;
+        for (int r = 0; r < 16; ++r) {
+          s[r] = keep_bit(s[r], word, 8 * (r >> 2) + (r & 3), 0.f);
+          dp[r] = keep_bit(dp[r], word, 8 * (r >> 2) + (r & 3), 0.f);
+        }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -392,16 +440,15 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
       }
     }
     if (wildq[t & 1] | wildg[t & 1]) {
-      const int h = hk * group + g0 + t / span;
-      add_wild<T, kMt, false>(grad + static_cast<int64_t>(h) * a.D, static_cast<int64_t>(a.Hq) * a.D, it, wildg[t & 1], vis,
-                              a.D, dva);
-      add_wild<T, kMt, true>(static_cast<const T*>(a.q) + h * a.q_sh, a.q_st, it, wildq[t & 1], vis, a.D, dka);
+      add_wild<T, kMt, false>(grad + static_cast<int64_t>(head) * a.D, static_cast<int64_t>(a.Hq) * a.D, now, wildg[t & 1],
+                              vis, a.D, dva);
+      add_wild<T, kMt, true>(static_cast<const T*>(a.q) + head * a.q_sh, a.q_st, now, wildq[t & 1], vis, a.D, dka);
     }
   }
   if (!real) return;
   if constexpr (PART) {
-    const int h = hk * group + g0;
-    float* row = f.part + ((static_cast<int64_t>(cut / f.len) * a.Hq + h) * a.sinks + (j - first)) * 2 * a.D;
+    const int h0 = hk * group + g0;
+    float* row = f.part + ((static_cast<int64_t>(cut / f.len) * a.Hq + h0) * a.sinks + (j - first)) * 2 * a.D;
     store_sums(row, dka, a.D);
     store_sums(row + a.D, dva, a.D);
   } else if (more) {
@@ -416,10 +463,11 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
 }
 
 // The sums of leading token s of the one sequence that begins in piece c and reaches past its end:
-// the key's own, then each later piece's, heads in order.
+// the key's own and each later piece's and head's, in four runs that are added in their order.
 template <typename T>
-__global__ __launch_bounds__(256) void attend_bwd_join(const Attend a, T* __restrict__ dk, T* __restrict__ dv, const Far f) {
+__global__ __launch_bounds__(1024) void attend_bwd_join(const Attend a, T* __restrict__ dk, T* __restrict__ dv, const Far f) {
   __shared__ int sptr[kStagedPtr];
+  __shared__ float runs[4][256];
   const int64_t w = blockIdx.x;
   const int s = static_cast<int>(w % a.sinks), hk = static_cast<int>(w / a.sinks % a.Hk);
   const int64_t c = w / a.sinks / a.Hk;
@@ -429,15 +477,27 @@ __global__ __launch_bounds__(256) void attend_bwd_join(const Attend a, T* __rest
   seq_of(a.seq, sptr, static_cast<int>((c + 1) * f.len), first, end);
   const int j = first + s;
   if (first / f.len != c || j >= end || own_end(f, j, a.left) >= end) return;
-  const int x = threadIdx.x;
-  if (x >= 2 * a.D) return;
-  const int group = a.Hq / a.Hk;
-  float sum = f.own[((c * a.Hk + hk) * a.sinks + s) * 2 * a.D + x];
-  const int64_t p0 = own_end(f, j, a.left) / f.len, p1 = (end - 1) / f.len;
-  const float* at = f.part + ((p0 * a.Hq + hk * group) * a.sinks + s) * 2 * a.D + x;
-  const int64_t step = static_cast<int64_t>(a.sinks) * 2 * a.D;
-  for (int64_t p = p0; p <= p1; ++p, at += a.Hq * step)
-    for (int g = 0; g < group; ++g) sum += at[g * step];
+  const int x = threadIdx.x & 255, run = threadIdx.x >> 8, group = a.Hq / a.Hk;
+  const int64_t p0 = own_end(f, j, a.left) / f.len, terms = ((end - 1) / f.len - p0 + 1) * group;
+  const int64_t per = (terms + 3) / 4, t0 = min(run * per, terms), t1 = min(t0 + per, terms);
+  float sum = 0.f;
+  if (x < 2 * a.D) {
+    auto term = [&](int64_t t) {
+      return f.part[(((p0 + t / group) * a.Hq + hk * group + t % group) * a.sinks + s) * 2 * a.D + x];
+    };
+    for (int64_t t = t0; t < t1; t += 8) {
+      float y[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) y[n] = term(min(t + n, t1 - 1));
+#pragma unroll
+      for (int n = 0; n < 8; ++n) sum += t + n < t1 ? y[n] : 0.f;
+    }
+  }
+  runs[run][x] = sum;
+  __syncthreads();
+  if (run || x >= 2 * a.D) return;
+  sum = f.own[((c * a.Hk + hk) * a.sinks + s) * 2 * a.D + x];
+  for (int n = 0; n < 4; ++n) sum += runs[n][x];
   const int64_t row = (static_cast<int64_t>(j) * a.Hk + hk) * a.D;
   if (x < a.D) dk[row + x] = static_cast<T>(sum * a.scale);
   else dv[row + x - a.D] = static_cast<T>(sum);
@@ -488,7 +548,7 @@ struct Grads {
 template <typename T, int DP, int NW, int BN, bool BIAS>
 int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
-                     (BIAS ? sizeof(float) * (32 * NW + BN + (2 * NW + 1) * (2 * a.bias.maxd + 1)) : 0);
+                     (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1 + NW * bias_slots(a.bias.maxd)) : 0);
   GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_q<T, DP, NW, BN, BIAS>), lds));
   attend_bwd_q<T, DP, NW, BN, BIAS><<<dim3(static_cast<uint32_t>(p.q_blocks * a.Hq)), dim3(64 * NW), lds, stream>>>(
       a, static_cast<const T*>(g.out), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
@@ -524,7 +584,7 @@ int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream
              ? launch_kv<T, DP, 1, 32, BIAS, false>(a, g, p, ceil_div(a.seq.T, 32) * a.Hk, stream)
              : launch_kv<T, DP, 4, 64, BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
   if (rc == GEO_OK && p.far.len) {
-    attend_bwd_join<T><<<dim3(static_cast<uint32_t>((p.pieces - 1) * a.Hk * a.sinks)), dim3(256), 0, stream>>>(
+    attend_bwd_join<T><<<dim3(static_cast<uint32_t>((p.pieces - 1) * a.Hk * a.sinks)), dim3(1024), 0, stream>>>(
         a, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
     GEO_LAUNCH_CHECK("attend_bwd_join");
   }
