@@ -77,31 +77,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* base, int6
                                            static_cast<int>(min(bytes, int64_t(0x7fffffff))), 0x00020000);
 }
 
-// A tile of ROWS rows in LDS, DP values each (a head's D, zeros beyond), in pieces of 16 bytes.
-// Rows adjoin (their pieces rounded up to a power of two), and piece c of row r lies in the place
-// c ^ turn(r), which keeps the wave's reads out of each other's banks (64 of 4 bytes): a read along
-// the rows takes one piece of eight neighbouring rows at a time, a transposing read two to four
-// neighbouring pieces of four rows.
+// A tile of ROWS rows in LDS, DP values each (a head's D, zeros beyond), in pieces of 16 bytes.  A
+// row is padded so that one piece of eight neighbouring rows, which a read along the rows takes at a
+// time, lies in eight different groups of the 64 banks, and the 64 bytes of four rows that a
+// transposing read takes meet at most in pairs.  (Turning the pieces by row instead kept those apart
+// too, but its addresses took registers that the products need: dq at D = 128 695 us, so 530.)
 template <typename T, int DP, int ROWS, int NT>
 struct Tile {
   static constexpr int kPer = 16 / sizeof(T);        // values in a piece
   static constexpr int kChunks = DP / kPer;          // pieces of a row
-  static constexpr int kPlaces = kChunks <= 4 ? 4 : kChunks <= 8 ? 8 : kChunks <= 16 ? 16 : 32;
-  static constexpr int kRow = kPlaces * 16;          // bytes from row to row
+  static constexpr int kRow = DP * sizeof(T) + (DP * sizeof(T) == 256 ? 48 : 16);  // bytes from row to row
   static constexpr int kLoads = ROWS * kChunks / NT; // per thread
   static constexpr int kBytes = ROWS * kRow;
   static_assert(ROWS * kChunks % NT == 0, "a thread loads whole pieces");
-
-  static __device__ __forceinline__ int turn(int r) {
-    if constexpr (sizeof(T) == 2) {
-      if constexpr (kPlaces == 4) return (r >> 2) & 3;
-      else if constexpr (kPlaces == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
-      else return (r & 3) << 2 | ((r >> 2) & 3);
-    } else {
-      if constexpr (kPlaces == 8) return (r >> 1) & 3;
-      else return (r & 3) | ((r >> 2) & 1) << 3;
-    }
-  }
 
   uint4 reg[kLoads];
   uint32_t off[kLoads];  // of the thread's pieces from the tile's first row, in bytes
@@ -120,7 +108,7 @@ struct Tile {
   }
   static __device__ __forceinline__ uint4* place(T* lds, int n) {
     const int c = threadIdx.x + n * NT, row = c / kChunks, at = c % kChunks;
-    return reinterpret_cast<uint4*>(reinterpret_cast<char*>(lds) + row * kRow + ((at ^ turn(row)) << 4));
+    return reinterpret_cast<uint4*>(reinterpret_cast<char*>(lds) + row * kRow + (at << 4));
   }
   // Rows whose bit is off as zeros (`some`: there may be such rows).
   __device__ __forceinline__ void drop(uint64_t rows, bool some) {
@@ -171,13 +159,8 @@ struct Tile {
   // along the row.
   static __device__ __forceinline__ typename Type<T>::Frag frag_along(const T* lds, int row0, int kc) {
     const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
-    const char* row = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow;
-    constexpr int kPieces = 8 / kPer;
-    union { uint4 u[kPieces]; typename Type<T>::Frag f; } x;
-#pragma unroll
-    for (int n = 0; n < kPieces; ++n)
-      x.u[n] = *reinterpret_cast<const uint4*>(row + ((((2 * kc + half) * kPieces + n) ^ turn(r)) << 4));
-    return x.f;
+    return *reinterpret_cast<const typename Type<T>::Frag*>(reinterpret_cast<const char*>(lds) + (row0 + r) * kRow +
+                                                            (16 * kc + 8 * half) * sizeof(T));
   }
   // Operand with this lane's column `32 mt + lane % 32`, k down the rows in a result's order:
   // rows row0 + 8 (j / 4) + 4 half + j % 4 (row0 a multiple of 16).  For 2-byte types by the
@@ -189,21 +172,17 @@ struct Tile {
     if constexpr (sizeof(T) == 2) {
       using LdsI16x4 = __attribute__((address_space(3))) i16x4;
       union { i16x4 h[2]; typename Type<T>::Frag f; } u;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int r = 8 * n + 4 * half + ((lane & 15) >> 2);
-        const int c = (4 * mt + ((lane & 16) >> 3) + ((lane & 3) >> 1)) ^ turn(r);
-        const char* p = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow + (c << 4) + 8 * (lane & 1);
-        u.h[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
-      }
+      const char* p = reinterpret_cast<const char*>(lds) + (row0 + 4 * half + ((lane & 15) >> 2)) * kRow +
+                      (32 * mt + (lane & 16) + 4 * (lane & 3)) * sizeof(T);
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)p);
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(p + 8 * kRow));
       f = u.f;
     } else {
       const int x = 32 * mt + (lane & 31);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = 8 * (j >> 2) + 4 * half + (j & 3);
-        const char* p = reinterpret_cast<const char*>(lds) + (row0 + r) * kRow + (((x >> 2) ^ turn(r)) << 4) + 4 * (x & 3);
-        f[j] = *reinterpret_cast<const float*>(p);
+        f[j] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lds) + (row0 + r) * kRow + 4 * x);
       }
     }
     return f;
@@ -214,6 +193,25 @@ struct Tile {
 __device__ __forceinline__ float keep_bit(float x, uint32_t word, int n, float other) {
   const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(word, n, 1));
   return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
+
+// At the head of a branch on what the whole wave agrees on, with a value that the branch works from:
+// keeps the compiler from carrying out the branch's instructions in every case.
+__device__ __forceinline__ void stay_branch(uint32_t& x) { asm volatile("" : "+v"(x)); }
+
+// The order of a product's LDS reads and matrix instructions, for the instructions written before it:
+// AHEAD reads first, then one more behind each of the TOTAL matrix instructions that still has one to
+// come (PER reads to an instruction).  Left alone the compiler, short of registers, reads one operand,
+// waits for it (about 100 clocks), multiplies (32) and reads the next.
+template <int TOTAL, int AHEAD, int PER>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * PER, 0);
+#pragma unroll
+  for (int n = 0; n < TOTAL - AHEAD; ++n) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
 // Registers 8 c .. 8 c + 7 of a result as an operand's chunk c.  Rounded to the inputs' type: the

@@ -5,15 +5,16 @@
 // h before a sequence's first token from `state`, or 0.  In reverse, the scan runs from each
 // sequence's last token to its first.
 //
-// A chunk of kLen tokens is one wave's, a lane V channels of it.  The chunk's map h -> A h + H is
-// formed from its inputs, the maps are composed over the chunks, and a second pass over the inputs
-// gives each chunk its outputs from the state it begins with.  All in float32, whatever the inputs.
+// A workgroup takes a chunk of kChunk tokens and 64 V channels, each of its waves kLen tokens in a
+// row, a lane V channels.  A stretch of tokens is a map h -> A h + H of the state before it; maps are
+// composed over the waves in LDS and over the chunks by scan_carry.  Pass 1 forms the chunks' maps,
+// pass 2 the outputs from the states that the chunks begin with.  All in float32, whatever the inputs.
 #include "common.hpp"
 
 namespace geo {
 namespace rec {
 
-constexpr int kLen = 32;
+constexpr int kLen = 16, kWaves = 8, kChunk = kLen * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T, int V> struct Pack;
@@ -47,18 +48,14 @@ __device__ __forceinline__ float sigmoid(float x) {
   const float err = __builtin_amdgcn_fmed3f(fmaf(-x, kLog2e, -t), -1.f, 1.f);
   return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(t), fmaf(err, 0.6931471805599453f, 1.f), 1.f));
 }
-// 1 - exp(u) for u <= 0 to a few units in the last place: near 0 the series of -expm1, since the
-// difference would cancel.
+// 1 - exp(u) for u <= 0, relatively to 5e-7: near 0 the series of -expm1, since the difference would
+// cancel (its first term left out is u^5 / 720).
 __device__ __forceinline__ float one_minus_exp(float u, float exp_u) {
-  float s = 1.f / 40320.f;
-  s = fmaf(s, u, 1.f / 5040.f);
-  s = fmaf(s, u, 1.f / 720.f);
-  s = fmaf(s, u, 1.f / 120.f);
-  s = fmaf(s, u, 1.f / 24.f);
+  float s = fmaf(u, 1.f / 120.f, 1.f / 24.f);
   s = fmaf(s, u, 1.f / 6.f);
   s = fmaf(s, u, 0.5f);
   s = fmaf(s, u, 1.f);
-  return u > -0.5f ? -u * s : 1.f - exp_u;
+  return u > -0.125f ? -u * s : 1.f - exp_u;
 }
 // A channel's log a per unit of the gate, -rate softplus(decay); softplus(x) = x for large x, where
 // exp(x) would overflow.
@@ -69,17 +66,14 @@ __device__ __forceinline__ float log_rate(float decay, float rate) {
 struct Gates {
   float a, m, r, z;
 };
+__device__ __forceinline__ float decay_of(float r, float lr) { return __builtin_amdgcn_exp2f(lr * kLog2e * r); }
 __device__ __forceinline__ Gates gates(float ga, float gx, float lr) {
   Gates g;
   g.r = sigmoid(ga);
   g.z = sigmoid(gx);
-  const float la = lr * g.r;
-  g.a = __builtin_amdgcn_exp2f(la * kLog2e);
-  g.m = __builtin_amdgcn_sqrtf(one_minus_exp(2.f * la, g.a * g.a));
+  g.a = decay_of(g.r, lr);
+  g.m = __builtin_amdgcn_sqrtf(one_minus_exp(2.f * lr * g.r, g.a * g.a));
   return g;
-}
-__device__ __forceinline__ float decay_of(float ga, float lr) {
-  return __builtin_amdgcn_exp2f(lr * sigmoid(ga) * kLog2e);
 }
 
 struct Scan {
@@ -94,15 +88,17 @@ struct Scan {
   int reverse;
 };
 
-// The tokens of a chunk in scan order: lane l < kLen looks at token number l of it.
-struct Chunk {
+// The tokens of a wave's stretch in scan order: lane l < kLen looks at token number l of it.
+struct Stretch {
+  int64_t n0;                    // the first token's number in scan order
   uint32_t begin, finish, live;  // bits: first of its sequence in scan order, last, of a sequence
   int64_t seq;                   // this lane's token's sequence
+  __device__ __forceinline__ bool plain() const { return live == (1u << kLen) - 1 && !(begin | finish); }
 };
 __device__ __forceinline__ int64_t token(const Scan& s, int64_t n) { return s.reverse ? s.T - 1 - n : n; }
-__device__ __forceinline__ Chunk look(const Scan& s, int64_t chunk) {
+__device__ __forceinline__ Stretch look(const Scan& s, int64_t n0) {
   const int lane = lane_id();
-  const int64_t n = chunk * kLen + (lane & (kLen - 1)), t = token(s, min(n, s.T - 1));
+  const int64_t n = n0 + (lane & (kLen - 1)), t = token(s, min(n, s.T - 1));
   int64_t lo = 0, first = 0, end = s.T;
   if (s.ptr) {
     int64_t hi = s.B - 1;
@@ -114,14 +110,17 @@ __device__ __forceinline__ Chunk look(const Scan& s, int64_t chunk) {
     end = min(s.ptr[lo + 1], s.T);
   }
   const bool live = n < s.T && first <= t && t < end;
-  Chunk c;
-  c.live = static_cast<uint32_t>(__ballot(live));
-  c.begin = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? end - 1 : max(first, int64_t(0)))));
-  c.finish = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? max(first, int64_t(0)) : end - 1)));
+  const int64_t first_in = max(first, int64_t(0));
+  constexpr uint32_t kAll = (1u << kLen) - 1;
+  Stretch c;
+  c.n0 = n0;
+  c.live = static_cast<uint32_t>(__ballot(live)) & kAll;
+  c.begin = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? end - 1 : first_in))) & kAll;
+  c.finish = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? first_in : end - 1))) & kAll;
   c.seq = lo;
   return c;
 }
-__device__ __forceinline__ int64_t seq_at(const Chunk& c, int l) {
+__device__ __forceinline__ int64_t seq_at(const Stretch& c, int l) {
   return (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq >> 32), l)) << 32) |
          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq), l));
 }
@@ -129,127 +128,177 @@ __device__ __forceinline__ int64_t seq_at(const Chunk& c, int l) {
 template <typename T, int V>
 struct Rows {
   typename Pack<T, V>::Raw raw[kLen];
-  __device__ __forceinline__ void load(const void* base, int64_t stride, const Scan& s, int64_t chunk, int64_t at) {
+  __device__ __forceinline__ void load(const void* base, int64_t stride, const Scan& s, int64_t n0, int64_t at) {
 #pragma unroll
     for (int l = 0; l < kLen; ++l) {
-      const int64_t n = min(chunk * kLen + l, s.T - 1);
-      raw[l] = *reinterpret_cast<const typename Pack<T, V>::Raw*>(static_cast<const T*>(base) + token(s, n) * stride + at);
+      const T* row = static_cast<const T*>(base) + token(s, min(n0 + l, s.T - 1)) * stride;
+      raw[l] = *reinterpret_cast<const typename Pack<T, V>::Raw*>(row + at);
     }
   }
 };
 
-// Grid of all passes: one wave per workgroup, (chunk, block of 64 V channels), channels fastest.
+// Grid of the passes: (chunk, block of 64 V channels), channels fastest.
 struct Place {
-  int64_t chunk, at;  // this lane's first channel, in range
+  int64_t chunk, n0, at;  // n0: the wave's first token's number; at: this lane's first channel, in range
+  int wave;
   bool mine;
 };
 template <int V>
 __device__ __forceinline__ Place place(const Scan& s) {
   const int64_t blocks = (s.C + 64 * V - 1) / (64 * V), w = xcd_block();
-  const int64_t at = (w % blocks * 64 + lane_id()) * V;
-  return {w / blocks, min(at, s.C - V), at < s.C};
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t at = (w % blocks * 64 + lane_id()) * V, chunk = w / blocks;
+  return {chunk, chunk * kChunk + wave * kLen, min(at, s.C - V), wave, at < s.C};
 }
 
 // The factor of a map across which nothing passes, as at the beginning of a sequence: a factor of 0
 // would let the infinities and NaN of the sequence before through.  No decay is negative.
 constexpr float kCut = -1.f;
 __device__ __forceinline__ float after(float a, float add, float h) { return a == kCut ? add : fmaf(a, h, add); }
+__device__ __forceinline__ float chain(float a1, float a2) { return a1 == kCut || a2 == kCut ? kCut : a1 * a2; }
 
-// Pass 1: the chunk's map.
-template <typename T, int V>
-__global__ __launch_bounds__(64) void scan_map(const Scan s, float* __restrict__ mapa, float* __restrict__ maph) {
-  const Place p = place<V>(s);
-  Rows<T, V> x, ga, gx;
-  x.load(s.x, s.x_st, s, p.chunk, p.at);
-  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
-  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
-  const Chunk c = look(s, p.chunk);
-  float lr[V], A[V], H[V];
+// The waves' maps of a chunk, in LDS.
+template <int V>
+struct Maps {
+  float a[kWaves][64 * V], h[kWaves][64 * V];
+  __device__ __forceinline__ void put(int wave, const float (&A)[V], const float (&H)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
-    A[v] = 1.f;
-    H[v] = 0.f;
+    for (int v = 0; v < V; ++v) {
+      a[wave][lane_id() * V + v] = A[v];
+      h[wave][lane_id() * V + v] = H[v];
+    }
   }
+  // state[v] through the maps of waves from .. to - 1 (or, to < from, from - 1 down to `to`)
+  __device__ __forceinline__ void run(int from, int to, float (&state)[V]) const {
+    const int step = to < from ? -1 : 1;
+    for (int w = to < from ? from - 1 : from; w != (to < from ? to - 1 : to); w += step)
+#pragma unroll
+      for (int v = 0; v < V; ++v) state[v] = after(a[w][lane_id() * V + v], h[w][lane_id() * V + v], state[v]);
+  }
+};
+
+// Factors and terms of a wave's tokens, and the map of its stretch.  PLAIN: no border of a sequence
+// lies in it.
+template <bool PLAIN, typename T, int V>
+__device__ __forceinline__ void steps(const Scan& s, const Stretch& c, const Place& p, const Rows<T, V>& x, const Rows<T, V>& ga,
+                                      const Rows<T, V>& gx, const float (&lr)[V], float (&fa)[kLen][V], float (&fb)[kLen][V],
+                                      float (&A)[V], float (&H)[V]) {
 #pragma unroll
   for (int l = 0; l < kLen; ++l) {
     float xf[V], af[V], gf[V];
     unpack<T, V>(x.raw[l], xf);
     unpack<T, V>(ga.raw[l], af);
     unpack<T, V>(gx.raw[l], gf);
-    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+    const bool begin = !PLAIN && ((c.begin >> l) & 1), live = PLAIN || ((c.live >> l) & 1);
     const int64_t b = begin ? seq_at(c, l) : 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const Gates g = gates(af[v], gf[v], lr[v]);
+      fa[l][v] = g.a;
+      fb[l][v] = g.m * g.z * xf[v];
       if (begin) {
         A[v] = kCut;
         H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
       }
-      A[v] = live && A[v] != kCut ? A[v] * g.a : kCut;
-      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
+      if (PLAIN) {
+        A[v] *= g.a;
+        H[v] = fmaf(g.a, H[v], fb[l][v]);
+      } else {
+        A[v] = live ? chain(A[v], g.a) : kCut;
+        H[v] = live ? fmaf(g.a, H[v], fb[l][v]) : 0.f;
+      }
     }
   }
-  if (p.mine) {
+}
+
+// Pass 1: the chunk's map.
+template <typename T, int V>
+__global__ __launch_bounds__(64 * kWaves) void scan_map(const Scan s, float* __restrict__ mapa, float* __restrict__ maph) {
+  __shared__ Maps<V> maps;
+  const Place p = place<V>(s);
+  Rows<T, V> x, ga, gx;
+  x.load(s.x, s.x_st, s, p.n0, p.at);
+  ga.load(s.ga, s.ga_st, s, p.n0, p.at);
+  gx.load(s.gx, s.gx_st, s, p.n0, p.at);
+  const Stretch c = look(s, p.n0);
+  float lr[V], A[V], H[V], fa[kLen][V], fb[kLen][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      mapa[p.chunk * s.C + p.at + v] = A[v];
-      maph[p.chunk * s.C + p.at + v] = H[v];
-    }
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    A[v] = 1.f;
+    H[v] = 0.f;
+  }
+  if (c.plain()) steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  else steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  maps.put(p.wave, A, H);
+  __syncthreads();
+  if (p.wave || !p.mine) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float Av = 1.f;
+    for (int w = 0; w < kWaves; ++w) Av = chain(Av, maps.a[w][lane_id() * V + v]);
+    A[v] = Av;
+    H[v] = 0.f;
+  }
+  maps.run(0, kWaves, H);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    mapa[p.chunk * s.C + p.at + v] = A[v];
+    maph[p.chunk * s.C + p.at + v] = H[v];
   }
 }
 
 // Between the passes: maps composed over the chunks, `maph` replaced by the state before each chunk
-// (or, `back`, after it, from the last chunk to the first).  Sixteen waves share 64 channels.
+// (or, `back`, after it, from the last chunk to the first).  Sixteen waves share 64 channels, each 32
+// chunks at a time held in registers, so that a round of 512 chunks costs one memory latency.
 __global__ __launch_bounds__(1024) void scan_carry(const float* __restrict__ mapa, float* __restrict__ maph, int64_t chunks,
                                                    int64_t C, int back) {
+  constexpr int kHeld = 32;
   __shared__ float sa[16][64], sh[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t at = min(static_cast<int64_t>(blockIdx.x) * 64 + lane, C - 1);
   const bool mine = static_cast<int64_t>(blockIdx.x) * 64 + lane < C;
-  const int64_t per = (chunks + 15) / 16, c0 = min(wave * per, chunks), c1 = min(c0 + per, chunks);
   auto index = [&](int64_t c) { return (back ? chunks - 1 - c : c) * C + at; };
-  float A = 1.f, H = 0.f;
-  for (int64_t c = c0; c < c1; c += 8) {
-    float a[8], h[8];
+  float ahead = 0.f;  // the state before the round
+  for (int64_t r = 0; r < chunks; r += 16 * kHeld) {
+    const int64_t c0 = r + wave * kHeld;
+    float a[kHeld], h[kHeld];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int64_t i = index(min(c + n, c1 - 1));
+    for (int n = 0; n < kHeld; ++n) {
+      const int64_t i = index(min(c0 + n, chunks - 1));
       a[n] = mapa[i];
       h[n] = maph[i];
     }
+    float A = 1.f, H = 0.f;
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-      if (c + n < c1) {
-        A = a[n] == kCut || A == kCut ? kCut : A * a[n];
+    for (int n = 0; n < kHeld; ++n)
+      if (c0 + n < chunks) {
+        A = chain(A, a[n]);
         H = after(a[n], h[n], H);
       }
-  }
-  sa[wave][lane] = A;
-  sh[wave][lane] = H;
-  __syncthreads();
-  float h0 = 0.f;
-  for (int n = 0; n < wave; ++n) h0 = after(sa[n][lane], sh[n][lane], h0);
-  for (int64_t c = c0; c < c1; c += 8) {
-    float a[8], h[8];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int64_t i = index(min(c + n, c1 - 1));
-      a[n] = mapa[i];
-      h[n] = maph[i];
+    __syncthreads();
+    sa[wave][lane] = A;
+    sh[wave][lane] = H;
+    __syncthreads();
+    float h0 = ahead;
+    for (int n = 0; n < 16; ++n) {
+      if (n == wave) H = h0;
+      h0 = after(sa[n][lane], sh[n][lane], h0);
     }
+    ahead = h0;
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
-      if (c + n < c1) {
-        if (mine) maph[index(c + n)] = h0;
-        h0 = after(a[n], h[n], h0);
+    for (int n = 0; n < kHeld; ++n)
+      if (c0 + n < chunks) {
+        if (mine) maph[index(c0 + n)] = H;
+        H = after(a[n], h[n], H);
       }
   }
 }
 
-// A sequence without tokens passes its state (or its state's gradient) on; chunk c sees to its share.
+// A sequence without tokens passes its state (or its state's gradient) on; a chunk's first wave sees
+// to its share of them.
 __device__ __forceinline__ void pass_empty(const Scan& s, const Place& p, int64_t chunks, int V, const float* from, float* to) {
-  if (!s.ptr || !to) return;
+  if (!s.ptr || !to || p.wave) return;
   const int64_t per = (s.B + chunks - 1) / chunks;
   for (int64_t b = p.chunk * per; b < min((p.chunk + 1) * per, s.B); ++b) {
     if (max(s.ptr[b], int64_t(0)) < min(s.ptr[b + 1], s.T) || !p.mine) continue;
@@ -259,39 +308,52 @@ __device__ __forceinline__ void pass_empty(const Scan& s, const Place& p, int64_
 
 // Pass 2: the outputs.
 template <typename T, int V>
-__global__ __launch_bounds__(64) void scan_out(const Scan s, int64_t chunks, const float* __restrict__ carry,
-                                               T* __restrict__ h, float* __restrict__ last) {
+__global__ __launch_bounds__(64 * kWaves) void scan_out(const Scan s, int64_t chunks, const float* __restrict__ carry,
+                                                        T* __restrict__ h, float* __restrict__ last) {
+  __shared__ Maps<V> maps;
   const Place p = place<V>(s);
   Rows<T, V> x, ga, gx;
-  x.load(s.x, s.x_st, s, p.chunk, p.at);
-  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
-  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
-  const Chunk c = look(s, p.chunk);
-  float lr[V], H[V];
+  x.load(s.x, s.x_st, s, p.n0, p.at);
+  ga.load(s.ga, s.ga_st, s, p.n0, p.at);
+  gx.load(s.gx, s.gx_st, s, p.n0, p.at);
+  const Stretch c = look(s, p.n0);
+  float lr[V], A[V], H[V], state[V], fa[kLen][V], fb[kLen][V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     lr[v] = log_rate(s.decay[p.at + v], s.rate);
-    H[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
+    A[v] = 1.f;
+    H[v] = 0.f;
+    state[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
   }
+  const bool plain = c.plain();
+  if (plain) steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  else steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  maps.put(p.wave, A, H);
+  __syncthreads();
+  maps.run(0, p.wave, state);
+  if (plain) {
 #pragma unroll
-  for (int l = 0; l < kLen; ++l) {
-    float xf[V], af[V], gf[V];
-    unpack<T, V>(x.raw[l], xf);
-    unpack<T, V>(ga.raw[l], af);
-    unpack<T, V>(gx.raw[l], gf);
-    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
-    const int64_t b = seq_at(c, l), n = p.chunk * kLen + l;
+    for (int l = 0; l < kLen; ++l) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Gates g = gates(af[v], gf[v], lr[v]);
-      if (begin) H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
-      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
+      for (int v = 0; v < V; ++v) state[v] = fmaf(fa[l][v], state[v], fb[l][v]);
+      if (p.mine) *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, p.n0 + l) * s.C + p.at) = pack<T, V>(state);
     }
-    if (p.mine && n < s.T)
-      *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, n) * s.C + p.at) = pack<T, V>(H);
-    if (((c.finish >> l) & 1) && p.mine)
+  } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) last[b * s.C + p.at + v] = H[v];
+    for (int l = 0; l < kLen; ++l) {
+      const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+      const int64_t b = seq_at(c, l), n = p.n0 + l;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (begin) state[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
+        state[v] = live ? fmaf(fa[l][v], state[v], fb[l][v]) : 0.f;
+      }
+      if (p.mine && n < s.T)
+        *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, n) * s.C + p.at) = pack<T, V>(state);
+      if (((c.finish >> l) & 1) && p.mine)
+#pragma unroll
+        for (int v = 0; v < V; ++v) last[b * s.C + p.at + v] = state[v];
+    }
   }
   pass_empty(s, p, chunks, V, s.state, last);
 }
@@ -307,15 +369,43 @@ struct Grad {
   float* ddecay;           // [chunks, C] sums of the chunks
 };
 
+// The map of a wave's stretch against the scan order, e before it from e behind it.
+template <bool PLAIN, typename T, int V>
+__device__ __forceinline__ void back_steps(const Scan& s, const Grad& d, const Stretch& c, const Place& p, const Rows<T, V>& dh,
+                                           const float (&fa)[kLen][V], float (&A)[V], float (&E)[V]) {
+#pragma unroll
+  for (int l = kLen - 1; l >= 0; --l) {
+    float hf[V] = {};
+    if (d.dh) unpack<T, V>(dh.raw[l], hf);
+    const bool finish = !PLAIN && ((c.finish >> l) & 1), live = PLAIN || ((c.live >> l) & 1);
+    const int64_t b = finish ? seq_at(c, l) : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (finish) {
+        A[v] = kCut;
+        E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
+      }
+      if (PLAIN) {
+        A[v] *= fa[l][v];
+        E[v] = fa[l][v] * (hf[v] + E[v]);
+      } else {
+        A[v] = live ? chain(A[v], fa[l][v]) : kCut;
+        E[v] = live ? fa[l][v] * (hf[v] + E[v]) : 0.f;
+      }
+    }
+  }
+}
+
 template <typename T, int V>
-__global__ __launch_bounds__(64) void scan_bwd_map(const Scan s, const Grad d, float* __restrict__ mapa,
-                                                   float* __restrict__ mape) {
+__global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const Grad d, float* __restrict__ mapa,
+                                                            float* __restrict__ mape) {
+  __shared__ Maps<V> maps;
   const Place p = place<V>(s);
   Rows<T, V> ga, dh;
-  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
-  if (d.dh) dh.load(d.dh, s.C, s, p.chunk, p.at);
-  const Chunk c = look(s, p.chunk);
-  float lr[V], A[V], E[V];
+  ga.load(s.ga, s.ga_st, s, p.n0, p.at);
+  if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
+  const Stretch c = look(s, p.n0);
+  float lr[V], A[V], E[V], fa[kLen][V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     lr[v] = log_rate(s.decay[p.at + v], s.rate);
@@ -323,67 +413,40 @@ __global__ __launch_bounds__(64) void scan_bwd_map(const Scan s, const Grad d, f
     E[v] = 0.f;
   }
 #pragma unroll
-  for (int l = kLen - 1; l >= 0; --l) {
-    float af[V], hf[V] = {};
+  for (int l = 0; l < kLen; ++l) {
+    float af[V];
     unpack<T, V>(ga.raw[l], af);
-    if (d.dh) unpack<T, V>(dh.raw[l], hf);
-    const bool finish = (c.finish >> l) & 1, live = (c.live >> l) & 1;
-    const int64_t b = seq_at(c, l);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float a = decay_of(af[v], lr[v]);
-      if (finish) {
-        A[v] = kCut;
-        E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
-      }
-      A[v] = live && A[v] != kCut ? A[v] * a : kCut;
-      E[v] = live ? a * (hf[v] + E[v]) : 0.f;
-    }
+    for (int v = 0; v < V; ++v) fa[l][v] = decay_of(sigmoid(af[v]), lr[v]);
   }
-  if (p.mine) {
+  if (c.plain()) back_steps<true>(s, d, c, p, dh, fa, A, E);
+  else back_steps<false>(s, d, c, p, dh, fa, A, E);
+  maps.put(p.wave, A, E);
+  __syncthreads();
+  if (p.wave || !p.mine) return;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      mapa[p.chunk * s.C + p.at + v] = A[v];
-      mape[p.chunk * s.C + p.at + v] = E[v];
-    }
+  for (int v = 0; v < V; ++v) {
+    float Av = 1.f;
+    for (int w = 0; w < kWaves; ++w) Av = chain(Av, maps.a[w][lane_id() * V + v]);
+    A[v] = Av;
+    E[v] = 0.f;
+  }
+  maps.run(kWaves, 0, E);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    mapa[p.chunk * s.C + p.at + v] = A[v];
+    mape[p.chunk * s.C + p.at + v] = E[v];
   }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(64) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks, const float* __restrict__ carry,
-                                                   const float* __restrict__ carry_e) {
+// Pass 2 of the backward: the states ahead of the wave's tokens again, then the gradients against the
+// scan order.
+template <bool PLAIN, typename T, int V>
+__device__ __forceinline__ void back_out(const Scan& s, const Grad& d, const Stretch& c, const Place& p, const Rows<T, V>& x,
+                                         const Rows<T, V>& ga, const Rows<T, V>& gx, const Rows<T, V>& dh, const float (&lr)[V],
+                                         const float (&fa)[kLen][V], const float (&before)[kLen][V], float (&E)[V],
+                                         float (&dlr)[V]) {
   using Raw = typename Pack<T, V>::Raw;
-  const Place p = place<V>(s);
-  Rows<T, V> x, ga, gx, dh;
-  x.load(s.x, s.x_st, s, p.chunk, p.at);
-  ga.load(s.ga, s.ga_st, s, p.chunk, p.at);
-  gx.load(s.gx, s.gx_st, s, p.chunk, p.at);
-  if (d.dh) dh.load(d.dh, s.C, s, p.chunk, p.at);
-  const Chunk c = look(s, p.chunk);
-  float lr[V], H[V], E[V], dlr[V] = {};
-  float before[kLen][V];  // the state ahead of each token, formed again from the chunk's first
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
-    H[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
-    E[v] = chunks > 1 ? carry_e[p.chunk * s.C + p.at + v] : 0.f;
-  }
-#pragma unroll
-  for (int l = 0; l < kLen; ++l) {
-    float xf[V], af[V], gf[V];
-    unpack<T, V>(x.raw[l], xf);
-    unpack<T, V>(ga.raw[l], af);
-    unpack<T, V>(gx.raw[l], gf);
-    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
-    const int64_t b = seq_at(c, l);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Gates g = gates(af[v], gf[v], lr[v]);
-      if (begin) H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
-      before[l][v] = H[v];
-      H[v] = live ? fmaf(g.a, H[v], g.m * g.z * xf[v]) : 0.f;
-    }
-  }
 #pragma unroll
   for (int l = kLen - 1; l >= 0; --l) {
     float xf[V], af[V], gf[V], hf[V] = {}, ox[V], oa[V], og[V];
@@ -391,38 +454,100 @@ __global__ __launch_bounds__(64) void scan_bwd_out(const Scan s, const Grad d, i
     unpack<T, V>(ga.raw[l], af);
     unpack<T, V>(gx.raw[l], gf);
     if (d.dh) unpack<T, V>(dh.raw[l], hf);
-    const bool finish = (c.finish >> l) & 1, live = (c.live >> l) & 1;
-    const int64_t b = seq_at(c, l), n = p.chunk * kLen + l;
+    const bool finish = !PLAIN && ((c.finish >> l) & 1), live = PLAIN || ((c.live >> l) & 1);
+    const int64_t b = PLAIN ? 0 : seq_at(c, l), n = p.n0 + l;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Gates g = gates(af[v], gf[v], lr[v]);
       if (finish) E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
-      const float G = live ? hf[v] + E[v] : 0.f;
-      E[v] = live ? g.a * G : 0.f;
-      const float in = g.z * xf[v];
-      ox[v] = live ? G * g.m * g.z : 0.f;
-      og[v] = live ? G * g.m * in * (1.f - g.z) : 0.f;
+      const float a = fa[l][v], r = sigmoid(af[v]), z = sigmoid(gf[v]), la = lr[v] * r;
+      const float m = __builtin_amdgcn_sqrtf(one_minus_exp(2.f * la, a * a));
+      const float G = hf[v] + E[v], in = z * xf[v], gm = G * m;
+      E[v] = a * G;
+      ox[v] = gm * z;
+      og[v] = gm * in * (1.f - z);
       // d log a of a h + m z x: a h - a^2 / m z x.  Times d log a / d gate = log a (1 - r), whose
       // log a / m has the limit 0 at m = 0 (no decay left in the type's range).
-      const float la = lr[v] * g.r, up = g.a * before[l][v];
-      const float lam = g.m > 0.f ? la * __builtin_amdgcn_rcpf(g.m) : 0.f;
-      const float dla = G * (up * la - g.a * g.a * in * lam);  // d log a times log a
-      oa[v] = live ? dla * (1.f - g.r) : 0.f;
-      dlr[v] += live ? dla : 0.f;
+      const float lam = m > 0.f ? la * __builtin_amdgcn_rcpf(m) : 0.f;
+      const float dla = G * a * (before[l][v] * la - a * in * lam);  // d log a times log a
+      oa[v] = dla * (1.f - r);
+      if (PLAIN || live) dlr[v] += dla;
+      if (!PLAIN && !live) E[v] = ox[v] = oa[v] = og[v] = 0.f;
     }
-    if (p.mine && n < s.T) {
+    if (p.mine && (PLAIN || n < s.T)) {
       const int64_t at = token(s, n) * s.C + p.at;
       *reinterpret_cast<Raw*>(static_cast<T*>(d.dx) + at) = pack<T, V>(ox);
       *reinterpret_cast<Raw*>(static_cast<T*>(d.dga) + at) = pack<T, V>(oa);
       *reinterpret_cast<Raw*>(static_cast<T*>(d.dgx) + at) = pack<T, V>(og);
     }
-    if (((c.begin >> l) & 1) && p.mine && d.dstate)
+    if (!PLAIN && ((c.begin >> l) & 1) && p.mine && d.dstate)
 #pragma unroll
       for (int v = 0; v < V; ++v) d.dstate[b * s.C + p.at + v] = E[v];
   }
-  if (p.mine)
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks,
+                                                               const float* __restrict__ carry,
+                                                               const float* __restrict__ carry_e) {
+  __shared__ Maps<V> maps, back;
+  __shared__ float sum[kWaves][64 * V];
+  const Place p = place<V>(s);
+  Rows<T, V> x, ga, gx, dh;
+  x.load(s.x, s.x_st, s, p.n0, p.at);
+  ga.load(s.ga, s.ga_st, s, p.n0, p.at);
+  gx.load(s.gx, s.gx_st, s, p.n0, p.at);
+  if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
+  const Stretch c = look(s, p.n0);
+  float lr[V], A[V], H[V], B[V], E[V], state[V], dlr[V] = {}, fa[kLen][V], fb[kLen][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) d.ddecay[p.chunk * s.C + p.at + v] = dlr[v];
+  for (int v = 0; v < V; ++v) {
+    lr[v] = log_rate(s.decay[p.at + v], s.rate);
+    A[v] = B[v] = 1.f;
+    H[v] = E[v] = 0.f;
+  }
+  const bool plain = c.plain();
+  if (plain) {
+    steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+    back_steps<true>(s, d, c, p, dh, fa, B, E);
+  } else {
+    steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+    back_steps<false>(s, d, c, p, dh, fa, B, E);
+  }
+  maps.put(p.wave, A, H);
+  back.put(p.wave, B, E);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    state[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
+    E[v] = chunks > 1 ? carry_e[p.chunk * s.C + p.at + v] : 0.f;
+  }
+  __syncthreads();
+  maps.run(0, p.wave, state);
+  back.run(kWaves, p.wave + 1, E);
+#pragma unroll
+  for (int l = 0; l < kLen; ++l) {  // fb becomes the state ahead of the token
+    const bool begin = (c.begin >> l) & 1, live = (c.live >> l) & 1;
+    const int64_t b = begin ? seq_at(c, l) : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (begin) state[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
+      const float now = live ? fmaf(fa[l][v], state[v], fb[l][v]) : 0.f;
+      fb[l][v] = state[v];
+      state[v] = now;
+    }
+  }
+  if (plain) back_out<true>(s, d, c, p, x, ga, gx, dh, lr, fa, fb, E, dlr);
+  else back_out<false>(s, d, c, p, x, ga, gx, dh, lr, fa, fb, E, dlr);
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[p.wave][lane_id() * V + v] = dlr[v];
+  __syncthreads();
+  if (p.wave == 0 && p.mine) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float y = dlr[v];
+      for (int w = 1; w < kWaves; ++w) y += sum[w][lane_id() * V + v];
+      d.ddecay[p.chunk * s.C + p.at + v] = y;
+    }
+  }
   pass_empty(s, p, chunks, V, d.dlast, d.dstate);
 }
 
@@ -434,7 +559,13 @@ __global__ __launch_bounds__(1024) void scan_bwd_decay(const float* __restrict__
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float x = 0.f;
-  for (int64_t c = wave; c < chunks; c += 16) x += part[c * C + min(at, C - 1)];
+  for (int64_t c = wave; c < chunks; c += 16 * 16) {
+    float y[16];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) y[n] = part[min(c + 16 * n, chunks - 1) * C + min(at, C - 1)];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) x += c + 16 * n < chunks ? y[n] : 0.f;
+  }
   sum[wave][lane] = x;
   __syncthreads();
   if (wave || at >= C) return;
@@ -467,7 +598,7 @@ __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict
 
 // ---------------------------------------------------------------------- host ---
 
-inline int64_t chunks_of(int64_t T) { return ceil_div(T, kLen); }
+inline int64_t chunks_of(int64_t T) { return ceil_div(T, kChunk); }
 
 inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
   GEO_REQUIRE(g, "gated recurrence: null arguments");
@@ -492,12 +623,12 @@ int forward(const Scan& s, void* h, float* last, float* maph, float* mapa, hipSt
   const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
   const dim3 grid(static_cast<uint32_t>(chunks * blocks));
   if (chunks > 1) {
-    scan_map<T, V><<<grid, dim3(64), 0, stream>>>(s, mapa, maph);
+    scan_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, mapa, maph);
     GEO_LAUNCH_CHECK("scan_map");
     scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, maph, chunks, s.C, 0);
     GEO_LAUNCH_CHECK("scan_carry");
   }
-  scan_out<T, V><<<grid, dim3(64), 0, stream>>>(s, chunks, maph, static_cast<T*>(h), last);
+  scan_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, chunks, maph, static_cast<T*>(h), last);
   GEO_LAUNCH_CHECK("scan_out");
   return GEO_OK;
 }
@@ -507,12 +638,12 @@ int backward(const Scan& s, const Grad& d, const float* carry, float* mape, floa
   const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
   const dim3 grid(static_cast<uint32_t>(chunks * blocks));
   if (chunks > 1) {
-    scan_bwd_map<T, V><<<grid, dim3(64), 0, stream>>>(s, d, mapa, mape);
+    scan_bwd_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, mapa, mape);
     GEO_LAUNCH_CHECK("scan_bwd_map");
     scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, mape, chunks, s.C, 1);
     GEO_LAUNCH_CHECK("scan_carry");
   }
-  scan_bwd_out<T, V><<<grid, dim3(64), 0, stream>>>(s, d, chunks, carry, mape);
+  scan_bwd_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, carry, mape);
   GEO_LAUNCH_CHECK("scan_bwd_out");
   scan_bwd_decay<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(d.ddecay, chunks, s.C, s.decay, ddecay);
   GEO_LAUNCH_CHECK("scan_bwd_decay");

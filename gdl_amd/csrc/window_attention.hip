@@ -17,8 +17,8 @@ namespace attn {
 //
 // Which of a tile's keys a query sees is a 64-bit word per lane: the tile is skipped by a wave
 // whose words are all zero, and takes no select where all bits are set.
-template <typename T, int DP, int NW, int BN, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restrict__ out, float* __restrict__ lse) {
+template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
+__global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* __restrict__ out, float* __restrict__ lse) {
   using Tl = Tile<T, DP, BN, 64 * NW>;
   using Frag = typename Type<T>::Frag;
   constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBm = 32 * NW;
@@ -116,6 +116,7 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
 #pragma unroll
       for (int kc = 0; kc < kKc; ++kc) s[u] = Type<T>::mma(Tl::frag_along(ks, 32 * u, kc), qf[kc], s[u]);
     }
+    if (sizeof(T) == 2) reads_ahead<kSub * kKc, 4, 1>();
     if (BIAS) {
       const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31);
 #pragma unroll
@@ -124,12 +125,13 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
         for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], scale2, bias[32 * u + 8 * (r >> 2) + (r & 3)]);
     }
     if (!whole) {
-      const uint64_t bits = vis >> (4 * half);
 #pragma unroll
-      for (int u = 0; u < kSub; ++u)
+      for (int u = 0; u < kSub; ++u) {
+        uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
+        stay_branch(word);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[u][r] = keep_bit(s[u][r], static_cast<uint32_t>(bits >> (32 * u)), 8 * (r >> 2) + (r & 3), -kInf);
+        for (int r = 0; r < 16; ++r) s[u][r] = keep_bit(s[u][r], word, 8 * (r >> 2) + (r & 3), -kInf);
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -163,6 +165,7 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
 #pragma unroll
         for (int mt = 0; mt < kMt; ++mt) o[mt] = Type<T>::mma(Tl::frag_down(vs, 32 * u + 16 * c, mt), p, o[mt]);
       }
+    if (sizeof(T) == 2) reads_ahead<kSub * 2 * kMt, 4, 2>();
     if (wild[t & 1]) add_wild<T, kMt, false>(vbase, a.v_st, j0, wild[t & 1], vis, a.D, o);
   }
   l = halves_sum(l);
@@ -174,14 +177,21 @@ __global__ __launch_bounds__(64 * NW) void attend_fwd(const Attend a, T* __restr
   }
 }
 
+// Waves per SIMD that the registers are bounded for: while one waits for LDS or forms exponentials
+// another keeps the matrix unit busy.
+template <typename T, int DP, int NW>
+constexpr int fwd_waves() {
+  return NW == 1 ? 1 : sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
+}
+
 template <typename T, int DP, int NW, int BN, bool BIAS>
 int launch_fwd(const Attend& a, void* out, float* lse, hipStream_t stream) {
   const int64_t blocks = ceil_div(a.seq.T, 32 * NW) * a.Hq;
   GEO_REQUIRE(blocks < (int64_t(1) << 31), "window attention: %lld workgroups", static_cast<long long>(blocks));
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
-  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_fwd<T, DP, NW, BN, BIAS>), lds));
-  attend_fwd<T, DP, NW, BN, BIAS><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_fwd<T, DP, NW, BN, BIAS, fwd_waves<T, DP, NW>()>), lds));
+  attend_fwd<T, DP, NW, BN, BIAS, fwd_waves<T, DP, NW>()><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
       a, static_cast<T*>(out), lse);
   GEO_LAUNCH_CHECK("attend_fwd");
   return GEO_OK;

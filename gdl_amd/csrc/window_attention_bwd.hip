@@ -47,8 +47,8 @@ __device__ __forceinline__ float sum_by_distance(const f32x16& x) {
 // As the forward, a wave's 32 queries over tiles of keys.  The bias gradient is summed by distance,
 // each wave into its own places; sub-tiles with no distance inside the ends go to two registers.  The
 // workgroup's sums leave by bucket.
-template <typename T, int DP, int NW, int BN, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T* __restrict__ out,
+template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
+__global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, const T* __restrict__ out,
                                                         const T* __restrict__ grad, const float* __restrict__ lse,
                                                         float* __restrict__ delta, T* __restrict__ dq,
                                                         const int32_t* __restrict__ range, float* __restrict__ part) {
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
     }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
+      uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
       if (!whole && __ballot((word & 0x0f0f0f0fu) != 0) == 0) continue;
       f32x16 s{}, dp{};
 #pragma unroll
@@ -164,6 +164,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
         s = Type<T>::mma(Tl::frag_along(ks, 32 * u, kc), qf[kc], s);
         dp = Type<T>::mma(Tl::frag_along(vs, 32 * u, kc), gf[kc], dp);
       }
+      if (sizeof(T) == 2) reads_ahead<2 * kKc, 4, 1>();
       const float* bias = near + 4 * half + kBm - 1 - 32 * wave - (lane & 31) + 32 * u;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -171,6 +172,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
         s[r] = exp2_hw(BIAS ? fmaf(s[r], scale2, bias[kk]) - ls : fmaf(s[r], scale2, -ls)) * (dp[r] - dl);
       }
       if (!whole) {
+        stay_branch(word);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[r] = keep_bit(s[r], word, 8 * (r >> 2) + (r & 3), 0.f);
@@ -196,6 +198,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_q(const Attend a, const T*
 #pragma unroll
         for (int mt = 0; mt < kMt; ++mt) o[mt] = Type<T>::mma(Tl::frag_down(ks, 32 * u + 16 * c, mt), p, o[mt]);
       }
+      if (sizeof(T) == 2) reads_ahead<2 * kMt, 4 < 2 * kMt ? 4 : 2 * kMt, 2>();
     }
     if (wild[t & 1]) add_wild<T, kMt, true>(kbase, a.k_st, j0, wild[t & 1], vis, a.D, o);
   }
@@ -260,23 +263,31 @@ __device__ __forceinline__ void store_sums(float* row, const f32x16 (&acc)[MT], 
   store_row<float>(row, acc, 1.f, D);
 }
 
+// Wide heads keep their rows of V in LDS: with K's, V's and both sums in registers one wave fits a
+// SIMD, and nothing hides its waits.
+template <int DP>
+constexpr bool kv_lds() { return DP >= 96; }
+
 // One workgroup holds 32 NW keys of one key head, a lane one of them, and walks the queries of all
 // heads that share it in tiles of BN.  S = Q K^T and dP = G V^T leave a key's weights of 16 queries
 // in a lane's registers, where dV^T = G^T P and dK^T = Q^T dS take them as operands; the sums over
 // heads and queries stay in registers.
-template <typename T, int DP, int NW, int BN, bool BIAS, bool PART>
-__global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T* __restrict__ grad,
+template <typename T, int DP, int NW, int BN, bool BIAS, bool PART, int WAVES>
+__global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_kv(const Attend a, const T* __restrict__ grad,
                                                          const float* __restrict__ lse, const float* __restrict__ delta,
                                                          T* __restrict__ dk, T* __restrict__ dv, const Far f) {
   using Tl = Tile<T, DP, BN, 64 * NW>;
   using Frag = typename Type<T>::Frag;
   constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBk = 32 * NW;
+  constexpr bool kVLds = kv_lds<DP>();
+  using Vl = Tile<T, DP, kBk, 64 * NW>;
   extern __shared__ __align__(16) unsigned char lds[];
   T* const qs = reinterpret_cast<T*>(lds);
   T* const gs = reinterpret_cast<T*>(lds + Tl::kBytes);
   float* const rowl = reinterpret_cast<float*>(lds + 2 * Tl::kBytes);  // the tile's log-sums and deltas
   float* const rowd = rowl + BN;
-  float* const near = rowd + BN;
+  T* const vl = reinterpret_cast<T*>(rowd + BN);  // kVLds: the workgroup's rows of V
+  float* const near = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(vl) + (kVLds ? Vl::kBytes : 0));
   float* const base = near + (BIAS ? kBk + BN : 0);
   __shared__ int sptr[kStagedPtr];
   __shared__ unsigned long long wildq[2], wildg[2];
@@ -347,14 +358,19 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
   const int span = ilast >= i0 ? (ilast - i0) / BN + 1 : 0;
   const int tiles = span * heads;
 
-  Frag kf[kKc], vf[kKc];
+  Frag kf[kKc], vf[kVLds ? 1 : kKc];
   {
     const T* kr = static_cast<const T*>(a.k) + static_cast<int64_t>(real ? j : 0) * a.k_st + hk * a.k_sh;
     const T* vr = static_cast<const T*>(a.v) + static_cast<int64_t>(real ? j : 0) * a.v_st + hk * a.v_sh;
 #pragma unroll
     for (int kc = 0; kc < kKc; ++kc) {
       kf[kc] = frag_global(kr, kc, a.D, on);
-      vf[kc] = frag_global(vr, kc, a.D, on);
+      if constexpr (kVLds) {  // its own wave reads a row only: no barrier
+        *reinterpret_cast<Frag*>(reinterpret_cast<char*>(vl) + (32 * wave + (lane & 31)) * Vl::kRow +
+                                 (16 * kc + 8 * half) * sizeof(T)) = frag_global(vr, kc, a.D, on);
+      } else {
+        vf[kc] = frag_global(vr, kc, a.D, on);
+      }
     }
   }
   f32x16 dka[kMt] = {}, dva[kMt] = {};
@@ -401,13 +417,23 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
     }
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      const uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
+      uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
       if (!whole && __ballot((word & 0x0f0f0f0fu) != 0) == 0) continue;
       f32x16 s{}, dp{};
 #pragma unroll
       for (int kc = 0; kc < kKc; ++kc) {
         s = Type<T>::mma(Tl::frag_along(qs, 32 * u, kc), kf[kc], s);
-        dp = Type<T>::mma(Tl::frag_along(gs, 32 * u, kc), vf[kc], dp);
+        if constexpr (!kVLds) dp = Type<T>::mma(Tl::frag_along(gs, 32 * u, kc), vf[kc], dp);
+      }
+      if constexpr (kVLds) {
+#pragma unroll
+        for (int kc = 0; kc < kKc; ++kc) dp = Type<T>::mma(Tl::frag_along(gs, 32 * u, kc), Vl::frag_along(vl, 32 * wave, kc), dp);
+        if (sizeof(T) == 2) {
+          reads_ahead<kKc, 2, 1>();
+          reads_ahead<kKc, 2, 2>();
+        }
+      } else if (sizeof(T) == 2) {
+        reads_ahead<2 * kKc, 4, 1>();
       }
       const float* bias = near + (lane & 31) + 32 * wave - 4 * half + (BN - 32 * u - 28);
 #pragma unroll
@@ -423,6 +449,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
         }
       }
       if (!whole) {
+        stay_branch(word);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] = keep_bit(s[r], word, 8 * (r >> 2) + (r & 3), 0.f);
@@ -438,6 +465,7 @@ __global__ __launch_bounds__(64 * NW) void attend_bwd_kv(const Attend a, const T
           dka[mt] = Type<T>::mma(Tl::frag_down(qs, 32 * u + 16 * c, mt), ds, dka[mt]);
         }
       }
+      if (sizeof(T) == 2) reads_ahead<4 * kMt, 4, 2>();
     }
     if (wildq[t & 1] | wildg[t & 1]) {
       add_wild<T, kMt, false>(grad + static_cast<int64_t>(head) * a.D, static_cast<int64_t>(a.Hq) * a.D, now, wildg[t & 1],
@@ -545,12 +573,29 @@ struct Grads {
   const int32_t* range;
 };
 
+// Waves per SIMD that the registers are bounded for.  dk and dv with wide heads keep 128 registers of
+// sums and take a SIMD for themselves: two waves there spilled into the loop (1166 us against 1009 at
+// 32,768 tokens, 8 (2) heads of 128, window 2047).
+template <typename T, int DP, int NW>
+constexpr int q_waves() {
+  return NW == 1 ? 1 : sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
+}
+template <typename T, int DP, int NW>
+constexpr int kv_waves() {
+  return NW == 1 ? 1 : sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 3 : DP <= 64 ? 2 : 1;
+}
+// Rows of a tile: 64, or 32 where the next tile's would not find registers.
+template <int DP>
+constexpr int q_rows() { return DP == 128 ? 32 : 64; }
+template <typename T, int DP>
+constexpr int kv_rows() { return DP == 128 && sizeof(T) == 4 ? 32 : 64; }
+
 template <typename T, int DP, int NW, int BN, bool BIAS>
 int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1 + NW * bias_slots(a.bias.maxd)) : 0);
-  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_q<T, DP, NW, BN, BIAS>), lds));
-  attend_bwd_q<T, DP, NW, BN, BIAS><<<dim3(static_cast<uint32_t>(p.q_blocks * a.Hq)), dim3(64 * NW), lds, stream>>>(
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_q<T, DP, NW, BN, BIAS, q_waves<T, DP, NW>()>), lds));
+  attend_bwd_q<T, DP, NW, BN, BIAS, q_waves<T, DP, NW>()><<<dim3(static_cast<uint32_t>(p.q_blocks * a.Hq)), dim3(64 * NW), lds, stream>>>(
       a, static_cast<const T*>(g.out), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
       p.part);
   GEO_LAUNCH_CHECK("attend_bwd_q");
@@ -565,9 +610,10 @@ int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream)
 template <typename T, int DP, int NW, int BN, bool BIAS, bool PART>
 int launch_kv(const Attend& a, const Grads& g, const Plan& p, int64_t blocks, hipStream_t stream) {
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes + 2 * BN * sizeof(float) +
+                     (kv_lds<DP>() ? Tile<T, DP, 32 * NW, 64 * NW>::kBytes : 0) +
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
-  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_kv<T, DP, NW, BN, BIAS, PART>), lds));
-  attend_bwd_kv<T, DP, NW, BN, BIAS, PART><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
+  GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_kv<T, DP, NW, BN, BIAS, PART, kv_waves<T, DP, NW>()>), lds));
+  attend_bwd_kv<T, DP, NW, BN, BIAS, PART, kv_waves<T, DP, NW>()><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
       a, static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
   GEO_LAUNCH_CHECK("attend_bwd_kv");
   return GEO_OK;
@@ -576,13 +622,13 @@ int launch_kv(const Attend& a, const Grads& g, const Plan& p, int64_t blocks, hi
 template <typename T, int DP, bool BIAS>
 int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
   int rc = few_blocks(a.seq.T, a.Hq) ? launch_q<T, DP, 1, 32, BIAS>(a, g, p, stream)
-                                     : launch_q<T, DP, 4, 64, BIAS>(a, g, p, stream);
+                                     : launch_q<T, DP, 4, q_rows<DP>(), BIAS>(a, g, p, stream);
   if (rc == GEO_OK && p.far.len)
     rc = launch_kv<T, DP, 1, 32, BIAS, true>(a, g, p, (p.pieces - 1) * ceil_div(a.sinks, 32) * a.Hq, stream);
   if (rc == GEO_OK)
     rc = few_blocks(a.seq.T, a.Hk)
              ? launch_kv<T, DP, 1, 32, BIAS, false>(a, g, p, ceil_div(a.seq.T, 32) * a.Hk, stream)
-             : launch_kv<T, DP, 4, 64, BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
+             : launch_kv<T, DP, 4, kv_rows<T, DP>(), BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
   if (rc == GEO_OK && p.far.len) {
     attend_bwd_join<T><<<dim3(static_cast<uint32_t>((p.pieces - 1) * a.Hk * a.sinks)), dim3(1024), 0, stream>>>(
         a, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
