@@ -10,6 +10,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -24,38 +25,23 @@ c_vp = ctypes.c_void_p
 c_size = ctypes.c_size_t
 c_f32 = ctypes.c_float
 c_i32 = ctypes.c_int32
+c_bytes = ctypes.c_char_p  # a packed struct
 
 
 
-class WindowAttentionArgs(ctypes.Structure):
-    """geo_window_attention_t of include/geo_api.h."""
-
-    _fields_ = [(n, c_vp) for n in ("q", "k", "v")] + \
-        [(n, c_i64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head")] + \
-        [(n, c_vp) for n in ("ptr", "mask", "bias", "bias_lut")] + \
-        [(n, c_i64) for n in ("tokens", "sequences", "left", "right", "sinks")] + \
-        [(n, c_i32) for n in ("dtype", "bias_dtype", "heads", "kv_heads", "head_dim", "buckets", "max_distance")] + \
-        [("scale", c_f32)]
-
-
-class WindowStepArgs(ctypes.Structure):
-    """geo_window_step_t of include/geo_api.h."""
-
-    _fields_ = [(n, c_vp) for n in ("q", "k", "v", "k_cache", "v_cache")] + \
-        [(n, c_i64) for n in ("q_stream", "q_head", "k_stream", "k_head", "v_stream", "v_head", "k_cache_stream",
-                              "k_cache_head", "v_cache_stream", "v_cache_head")] + \
-        [(n, c_vp) for n in ("positions", "bias", "bias_lut")] + [(n, c_i64) for n in ("batch", "slots", "sinks")] + \
-        [(n, c_i32) for n in ("dtype", "bias_dtype", "heads", "kv_heads", "head_dim", "buckets", "max_distance")] + \
-        [("scale", c_f32)]
+# The argument structs of the sequence operators (include/geo_api.h) as packed bytes, which cost a
+# fraction of a ctypes.Structure of so many fields; null pointers are 0.
+# geo_window_attention_t: 3 tensors, 6 strides, ptr, mask, bias, bias_lut, 5 sizes, 7 codes, scale
+pack_window_attention = struct.Struct("=3Q6q4Q5q7if").pack
+# geo_window_step_t: 5 tensors, 10 strides, positions, bias, bias_lut, 3 sizes, 7 codes, scale
+pack_window_step = struct.Struct("=5Q10q3Q3q7if").pack
+# geo_recurrence_t: 3 tensors, 3 strides, decay, ptr, state, 3 sizes, 2 codes, rate, 4 bytes to the end
+pack_recurrence = struct.Struct("=3Q3q3Q3q2if4x").pack
 
 
-class RecurrenceArgs(ctypes.Structure):
-    """geo_recurrence_t of include/geo_api.h."""
-
-    _fields_ = [(n, c_vp) for n in ("x", "gate_a", "gate_x")] + \
-        [(n, c_i64) for n in ("x_token", "gate_a_token", "gate_x_token")] + \
-        [(n, c_vp) for n in ("decay", "ptr", "state")] + [(n, c_i64) for n in ("tokens", "channels", "sequences")] + \
-        [("dtype", c_i32), ("reverse", c_i32), ("rate", c_f32)]
+def at(t: torch.Tensor | None) -> int:
+    """Address for the structs above."""
+    return 0 if t is None else t.data_ptr()
 
 
 # name -> (restype, argtypes)
@@ -161,20 +147,20 @@ _SIGNATURES = {
                                       c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32,
                                       c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp,
                                       c_vp]),
-    "geo_window_attention_fwd": (c_int, [ctypes.POINTER(WindowAttentionArgs), c_vp, c_vp, c_vp]),
-    "geo_window_attention_bwd_workspace_bytes": (c_size, [ctypes.POINTER(WindowAttentionArgs)]),
-    "geo_window_attention_bwd": (c_int, [ctypes.POINTER(WindowAttentionArgs), c_vp, c_vp, c_vp, c_vp, c_vp,
+    "geo_window_attention_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp]),
+    "geo_window_attention_bwd_workspace_bytes": (c_size, [c_bytes]),
+    "geo_window_attention_bwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_vp,
                                          c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "geo_window_attention_step_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i64]),
-    "geo_window_attention_step": (c_int, [ctypes.POINTER(WindowStepArgs), c_vp, c_vp, c_size, c_vp]),
+    "geo_window_attention_step": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
     "geo_window_cache_fill": (c_int, [c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
                                       c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
-    "geo_recurrence_chunks": (c_i64, [c_i64]),
-    "geo_recurrence_fwd": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "geo_recurrence_carry_size": (c_i64, [c_i64, c_i64]),
+    "geo_recurrence_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_bwd_workspace_bytes": (c_size, [c_i64, c_i64]),
-    "geo_recurrence_bwd": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+    "geo_recurrence_bwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                    c_size, c_vp]),
-    "geo_recurrence_step": (c_int, [ctypes.POINTER(RecurrenceArgs), c_vp, c_vp, c_vp]),
+    "geo_recurrence_step": (c_int, [c_bytes, c_vp, c_vp, c_vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -503,17 +503,24 @@ def segment_softmax_backward_hip(
 
 def _sequence_code(name: str, *tensors: Tensor) -> int:
     """Type code of a sequence operator's tensors, which have one type."""
-    code = _nat.SEQUENCE_DTYPES.get(tensors[0].dtype)
-    if code is None or any(t.dtype is not tensors[0].dtype for t in tensors):
-        raise TypeError(f"{name}: float32, bfloat16 or float16 tensors of one type, got "
-                        f"{', '.join(str(t.dtype) for t in tensors)}")
+    dtype = tensors[0].dtype
+    code = _nat.SEQUENCE_DTYPES.get(dtype)
+    for t in tensors:
+        if code is None or t.dtype is not dtype:
+            raise TypeError(f"{name}: float32, bfloat16 or float16 tensors of one type, got "
+                            f"{', '.join(str(t.dtype) for t in tensors)}")
     return code
 
 
-def _same_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
+def _sequence_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
+    """The GPU that holds all of an operator's tensors."""
     dev = tensors[0].device
-    if any(t is not None and t.device != dev for t in tensors):
-        raise ValueError(f"{name}: tensors on different devices")
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                _require_gpu(name, t)
+            if t.device != dev:
+                raise ValueError(f"{name}: tensors on different devices")
     return dev
 
 
@@ -527,10 +534,9 @@ def _in_pieces(t: Tensor) -> Tensor:
 
 
 def _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
-    """geo_window_attention_t of the call, and the tensors that it points into."""
-    _require_gpu(name, q, k, v, ptr, mask, bias)
+    """geo_window_attention_t of the call (packed), and the tensors that it points into."""
+    dev = _sequence_device(name, q, k, v, ptr, mask, bias)
     code = _sequence_code(name, q, k, v)
-    dev = _same_device(name, q, k, v, ptr, mask, bias)
     q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
     T, H, D = q.shape
     if k.shape[1] < 1 or H < 1 or H % k.shape[1]:
@@ -550,9 +556,10 @@ def _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, p
         bias = bias.contiguous()
         lut, _, maxd = plan
         buckets = bias.shape[0]
-    args = _nat.WindowAttentionArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-        v.stride(1), _nat.ptr(ptr), _nat.ptr(mask), _nat.ptr(bias), _nat.ptr(lut), T,
+    at = _nat.at
+    (qs, qh, _), (ks, kh, _), (vs, vh, _) = q.stride(), k.stride(), v.stride()
+    args = _nat.pack_window_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, qh, ks, kh, vs, vh, at(ptr), at(mask), at(bias), at(lut), T,
         1 if ptr is None else ptr.numel() - 1, left, right, sinks, code, bias_code, H, k.shape[1], D, buckets, maxd, scale)
     return args, (q, k, v, ptr, mask, bias, lut), dev
 
@@ -593,9 +600,8 @@ def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale
     """[B, H, D] of the tokens at ``positions``, whose k and v go into the caches [B, Hk, slots, D];
     ``workspace(bytes)`` gives the scratch."""
     name = "window_attention_step"
-    _require_gpu(name, q, k, v, k_cache, v_cache, positions, bias)
+    dev = _sequence_device(name, q, k, v, k_cache, v_cache, positions, bias)
     code = _sequence_code(name, q, k, v, k_cache, v_cache)
-    dev = _same_device(name, q, k, v, k_cache, v_cache, positions, bias)
     q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
     positions = _i64(positions, dev)
     B, H, D = q.shape
@@ -607,11 +613,12 @@ def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale
         bias = bias.contiguous()
         lut, _, maxd = plan
         buckets = bias.shape[0]
-    args = _nat.WindowStepArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q.stride(0), q.stride(1),
-        k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
-        v_cache.stride(1), positions.data_ptr(), _nat.ptr(bias), _nat.ptr(lut), B, slots, sinks, code, bias_code, H, Hk, D,
-        buckets, maxd, scale)
+    at = _nat.at
+    (qs, qh, _), (ks, kh, _), (vs, vh, _) = q.stride(), k.stride(), v.stride()
+    (kcs, kch, _, _), (vcs, vch, _, _) = k_cache.stride(), v_cache.stride()
+    args = _nat.pack_window_step(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), qs, qh, ks, kh, vs, vh, kcs, kch,
+        vcs, vch, positions.data_ptr(), at(bias), at(lut), B, slots, sinks, code, bias_code, H, Hk, D, buckets, maxd, scale)
     out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
     L = _nat.lib()
     with _nat.on_device(dev):
@@ -624,9 +631,8 @@ def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale
 def window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start):
     """Tokens k, v [T, Hk, D] of packed sequences into the caches [B, Hk, slots, D]."""
     name = "WindowCache.fill"
-    _require_gpu(name, k, v, k_cache, v_cache, ptr, start)
+    dev = _sequence_device(name, k, v, k_cache, v_cache, ptr, start)
     code = _sequence_code(name, k, v, k_cache, v_cache)
-    dev = _same_device(name, k, v, k_cache, v_cache, ptr, start)
     k, v = _in_pieces(k), _in_pieces(v)
     ptr = None if ptr is None else _i64(ptr, dev)
     start = None if start is None else _i64(start, dev)
@@ -638,20 +644,23 @@ def window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start):
             _nat.stream_of(dev)), "geo_window_cache_fill")
 
 
-def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate):
-    """geo_recurrence_t of the call, and the tensors that it points into."""
-    _require_gpu(name, x, gate_a, gate_x, decay, ptr, state)
+def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate, streams=None):
+    """geo_recurrence_t of the call (packed), the tensors that it points into, the device and the
+    number of sequences (``streams``: that many of one token each)."""
+    dev = _sequence_device(name, x, gate_a, gate_x, decay, ptr, state)
     code = _sequence_code(name, x, gate_a, gate_x)
-    dev = _same_device(name, x, gate_a, gate_x, decay, ptr, state)
-    x, gate_a, gate_x = (t if t.stride(1) == 1 else t.contiguous() for t in (x, gate_a, gate_x))
+    (xs, xd), (gas, gad), (gxs, gxd) = x.stride(), gate_a.stride(), gate_x.stride()
+    if xd != 1 or gad != 1 or gxd != 1:
+        x, gate_a, gate_x = x.contiguous(), gate_a.contiguous(), gate_x.contiguous()
+        xs, gas, gxs = x.stride(0), gate_a.stride(0), gate_x.stride(0)
     decay = _nat.f32c(decay)
     ptr = None if ptr is None else _i64(ptr, dev)
     state = None if state is None else _nat.f32c(state)
     T, C = x.shape
-    B = ptr.numel() - 1 if ptr is not None else 1
-    args = _nat.RecurrenceArgs(x.data_ptr(), gate_a.data_ptr(), gate_x.data_ptr(), x.stride(0), gate_a.stride(0),
-                               gate_x.stride(0), decay.data_ptr(), _nat.ptr(ptr), _nat.ptr(state), T, C, B, code,
-                               int(bool(reverse)), rate)
+    B = streams if streams is not None else ptr.numel() - 1 if ptr is not None else 1
+    at = _nat.at
+    args = _nat.pack_recurrence(x.data_ptr(), gate_a.data_ptr(), gate_x.data_ptr(), xs, gas, gxs, decay.data_ptr(), at(ptr),
+                                at(state), T, C, max(B, 1), code, 1 if reverse else 0, rate)
     return args, (x, gate_a, gate_x, decay, ptr, state), dev, B
 
 
@@ -663,13 +672,14 @@ def gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, 
     h = torch.empty(T, C, dtype=x.dtype, device=dev)
     if T == 0 or C == 0:
         last = torch.zeros(B, C, dtype=torch.float32, device=dev) if state is None else held[5].clone()
-        return h, last, h.new_empty(0, C, dtype=torch.float32)
+        return h, last, h.new_empty(0, dtype=torch.float32)
     last = torch.empty(B, C, dtype=torch.float32, device=dev)
-    carry = torch.empty(L.geo_recurrence_chunks(T), C, dtype=torch.float32, device=dev)
-    ws = torch.empty_like(carry)
+    n = L.geo_recurrence_carry_size(T, C)
+    carry = torch.empty(n, dtype=torch.float32, device=dev)
+    ws = torch.empty(2 * n, dtype=torch.float32, device=dev)
     with _nat.on_device(dev):
-        _nat.check(L.geo_recurrence_fwd(args, h.data_ptr(), last.data_ptr(), carry.data_ptr(), ws.data_ptr(),
-                                        ws.numel() * 4, _nat.stream_of(dev)), "geo_recurrence_fwd")
+        _nat.check(L.geo_recurrence_fwd(args, h.data_ptr(), last.data_ptr(), carry.data_ptr(), ws.data_ptr(), 8 * n,
+                                        _nat.stream_of(dev)), "geo_recurrence_fwd")
     return h, last, carry
 
 
@@ -701,8 +711,8 @@ def gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, pt
 
 def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate):
     """(h [B, C], new state float32 [B, C]) of one token per stream."""
-    args, held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, None, state, False, rate)
-    args.sequences = x.shape[0]
+    args, _held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, None, state, False, rate,
+                                           x.shape[0])
     h = torch.empty(x.shape, dtype=x.dtype, device=dev)
     new = torch.empty(x.shape, dtype=torch.float32, device=dev)
     if x.numel():

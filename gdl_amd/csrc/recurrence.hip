@@ -14,7 +14,9 @@
 namespace geo {
 namespace rec {
 
-constexpr int kLen = 16, kWaves = 8, kChunk = kLen * kWaves;
+// Longer stretches would hold more rows in registers than leave two workgroups a CU (16 tokens a wave:
+// the backward's second pass 208 us against 151 us at 131,072 x 256 bfloat16).
+constexpr int kLen = 8, kWaves = 8, kChunk = kLen * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T, int V> struct Pack;
@@ -157,6 +159,15 @@ constexpr float kCut = -1.f;
 __device__ __forceinline__ float after(float a, float add, float h) { return a == kCut ? add : fmaf(a, h, add); }
 __device__ __forceinline__ float chain(float a1, float a2) { return a1 == kCut || a2 == kCut ? kCut : a1 * a2; }
 
+// Where a chunk's map, state or sum of a channel lies: blocks of kCarryChannels channels, chunk after
+// chunk, so that the workgroup that carries a block over the chunks reads and writes whole lines.  Narrow
+// blocks spread the reading over CUs.
+constexpr int kCarryChannels = 4;
+__host__ __device__ inline int64_t padded(int64_t C) { return (C + kCarryChannels - 1) / kCarryChannels * kCarryChannels; }
+__device__ __forceinline__ int64_t chunk_place(int64_t chunk, int64_t chunks, int64_t at) {
+  return (at / kCarryChannels * chunks + chunk) * kCarryChannels + at % kCarryChannels;
+}
+
 // The waves' maps of a chunk, in LDS.
 template <int V>
 struct Maps {
@@ -213,7 +224,7 @@ __device__ __forceinline__ void steps(const Scan& s, const Stretch& c, const Pla
 
 // Pass 1: the chunk's map.
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves) void scan_map(const Scan s, float* __restrict__ mapa, float* __restrict__ maph) {
+__global__ __launch_bounds__(64 * kWaves, 4) void scan_map(const Scan s, int64_t chunks, float2* __restrict__ map) {
   __shared__ Maps<V> maps;
   const Place p = place<V>(s);
   Rows<T, V> x, ga, gx;
@@ -243,54 +254,59 @@ __global__ __launch_bounds__(64 * kWaves) void scan_map(const Scan s, float* __r
   maps.run(0, kWaves, H);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    mapa[p.chunk * s.C + p.at + v] = A[v];
-    maph[p.chunk * s.C + p.at + v] = H[v];
+    map[chunk_place(p.chunk, chunks, p.at + v)] = make_float2(A[v], H[v]);
   }
 }
 
-// Between the passes: maps composed over the chunks, `maph` replaced by the state before each chunk
-// (or, `back`, after it, from the last chunk to the first).  Sixteen waves share 64 channels, each 32
-// chunks at a time held in registers, so that a round of 512 chunks costs one memory latency.
-__global__ __launch_bounds__(1024) void scan_carry(const float* __restrict__ mapa, float* __restrict__ maph, int64_t chunks,
-                                                   int64_t C, int back) {
-  constexpr int kHeld = 32;
-  __shared__ float sa[16][64], sh[16][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t at = min(static_cast<int64_t>(blockIdx.x) * 64 + lane, C - 1);
-  const bool mine = static_cast<int64_t>(blockIdx.x) * 64 + lane < C;
-  auto index = [&](int64_t c) { return (back ? chunks - 1 - c : c) * C + at; };
+// Between the passes: maps composed over the chunks to the state before each chunk (or, `back`, after
+// it, from the last chunk to the first).  A workgroup shares its channels among 64 runs of chunks, each
+// held in registers by one thread per channel, so that a round of 2048 chunks costs one memory latency
+// (the loads are at clamped places: under a condition each waited for the one before, 26 us instead of
+// 9.4 us at 2048 chunks of 256 channels) and 64 steps over LDS.
+constexpr int kRuns = 64, kHeld = 32;
+__global__ __launch_bounds__(kCarryChannels * kRuns) void scan_carry(const float2* __restrict__ map, float* __restrict__ carry,
+                                                                     int64_t chunks, int back) {
+  __shared__ float2 runs[kRuns][kCarryChannels];
+  const int ch = threadIdx.x % kCarryChannels, run = threadIdx.x / kCarryChannels;
+  auto index = [&](int64_t c) { return (blockIdx.x * chunks + (back ? chunks - 1 - c : c)) * kCarryChannels + ch; };
   float ahead = 0.f;  // the state before the round
-  for (int64_t r = 0; r < chunks; r += 16 * kHeld) {
-    const int64_t c0 = r + wave * kHeld;
-    float a[kHeld], h[kHeld];
-#pragma unroll
-    for (int n = 0; n < kHeld; ++n) {
-      const int64_t i = index(min(c0 + n, chunks - 1));
-      a[n] = mapa[i];
-      h[n] = maph[i];
-    }
+  for (int64_t r = 0; r < chunks; r += kRuns * kHeld) {
+    // a run's length: the round's chunks shared evenly
+    const int per = static_cast<int>(min((chunks - r + kRuns - 1) / kRuns, int64_t(kHeld)));
+    const int64_t c0 = r + static_cast<int64_t>(run) * per, c1 = min(c0 + per, chunks);
+    float2 m[kHeld];
     float A = 1.f, H = 0.f;
 #pragma unroll
-    for (int n = 0; n < kHeld; ++n)
-      if (c0 + n < chunks) {
-        A = chain(A, a[n]);
-        H = after(a[n], h[n], H);
-      }
-    __syncthreads();
-    sa[wave][lane] = A;
-    sh[wave][lane] = H;
-    __syncthreads();
-    float h0 = ahead;
-    for (int n = 0; n < 16; ++n) {
-      if (n == wave) H = h0;
-      h0 = after(sa[n][lane], sh[n][lane], h0);
-    }
-    ahead = h0;
+    for (int n = 0; n < kHeld; ++n) m[n] = map[index(min(c0 + min(n, per - 1), chunks - 1))];
 #pragma unroll
     for (int n = 0; n < kHeld; ++n)
-      if (c0 + n < chunks) {
-        if (mine) maph[index(c0 + n)] = H;
-        H = after(a[n], h[n], H);
+      if (c0 + n < c1) {
+        A = chain(A, m[n].x);
+        H = after(m[n].x, m[n].y, H);
+      }
+    __syncthreads();
+    runs[run][ch] = make_float2(A, H);
+    __syncthreads();
+    if (threadIdx.x < kCarryChannels) {  // the state before each run, in the place of its map
+      const int used = static_cast<int>(min((chunks - r + per - 1) / per, int64_t(kRuns)));
+      for (int n0 = 0; n0 < used; n0 += 16) {
+        float2 y[16];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) y[n] = runs[n0 + n][ch];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          runs[n0 + n][ch].y = ahead;
+          if (n0 + n < used) ahead = after(y[n].x, y[n].y, ahead);
+        }
+      }
+    }
+    __syncthreads();
+    H = runs[run][ch].y;
+#pragma unroll
+    for (int n = 0; n < kHeld; ++n)
+      if (c0 + n < c1) {
+        carry[index(c0 + n)] = H;
+        H = after(m[n].x, m[n].y, H);
       }
   }
 }
@@ -308,7 +324,7 @@ __device__ __forceinline__ void pass_empty(const Scan& s, const Place& p, int64_
 
 // Pass 2: the outputs.
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves) void scan_out(const Scan s, int64_t chunks, const float* __restrict__ carry,
+__global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t chunks, const float* __restrict__ carry,
                                                         T* __restrict__ h, float* __restrict__ last) {
   __shared__ Maps<V> maps;
   const Place p = place<V>(s);
@@ -323,7 +339,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_out(const Scan s, int64_t ch
     lr[v] = log_rate(s.decay[p.at + v], s.rate);
     A[v] = 1.f;
     H[v] = 0.f;
-    state[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
+    state[v] = chunks > 1 ? carry[chunk_place(p.chunk, chunks, p.at + v)] : 0.f;
   }
   const bool plain = c.plain();
   if (plain) steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
@@ -366,7 +382,7 @@ struct Grad {
   const float* dlast;      // [B, C], or null
   void *dx, *dga, *dgx;    // contiguous [T, C]
   float *dstate;           // [B, C], or null
-  float* ddecay;           // [chunks, C] sums of the chunks
+  float* ddecay;           // sums of the chunks, by chunk_place
 };
 
 // The map of a wave's stretch against the scan order, e before it from e behind it.
@@ -397,8 +413,8 @@ __device__ __forceinline__ void back_steps(const Scan& s, const Grad& d, const S
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const Grad d, float* __restrict__ mapa,
-                                                            float* __restrict__ mape) {
+__global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const Grad d, int64_t chunks,
+                                                            float2* __restrict__ map) {
   __shared__ Maps<V> maps;
   const Place p = place<V>(s);
   Rows<T, V> ga, dh;
@@ -434,8 +450,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const 
   maps.run(kWaves, 0, E);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    mapa[p.chunk * s.C + p.at + v] = A[v];
-    mape[p.chunk * s.C + p.at + v] = E[v];
+    map[chunk_place(p.chunk, chunks, p.at + v)] = make_float2(A[v], E[v]);
   }
 }
 
@@ -486,7 +501,7 @@ __device__ __forceinline__ void back_out(const Scan& s, const Grad& d, const Str
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks,
+__global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks,
                                                                const float* __restrict__ carry,
                                                                const float* __restrict__ carry_e) {
   __shared__ Maps<V> maps, back;
@@ -517,8 +532,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_out(const Scan s, con
   back.put(p.wave, B, E);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    state[v] = chunks > 1 ? carry[p.chunk * s.C + p.at + v] : 0.f;
-    E[v] = chunks > 1 ? carry_e[p.chunk * s.C + p.at + v] : 0.f;
+    state[v] = chunks > 1 ? carry[chunk_place(p.chunk, chunks, p.at + v)] : 0.f;
+    E[v] = chunks > 1 ? carry_e[chunk_place(p.chunk, chunks, p.at + v)] : 0.f;
   }
   __syncthreads();
   maps.run(0, p.wave, state);
@@ -545,7 +560,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_out(const Scan s, con
     for (int v = 0; v < V; ++v) {
       float y = dlr[v];
       for (int w = 1; w < kWaves; ++w) y += sum[w][lane_id() * V + v];
-      d.ddecay[p.chunk * s.C + p.at + v] = y;
+      d.ddecay[chunk_place(p.chunk, chunks, p.at + v)] = y;
     }
   }
   pass_empty(s, p, chunks, V, d.dlast, d.dstate);
@@ -553,23 +568,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_out(const Scan s, con
 
 // The chunks' sums of d log a times log a, added in their order; d log a / d decay = log a times
 // sigmoid(decay) / softplus(decay).
-__global__ __launch_bounds__(1024) void scan_bwd_decay(const float* __restrict__ part, int64_t chunks, int64_t C,
-                                                       const float* __restrict__ decay, float* __restrict__ out) {
-  __shared__ float sum[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+__global__ __launch_bounds__(kCarryChannels * kRuns) void scan_bwd_decay(const float* __restrict__ part, int64_t chunks,
+                                                                         int64_t C, const float* __restrict__ decay,
+                                                                         float* __restrict__ out) {
+  __shared__ float sum[kRuns][kCarryChannels];
+  const int ch = threadIdx.x % kCarryChannels, run = threadIdx.x / kCarryChannels;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kCarryChannels + ch;
   float x = 0.f;
-  for (int64_t c = wave; c < chunks; c += 16 * 16) {
+  for (int64_t c = run; c < chunks; c += kRuns * 16) {
     float y[16];
 #pragma unroll
-    for (int n = 0; n < 16; ++n) y[n] = part[min(c + 16 * n, chunks - 1) * C + min(at, C - 1)];
+    for (int n = 0; n < 16; ++n) y[n] = part[chunk_place(min(c + kRuns * n, chunks - 1), chunks, at)];
 #pragma unroll
-    for (int n = 0; n < 16; ++n) x += c + 16 * n < chunks ? y[n] : 0.f;
+    for (int n = 0; n < 16; ++n) x += c + kRuns * n < chunks ? y[n] : 0.f;
   }
-  sum[wave][lane] = x;
+  sum[run][ch] = x;
   __syncthreads();
-  if (wave || at >= C) return;
-  for (int n = 1; n < 16; ++n) x += sum[n][lane];
+  if (run || at >= C) return;
+  for (int n = 1; n < kRuns; ++n) x += sum[n][ch];
   const float y = decay[at];
   // sigmoid / softplus, near 1 where both are exp(y)
   const float ratio = y < -15.f ? 1.f - 0.5f * expf(y) : (y > 20.f ? 1.f / y : 1.f / (1.f + expf(-y)) / log1pf(expf(y)));
@@ -619,33 +635,33 @@ inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
 }
 
 template <typename T, int V>
-int forward(const Scan& s, void* h, float* last, float* maph, float* mapa, hipStream_t stream) {
+int forward(const Scan& s, void* h, float* last, float* carry, float2* map, hipStream_t stream) {
   const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
   const dim3 grid(static_cast<uint32_t>(chunks * blocks));
   if (chunks > 1) {
-    scan_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, mapa, maph);
+    scan_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, chunks, map);
     GEO_LAUNCH_CHECK("scan_map");
-    scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, maph, chunks, s.C, 0);
+    scan_carry<<<dim3(static_cast<uint32_t>(padded(s.C) / kCarryChannels)), dim3(kCarryChannels * kRuns), 0, stream>>>(map, carry, chunks, 0);
     GEO_LAUNCH_CHECK("scan_carry");
   }
-  scan_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, chunks, maph, static_cast<T*>(h), last);
+  scan_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, chunks, carry, static_cast<T*>(h), last);
   GEO_LAUNCH_CHECK("scan_out");
   return GEO_OK;
 }
 
 template <typename T, int V>
-int backward(const Scan& s, const Grad& d, const float* carry, float* mape, float* mapa, float* ddecay, hipStream_t stream) {
+int backward(const Scan& s, const Grad& d, const float* carry, float* carry_e, float2* map, float* ddecay, hipStream_t stream) {
   const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
-  const dim3 grid(static_cast<uint32_t>(chunks * blocks));
+  const dim3 grid(static_cast<uint32_t>(chunks * blocks)), across(static_cast<uint32_t>(padded(s.C) / kCarryChannels));
   if (chunks > 1) {
-    scan_bwd_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, mapa, mape);
+    scan_bwd_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, map);
     GEO_LAUNCH_CHECK("scan_bwd_map");
-    scan_carry<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(mapa, mape, chunks, s.C, 1);
+    scan_carry<<<across, dim3(kCarryChannels * kRuns), 0, stream>>>(map, carry_e, chunks, 1);
     GEO_LAUNCH_CHECK("scan_carry");
   }
-  scan_bwd_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, carry, mape);
+  scan_bwd_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, carry, carry_e);
   GEO_LAUNCH_CHECK("scan_bwd_out");
-  scan_bwd_decay<<<dim3(static_cast<uint32_t>(ceil_div(s.C, 64))), dim3(1024), 0, stream>>>(d.ddecay, chunks, s.C, s.decay, ddecay);
+  scan_bwd_decay<<<across, dim3(kCarryChannels * kRuns), 0, stream>>>(d.ddecay, chunks, s.C, s.decay, ddecay);
   GEO_LAUNCH_CHECK("scan_bwd_decay");
   return GEO_OK;
 }
@@ -658,7 +674,9 @@ int backward(const Scan& s, const Grad& d, const float* carry, float* mape, floa
    : g->dtype == GEO_BF16 ? (v == 2 ? geo::rec::F<__bf16, 2>(__VA_ARGS__) : geo::rec::F<__bf16, 1>(__VA_ARGS__)) \
                           : (v == 2 ? geo::rec::F<_Float16, 2>(__VA_ARGS__) : geo::rec::F<_Float16, 1>(__VA_ARGS__)))
 
-extern "C" int64_t geo_recurrence_chunks(int64_t tokens) { return tokens < 0 ? 0 : geo::rec::chunks_of(tokens); }
+extern "C" int64_t geo_recurrence_carry_size(int64_t tokens, int64_t channels) {
+  return tokens < 1 || channels < 1 ? 0 : geo::rec::chunks_of(tokens) * geo::rec::padded(channels);
+}
 
 extern "C" int geo_recurrence_fwd(const geo_recurrence_t* g, void* h, float* last, float* carry, void* workspace,
                                   size_t workspace_bytes, void* stream) {
@@ -667,16 +685,15 @@ extern "C" int geo_recurrence_fwd(const geo_recurrence_t* g, void* h, float* las
   const int rc = geo::rec::scan_args(g, &s, &v);
   if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
   GEO_REQUIRE(h && last && carry, "gated recurrence: null output");
-  const size_t need = static_cast<size_t>(geo::rec::chunks_of(s.T)) * s.C * sizeof(float);
+  const size_t need = static_cast<size_t>(geo_recurrence_carry_size(s.T, s.C)) * sizeof(float2);
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
-  return GEO_REC_CALL(forward, s, h, last, carry, static_cast<float*>(workspace), geo::as_stream(stream));
+  return GEO_REC_CALL(forward, s, h, last, carry, static_cast<float2*>(workspace), geo::as_stream(stream));
 }
 
 extern "C" size_t geo_recurrence_bwd_workspace_bytes(int64_t tokens, int64_t channels) {
-  if (tokens < 1 || channels < 1) return 0;
-  return static_cast<size_t>(geo::rec::chunks_of(tokens)) * channels * 3 * sizeof(float);
+  return static_cast<size_t>(geo_recurrence_carry_size(tokens, channels)) * 4 * sizeof(float);
 }
 
 extern "C" int geo_recurrence_bwd(const geo_recurrence_t* g, const float* carry, const void* dh, const float* dlast, void* dx,
@@ -692,10 +709,10 @@ extern "C" int geo_recurrence_bwd(const geo_recurrence_t* g, const float* carry,
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence backward: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
-  const int64_t n = geo::rec::chunks_of(s.T) * s.C;
-  float* w = static_cast<float*>(workspace);
-  const geo::rec::Grad d{dh, dlast, dx, dgate_a, dgate_x, dstate, w + 2 * n};
-  return GEO_REC_CALL(backward, s, d, carry, w, w + n, ddecay, geo::as_stream(stream));
+  const int64_t n = geo_recurrence_carry_size(s.T, s.C);
+  float* w = static_cast<float*>(workspace);  // maps, states, sums
+  const geo::rec::Grad d{dh, dlast, dx, dgate_a, dgate_x, dstate, w + 3 * n};
+  return GEO_REC_CALL(backward, s, d, carry, w + 2 * n, reinterpret_cast<float2*>(w), ddecay, geo::as_stream(stream));
 }
 
 namespace geo {

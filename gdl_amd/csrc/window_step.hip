@@ -20,26 +20,66 @@ struct Step {
   float scale;
 };
 
-// The position that slot s holds once position p is written, s one of the slots in use.
-__device__ __forceinline__ int64_t held(int s, int64_t p, int sinks, int ring) {
-  if (s < sinks) return s;
-  const int now = static_cast<int>((p - sinks) % ring), at = s - sinks;
-  return p - (at <= now ? now - at : now + ring - at);
+constexpr int kStepThreads = 256;
+constexpr int kAhead = 4;  // keys of a lane group in flight
+
+// Eight values of a row; their products are summed in float32 (pairs of 16-bit values by one
+// instruction, exact products).
+template <typename T>
+struct Eight {
+  union { uint4 u[sizeof(T) / 2]; T t[8]; };
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) u[n] = reinterpret_cast<const uint4*>(p)[n];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) reinterpret_cast<uint4*>(p)[n] = u[n];
+  }
+  __device__ __forceinline__ float operator[](int e) const { return static_cast<float>(t[e]); }
+};
+template <typename T>
+__device__ __forceinline__ float dot(const Eight<T>& a, const Eight<T>& b) {
+  float x = 0.f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x = fmaf(a.t[e], b.t[e], x);
+  } else {
+    const uint32_t p[4] = {a.u[0].x, a.u[0].y, a.u[0].z, a.u[0].w}, q[4] = {b.u[0].x, b.u[0].y, b.u[0].z, b.u[0].w};
+    using Two = T __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (__is_same(T, __bf16)) x = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, p[e]), __builtin_bit_cast(Two, q[e]), x, false);
+      else x = __builtin_amdgcn_fdot2(__builtin_bit_cast(Two, p[e]), __builtin_bit_cast(Two, q[e]), x, false);
+    }
+  }
+  return x;
+}
+// Sum over a group of LW = 4, 8 or 16 lanes, in all of them: each mirrored half holds the same sums
+// by the time that it is added.
+template <int LW>
+__device__ __forceinline__ float group_sum(float x) {
+  x += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(x)));
+  if constexpr (LW >= 8) x += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(x)));
+  if constexpr (LW >= 16) x += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(x)));
+  return x;
 }
 
-constexpr int kStepThreads = 256;
-
 // One workgroup: a piece of the slots of one stream and key head, for GB of the query heads that
-// share it.  LW = D / 8 lanes (rounded up to a power of two) hold a key, 8 values each, and 64 / LW
-// keys a wave goes on at once; every lane group keeps its own running maximum, sum and output,
-// which are joined through LDS at the end.  Partial results of the pieces go to the workspace.
+// share it.  LW lanes hold a key, 8 values each (D / 8 rounded up to a power of two); every lane group
+// takes kAhead keys at a time, their reads in flight together, and keeps its own running maximum, sum
+// and output, which are joined through LDS at the end.  Partial results of the pieces go to the
+// workspace.  The work is the reading of the cache: 256 streams, 4112 slots, 16 (4) heads of 128 in
+// bfloat16 712 us with one key at a time and its lane sums through LDS.
 template <typename T, int LW, int GB>
 __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pieces, float* __restrict__ part,
                                                            T* __restrict__ out) {
-  constexpr int kGroups = kStepThreads / LW;  // keys at once
+  constexpr int kGroups = kStepThreads / LW;  // lane groups
   constexpr int kDp = 8 * LW;
-  __shared__ float sm[kGroups][GB], sl[kGroups][GB];
+  __shared__ float sm[4][GB], sl[4][GB];
   __shared__ float so[4][GB][kDp];
+  extern __shared__ float sbias[];  // [GB][maxd + 1]: biases of distances 0 .. maxd back, times log2 e
   const int group = a.Hq / a.Hk, chunks = (group + GB - 1) / GB;
   int64_t w = blockIdx.x;
   const int piece = static_cast<int>(w % pieces); w /= pieces;
@@ -55,57 +95,92 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
   T* const vc = static_cast<T*>(a.vc) + b * a.vc_b + hk * a.vc_h;
   const T* const kn = static_cast<const T*>(a.k) + b * a.k_st + hk * a.k_sh;
   const T* const vn = static_cast<const T*>(a.v) + b * a.v_st + hk * a.v_sh;
-  const int fresh = p < 0 ? -1 : static_cast<int>(p < a.sinks ? p : a.sinks + (p - a.sinks) % a.ring);
-
-  float q[GB][8], o[GB][8] = {}, m[GB], l[GB];
-#pragma unroll
-  for (int g = 0; g < GB; ++g) {
-    m[g] = -kInf;
-    l[g] = 0.f;
-    const T* row = static_cast<const T*>(a.q) + b * a.q_st + (h0 + min(g, heads - 1)) * a.q_sh;
-    union { uint4 u[sizeof(T) / 2]; T t[8]; } x;
-#pragma unroll
-    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) x.u[n] = reinterpret_cast<const uint4*>(row + (wide ? d : 0))[n];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[g][e] = wide ? static_cast<float>(x.t[e]) * a.scale * kLog2e : 0.f;
-  }
+  const int now = p < a.sinks ? -1 : static_cast<int>((p - a.sinks) % a.ring);  // the new token's place in the ring
+  const int fresh = p < 0 ? -1 : now < 0 ? static_cast<int>(p) : a.sinks + now;
   // slots in use: all once the window is full
   const int used = p < 0 ? 0 : static_cast<int>(min(p + 1, int64_t(a.slots)));
   const int per = (used + pieces - 1) / pieces;
   const int s0 = piece * per, s1 = min(used, s0 + per);
-  for (int s = s0 + kg; s < s1; s += kGroups) {
-    union { uint4 u[sizeof(T) / 2]; T t[8]; } kx, vx;
-    const T* kr = s == fresh ? kn : kc + static_cast<int64_t>(s) * a.D;
-    const T* vr = s == fresh ? vn : vc + static_cast<int64_t>(s) * a.D;
+  const int ds = wide ? d : 0;
+
+  Eight<T> kx[kAhead], vx[kAhead];
+  auto fetch = [&](int s) {
 #pragma unroll
-    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) {
-      kx.u[n] = reinterpret_cast<const uint4*>(kr + (wide ? d : 0))[n];
-      vx.u[n] = reinterpret_cast<const uint4*>(vr + (wide ? d : 0))[n];
+    for (int n = 0; n < kAhead; ++n) {
+      const int at = min(s + n * kGroups, s1 - 1);
+      kx[n].load((at == fresh ? kn : kc + static_cast<int64_t>(at) * a.D) + ds);
+      vx[n].load((at == fresh ? vn : vc + static_cast<int64_t>(at) * a.D) + ds);
     }
-    if (s == fresh && gc == 0 && wide) {
+  };
+  if (s0 < s1) fetch(s0 + kg);
+  Eight<T> q[GB];
+  float o[GB][8] = {}, m[GB], l[GB];
 #pragma unroll
-      for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) {
-        reinterpret_cast<uint4*>(kc + static_cast<int64_t>(s) * a.D + d)[n] = kx.u[n];
-        reinterpret_cast<uint4*>(vc + static_cast<int64_t>(s) * a.D + d)[n] = vx.u[n];
+  for (int g = 0; g < GB; ++g) {
+    m[g] = -kInf;
+    l[g] = 0.f;
+    q[g].load(static_cast<const T*>(a.q) + b * a.q_st + (h0 + min(g, heads - 1)) * a.q_sh + ds);
+    if (!wide) q[g] = Eight<T>{};
+  }
+  if (a.bias.table) {
+    for (int x = threadIdx.x; x <= a.bias.maxd; x += kStepThreads) {
+      const int64_t row = static_cast<int64_t>(a.bias.lut[a.bias.maxd - x]) * a.Hq + h0;
+#pragma unroll
+      for (int g = 0; g < GB; ++g)
+        sbias[g * (a.bias.maxd + 1) + x] = table_value(a.bias.table, a.bias.dtype, row + min(g, heads - 1)) * kLog2e;
+    }
+    __syncthreads();
+  }
+  const float scale2 = a.scale * kLog2e;
+  for (int s = s0 + kg; s - kg < s1; s += kAhead * kGroups) {
+    float x[kAhead][GB];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int at = s + n * kGroups;
+      const bool in = at < s1;
+      if (at == fresh && gc == 0 && wide && in) {
+        kx[n].store(kc + static_cast<int64_t>(at) * a.D + d);
+        vx[n].store(vc + static_cast<int64_t>(at) * a.D + d);
+      }
+      const float* bias = nullptr;
+      if (a.bias.table) {
+        // how far back the slot's token lies (at most maxd): the ring is read backwards from `now`
+        const int ring = at - a.sinks <= now ? now - (at - a.sinks) : now + a.ring - (at - a.sinks);
+        const int64_t back = at < a.sinks ? p - at : ring;
+        bias = sbias + static_cast<int>(min(max(back, int64_t(0)), int64_t(a.bias.maxd)));
+      }
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        const float y = group_sum<LW>(dot(q[g], kx[n])) * scale2;
+        x[n][g] = in ? (bias ? y + bias[g * (a.bias.maxd + 1)] : y) : -kInf;
       }
     }
-    int bucket = 0;
-    if (a.bias.table) bucket = a.bias.lut[max(held(s, p, a.sinks, a.ring) - p, int64_t(-a.bias.maxd)) + a.bias.maxd];
 #pragma unroll
     for (int g = 0; g < GB; ++g) {
-      float x = 0.f;
+      float top = m[g];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x = fmaf(q[g][e], static_cast<float>(kx.t[e]), x);
-#pragma unroll
-      for (int n = 1; n < LW; n *= 2) x += __shfl_xor(x, n, 64);
-      if (a.bias.table)
-        x += table_value(a.bias.table, a.bias.dtype, static_cast<int64_t>(bucket) * a.Hq + h0 + min(g, heads - 1)) * kLog2e;
-      const float top = fmaxf(m[g], x), keep = m[g] == -kInf ? 0.f : exp2_hw(m[g] - top), y = exp2_hw(x - (top == -kInf ? 0.f : top));
+      for (int n = 0; n < kAhead; ++n) top = fmaxf(top, x[n][g]);
+      const float shift = top == -kInf ? 0.f : top, keep = exp2_hw(m[g] - shift);
       m[g] = top;
-      l[g] = l[g] * keep + y;
+      l[g] *= keep;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[g][e] = fmaf(y, wide ? static_cast<float>(vx.t[e]) : 0.f, o[g][e] * keep);
+      for (int e = 0; e < 8; ++e) o[g][e] *= keep;
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        x[n][g] = exp2_hw(x[n][g] - shift);
+        l[g] += x[n][g];
+      }
     }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // a repeated last key (no key of this place) has the weight 0, its values may be anything
+        const float y = s + n * kGroups < s1 ? vx[n][e] : 0.f;
+#pragma unroll
+        for (int g = 0; g < GB; ++g) o[g][e] = fmaf(x[n][g], y, o[g][e]);
+      }
+    if (s - kg + kAhead * kGroups < s1) fetch(s + kAhead * kGroups);
   }
   // the groups' results joined: the wave's first, then the four waves'
   const int wave = threadIdx.x >> 6;
@@ -202,10 +277,15 @@ __global__ __launch_bounds__(256) void cache_fill(const char* __restrict__ k, co
       *reinterpret_cast<const uint4*>(v + (t * v_st + h * v_sh) * SIZE + e);
 }
 
-// Pieces of a stream's slots: enough workgroups for the 256 CUs, at least 128 slots each.
-inline int step_pieces(int64_t rows, int slots) {
+inline int lanes_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : 16; }
+
+// Pieces of a stream's slots: sixteen workgroups for each of the 256 CUs where there is work, at least
+// four rounds of a workgroup's keys each (a stream of 260 slots of 32 values in two pieces and a
+// join 9.8 us, in one 6 us).
+inline int step_pieces(int64_t rows, int64_t slots, int D) {
+  const int64_t least = 4 * kAhead * kStepThreads / lanes_of(D);
   int64_t n = 1;
-  while (rows * n < 1024 && slots / (2 * n) >= 128) n *= 2;
+  while (rows * n < 4096 && slots / (2 * n) >= least) n *= 2;
   return static_cast<int>(n);
 }
 
@@ -213,9 +293,10 @@ template <typename T, int LW, int GB>
 int launch_step(const Step& a, void* out, float* part, hipStream_t stream) {
   const int group = a.Hq / a.Hk;
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * ceil_div(group, GB);
-  const int pieces = step_pieces(rows, a.slots);
+  const int pieces = step_pieces(rows, a.slots, a.D);
   GEO_REQUIRE(rows * pieces < (int64_t(1) << 31), "window attention step: too many workgroups");
-  step_piece<T, LW, GB><<<dim3(static_cast<uint32_t>(rows * pieces)), dim3(kStepThreads), 0, stream>>>(a, pieces, part, static_cast<T*>(out));
+  const size_t lds = a.bias.table ? sizeof(float) * GB * (a.bias.maxd + 1) : 0;
+  step_piece<T, LW, GB><<<dim3(static_cast<uint32_t>(rows * pieces)), dim3(kStepThreads), lds, stream>>>(a, pieces, part, static_cast<T*>(out));
   GEO_LAUNCH_CHECK("step_piece");
   if (pieces > 1) {
     step_join<T, LW><<<dim3(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.Hq)), dim3(8 * LW), 0, stream>>>(a.D, pieces, part, static_cast<T*>(out));
@@ -232,7 +313,6 @@ int choose_group(const Step& a, void* out, float* part, hipStream_t stream) {
     default: return launch_step<T, LW, 1>(a, out, part, stream);
   }
 }
-inline int lanes_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : 16; }
 template <typename T>
 int choose_step(const Step& a, void* out, float* part, hipStream_t stream) {
   switch (lanes_of(a.D)) {
@@ -249,7 +329,7 @@ extern "C" size_t geo_window_attention_step_workspace_bytes(int64_t batch, int64
                                                             int64_t head_dim) {
   if (batch < 1 || heads < 1 || kv_heads < 1 || slots < 1 || head_dim < 1) return 0;
   const int64_t rows = batch * kv_heads * geo::ceil_div(heads / kv_heads, geo::attn::group_block(static_cast<int>(heads / kv_heads)));
-  const int pieces = geo::attn::step_pieces(rows, static_cast<int>(slots));
+  const int pieces = geo::attn::step_pieces(rows, slots, static_cast<int>(head_dim));
   return pieces == 1 ? 0 : static_cast<size_t>(batch * heads) * pieces * (8 * geo::attn::lanes_of(static_cast<int>(head_dim)) + 2) * sizeof(float);
 }
 
@@ -269,7 +349,8 @@ extern "C" int geo_window_attention_step(const geo_window_step_t* g, void* out, 
   if (g->bias) {
     GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16,
                 "window attention step: bias dtype code %d", static_cast<int>(g->bias_dtype));
-    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->max_distance >= 1, "window attention step: bias without its buckets");
+    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->max_distance >= 1 && g->max_distance <= 1024,
+                "window attention step: bias of %d buckets up to distance %d (at most 1024)", g->buckets, g->max_distance);
   }
   if (g->batch == 0) return GEO_OK;
   const int size = g->dtype == GEO_F32 ? 4 : 2;

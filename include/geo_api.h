@@ -698,11 +698,12 @@ typedef struct {
   int32_t dtype, reverse;
   float rate;
 } geo_recurrence_t;
-/* Chunks of the scan: carry is [chunks, channels], the states that the chunks begin with, which the
- * backward reads. */
-int64_t geo_recurrence_chunks(int64_t tokens);
+/* Elements of carry, float32: the states that the scan's chunks begin with, which the backward
+ * reads. */
+int64_t geo_recurrence_carry_size(int64_t tokens, int64_t channels);
 /* h [tokens, channels]; last float32 [sequences, channels], the states after each sequence's last
- * token in scan order (its state where it has none).  Workspace: as large as carry. */
+ * token in scan order (its state where it has none).  Workspace: twice as large as carry, 8-byte
+ * aligned. */
 int geo_recurrence_fwd(const geo_recurrence_t* args, void* h, float* last, float* carry,
                        void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients from dh [tokens, channels] and dlast (each may be NULL: zero); dstate may be NULL. */
