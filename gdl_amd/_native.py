@@ -147,9 +147,9 @@ _SIGNATURES = {
                                       c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32,
                                       c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp,
                                       c_vp]),
-    "geo_window_attention_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp]),
+    "geo_window_attention_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp]),
     "geo_window_attention_bwd_workspace_bytes": (c_size, [c_bytes]),
-    "geo_window_attention_bwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_vp,
+    "geo_window_attention_bwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                          c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "geo_window_attention_step_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     "geo_window_attention_step": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),

@@ -564,19 +564,23 @@ def _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, p
     return args, (q, k, v, ptr, mask, bias, lut), dev
 
 
-def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, with_lse):
-    """(out [T, H, D], log-sums float32 [H, T] or None); ``plan``: (bucket of each distance, spans,
-    max_distance) of the bias."""
+def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, train):
+    """(out [T, H, D], and for the backward, with ``train``: what its rounding took, for 16-bit types,
+    and the log-sums float32 [H, T]); ``plan``: (bucket of each distance, spans, max_distance) of the
+    bias."""
     args, _held, dev = _attention_args("window_attention", q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=dev) if with_lse else None
+    rest = lse = None
+    if train:
+        rest = torch.empty_like(out) if q.dtype is not torch.float32 else None
+        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=dev)
     with _nat.on_device(dev):
-        _nat.check(_nat.lib().geo_window_attention_fwd(args, out.data_ptr(), _nat.ptr(lse), _nat.stream_of(dev)),
-                   "geo_window_attention_fwd")
-    return out, lse
+        _nat.check(_nat.lib().geo_window_attention_fwd(args, out.data_ptr(), _nat.ptr(rest), _nat.ptr(lse),
+                                                       _nat.stream_of(dev)), "geo_window_attention_fwd")
+    return out, rest, lse
 
 
-def window_attention_backward_hip(grad, out, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
+def window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
     """(dq, dk, dv, dbias or None), contiguous and of the inputs' types."""
     name = "window_attention backward"
     args, _held, dev = _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
@@ -588,8 +592,8 @@ def window_attention_backward_hip(grad, out, lse, q, k, v, left, right, sinks, s
         ws_bytes = L.geo_window_attention_bwd_workspace_bytes(args)
         ws = _nat.workspace(ws_bytes, dev)
         _nat.check(L.geo_window_attention_bwd(
-            args, out.data_ptr(), grad.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            None if bias is None else plan[1].data_ptr(), _nat.ptr(dbias), ws.data_ptr(), ws_bytes,
+            args, out.data_ptr(), _nat.ptr(rest), grad.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), None if bias is None else plan[1].data_ptr(), _nat.ptr(dbias), ws.data_ptr(), ws_bytes,
             _nat.stream_of(dev)), "geo_window_attention_bwd")
     if dbias is not None and q.shape[0] == 0:
         dbias.zero_()

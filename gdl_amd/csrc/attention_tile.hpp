@@ -274,8 +274,9 @@ __device__ __forceinline__ void add_wild(const T* base, int64_t stride, int row0
 }
 
 // A lane's register quads (four values along the row) of a transposed result, to a row of global
-// memory: rows of the result are columns 32 mt + 8 g + 4 half + 0..3.
-template <typename T, int MT>
+// memory: rows of the result are columns 32 mt + 8 g + 4 half + 0..3.  REST: what rounding to T takes
+// from each value, in its place.
+template <typename T, int MT, bool REST = false>
 __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[MT], float scale, int D) {
   const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
@@ -286,7 +287,11 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[MT], float
       if (d < D) {
         union { T t[4]; uint2 u2; uint4 u4; } w;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w.t[j] = static_cast<T>(acc[mt][4 * g + j] * scale);
+        for (int j = 0; j < 4; ++j) {
+          const float x = acc[mt][4 * g + j] * scale;
+          w.t[j] = static_cast<T>(x);
+          if constexpr (REST) w.t[j] = static_cast<T>(x - static_cast<float>(w.t[j]));
+        }
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + d) = w.u2;
         else *reinterpret_cast<uint4*>(row + d) = w.u4;
       }

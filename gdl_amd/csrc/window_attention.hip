@@ -18,7 +18,8 @@ namespace attn {
 // Which of a tile's keys a query sees is a 64-bit word per lane: the tile is skipped by a wave
 // whose words are all zero, and takes no select where all bits are set.
 template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
-__global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* __restrict__ out, float* __restrict__ lse) {
+__global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* __restrict__ out, T* __restrict__ rest,
+                                                            float* __restrict__ lse) {
   using Tl = Tile<T, DP, BN, 64 * NW>;
   using Frag = typename Type<T>::Frag;
   constexpr int kSub = BN / 32, kMt = DP / 32, kKc = DP / 16, kBm = 32 * NW;
@@ -170,8 +171,10 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
   }
   l = halves_sum(l);
   if (real) {
-    T* row = out + (static_cast<int64_t>(i) * a.Hq + h) * a.D;
-    store_row<T>(row, o, l == 0.f ? 0.f : 1.f / l, a.D);
+    const int64_t row = (static_cast<int64_t>(i) * a.Hq + h) * a.D;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store_row<T>(out + row, o, inv, a.D);
+    if (sizeof(T) == 2 && rest) store_row<T, kMt, true>(rest + row, o, inv, a.D);
     // +inf where no key is seen: the backward's exp2(s - lse) is 0 there
     if (lse && half == 0) lse[static_cast<int64_t>(h) * a.seq.T + i] = l == 0.f ? kInf : m + log2f(l);
   }
@@ -185,46 +188,47 @@ constexpr int fwd_waves() {
 }
 
 template <typename T, int DP, int NW, int BN, bool BIAS>
-int launch_fwd(const Attend& a, void* out, float* lse, hipStream_t stream) {
+int launch_fwd(const Attend& a, void* out, void* rest, float* lse, hipStream_t stream) {
   const int64_t blocks = ceil_div(a.seq.T, 32 * NW) * a.Hq;
   GEO_REQUIRE(blocks < (int64_t(1) << 31), "window attention: %lld workgroups", static_cast<long long>(blocks));
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
   GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_fwd<T, DP, NW, BN, BIAS, fwd_waves<T, DP, NW>()>), lds));
   attend_fwd<T, DP, NW, BN, BIAS, fwd_waves<T, DP, NW>()><<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * NW), lds, stream>>>(
-      a, static_cast<T*>(out), lse);
+      a, static_cast<T*>(out), static_cast<T*>(rest), lse);
   GEO_LAUNCH_CHECK("attend_fwd");
   return GEO_OK;
 }
 
 template <typename T, int DP>
-int choose_fwd(const Attend& a, void* out, float* lse, hipStream_t stream) {
+int choose_fwd(const Attend& a, void* out, void* rest, float* lse, hipStream_t stream) {
   // Four waves share a tile's loads; one wave alone where that leaves less than a workgroup for
   // each of the 256 CUs.
   const bool few = ceil_div(a.seq.T, 128) * a.Hq < 256;
   if (a.bias.table)
-    return few ? launch_fwd<T, DP, 1, 32, true>(a, out, lse, stream) : launch_fwd<T, DP, 4, 64, true>(a, out, lse, stream);
-  return few ? launch_fwd<T, DP, 1, 32, false>(a, out, lse, stream) : launch_fwd<T, DP, 4, 64, false>(a, out, lse, stream);
+    return few ? launch_fwd<T, DP, 1, 32, true>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, true>(a, out, rest, lse, stream);
+  return few ? launch_fwd<T, DP, 1, 32, false>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, false>(a, out, rest, lse, stream);
 }
 
 template <typename T>
-int choose_width(const Attend& a, void* out, float* lse, hipStream_t stream) {
-  if (a.D <= 32) return choose_fwd<T, 32>(a, out, lse, stream);
-  if (a.D <= 64) return choose_fwd<T, 64>(a, out, lse, stream);
-  if (a.D <= 96) return choose_fwd<T, 96>(a, out, lse, stream);
-  return choose_fwd<T, 128>(a, out, lse, stream);
+int choose_width(const Attend& a, void* out, void* rest, float* lse, hipStream_t stream) {
+  if (a.D <= 32) return choose_fwd<T, 32>(a, out, rest, lse, stream);
+  if (a.D <= 64) return choose_fwd<T, 64>(a, out, rest, lse, stream);
+  if (a.D <= 96) return choose_fwd<T, 96>(a, out, rest, lse, stream);
+  return choose_fwd<T, 128>(a, out, rest, lse, stream);
 }
 
 }  // namespace attn
 }  // namespace geo
 
-extern "C" int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, float* lse, void* stream) {
+extern "C" int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, void* rest, float* lse,
+                                        void* stream) {
   geo::attn::Attend a;
   const int rc = geo::attn::attend_args(args, &a);
   if (rc != GEO_OK || args->tokens == 0) return rc;
   GEO_REQUIRE(out, "window attention: null output");
   const hipStream_t s = geo::as_stream(stream);
-  if (args->dtype == GEO_F32) return geo::attn::choose_width<float>(a, out, lse, s);
-  if (args->dtype == GEO_BF16) return geo::attn::choose_width<__bf16>(a, out, lse, s);
-  return geo::attn::choose_width<_Float16>(a, out, lse, s);
+  if (args->dtype == GEO_F32) return geo::attn::choose_width<float>(a, out, rest, lse, s);
+  if (args->dtype == GEO_BF16) return geo::attn::choose_width<__bf16>(a, out, rest, lse, s);
+  return geo::attn::choose_width<_Float16>(a, out, rest, lse, s);
 }

@@ -3,7 +3,8 @@
 // With p_ij the weights, g_i the output's gradient and delta_i = g_i.o_i:
 //   dv_j = sum_i p_ij g_i,  ds_ij = p_ij (g_i.v_j - delta_i),
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dbias(d) = sum of ds_ij, j - i = d.
-// The weights are formed again from the scores and the forward's log-sums, once for dq (and the
+// delta is formed from the output before its rounding (out + rest): the rounding would cost as much
+// again as the rounding of ds does.  The weights are formed again from the scores and the forward's log-sums, once for dq (and the
 // bias) and once for dk and dv: seven products instead of five, for sums that no two workgroups
 // share, so every gradient is the same from run to run.
 #include "attention_args.hpp"
@@ -49,6 +50,7 @@ __device__ __forceinline__ float sum_by_distance(const f32x16& x) {
 // workgroup's sums leave by bucket.
 template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
 __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, const T* __restrict__ out,
+                                                        const T* __restrict__ rest,
                                                         const T* __restrict__ grad, const float* __restrict__ lse,
                                                         float* __restrict__ delta, T* __restrict__ dq,
                                                         const int32_t* __restrict__ range, float* __restrict__ part) {
@@ -101,8 +103,14 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
       qf[kc] = frag_global(q, kc, a.D, real);
       gf[kc] = frag_global(grad + row, kc, a.D, real);
       const Frag of = frag_global(out + row, kc, a.D, real);
+      Frag rf{};
+      if (sizeof(T) == 2 && rest) rf = frag_global(rest + row, kc, a.D, real);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dl += static_cast<float>(gf[kc][j]) * static_cast<float>(of[j]);
+      for (int j = 0; j < 8; ++j) {
+        float y = static_cast<float>(of[j]);
+        if (sizeof(T) == 2 && rest) y += static_cast<float>(rf[j]);
+        dl = fmaf(static_cast<float>(gf[kc][j]), y, dl);
+      }
     }
     dl = halves_sum(dl);
     if (real && half == 0) delta[static_cast<int64_t>(h) * a.seq.T + i] = dl;
@@ -567,7 +575,7 @@ inline size_t plan(const geo_window_attention_t& g, void* workspace, Plan* p) {
 }
 
 struct Grads {
-  const void *out, *grad;
+  const void *out, *rest, *grad;
   const float* lse;
   void *dq, *dk, *dv, *dbias;
   const int32_t* range;
@@ -596,7 +604,7 @@ int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream)
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1 + NW * bias_slots(a.bias.maxd)) : 0);
   GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_bwd_q<T, DP, NW, BN, BIAS, q_waves<T, DP, NW>()>), lds));
   attend_bwd_q<T, DP, NW, BN, BIAS, q_waves<T, DP, NW>()><<<dim3(static_cast<uint32_t>(p.q_blocks * a.Hq)), dim3(64 * NW), lds, stream>>>(
-      a, static_cast<const T*>(g.out), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
+      a, static_cast<const T*>(g.out), static_cast<const T*>(g.rest), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
       p.part);
   GEO_LAUNCH_CHECK("attend_bwd_q");
   if (BIAS) {
@@ -659,15 +667,16 @@ extern "C" size_t geo_window_attention_bwd_workspace_bytes(const geo_window_atte
   return geo::attn::plan(*args, nullptr, &p);
 }
 
-extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* grad,
+extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* rest, const void* grad,
                                         const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
                                         void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
   geo::attn::Attend a;
   const int rc = geo::attn::attend_args(args, &a);
   if (rc != GEO_OK || args->tokens == 0) return rc;
   GEO_REQUIRE(out && grad && lse && dq && dk && dv, "window attention backward: null tensor");
-  GEO_REQUIRE(reinterpret_cast<uintptr_t>(grad) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
-              "window attention backward: out and grad must lie on multiples of 16 bytes");
+  GEO_REQUIRE(reinterpret_cast<uintptr_t>(grad) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(rest) % 16 == 0,
+              "window attention backward: out, rest and grad must lie on multiples of 16 bytes");
   GEO_REQUIRE(!args->bias || (bucket_range && dbias), "window attention backward: null bucket_range or dbias");
   geo::attn::Plan p;
   const size_t need = geo::attn::plan(*args, workspace, &p);
@@ -676,7 +685,7 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
                           workspace ? workspace_bytes : size_t(0), need);
   GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks < (int64_t(1) << 31),
               "window attention backward: too many workgroups");
-  const geo::attn::Grads g{out, grad, lse, dq, dk, dv, dbias, bucket_range};
+  const geo::attn::Grads g{out, rest, grad, lse, dq, dk, dv, dbias, bucket_range};
   const hipStream_t s = geo::as_stream(stream);
   if (args->dtype == GEO_F32) return geo::attn::choose_grads<float>(a, g, p, s);
   if (args->dtype == GEO_BF16) return geo::attn::choose_grads<__bf16>(a, g, p, s);

@@ -40,18 +40,18 @@ _UNBOUNDED = 1 << 40
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, plan, ptr, mask, left, right, sinks, scale):
-        out, lse = window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, True)
-        ctx.save_for_backward(q, k, v, bias, out, lse, ptr, mask)
+        out, rest, lse = window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, True)
+        ctx.save_for_backward(q, k, v, bias, out, rest, lse, ptr, mask)
         ctx.rest = (plan, left, right, sinks, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, bias, out, lse, ptr, mask = ctx.saved_tensors
+        q, k, v, bias, out, rest, lse, ptr, mask = ctx.saved_tensors
         plan, left, right, sinks, scale = ctx.rest
-        dq, dk, dv, dbias = window_attention_backward_hip(grad, out, lse, q, k, v, left, right, sinks, scale, ptr, mask,
-                                                          bias, plan)
+        dq, dk, dv, dbias = window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr,
+                                                          mask, bias, plan)
         return dq, dk, dv, dbias, None, None, None, None, None, None, None
 
 
@@ -116,7 +116,7 @@ def window_attention(
                                     or (bias is not None and bias.requires_grad)):
         out = _WindowAttention.apply(q, k, v, bias, plan, ptr, mask, left, right, int(sinks), scale)
     else:
-        out, _ = window_attention_forward_hip(q, k, v, left, right, int(sinks), scale, ptr, mask, bias, plan, False)
+        out, _, _ = window_attention_forward_hip(q, k, v, left, right, int(sinks), scale, ptr, mask, bias, plan, False)
     return out[..., :d] if d % 8 else out
 
 

@@ -636,15 +636,16 @@ typedef struct {
   float scale;
 } geo_window_attention_t;
 
-/* out [tokens, heads, head_dim]; lse [heads, tokens] (may be NULL): log2 of the softmax's sum, for
- * the backward. */
-int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, float* lse, void* stream);
-/* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out and
- * lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of
+/* out [tokens, heads, head_dim]; for the backward (each may be NULL): rest, what the rounding of out
+ * took from its values, of out's shape and type (16-bit types); lse [heads, tokens], log2 of the
+ * softmax's sum. */
+int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, void* rest, float* lse, void* stream);
+/* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out,
+ * rest (may be NULL) and lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of
  * bias_lut that hold the bucket (each bucket's places are consecutive).  Sums have a fixed order. */
 size_t geo_window_attention_bwd_workspace_bytes(const geo_window_attention_t* args);
-int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* grad,
-                             const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
+int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* rest,
+                             const void* grad, const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
                              void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
