@@ -524,6 +524,11 @@ def _sequence_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
     return dev
 
 
+def _like(t: Tensor) -> Tensor:
+    """An empty contiguous tensor of t's shape and type (empty_like costs half of empty)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _in_pieces(t: Tensor) -> Tensor:
     """t [T, H, D] itself where its rows are contiguous, begin on multiples of 16 bytes and do not
     overlap."""
@@ -569,10 +574,10 @@ def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, 
     and the log-sums float32 [H, T]); ``plan``: (bucket of each distance, spans, max_distance) of the
     bias."""
     args, _held, dev = _attention_args("window_attention", q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = _like(q)
     rest = lse = None
     if train:
-        rest = torch.empty_like(out) if q.dtype is not torch.float32 else None
+        rest = _like(q) if q.dtype is not torch.float32 else None
         lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=dev)
     with _nat.on_device(dev):
         _nat.check(_nat.lib().geo_window_attention_fwd(args, out.data_ptr(), _nat.ptr(rest), _nat.ptr(lse),
@@ -585,8 +590,8 @@ def window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, si
     name = "window_attention backward"
     args, _held, dev = _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
     grad = _in_pieces(grad.to(out.dtype).contiguous())
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-    dbias = None if bias is None else torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    dbias = None if bias is None else _like(bias)
     L = _nat.lib()
     with _nat.on_device(dev):
         ws_bytes = L.geo_window_attention_bwd_workspace_bytes(args)
@@ -623,7 +628,7 @@ def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale
     args = _nat.pack_window_step(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), qs, qh, ks, kh, vs, vh, kcs, kch,
         vcs, vch, positions.data_ptr(), at(bias), at(lut), B, slots, sinks, code, bias_code, H, Hk, D, buckets, maxd, scale)
-    out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
+    out = _like(q)
     L = _nat.lib()
     with _nat.on_device(dev):
         ws = workspace(L.geo_window_attention_step_workspace_bytes(B, H, Hk, slots, D))
@@ -668,22 +673,23 @@ def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate, 
     return args, (x, gate_a, gate_x, decay, ptr, state), dev, B
 
 
-def gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate):
-    """(h [T, C], last float32 [B, C], states that the scan's chunks begin with)."""
+def gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate, train):
+    """(h [T, C], last float32 [B, C], with ``train`` the states that the scan's chunks begin with)."""
     args, held, dev, B = _recurrence_args("gated_recurrence", x, gate_a, gate_x, decay, ptr, state, reverse, rate)
     T, C = x.shape
     L = _nat.lib()
-    h = torch.empty(T, C, dtype=x.dtype, device=dev)
+    h = _like(x)
     if T == 0 or C == 0:
         last = torch.zeros(B, C, dtype=torch.float32, device=dev) if state is None else held[5].clone()
-        return h, last, h.new_empty(0, dtype=torch.float32)
-    last = torch.empty(B, C, dtype=torch.float32, device=dev)
+        return h, last, last.new_empty(0)
+    last = torch.empty(B, C, dtype=torch.float32, device=dev) if state is None else _like(held[5])
     n = L.geo_recurrence_carry_size(T, C)
-    carry = torch.empty(n, dtype=torch.float32, device=dev)
-    ws = torch.empty(2 * n, dtype=torch.float32, device=dev)
+    scratch = torch.empty(2 * n if train else 3 * n, dtype=torch.float32, device=dev)
+    carry = torch.empty(n, dtype=torch.float32, device=dev) if train else None
+    maps = scratch.data_ptr()
     with _nat.on_device(dev):
-        _nat.check(L.geo_recurrence_fwd(args, h.data_ptr(), last.data_ptr(), carry.data_ptr(), ws.data_ptr(), 8 * n,
-                                        _nat.stream_of(dev)), "geo_recurrence_fwd")
+        _nat.check(L.geo_recurrence_fwd(args, h.data_ptr(), last.data_ptr(), carry.data_ptr() if train else maps + 8 * n,
+                                        maps, 8 * n, _nat.stream_of(dev)), "geo_recurrence_fwd")
     return h, last, carry
 
 
@@ -697,12 +703,12 @@ def gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, pt
         if dh.data_ptr() % 4:
             dh = dh.clone()
     dlast = None if dlast is None else _nat.f32c(dlast)
-    dx, dga, dgx = (torch.empty(T, C, dtype=x.dtype, device=dev) for _ in range(3))
+    dx, dga, dgx = _like(x), _like(x), _like(x)
     if T == 0 or C == 0:
         dstate = None if state is None else (torch.zeros_like(held[5]) if dlast is None else dlast.clone())
         return dx, dga, dgx, torch.zeros(C, dtype=torch.float32, device=dev), dstate
-    ddecay = torch.empty(C, dtype=torch.float32, device=dev)
-    dstate = None if state is None else torch.empty(B, C, dtype=torch.float32, device=dev)
+    ddecay = _like(held[3])
+    dstate = None if state is None else _like(held[5])
     L = _nat.lib()
     with _nat.on_device(dev):
         ws_bytes = L.geo_recurrence_bwd_workspace_bytes(T, C)
@@ -717,8 +723,7 @@ def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate):
     """(h [B, C], new state float32 [B, C]) of one token per stream."""
     args, _held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, None, state, False, rate,
                                            x.shape[0])
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    new = torch.empty(x.shape, dtype=torch.float32, device=dev)
+    h, new = _like(x), _like(state)
     if x.numel():
         with _nat.on_device(dev):
             _nat.check(_nat.lib().geo_recurrence_step(args, new.data_ptr(), h.data_ptr(), _nat.stream_of(dev)),

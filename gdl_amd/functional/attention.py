@@ -203,7 +203,8 @@ def window_attention_step(
         if bias.dim() != 2 or bias.shape[1] != q.shape[1]:
             raise ValueError(f"window_attention_step: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
         plan = bucket_plan(bias.shape[0], int(max_distance), False, q.device) + (int(max_distance),)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
         raise RuntimeError("window_attention_step has no backward: call it under torch.no_grad()")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     return window_attention_step_hip(q, k, v, cache.k, cache.v, cache.sinks, positions, scale, bias, plan, cache._workspace)

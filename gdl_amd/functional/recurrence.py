@@ -31,7 +31,7 @@ from gdl_amd.csrc import (
 class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_a, gate_x, decay, state, ptr, reverse, rate):
-        h, last, carry = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate)
+        h, last, carry = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate, True)
         ctx.save_for_backward(x, gate_a, gate_x, decay, state, ptr, carry)
         ctx.rest = (reverse, rate)
         ctx.set_materialize_grads(False)
@@ -48,7 +48,8 @@ class _GatedRecurrence(torch.autograd.Function):
 
 
 def _check(name: str, x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor) -> None:
-    if x.dim() != 2 or gate_a.shape != x.shape or gate_x.shape != x.shape or decay.shape != x.shape[1:]:
+    shape = x.shape
+    if len(shape) != 2 or gate_a.shape != shape or gate_x.shape != shape or decay.dim() != 1 or decay.shape[0] != shape[1]:
         raise ValueError(f"{name}: x, gate_a and gate_x [T, C], decay [C]; got {tuple(x.shape)}, {tuple(gate_a.shape)}, "
                          f"{tuple(gate_x.shape)}, {tuple(decay.shape)}")
     if not decay.dtype.is_floating_point:
@@ -89,9 +90,10 @@ def gated_recurrence(
     rate = float(rate)
     if not rate > 0:
         raise ValueError(f"gated_recurrence: rate {rate} must be positive")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate_a, gate_x, decay, state)):
+    if torch.is_grad_enabled() and (x.requires_grad or gate_a.requires_grad or gate_x.requires_grad or decay.requires_grad
+                                    or (state is not None and state.requires_grad)):
         return _GatedRecurrence.apply(x, gate_a, gate_x, decay, state, ptr, bool(reverse), rate)
-    h, last, _ = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, bool(reverse), rate)
+    h, last, _ = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, bool(reverse), rate, False)
     return h, last
 
 
@@ -111,6 +113,7 @@ def gated_recurrence_step(
         raise ValueError(f"gated_recurrence_step: state must be float32 {tuple(x.shape)}, got {state.dtype} {tuple(state.shape)}")
     if not rate > 0:
         raise ValueError(f"gated_recurrence_step: rate {rate} must be positive")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_a, gate_x, decay, state)):
+    if torch.is_grad_enabled() and (x.requires_grad or gate_a.requires_grad or gate_x.requires_grad or decay.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad()")
     return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, float(rate))
