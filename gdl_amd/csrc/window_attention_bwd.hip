@@ -498,42 +498,55 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_kv(const Attend a, 
   }
 }
 
-// The sums of leading token s of the one sequence that begins in piece c and reaches past its end:
-// the key's own and each later piece's and head's, in four runs that are added in their order.
+// The sums of leading token s of a sequence that reaches past the piece c that it begins in (one alone
+// does): the key's own and each later piece's and head's, in kJoinRuns runs that are added in their
+// order.  A workgroup for 64 of dk's and dv's values of every sequence, or where there are more of them
+// of every piece (by_piece).
+constexpr int kJoinRuns = 16;
 template <typename T>
-__global__ __launch_bounds__(1024) void attend_bwd_join(const Attend a, T* __restrict__ dk, T* __restrict__ dv, const Far f) {
+__global__ __launch_bounds__(64 * kJoinRuns) void attend_bwd_join(const Attend a, T* __restrict__ dk, T* __restrict__ dv, const Far f,
+                                                        bool by_piece) {
   __shared__ int sptr[kStagedPtr];
-  __shared__ float runs[4][256];
-  const int64_t w = blockIdx.x;
+  __shared__ float runs[kJoinRuns][64];
+  const int blocks = (2 * a.D + 63) / 64;
+  const int64_t w = blockIdx.x / blocks;
   const int s = static_cast<int>(w % a.sinks), hk = static_cast<int>(w / a.sinks % a.Hk);
-  const int64_t c = w / a.sinks / a.Hk;
-  stage_ptr(a.seq, sptr);
-  __syncthreads();
-  int first, end;
-  seq_of(a.seq, sptr, static_cast<int>((c + 1) * f.len), first, end);
+  const int n = static_cast<int>(w / a.sinks / a.Hk);
+  int first = 0, end = a.seq.T;
+  if (by_piece) {
+    stage_ptr(a.seq, sptr);
+    __syncthreads();
+    seq_of(a.seq, sptr, (n + 1) * f.len, first, end);
+    if (first / f.len != n) return;
+  } else if (a.seq.ptr) {
+    first = static_cast<int>(min(max(a.seq.ptr[n], int64_t(0)), int64_t(a.seq.T)));
+    end = static_cast<int>(min(max(a.seq.ptr[n + 1], int64_t(0)), int64_t(a.seq.T)));
+  }
   const int j = first + s;
-  if (first / f.len != c || j >= end || own_end(f, j, a.left) >= end) return;
-  const int x = threadIdx.x & 255, run = threadIdx.x >> 8, group = a.Hq / a.Hk;
+  const int64_t c = first / f.len;
+  if (j >= end || own_end(f, j, a.left) >= end) return;
+  const int column = threadIdx.x & 63, x = static_cast<int>(blockIdx.x % blocks) * 64 + column, run = threadIdx.x >> 6;
+  const int group = a.Hq / a.Hk;
   const int64_t p0 = own_end(f, j, a.left) / f.len, terms = ((end - 1) / f.len - p0 + 1) * group;
-  const int64_t per = (terms + 3) / 4, t0 = min(run * per, terms), t1 = min(t0 + per, terms);
+  const int64_t per = (terms + kJoinRuns - 1) / kJoinRuns, t0 = min(run * per, terms), t1 = min(t0 + per, terms);
   float sum = 0.f;
   if (x < 2 * a.D) {
     auto term = [&](int64_t t) {
       return f.part[(((p0 + t / group) * a.Hq + hk * group + t % group) * a.sinks + s) * 2 * a.D + x];
     };
-    for (int64_t t = t0; t < t1; t += 8) {
-      float y[8];
+    for (int64_t t = t0; t < t1; t += 16) {
+      float y[16];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) y[n] = term(min(t + n, t1 - 1));
+      for (int q = 0; q < 16; ++q) y[q] = term(min(t + q, t1 - 1));
 #pragma unroll
-      for (int n = 0; n < 8; ++n) sum += t + n < t1 ? y[n] : 0.f;
+      for (int q = 0; q < 16; ++q) sum += t + q < t1 ? y[q] : 0.f;
     }
   }
-  runs[run][x] = sum;
+  runs[run][column] = sum;
   __syncthreads();
   if (run || x >= 2 * a.D) return;
   sum = f.own[((c * a.Hk + hk) * a.sinks + s) * 2 * a.D + x];
-  for (int n = 0; n < 4; ++n) sum += runs[n][x];
+  for (int q = 0; q < kJoinRuns; ++q) sum += runs[q][column];
   const int64_t row = (static_cast<int64_t>(j) * a.Hk + hk) * a.D;
   if (x < a.D) dk[row + x] = static_cast<T>(sum * a.scale);
   else dv[row + x - a.D] = static_cast<T>(sum);
@@ -638,8 +651,10 @@ int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream
              ? launch_kv<T, DP, 1, 32, BIAS, false>(a, g, p, ceil_div(a.seq.T, 32) * a.Hk, stream)
              : launch_kv<T, DP, 4, kv_rows<T, DP>(), BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
   if (rc == GEO_OK && p.far.len) {
-    attend_bwd_join<T><<<dim3(static_cast<uint32_t>((p.pieces - 1) * a.Hk * a.sinks)), dim3(1024), 0, stream>>>(
-        a, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far);
+    const bool by_piece = a.seq.B > p.pieces - 1;
+    const int64_t each = by_piece ? p.pieces - 1 : a.seq.B;
+    attend_bwd_join<T><<<dim3(static_cast<uint32_t>(each * a.Hk * a.sinks * ceil_div(2 * a.D, 64))), dim3(64 * kJoinRuns), 0, stream>>>(
+        a, static_cast<T*>(g.dk), static_cast<T*>(g.dv), p.far, by_piece);
     GEO_LAUNCH_CHECK("attend_bwd_join");
   }
   return rc;
@@ -683,7 +698,7 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
-  GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks < (int64_t(1) << 31),
+  GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks * 4 < (int64_t(1) << 31),
               "window attention backward: too many workgroups");
   const geo::attn::Grads g{out, rest, grad, lse, dq, dk, dv, dbias, bucket_range};
   const hipStream_t s = geo::as_stream(stream);
