@@ -94,38 +94,39 @@ struct Scan {
 struct Stretch {
   int64_t n0;                    // the first token's number in scan order
   uint32_t begin, finish, live;  // bits: first of its sequence in scan order, last, of a sequence
-  int64_t seq;                   // this lane's token's sequence
+  int seq;                       // this lane's token's sequence
   __device__ __forceinline__ bool plain() const { return live == (1u << kLen) - 1 && !(begin | finish); }
 };
 __device__ __forceinline__ int64_t token(const Scan& s, int64_t n) { return s.reverse ? s.T - 1 - n : n; }
 __device__ __forceinline__ Stretch look(const Scan& s, int64_t n0) {
-  const int lane = lane_id();
-  const int64_t n = n0 + (lane & (kLen - 1)), t = token(s, min(n, s.T - 1));
-  int64_t lo = 0, first = 0, end = s.T;
-  if (s.ptr) {
-    int64_t hi = s.B - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (s.ptr[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    first = s.ptr[lo];
-    end = min(s.ptr[lo + 1], s.T);
-  }
-  const bool live = n < s.T && first <= t && t < end;
-  const int64_t first_in = max(first, int64_t(0));
   constexpr uint32_t kAll = (1u << kLen) - 1;
   Stretch c;
   c.n0 = n0;
+  c.seq = 0;
+  if (!s.ptr) {  // one sequence: on the scalar unit
+    const int64_t left = s.T - n0;
+    c.live = left >= kLen ? kAll : left > 0 ? (1u << left) - 1 : 0u;
+    c.begin = n0 == 0 ? 1u : 0u;
+    c.finish = left > 0 && left <= kLen ? 1u << (left - 1) : 0u;
+    return c;
+  }
+  const int T = static_cast<int>(s.T), n = static_cast<int>(n0) + (lane_id() & (kLen - 1));
+  const int t = s.reverse ? T - 1 - min(n, T - 1) : min(n, T - 1);
+  auto at = [&](int b) { return static_cast<int>(min(max(s.ptr[b], int64_t(-1)), int64_t(T))); };
+  int lo = 0, hi = static_cast<int>(s.B) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at(mid) <= t) lo = mid; else hi = mid - 1;
+  }
+  const int first = at(lo), end = at(lo + 1), first_in = max(first, 0);
+  const bool live = n < T && first <= t && t < end;
   c.live = static_cast<uint32_t>(__ballot(live)) & kAll;
   c.begin = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? end - 1 : first_in))) & kAll;
   c.finish = static_cast<uint32_t>(__ballot(live && t == (s.reverse ? first_in : end - 1))) & kAll;
   c.seq = lo;
   return c;
 }
-__device__ __forceinline__ int64_t seq_at(const Stretch& c, int l) {
-  return (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq >> 32), l)) << 32) |
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(c.seq), l));
-}
+__device__ __forceinline__ int64_t seq_at(const Stretch& c, int l) { return __builtin_amdgcn_readlane(c.seq, l); }
 
 template <typename T, int V>
 struct Rows {
@@ -142,6 +143,7 @@ struct Rows {
 // Grid of the passes: (chunk, block of 64 V channels), channels fastest.
 struct Place {
   int64_t chunk, n0, at;  // n0: the wave's first token's number; at: this lane's first channel, in range
+  int64_t base;           // the workgroup's first channel
   int wave;
   bool mine;
 };
@@ -149,8 +151,19 @@ template <int V>
 __device__ __forceinline__ Place place(const Scan& s) {
   const int64_t blocks = (s.C + 64 * V - 1) / (64 * V), w = xcd_block();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t at = (w % blocks * 64 + lane_id()) * V, chunk = w / blocks;
-  return {chunk, chunk * kChunk + wave * kLen, min(at, s.C - V), wave, at < s.C};
+  const int64_t base = w % blocks * 64 * V, at = base + lane_id() * V, chunk = w / blocks;
+  return {chunk, chunk * kChunk + wave * kLen, min(at, s.C - V), base, wave, at < s.C};
+}
+
+// log_rate of the lane's channels, formed once for the workgroup: its logarithm and exponential take
+// as many instructions as two tokens.  The barrier leaves the rows' loads in flight.
+template <int V>
+__device__ __forceinline__ void share_rates(const Scan& s, const Place& p, float (&lr)[V]) {
+  __shared__ float rates[64 * V];
+  if (threadIdx.x < 64 * V) rates[threadIdx.x] = log_rate(s.decay[min(p.base + threadIdx.x, s.C - 1)], s.rate);
+  lds_barrier();
+#pragma unroll
+  for (int v = 0; v < V; ++v) lr[v] = rates[lane_id() * V + v];
 }
 
 // The factor of a map across which nothing passes, as at the beginning of a sequence: a factor of 0
@@ -267,9 +280,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_map(const Scan s, int64_t
   gx.load(s.gx, s.gx_st, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
   float lr[V], A[V], H[V], fa[kLen][V], fb[kLen][V];
+  share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
     A[v] = 1.f;
     H[v] = 0.f;
   }
@@ -368,9 +381,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
   gx.load(s.gx, s.gx_st, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
   float lr[V], A[V], H[V], state[V], fa[kLen][V], fb[kLen][V];
+  share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
     A[v] = 1.f;
     H[v] = 0.f;
     state[v] = chunks > kFew ? carry[chunk_place(p.chunk, chunks, p.at + v)] : 0.f;
@@ -462,9 +475,9 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const 
   if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
   float lr[V], A[V], E[V], fa[kLen][V];
+  share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
     A[v] = 1.f;
     E[v] = 0.f;
   }
@@ -554,9 +567,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, con
   if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
   float lr[V], A[V], H[V], B[V], E[V], state[V], dlr[V] = {}, fa[kLen][V], fb[kLen][V];
+  share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    lr[v] = log_rate(s.decay[p.at + v], s.rate);
     A[v] = B[v] = 1.f;
     H[v] = E[v] = 0.f;
   }
@@ -660,7 +673,8 @@ inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
   GEO_REQUIRE(g, "gated recurrence: null arguments");
   GEO_REQUIRE(g->dtype == GEO_F32 || g->dtype == GEO_BF16 || g->dtype == GEO_F16, "gated recurrence: dtype code %d",
               static_cast<int>(g->dtype));
-  GEO_REQUIRE(g->tokens >= 0 && g->channels >= 0 && g->sequences >= 1, "gated recurrence: %lld tokens, %lld channels, %lld sequences",
+  GEO_REQUIRE(g->tokens >= 0 && g->tokens < (int64_t(1) << 31) - kChunk && g->channels >= 0 && g->sequences >= 1 &&
+                  g->sequences < (int64_t(1) << 31) - 1, "gated recurrence: %lld tokens, %lld channels, %lld sequences",
               static_cast<long long>(g->tokens), static_cast<long long>(g->channels), static_cast<long long>(g->sequences));
   *s = Scan{g->x, g->gate_a, g->gate_x, g->x_token, g->gate_a_token, g->gate_x_token, g->decay, g->ptr, g->state,
             g->tokens, g->channels, g->sequences, g->rate, g->reverse};
