@@ -79,6 +79,20 @@ inline int attend_args(const geo_window_attention_t* g, Attend* a) {
   return GEO_OK;
 }
 
+// Rows are taken by workgroups of four waves, which share tiles of 64 rows of the other side, or by one
+// wave alone with tiles of 32.  Alone, a wave loads little that it does not need: better where four would
+// leave CUs without a workgroup and the window is narrow.  1024 tokens of 8 heads of 64, windows to both
+// sides, forward and backward in us, four waves | one:
+//   bfloat16, 129 keys   9.1  25.7 |  8.3  21.5      float32, 129 keys   24.2   76.5 | 18.4   54.8
+//             385       13.6  38.8 | 15.4  37.8               513        52.3  170.9 | 50.3  161.1
+//             769       20.3  57.0 | 25.3  61.2              2049        82.0  265.4 | 92.2  293.1
+// and at 8192 tokens, 512 workgroups of four waves, with 257 keys 16.7 49.9 | 18.9 53.1 and 63.7 214.4 |
+// 79.8 200.6.
+inline bool lone_wave(const Attend& a, int heads, bool f32) {
+  const int64_t keys = int64_t(a.left) + a.right + 1;
+  return ceil_div(a.seq.T, 128) * heads < 256 && keys <= (f32 ? 512 : 256);
+}
+
 // Dynamic LDS beyond 64 KB has to be asked for.
 inline hipError_t allow_lds(const void* kernel, size_t bytes) {
   return bytes <= 60 * 1024 ? hipSuccess

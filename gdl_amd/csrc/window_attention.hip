@@ -202,12 +202,10 @@ int launch_fwd(const Attend& a, void* out, void* rest, float* lse, hipStream_t s
 
 template <typename T, int DP>
 int choose_fwd(const Attend& a, void* out, void* rest, float* lse, hipStream_t stream) {
-  // Four waves share a tile's loads; one wave alone where that leaves less than a workgroup for
-  // each of the 256 CUs.
-  const bool few = ceil_div(a.seq.T, 128) * a.Hq < 256;
+  const bool lone = lone_wave(a, a.Hq, sizeof(T) == 4);
   if (a.bias.table)
-    return few ? launch_fwd<T, DP, 1, 32, true>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, true>(a, out, rest, lse, stream);
-  return few ? launch_fwd<T, DP, 1, 32, false>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, false>(a, out, rest, lse, stream);
+    return lone ? launch_fwd<T, DP, 1, 32, true>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, true>(a, out, rest, lse, stream);
+  return lone ? launch_fwd<T, DP, 1, 32, false>(a, out, rest, lse, stream) : launch_fwd<T, DP, 4, 64, false>(a, out, rest, lse, stream);
 }
 
 template <typename T>

@@ -554,10 +554,6 @@ __global__ __launch_bounds__(64 * kJoinRuns) void attend_bwd_join(const Attend a
 
 // ---------------------------------------------------------------------- host ---
 
-// Workgroups of four waves share a tile; one wave alone where that leaves less than one workgroup
-// for each of the 256 CUs.
-inline bool few_blocks(int T, int heads) { return ceil_div(T, 128) * heads < 256; }
-
 // Pieces of the queries past a leading token's window: 256 tokens (64 pieces keep the sums of a
 // sequence of 16,384 small), longer where that would be more than 512 pieces.
 inline int far_len(int T, int left, int sinks) {
@@ -573,14 +569,13 @@ struct Plan {
   Far far;
   int64_t pieces;
 };
-inline size_t plan(const geo_window_attention_t& g, void* workspace, Plan* p) {
-  const int T = static_cast<int>(g.tokens);
+inline size_t plan(const geo_window_attention_t& g, const Attend& a, void* workspace, Plan* p) {
+  const int T = a.seq.T, sinks = a.sinks;
   Carver c(workspace);
-  p->q_blocks = ceil_div(T, few_blocks(T, g.heads) ? 32 : 128);
+  p->q_blocks = ceil_div(T, lone_wave(a, a.Hq, g.dtype == GEO_F32) ? 32 : 128);
   p->delta = c.take<float>(static_cast<size_t>(g.heads) * T);
   p->part = c.take<float>(g.bias ? static_cast<size_t>(p->q_blocks) * g.heads * g.buckets : 0);
-  const int sinks = static_cast<int>(g.sinks < T ? g.sinks : T);
-  p->far.len = far_len(T, static_cast<int>(g.left < T ? g.left : T), sinks);
+  p->far.len = far_len(T, a.left, sinks);
   p->pieces = p->far.len ? ceil_div(T, p->far.len) : 0;
   p->far.own = c.take<float>(static_cast<size_t>(p->pieces) * g.kv_heads * sinks * 2 * g.head_dim);
   p->far.part = c.take<float>(static_cast<size_t>(p->pieces) * g.heads * sinks * 2 * g.head_dim);
@@ -642,12 +637,12 @@ int launch_kv(const Attend& a, const Grads& g, const Plan& p, int64_t blocks, hi
 
 template <typename T, int DP, bool BIAS>
 int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
-  int rc = few_blocks(a.seq.T, a.Hq) ? launch_q<T, DP, 1, 32, BIAS>(a, g, p, stream)
-                                     : launch_q<T, DP, 4, q_rows<DP>(), BIAS>(a, g, p, stream);
+  int rc = lone_wave(a, a.Hq, sizeof(T) == 4) ? launch_q<T, DP, 1, 32, BIAS>(a, g, p, stream)
+                                              : launch_q<T, DP, 4, q_rows<DP>(), BIAS>(a, g, p, stream);
   if (rc == GEO_OK && p.far.len)
     rc = launch_kv<T, DP, 1, 32, BIAS, true>(a, g, p, (p.pieces - 1) * ceil_div(a.sinks, 32) * a.Hq, stream);
   if (rc == GEO_OK)
-    rc = few_blocks(a.seq.T, a.Hk)
+    rc = lone_wave(a, a.Hk, sizeof(T) == 4)
              ? launch_kv<T, DP, 1, 32, BIAS, false>(a, g, p, ceil_div(a.seq.T, 32) * a.Hk, stream)
              : launch_kv<T, DP, 4, kv_rows<T, DP>(), BIAS, false>(a, g, p, ceil_div(a.seq.T, 128) * a.Hk, stream);
   if (rc == GEO_OK && p.far.len) {
@@ -679,7 +674,7 @@ extern "C" size_t geo_window_attention_bwd_workspace_bytes(const geo_window_atte
   geo::attn::Attend a;
   if (geo::attn::attend_args(args, &a) != GEO_OK || args->tokens == 0) return 0;
   geo::attn::Plan p;
-  return geo::attn::plan(*args, nullptr, &p);
+  return geo::attn::plan(*args, a, nullptr, &p);
 }
 
 extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* rest, const void* grad,
@@ -694,7 +689,7 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
               "window attention backward: out, rest and grad must lie on multiples of 16 bytes");
   GEO_REQUIRE(!args->bias || (bucket_range && dbias), "window attention backward: null bucket_range or dbias");
   geo::attn::Plan p;
-  const size_t need = geo::attn::plan(*args, workspace, &p);
+  const size_t need = geo::attn::plan(*args, a, workspace, &p);
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
