@@ -9,13 +9,17 @@
 // row, a lane V channels.  A stretch of tokens is a map h -> A h + H of the state before it; maps are
 // composed over the waves in LDS and over the chunks by scan_carry.  Pass 1 forms the chunks' maps,
 // pass 2 the outputs from the states that the chunks begin with.  All in float32, whatever the inputs.
+//
+// The inputs are read twice in each direction, and still vector instructions bound the passes: 89 to 95%
+// of a SIMD's cycles, for two sigmoids, a decay, a root and 1 - a^2 of every element.  131,072 tokens of
+// 256 channels in bfloat16: pass 1 60 us, carry 9, pass 2 62; backward 34, 9 and 121, decay's sums 4.
 #include "common.hpp"
 
 namespace geo {
 namespace rec {
 
-// Longer stretches would hold more rows in registers than leave two workgroups a CU (16 tokens a wave:
-// the backward's second pass 208 us against 151 us at 131,072 x 256 bfloat16).
+// Longer stretches would hold more rows in registers than leave three workgroups a CU in the backward's
+// second pass (which with two takes 145 us instead of 121 at 131,072 x 256 bfloat16).
 constexpr int kLen = 8, kWaves = 8, kChunk = kLen * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -201,35 +205,44 @@ struct Maps {
   }
 };
 
-// Factors and terms of a wave's tokens, and the map of its stretch.  PLAIN: no border of a sequence
-// lies in it.
-template <bool PLAIN, typename T, int V>
-__device__ __forceinline__ void steps(const Scan& s, const Stretch& c, const Place& p, const Rows<T, V>& x, const Rows<T, V>& ga,
-                                      const Rows<T, V>& gx, const float (&lr)[V], float (&fa)[kLen][V], float (&fb)[kLen][V],
-                                      float (&A)[V], float (&H)[V]) {
+// Factors and terms of a wave's tokens.
+template <typename T, int V>
+__device__ __forceinline__ void terms(const Rows<T, V>& x, const Rows<T, V>& ga, const Rows<T, V>& gx, const float (&lr)[V],
+                                      Gates (&g)[kLen][V], float (&fb)[kLen][V]) {
 #pragma unroll
   for (int l = 0; l < kLen; ++l) {
     float xf[V], af[V], gf[V];
     unpack<T, V>(x.raw[l], xf);
     unpack<T, V>(ga.raw[l], af);
     unpack<T, V>(gx.raw[l], gf);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      g[l][v] = gates(af[v], gf[v], lr[v]);
+      fb[l][v] = g[l][v].m * g[l][v].z * xf[v];
+    }
+  }
+}
+// The map of a wave's stretch.  PLAIN: no border of a sequence lies in it.
+template <bool PLAIN, int V>
+__device__ __forceinline__ void steps(const Scan& s, const Stretch& c, const Place& p, const Gates (&g)[kLen][V],
+                                      const float (&fb)[kLen][V], float (&A)[V], float (&H)[V]) {
+#pragma unroll
+  for (int l = 0; l < kLen; ++l) {
     const bool begin = !PLAIN && ((c.begin >> l) & 1), live = PLAIN || ((c.live >> l) & 1);
     const int64_t b = begin ? seq_at(c, l) : 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Gates g = gates(af[v], gf[v], lr[v]);
-      fa[l][v] = g.a;
-      fb[l][v] = g.m * g.z * xf[v];
+      const float a = g[l][v].a;
       if (begin) {
         A[v] = kCut;
         H[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
       }
       if (PLAIN) {
-        A[v] *= g.a;
-        H[v] = fmaf(g.a, H[v], fb[l][v]);
+        A[v] *= a;
+        H[v] = fmaf(a, H[v], fb[l][v]);
       } else {
-        A[v] = live ? chain(A[v], g.a) : kCut;
-        H[v] = live ? fmaf(g.a, H[v], fb[l][v]) : 0.f;
+        A[v] = live ? chain(A[v], a) : kCut;
+        H[v] = live ? fmaf(a, H[v], fb[l][v]) : 0.f;
       }
     }
   }
@@ -279,15 +292,17 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_map(const Scan s, int64_t
   ga.load(s.ga, s.ga_st, s, p.n0, p.at);
   gx.load(s.gx, s.gx_st, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
-  float lr[V], A[V], H[V], fa[kLen][V], fb[kLen][V];
+  float lr[V], A[V], H[V], fb[kLen][V];
+  Gates g[kLen][V];
   share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     A[v] = 1.f;
     H[v] = 0.f;
   }
-  if (c.plain()) steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
-  else steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  terms(x, ga, gx, lr, g, fb);
+  if (c.plain()) steps<true>(s, c, p, g, fb, A, H);
+  else steps<false>(s, c, p, g, fb, A, H);
   maps.put(p.wave, A, H);
   __syncthreads();
   if (p.wave || !p.mine) return;
@@ -380,7 +395,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
   ga.load(s.ga, s.ga_st, s, p.n0, p.at);
   gx.load(s.gx, s.gx_st, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
-  float lr[V], A[V], H[V], state[V], fa[kLen][V], fb[kLen][V];
+  float lr[V], A[V], H[V], state[V], fb[kLen][V];
+  Gates g[kLen][V];
   share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -395,8 +411,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
       for (int v = 0; v < V; ++v) carry[chunk_place(p.chunk, chunks, p.at + v)] = state[v];
   }
   const bool plain = c.plain();
-  if (plain) steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
-  else steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
+  terms(x, ga, gx, lr, g, fb);
+  if (plain) steps<true>(s, c, p, g, fb, A, H);
+  else steps<false>(s, c, p, g, fb, A, H);
   maps.put(p.wave, A, H);
   __syncthreads();
   maps.run(0, p.wave, state);
@@ -404,7 +421,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
 #pragma unroll
     for (int l = 0; l < kLen; ++l) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) state[v] = fmaf(fa[l][v], state[v], fb[l][v]);
+      for (int v = 0; v < V; ++v) state[v] = fmaf(g[l][v].a, state[v], fb[l][v]);
       if (p.mine) *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, p.n0 + l) * s.C + p.at) = pack<T, V>(state);
     }
   } else {
@@ -415,7 +432,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (begin) state[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
-        state[v] = live ? fmaf(fa[l][v], state[v], fb[l][v]) : 0.f;
+        state[v] = live ? fmaf(g[l][v].a, state[v], fb[l][v]) : 0.f;
       }
       if (p.mine && n < s.T)
         *reinterpret_cast<typename Pack<T, V>::Raw*>(h + token(s, n) * s.C + p.at) = pack<T, V>(state);
@@ -441,7 +458,7 @@ struct Grad {
 // The map of a wave's stretch against the scan order, e before it from e behind it.
 template <bool PLAIN, typename T, int V>
 __device__ __forceinline__ void back_steps(const Scan& s, const Grad& d, const Stretch& c, const Place& p, const Rows<T, V>& dh,
-                                           const float (&fa)[kLen][V], float (&A)[V], float (&E)[V]) {
+                                           const Gates (&g)[kLen][V], float (&A)[V], float (&E)[V]) {
 #pragma unroll
   for (int l = kLen - 1; l >= 0; --l) {
     float hf[V] = {};
@@ -450,16 +467,17 @@ __device__ __forceinline__ void back_steps(const Scan& s, const Grad& d, const S
     const int64_t b = finish ? seq_at(c, l) : 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+      const float a = g[l][v].a;
       if (finish) {
         A[v] = kCut;
         E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
       }
       if (PLAIN) {
-        A[v] *= fa[l][v];
-        E[v] = fa[l][v] * (hf[v] + E[v]);
+        A[v] *= a;
+        E[v] = a * (hf[v] + E[v]);
       } else {
-        A[v] = live ? chain(A[v], fa[l][v]) : kCut;
-        E[v] = live ? fa[l][v] * (hf[v] + E[v]) : 0.f;
+        A[v] = live ? chain(A[v], a) : kCut;
+        E[v] = live ? a * (hf[v] + E[v]) : 0.f;
       }
     }
   }
@@ -474,7 +492,8 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const 
   ga.load(s.ga, s.ga_st, s, p.n0, p.at);
   if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
-  float lr[V], A[V], E[V], fa[kLen][V];
+  float lr[V], A[V], E[V];
+  Gates g[kLen][V];
   share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -486,10 +505,10 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const 
     float af[V];
     unpack<T, V>(ga.raw[l], af);
 #pragma unroll
-    for (int v = 0; v < V; ++v) fa[l][v] = decay_of(sigmoid(af[v]), lr[v]);
+    for (int v = 0; v < V; ++v) g[l][v].a = decay_of(sigmoid(af[v]), lr[v]);
   }
-  if (c.plain()) back_steps<true>(s, d, c, p, dh, fa, A, E);
-  else back_steps<false>(s, d, c, p, dh, fa, A, E);
+  if (c.plain()) back_steps<true>(s, d, c, p, dh, g, A, E);
+  else back_steps<false>(s, d, c, p, dh, g, A, E);
   maps.put(p.wave, A, E);
   __syncthreads();
   if (p.wave || !p.mine) return;
@@ -508,27 +527,24 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_map(const Scan s, const 
 }
 
 // Pass 2 of the backward: the states ahead of the wave's tokens again, then the gradients against the
-// scan order.
+// scan order.  The gates stay in registers between the two.
 template <bool PLAIN, typename T, int V>
 __device__ __forceinline__ void back_out(const Scan& s, const Grad& d, const Stretch& c, const Place& p, const Rows<T, V>& x,
-                                         const Rows<T, V>& ga, const Rows<T, V>& gx, const Rows<T, V>& dh, const float (&lr)[V],
-                                         const float (&fa)[kLen][V], const float (&before)[kLen][V], float (&E)[V],
+                                         const Rows<T, V>& dh, const float (&lr)[V], const Gates (&g)[kLen][V],
+                                         const float (&before)[kLen][V], float (&E)[V],
                                          float (&dlr)[V]) {
   using Raw = typename Pack<T, V>::Raw;
 #pragma unroll
   for (int l = kLen - 1; l >= 0; --l) {
-    float xf[V], af[V], gf[V], hf[V] = {}, ox[V], oa[V], og[V];
+    float xf[V], hf[V] = {}, ox[V], oa[V], og[V];
     unpack<T, V>(x.raw[l], xf);
-    unpack<T, V>(ga.raw[l], af);
-    unpack<T, V>(gx.raw[l], gf);
     if (d.dh) unpack<T, V>(dh.raw[l], hf);
     const bool finish = !PLAIN && ((c.finish >> l) & 1), live = PLAIN || ((c.live >> l) & 1);
     const int64_t b = PLAIN ? 0 : seq_at(c, l), n = p.n0 + l;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       if (finish) E[v] = d.dlast ? d.dlast[b * s.C + p.at + v] : 0.f;
-      const float a = fa[l][v], r = sigmoid(af[v]), z = sigmoid(gf[v]), la = lr[v] * r;
-      const float m = __builtin_amdgcn_sqrtf(one_minus_exp(2.f * la, a * a));
+      const float a = g[l][v].a, m = g[l][v].m, r = g[l][v].r, z = g[l][v].z, la = lr[v] * r;
       const float G = hf[v] + E[v], in = z * xf[v], gm = G * m;
       E[v] = a * G;
       ox[v] = gm * z;
@@ -553,10 +569,11 @@ __device__ __forceinline__ void back_out(const Scan& s, const Grad& d, const Str
   }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks,
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves, 6) void scan_bwd_out(const Scan s, const Grad d, int64_t chunks,
                                                                const float* __restrict__ carry,
                                                                const float* __restrict__ carry_e) {
+  constexpr int V = 1;
   __shared__ Maps<V> maps, back;
   __shared__ float sum[kWaves][64 * V];
   const Place p = place<V>(s);
@@ -566,7 +583,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, con
   gx.load(s.gx, s.gx_st, s, p.n0, p.at);
   if (d.dh) dh.load(d.dh, s.C, s, p.n0, p.at);
   const Stretch c = look(s, p.n0);
-  float lr[V], A[V], H[V], B[V], E[V], state[V], dlr[V] = {}, fa[kLen][V], fb[kLen][V];
+  float lr[V], A[V], H[V], B[V], E[V], state[V], dlr[V] = {}, fb[kLen][V];
+  Gates g[kLen][V];
   share_rates(s, p, lr);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -574,12 +592,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, con
     H[v] = E[v] = 0.f;
   }
   const bool plain = c.plain();
+  terms(x, ga, gx, lr, g, fb);
   if (plain) {
-    steps<true>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
-    back_steps<true>(s, d, c, p, dh, fa, B, E);
+    steps<true>(s, c, p, g, fb, A, H);
+    back_steps<true>(s, d, c, p, dh, g, B, E);
   } else {
-    steps<false>(s, c, p, x, ga, gx, lr, fa, fb, A, H);
-    back_steps<false>(s, d, c, p, dh, fa, B, E);
+    steps<false>(s, c, p, g, fb, A, H);
+    back_steps<false>(s, d, c, p, dh, g, B, E);
   }
   maps.put(p.wave, A, H);
   back.put(p.wave, B, E);
@@ -598,13 +617,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_bwd_out(const Scan s, con
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       if (begin) state[v] = s.state ? s.state[b * s.C + p.at + v] : 0.f;
-      const float now = live ? fmaf(fa[l][v], state[v], fb[l][v]) : 0.f;
+      const float now = live ? fmaf(g[l][v].a, state[v], fb[l][v]) : 0.f;
       fb[l][v] = state[v];
       state[v] = now;
     }
   }
-  if (plain) back_out<true>(s, d, c, p, x, ga, gx, dh, lr, fa, fb, E, dlr);
-  else back_out<false>(s, d, c, p, x, ga, gx, dh, lr, fa, fb, E, dlr);
+  if (plain) back_out<true>(s, d, c, p, x, dh, lr, g, fb, E, dlr);
+  else back_out<false>(s, d, c, p, x, dh, lr, g, fb, E, dlr);
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[p.wave][lane_id() * V + v] = dlr[v];
   __syncthreads();
@@ -645,7 +664,8 @@ __global__ __launch_bounds__(kCarryChannels * kRuns) void scan_bwd_decay(const f
   out[at] = x * ratio;
 }
 
-// One token of each of B streams.
+// One token of each of B streams, a thread for each lane's channels: 256 streams of 1024 channels in
+// bfloat16 4.4 us, as long as a launch whose loads wait for one another once.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict__ state_out, T* __restrict__ h) {
   const int64_t per = s.C / V, n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -669,7 +689,7 @@ __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict
 
 inline int64_t chunks_of(int64_t T) { return ceil_div(T, kChunk); }
 
-inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
+inline int scan_args(const geo_recurrence_t* g, Scan* s) {
   GEO_REQUIRE(g, "gated recurrence: null arguments");
   GEO_REQUIRE(g->dtype == GEO_F32 || g->dtype == GEO_BF16 || g->dtype == GEO_F16, "gated recurrence: dtype code %d",
               static_cast<int>(g->dtype));
@@ -678,14 +698,21 @@ inline int scan_args(const geo_recurrence_t* g, Scan* s, int* v) {
               static_cast<long long>(g->tokens), static_cast<long long>(g->channels), static_cast<long long>(g->sequences));
   *s = Scan{g->x, g->gate_a, g->gate_x, g->x_token, g->gate_a_token, g->gate_x_token, g->decay, g->ptr, g->state,
             g->tokens, g->channels, g->sequences, g->rate, g->reverse};
-  const int size = g->dtype == GEO_F32 ? 4 : 2;
-  auto even = [size](const void* p, int64_t st) { return reinterpret_cast<uintptr_t>(p) % (2 * size) == 0 && st % 2 == 0; };
-  // two 16-bit channels to a lane where every row begins on a multiple of 4 bytes
-  *v = size == 2 && g->channels % 2 == 0 && even(g->x, g->x_token) && even(g->gate_a, g->gate_a_token) &&
-               even(g->gate_x, g->gate_x_token) ? 2 : 1;
   GEO_REQUIRE(g->tokens == 0 || g->channels == 0 || (g->x && g->gate_a && g->gate_x && g->decay), "gated recurrence: null tensor");
-  GEO_REQUIRE(chunks_of(g->tokens) * ceil_div(g->channels, 64 * *v) < (int64_t(1) << 31), "gated recurrence: too many workgroups");
+  GEO_REQUIRE(chunks_of(g->tokens) * ceil_div(g->channels, 64) < (int64_t(1) << 31), "gated recurrence: too many workgroups");
   return GEO_OK;
+}
+
+// Two 16-bit channels to a lane, half the loads, where every row begins on a multiple of 4 bytes and
+// there are `least` elements.  Below that twice the waves are as good or better.  In bfloat16, us with
+// two | one: forward of 2048 x 64 17.2 | 12.1, 8192 x 256 23.0 | 21.1, 65,536 x 256 66.6 | 71.7,
+// 131,072 x 256 115.8 | 130.9, its backward's pass 1 34 | 46; step of 256 x 1024 4.8 | 4.2,
+// 1024 x 4096 21.8 | 23.5.  Pass 2 of the backward holds too many values for two.
+constexpr int64_t kPairsScan = int64_t(1) << 24, kPairsStep = int64_t(1) << 22;
+inline bool in_pairs(const geo_recurrence_t& g, int64_t least) {
+  auto even = [](const void* p, int64_t st) { return reinterpret_cast<uintptr_t>(p) % 4 == 0 && st % 2 == 0; };
+  return g.dtype != GEO_F32 && g.tokens * g.channels >= least && g.channels % 2 == 0 && even(g.x, g.x_token) &&
+         even(g.gate_a, g.gate_a_token) && even(g.gate_x, g.gate_x_token);
 }
 
 template <typename T, int V>
@@ -707,15 +734,15 @@ int forward(const Scan& s, void* h, float* last, float* carry, float2* map, hipS
 
 template <typename T, int V>
 int backward(const Scan& s, const Grad& d, const float* carry, float* carry_e, float2* map, float* ddecay, hipStream_t stream) {
-  const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64 * V);
-  const dim3 grid(static_cast<uint32_t>(chunks * blocks)), across(static_cast<uint32_t>(padded(s.C) / kCarryChannels));
+  const int64_t chunks = chunks_of(s.T), blocks = ceil_div(s.C, 64);
+  const dim3 across(static_cast<uint32_t>(padded(s.C) / kCarryChannels));
   if (chunks > 1) {
-    scan_bwd_map<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, map);
+    scan_bwd_map<T, V><<<dim3(static_cast<uint32_t>(chunks * ceil_div(s.C, 64 * V))), dim3(64 * kWaves), 0, stream>>>(s, d, chunks, map);
     GEO_LAUNCH_CHECK("scan_bwd_map");
     scan_carry<<<across, dim3(kCarryChannels * kRuns), 0, stream>>>(map, carry_e, chunks, 1);
     GEO_LAUNCH_CHECK("scan_carry");
   }
-  scan_bwd_out<T, V><<<grid, dim3(64 * kWaves), 0, stream>>>(s, d, chunks, carry, carry_e);
+  scan_bwd_out<T><<<dim3(static_cast<uint32_t>(chunks * blocks)), dim3(64 * kWaves), 0, stream>>>(s, d, chunks, carry, carry_e);
   GEO_LAUNCH_CHECK("scan_bwd_out");
   scan_bwd_decay<<<across, dim3(kCarryChannels * kRuns), 0, stream>>>(d.ddecay, chunks, s.C, s.decay, ddecay);
   GEO_LAUNCH_CHECK("scan_bwd_decay");
@@ -725,10 +752,10 @@ int backward(const Scan& s, const Grad& d, const float* carry, float* carry_e, f
 }  // namespace rec
 }  // namespace geo
 
-#define GEO_REC_CALL(F, ...)                                                                      \
-  (g->dtype == GEO_F32    ? geo::rec::F<float, 1>(__VA_ARGS__)                                    \
-   : g->dtype == GEO_BF16 ? (v == 2 ? geo::rec::F<__bf16, 2>(__VA_ARGS__) : geo::rec::F<__bf16, 1>(__VA_ARGS__)) \
-                          : (v == 2 ? geo::rec::F<_Float16, 2>(__VA_ARGS__) : geo::rec::F<_Float16, 1>(__VA_ARGS__)))
+#define GEO_REC_CALL(F, pairs, ...)                                                              \
+  (g->dtype == GEO_F32    ? geo::rec::F<float, 1>(__VA_ARGS__)                                   \
+   : g->dtype == GEO_BF16 ? (pairs ? geo::rec::F<__bf16, 2>(__VA_ARGS__) : geo::rec::F<__bf16, 1>(__VA_ARGS__)) \
+                          : (pairs ? geo::rec::F<_Float16, 2>(__VA_ARGS__) : geo::rec::F<_Float16, 1>(__VA_ARGS__)))
 
 extern "C" int64_t geo_recurrence_carry_size(int64_t tokens, int64_t channels) {
   return tokens < 1 || channels < 1 ? 0 : geo::rec::chunks_of(tokens) * geo::rec::padded(channels);
@@ -737,15 +764,16 @@ extern "C" int64_t geo_recurrence_carry_size(int64_t tokens, int64_t channels) {
 extern "C" int geo_recurrence_fwd(const geo_recurrence_t* g, void* h, float* last, float* carry, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   geo::rec::Scan s;
-  int v;
-  const int rc = geo::rec::scan_args(g, &s, &v);
+  const int rc = geo::rec::scan_args(g, &s);
   if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
   GEO_REQUIRE(h && last && carry, "gated recurrence: null output");
   const size_t need = static_cast<size_t>(geo_recurrence_carry_size(s.T, s.C)) * sizeof(float2);
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
-  return GEO_REC_CALL(forward, s, h, last, carry, static_cast<float2*>(workspace), geo::as_stream(stream));
+  // half a block of channels would leave half the lanes idle
+  const bool pairs = s.C % 128 == 0 && geo::rec::in_pairs(*g, geo::rec::kPairsScan) && reinterpret_cast<uintptr_t>(h) % 4 == 0;
+  return GEO_REC_CALL(forward, pairs, s, h, last, carry, static_cast<float2*>(workspace), geo::as_stream(stream));
 }
 
 extern "C" size_t geo_recurrence_bwd_workspace_bytes(int64_t tokens, int64_t channels) {
@@ -756,11 +784,9 @@ extern "C" int geo_recurrence_bwd(const geo_recurrence_t* g, const float* carry,
                                   void* dgate_a, void* dgate_x, float* ddecay, float* dstate, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   geo::rec::Scan s;
-  int v;
-  const int rc = geo::rec::scan_args(g, &s, &v);
+  const int rc = geo::rec::scan_args(g, &s);
   if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
   GEO_REQUIRE(carry && dx && dgate_a && dgate_x && ddecay, "gated recurrence backward: null tensor");
-  GEO_REQUIRE(v == 1 || reinterpret_cast<uintptr_t>(dh) % 4 == 0, "gated recurrence backward: dh must lie on a multiple of 4 bytes");
   const size_t need = geo_recurrence_bwd_workspace_bytes(s.T, s.C);
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "gated recurrence backward: workspace of %zu bytes, %zu needed",
@@ -768,7 +794,8 @@ extern "C" int geo_recurrence_bwd(const geo_recurrence_t* g, const float* carry,
   const int64_t n = geo_recurrence_carry_size(s.T, s.C);
   float* w = static_cast<float*>(workspace);  // maps, states, sums
   const geo::rec::Grad d{dh, dlast, dx, dgate_a, dgate_x, dstate, w + 3 * n};
-  return GEO_REC_CALL(backward, s, d, carry, w + 2 * n, reinterpret_cast<float2*>(w), ddecay, geo::as_stream(stream));
+  const bool pairs = s.C % 128 == 0 && geo::rec::in_pairs(*g, geo::rec::kPairsScan) && reinterpret_cast<uintptr_t>(dh) % 4 == 0;
+  return GEO_REC_CALL(backward, pairs, s, d, carry, w + 2 * n, reinterpret_cast<float2*>(w), ddecay, geo::as_stream(stream));
 }
 
 namespace geo {
@@ -786,11 +813,11 @@ int step(const Scan& s, float* state_out, void* h, hipStream_t stream) {
 
 extern "C" int geo_recurrence_step(const geo_recurrence_t* g, float* state_out, void* h, void* stream) {
   geo::rec::Scan s;
-  int v;
-  const int rc = geo::rec::scan_args(g, &s, &v);
+  const int rc = geo::rec::scan_args(g, &s);
   if (rc != GEO_OK || s.T == 0 || s.C == 0) return rc;
   GEO_REQUIRE(g->sequences == g->tokens, "gated recurrence step: one token for each of %lld streams, got %lld",
               static_cast<long long>(g->sequences), static_cast<long long>(g->tokens));
   GEO_REQUIRE(s.state && state_out && h, "gated recurrence step: null tensor");
-  return GEO_REC_CALL(step, s, state_out, h, geo::as_stream(stream));
+  const bool pairs = geo::rec::in_pairs(*g, geo::rec::kPairsStep) && reinterpret_cast<uintptr_t>(h) % 4 == 0;
+  return GEO_REC_CALL(step, pairs, s, state_out, h, geo::as_stream(stream));
 }

@@ -71,7 +71,8 @@ __device__ __forceinline__ float group_sum(float x) {
 // takes kAhead keys at a time, their reads in flight together, and keeps its own running maximum, sum
 // and output, which are joined through LDS at the end.  Partial results of the pieces go to the
 // workspace.  The work is the reading of the cache: 256 streams, 4112 slots, 16 (4) heads of 128 in
-// bfloat16 712 us with one key at a time and its lane sums through LDS.
+// bfloat16 409-415 us, 4.55 TB/s with the join (a large copy: 5.19); 712 us with one key at a time and
+// its lane sums through LDS.
 template <typename T, int LW, int GB>
 __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pieces, float* __restrict__ part,
                                                            T* __restrict__ out) {
