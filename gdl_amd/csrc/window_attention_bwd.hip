@@ -49,7 +49,7 @@ __device__ __forceinline__ float sum_by_distance(const f32x16& x) {
 // each wave into its own places; sub-tiles with no distance inside the ends go to two registers.  The
 // workgroup's sums leave by bucket.
 //
-// 32,768 tokens, 8 (2) heads of 128 in bfloat16, window 2047 back: 525 us, 805 TFLOP/s of its three
+// 32,768 tokens, 8 (2) heads of 128 in bfloat16, window 2047 back: 525 us, 767 TFLOP/s of its three
 // products; matrix instructions 41% of a SIMD's cycles, vector instructions 34%.  With the bias, 65,536
 // tokens, 8 heads of 32, window 128 to both sides: 140 us, vector instructions.
 template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
@@ -285,7 +285,7 @@ constexpr bool kv_lds() { return DP >= 96; }
 // in a lane's registers, where dV^T = G^T P and dK^T = Q^T dS take them as operands; the sums over
 // heads and queries stay in registers.
 //
-// 32,768 tokens, 8 (2) heads of 128 in bfloat16, window 2047 back: 1030 us, 547 TFLOP/s of its four
+// 32,768 tokens, 8 (2) heads of 128 in bfloat16, window 2047 back: 1030 us, 521 TFLOP/s of its four
 // products.  With one wave a SIMD, LDS reads, matrix (25% of the cycles) and vector instructions (21%)
 // follow one another.  65,536 tokens, 8 (2) heads of 64, window 255 back, two waves a SIMD: 140 us.
 template <typename T, int DP, int NW, int BN, bool BIAS, bool PART, int WAVES>
