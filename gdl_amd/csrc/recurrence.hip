@@ -10,7 +10,7 @@
 // composed over the waves in LDS and over the chunks by scan_carry.  Pass 1 forms the chunks' maps,
 // pass 2 the outputs from the states that the chunks begin with.  All in float32, whatever the inputs.
 //
-// The inputs are read twice in each direction, and still vector instructions bound the passes: 89 to 95%
+// The inputs are read twice in each direction, and still vector instructions bound the passes: 79 to 94%
 // of a SIMD's cycles, for two sigmoids, a decay, a root and 1 - a^2 of every element.  131,072 tokens of
 // 256 channels in bfloat16: pass 1 60 us, carry 9, pass 2 62; backward 34, 9 and 121, decay's sums 4.
 #include "common.hpp"
