@@ -406,7 +406,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void scan_out(const Scan s, int64_t
   }
   if (chunks <= kFew) {
     if (chunks > 1) state_from_maps(maps, map, p, chunks, state);
-    if (carry && p.wave == 0 && p.mine)
+    if (p.wave == 0 && p.mine)
 #pragma unroll
       for (int v = 0; v < V; ++v) carry[chunk_place(p.chunk, chunks, p.at + v)] = state[v];
   }
