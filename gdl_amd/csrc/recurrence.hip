@@ -38,11 +38,17 @@ __device__ __forceinline__ void unpack(typename Pack<T, V>::Raw r, float (&f)[V]
 #pragma unroll
   for (int v = 0; v < V; ++v) f[v] = static_cast<float>(u.t[v]);
 }
+// Each value's float32 rounded.  (The product and sum that formed it would else be rounded to float16 at
+// once in one instruction, here and there, and an output then not be its state's rounding.)
 template <typename T, int V>
 __device__ __forceinline__ typename Pack<T, V>::Raw pack(const float (&f)[V]) {
   union { typename Pack<T, V>::Raw r; T t[V]; } u;
 #pragma unroll
-  for (int v = 0; v < V; ++v) u.t[v] = static_cast<T>(f[v]);
+  for (int v = 0; v < V; ++v) {
+    float x = f[v];
+    asm("" : "+v"(x));
+    u.t[v] = static_cast<T>(x);
+  }
   return u.r;
 }
 
