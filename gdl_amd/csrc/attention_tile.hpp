@@ -189,6 +189,12 @@ struct Tile {
   }
 };
 
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x)));
+}
+
 // x where bit n of `word` is set, else `other`: two instructions, with no condition mask.
 __device__ __forceinline__ float keep_bit(float x, uint32_t word, int n, float other) {
   const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(word, n, 1));

@@ -166,6 +166,10 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
       vis &= rows;
       if (__ballot(vis != 0) == 0) continue;
     }
+    // The scores below take infinities and NaN of K for zeros.  A query with a number as its log-sum
+    // can see such a key only at a score of -inf, with the weight 0 (any other leaves NaN there).
+    const uint64_t odd = uniform(wild[t & 1]);
+    const uint64_t weighed = odd && ls == ls ? vis & ~odd : vis;
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
@@ -183,7 +187,8 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
         const int kk = 8 * (r >> 2) + (r & 3);
         s[r] = exp2_hw(BIAS ? fmaf(s[r], scale2, bias[kk]) - ls : fmaf(s[r], scale2, -ls)) * (dp[r] - dl);
       }
-      if (!whole) {
+      if (!whole || odd) {
+        word = static_cast<uint32_t>(weighed >> (32 * u + 4 * half));
         stay_branch(word);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -212,7 +217,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
       }
       if (sizeof(T) == 2) reads_ahead<2 * kMt, 4 < 2 * kMt ? 4 : 2 * kMt, 2>();
     }
-    if (wild[t & 1]) add_wild<T, kMt, true>(kbase, a.k_st, j0, wild[t & 1], vis, a.D, o);
+    if (odd) add_wild<T, kMt, true>(kbase, a.k_st, j0, odd, vis, a.D, o);
   }
   if (real) store_row<T>(dq + (static_cast<int64_t>(i) * a.Hq + h) * a.D, o, a.scale, a.D);
   if (BIAS) {
