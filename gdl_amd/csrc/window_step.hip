@@ -89,7 +89,9 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
   const int64_t b = w / a.Hk;
   const int64_t p = a.pos[b];
   const int lane = threadIdx.x % LW, kg = threadIdx.x / LW, d = 8 * lane;
-  const bool wide = d < a.D;
+  // lanes past the head size repeat its first values, which count as zeros on both sides: an infinity
+  // times a query's zero would be NaN
+  const bool wide = d < a.D, idle = a.D < kDp;
   const int heads = min(GB, group - gc * GB), h0 = hk * group + gc * GB;
 
   T* const kc = static_cast<T*>(a.kc) + b * a.kc_b + hk * a.kc_h;
@@ -143,6 +145,7 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
         kx[n].store(kc + static_cast<int64_t>(at) * a.D + d);
         vx[n].store(vc + static_cast<int64_t>(at) * a.D + d);
       }
+      if (idle && !wide) kx[n] = Eight<T>{};
       const float* bias = nullptr;
       if (a.bias.table) {
         // how far back the slot's token lies (at most maxd): the ring is read backwards from `now`
