@@ -56,6 +56,7 @@ template <> struct Type<float> {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kMost = 0x1.fffffep127f;  // the largest finite float32
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -367,9 +368,15 @@ struct Bias {
   const int32_t* lut;  // [2 maxd + 1]: bucket of each distance
   int dtype, buckets, maxd;
 };
+// An element of the table times log2 e.  A finite one stays finite: where the type's lowest value is all
+// that a query's keys have, the factor would leave it keys of the weight exp(-inf) alone.
+__device__ __forceinline__ float bias_value(const Bias& b, int64_t at) {
+  const float x = table_value(b.table, b.dtype, at), y = x * kLog2e;
+  return fabsf(x) < kInf ? fminf(fmaxf(y, -kMost), kMost) : y;
+}
 __device__ __forceinline__ void stage_bias(const Bias& b, int Hq, int h, float* lds) {
   for (int x = threadIdx.x; x <= 2 * b.maxd; x += blockDim.x)
-    lds[x] = table_value(b.table, b.dtype, static_cast<int64_t>(b.lut[x]) * Hq + h) * kLog2e;
+    lds[x] = bias_value(b, static_cast<int64_t>(b.lut[x]) * Hq + h);
 }
 
 }  // namespace attn

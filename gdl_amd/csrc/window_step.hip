@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
       const int64_t row = static_cast<int64_t>(a.bias.lut[a.bias.maxd - x]) * a.Hq + h0;
 #pragma unroll
       for (int g = 0; g < GB; ++g)
-        sbias[g * (a.bias.maxd + 1) + x] = table_value(a.bias.table, a.bias.dtype, row + min(g, heads - 1)) * kLog2e;
+        sbias[g * (a.bias.maxd + 1) + x] = bias_value(a.bias, row + min(g, heads - 1));
     }
     __syncthreads();
   }
