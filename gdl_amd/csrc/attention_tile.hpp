@@ -58,6 +58,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kMost = 0x1.fffffep127f;  // the largest finite float32
 
+// Log-sums above this are rounded by more than 2^-12, from 10^8 on they keep nothing of a sum of several weights.
+// Biases that a query's keys share bring that about (scores as large leave it one key, and are rounded as much
+// themselves), so with a bias the forward keeps the factor that such a row's exp2(score - log-sum) lack.
+constexpr float kFarSum = 4096.f;
+__device__ __forceinline__ bool far_sum(float lse) { return fabsf(lse) > kFarSum && lse < kInf; }
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The value of the same column in the wave's other half combined with this lane's.
@@ -154,6 +160,19 @@ struct Tile {
         atomicOr(wild, 1ull << ((threadIdx.x + n * NT) / kChunks));
         *place(lds, n) = v.u;
       }
+    }
+  }
+  // The stored pieces of this thread times by(row).
+  template <typename By>
+  static __device__ __forceinline__ void scale_rows(T* lds, By by) {
+#pragma unroll 1
+    for (int n = 0; n < kLoads; ++n) {
+      const float x = by((threadIdx.x + n * NT) / kChunks);
+      union { uint4 u; T t[kPer]; } v;
+      v.u = *place(lds, n);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v.t[e] = static_cast<T>(static_cast<float>(v.t[e]) * x);
+      *place(lds, n) = v.u;
     }
   }
   // Operand with this lane's row `row0 + lane % 32` (row0 a multiple of 32), k = 16 kc + 8 half + 0..7

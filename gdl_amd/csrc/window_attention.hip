@@ -181,7 +181,12 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
     store_row<T>(out + row, o, inv, a.D);
     if (sizeof(T) == 2 && rest) store_row<T, kMt, true>(rest + row, o, inv, a.D);
     // +inf where no key is seen: the backward's exp2(s - lse) is 0 there
-    if (lse && half == 0) lse[static_cast<int64_t>(h) * a.seq.T + i] = l == 0.f ? kInf : m + log2f(l);
+    if (lse && half == 0) {
+      const int64_t at = static_cast<int64_t>(h) * a.seq.T + i;
+      const float sum = log2f(l), x = m + sum;
+      lse[at] = l == 0.f ? kInf : x;
+      if (BIAS && far_sum(x)) lse[static_cast<int64_t>(a.Hq) * a.seq.T + at] = exp2_hw(x - m - sum);
+    }
   }
 }
 

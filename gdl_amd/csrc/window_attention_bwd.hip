@@ -120,6 +120,14 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
     if (real && half == 0) delta[static_cast<int64_t>(h) * a.seq.T + i] = dl;
   }
   const float ls = real ? lse[static_cast<int64_t>(h) * a.seq.T + i] : kInf;
+  if (BIAS && far_sum(ls)) {  // the factor of the row's weights, as one of what they are multiplied with
+    const float norm = lse[static_cast<int64_t>(a.Hq + h) * a.seq.T + i];
+    dl *= norm;
+#pragma unroll
+    for (int kc = 0; kc < kKc; ++kc)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gf[kc][j] = static_cast<T>(static_cast<float>(gf[kc][j]) * norm);
+  }
   f32x16 o[kMt] = {};
   float below = 0.f, above = 0.f;
   const float scale2 = a.scale * kLog2e;
@@ -169,7 +177,6 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
     // The scores below take infinities and NaN of K for zeros.  A query with a number as its log-sum
     // can see such a key only at a score of -inf, with the weight 0 (any other leaves NaN there).
     const uint64_t odd = uniform(wild[t & 1]);
-    const uint64_t weighed = odd && ls == ls ? vis & ~odd : vis;
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       uint32_t word = static_cast<uint32_t>(vis >> (32 * u + 4 * half));
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
         s[r] = exp2_hw(BIAS ? fmaf(s[r], scale2, bias[kk]) - ls : fmaf(s[r], scale2, -ls)) * (dp[r] - dl);
       }
       if (!whole || odd) {
-        word = static_cast<uint32_t>(weighed >> (32 * u + 4 * half));
+        if (odd && ls == ls) word = static_cast<uint32_t>((vis & ~odd) >> (32 * u + 4 * half));
         stay_branch(word);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -312,7 +319,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_kv(const Attend a, 
   float* const base = near + (BIAS ? kBk + BN : 0);
   __shared__ int sptr[kStagedPtr];
   __shared__ unsigned long long wildq[2], wildg[2];
-  __shared__ int last;
+  __shared__ int last, far[2];  // far: a row of the tile has a far_sum
 
   const int group = a.Hq / a.Hk;
   const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -334,6 +341,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_kv(const Attend a, 
 
   stage_ptr(a.seq, sptr);
   if (threadIdx.x < 2) wildq[threadIdx.x] = wildg[threadIdx.x] = 0;
+  if (BIAS && threadIdx.x < 2) far[threadIdx.x] = 0;
   if (threadIdx.x == 0) last = -1;
   __syncthreads();
 
@@ -414,15 +422,25 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_kv(const Attend a, 
     const int now = it, head = h;
     const uint64_t rows = bit_range(0, min(ilast + 1 - now, BN) - 1);
     if (BIAS && now == i0) stage_bias(a.bias, a.Hq, head, base);
+    if (BIAS && threadIdx.x < BN && far_sum(row_value)) far[t & 1] = 1;
     __syncthreads();
+    const int any_far = BIAS ? far[t & 1] : 0;
     qt.store_finite(qs, &wildq[t & 1]);
     gt.store_finite(gs, &wildg[t & 1]);
     if (threadIdx.x < 2 * BN) rowl[threadIdx.x] = row_value;
     if (threadIdx.x == 0) wildq[(t + 1) & 1] = wildg[(t + 1) & 1] = 0;
-    if (BIAS)
+    if (BIAS) {
+      if (threadIdx.x == 0) far[(t + 1) & 1] = 0;
       for (int x = threadIdx.x; x < kBk + BN - 1; x += 64 * NW)
         near[x] = base[min(max(key0 - now + x - (BN - 1), -a.bias.maxd), a.bias.maxd) + a.bias.maxd];
+    }
     __syncthreads();
+    if (BIAS && __builtin_amdgcn_readfirstlane(any_far)) {  // the rows' factors, as in attend_bwd_q
+      const float* norm = lse + static_cast<int64_t>(a.Hq + head) * a.seq.T;
+      gt.scale_rows(gs, [&](int n) { return far_sum(rowl[n]) ? norm[min(now + n, ilast)] : 1.f; });
+      if (threadIdx.x < BN && far_sum(rowl[threadIdx.x])) rowd[threadIdx.x] *= norm[min(now + static_cast<int>(threadIdx.x), ilast)];
+      __syncthreads();
+    }
     it += BN;
     if (it > ilast) {
       it = i0;
@@ -612,7 +630,7 @@ constexpr int q_waves() {
 }
 template <typename T, int DP, int NW>
 constexpr int kv_waves() {
-  return NW == 1 ? 1 : sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 3 : DP <= 64 ? 2 : 1;
+  return NW == 1 ? 1 : sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 32 ? 3 : DP <= 96 ? 2 : 1;
 }
 // Rows of a tile: 64, or 32 where the next tile's would not find registers.
 template <int DP>
