@@ -70,6 +70,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
   }
   f32x16 o[kMt] = {};
   float m = -kInf, l = 0.f;
+  uint64_t looked = 0;  // lanes whose query has seen a key
   // positive, so that the products' maximum is the scores': the queries carry its sign, or are zeros
   const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
 
@@ -113,7 +114,11 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
       vis = bit_range(lo - j0, hi - j0);
       if (a.sinks) vis |= bit_range(first - j0, far - j0);
       vis &= rows;
-      if (__ballot(vis != 0) == 0) continue;
+      const uint64_t any = __ballot(vis != 0);
+      if (any == 0) continue;
+      looked |= any;
+    } else {
+      looked = ~0ull;
     }
     f32x16 s[kSub];
 #pragma unroll
@@ -177,6 +182,8 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
   l = halves_sum(l);
   if (real) {
     const int64_t row = (static_cast<int64_t>(i) * a.Hq + h) * a.D;
+    // keys are seen, but with scores of -inf alone: 0 / 0
+    if (l == 0.f && (looked >> lane) & 1) l = __builtin_nanf("");
     const float inv = l == 0.f ? 0.f : 1.f / l;
     store_row<T>(out + row, o, inv, a.D);
     if (sizeof(T) == 2 && rest) store_row<T, kMt, true>(rest + row, o, inv, a.D);

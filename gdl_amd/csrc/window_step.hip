@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
       y += so[n][g][e] * keep;
     }
     if (pieces == 1) {
-      if (e < a.D) out[(b * a.Hq + h0 + g) * a.D + e] = static_cast<T>(sum == 0.f ? 0.f : y / sum);
+      if (e < a.D) out[(b * a.Hq + h0 + g) * a.D + e] = static_cast<T>(used == 0 ? 0.f : y / sum);
     } else {
       float* row = part + ((b * a.Hq + h0 + g) * pieces + piece) * (kDp + 2);
       row[2 + e] = y;
@@ -234,7 +234,8 @@ __global__ __launch_bounds__(kStepThreads) void step_piece(const Step a, int pie
 }
 
 template <typename T, int LW>
-__global__ __launch_bounds__(8 * LW) void step_join(int D, int pieces, const float* __restrict__ part, T* __restrict__ out) {
+__global__ __launch_bounds__(8 * LW) void step_join(int D, int Hq, int pieces, const int64_t* __restrict__ pos,
+                                                    const float* __restrict__ part, T* __restrict__ out) {
   constexpr int kDp = 8 * LW;
   const float* row = part + static_cast<int64_t>(blockIdx.x) * pieces * (kDp + 2);
   const int e = threadIdx.x;
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(8 * LW) void step_join(int D, int pieces, const flo
     sum += row[n * (kDp + 2) + 1] * keep;
     y += row[n * (kDp + 2) + 2 + e] * keep;
   }
-  if (e < D) out[static_cast<int64_t>(blockIdx.x) * D + e] = static_cast<T>(sum == 0.f ? 0.f : y / sum);
+  if (e < D) out[static_cast<int64_t>(blockIdx.x) * D + e] = static_cast<T>(pos[blockIdx.x / Hq] < 0 ? 0.f : y / sum);
 }
 
 // Tokens into caches: one thread per 16 bytes of a token's and head's row, k and v.
@@ -303,7 +304,7 @@ int launch_step(const Step& a, void* out, float* part, hipStream_t stream) {
   step_piece<T, LW, GB><<<dim3(static_cast<uint32_t>(rows * pieces)), dim3(kStepThreads), lds, stream>>>(a, pieces, part, static_cast<T*>(out));
   GEO_LAUNCH_CHECK("step_piece");
   if (pieces > 1) {
-    step_join<T, LW><<<dim3(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.Hq)), dim3(8 * LW), 0, stream>>>(a.D, pieces, part, static_cast<T*>(out));
+    step_join<T, LW><<<dim3(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.Hq)), dim3(8 * LW), 0, stream>>>(a.D, a.Hq, pieces, a.pos, part, static_cast<T*>(out));
     GEO_LAUNCH_CHECK("step_join");
   }
   return GEO_OK;

@@ -94,7 +94,8 @@ def window_attention(
         scale: of the scores; ``D ** -0.5`` by default.
 
     Returns:
-        [T, H, D] of q's type; 0 for a token that sees no key.
+        [T, H, D] of q's type; 0 for a token that sees no key, NaN for one that sees keys with scores
+        of -inf alone.
     """
     left, right = window if isinstance(window, (tuple, list)) else (window, window)
     left, right = _reach("left", left), _reach("right", right)

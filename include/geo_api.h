@@ -621,7 +621,7 @@ int geo_radial_mlp_bwd(const float* dist, int64_t E, const float* freqs, int32_t
  * of the sequence's first `sinks` tokens, and mask[j] (if given).  Query head h reads key head
  * h / (heads / kv_heads).  Scores are scale * q.k, plus, with a bias,
  * bias[bias_lut[clamp(j - i, -max_distance, max_distance) + max_distance], h].  A query that sees
- * nothing gives 0.  Values of keys that a query does not see have no effect on it, infinities and
+ * nothing gives 0, one that sees keys with scores of -inf alone NaN.  Values of keys that a query does not see have no effect on it, infinities and
  * NaN included; keys whose mask is 0 are not looked at.  Tokens that lie in no sequence see nothing.
  */
 typedef struct {
