@@ -239,18 +239,40 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+_Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
+_interpreter = torch._C._functorch.peek_interpreter_stack
+_legacy_batched = torch._C._functorch.is_legacy_batchedtensor
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_tracing = torch._C._get_tracing_state
+_compiling, _forward_ad = torch.compiler.is_compiling, torch.autograd.forward_ad
+
+
 def plain_eager(x: torch.Tensor) -> bool:
     """True for a plain tensor in ordinary eager execution: an op may call its implementation
     directly.  Tensor subclasses, torch.compile, jit tracing, function transforms (torch.func),
     forward-mode differentiation, batched gradients and dispatch or function modes take the
     registered custom op, which all of them can see."""
-    return (type(x) is torch.Tensor and not torch.compiler.is_compiling()
-            and torch._C._functorch.peek_interpreter_stack() is None
-            and not torch._C._functorch.is_legacy_batchedtensor(x)
-            and torch._C._len_torch_dispatch_stack() == 0
-            and torch._C._len_torch_function_stack() == 0
-            and torch.autograd.forward_ad._current_level < 0
-            and torch._C._get_tracing_state() is None)
+    return (type(x) is _Tensor and not _compiling() and _interpreter() is None and not _legacy_batched(x)
+            and _dispatch_modes() == 0 and _function_modes() == 0 and _forward_ad._current_level < 0
+            and _tracing() is None)
+
+
+def plain_call(x: torch.Tensor, *rest: torch.Tensor | None) -> bool:
+    """plain_eager for an op of several tensors, of which some are parameters and some may be absent."""
+    for t in rest:
+        kind = type(t)
+        if kind is not _Tensor and t is not None and kind is not _Parameter:
+            return False
+    return plain_eager(x)
+
+
+def no_tangents(name: str, *tensors: torch.Tensor | None) -> None:
+    """Raises in forward-mode differentiation of one of the tensors: a custom op would drop its tangent
+    without a word."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name}: no forward-mode derivative")
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

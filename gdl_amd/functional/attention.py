@@ -32,27 +32,112 @@ from gdl_amd.csrc import (
     window_attention_step_hip,
     window_cache_fill_hip,
 )
-from gdl_amd.functional.relative_bias import bucket_plan
+from gdl_amd.functional.relative_bias import bucket_plan, check_buckets
 
 _UNBOUNDED = 1 << 40
 
 
+def _plan(bias: Optional[Tensor], max_distance: int, two_sided: bool):
+    """(bucket of each distance, spans, max_distance) of a bias table on its device, None without one."""
+    if bias is None:
+        return None
+    return bucket_plan(bias.shape[0], max_distance, two_sided, bias.device) + (max_distance,)
+
+
+# ═══════════════════════════════════════════════════════════════════
+# Custom ops: what everything but plain eager execution uses (_native.plain_eager)
+# ═══════════════════════════════════════════════════════════════════
+
+
+@torch.library.custom_op("geoembodied::window_attention", mutates_args=())
+def _attention_op(q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], ptr: Optional[Tensor], mask: Optional[Tensor],
+                  left: int, right: int, sinks: int, max_distance: int, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    out, rest, lse = window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias,
+                                                  _plan(bias, max_distance, right != 0), True)
+    return out, out.new_empty(0) if rest is None else rest, lse
+
+
+@_attention_op.register_fake
+def _(q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
+    rest = q.new_empty(0) if q.dtype is torch.float32 else q.new_empty(q.shape)
+    return q.new_empty(q.shape), rest, q.new_empty((2, q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op("geoembodied::window_attention_backward", mutates_args=())
+def _attention_backward_op(grad: Tensor, out: Tensor, rest: Tensor, lse: Tensor, q: Tensor, k: Tensor, v: Tensor,
+                           bias: Optional[Tensor], ptr: Optional[Tensor], mask: Optional[Tensor], left: int, right: int,
+                           sinks: int, max_distance: int, scale: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    dq, dk, dv, dbias = window_attention_backward_hip(
+        grad, out, rest if rest.numel() else None, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias,
+        _plan(bias, max_distance, right != 0))
+    return dq, dk, dv, lse.new_empty(0) if dbias is None else dbias
+
+
+@_attention_backward_op.register_fake
+def _(grad, out, rest, lse, q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+            lse.new_empty(0) if bias is None else bias.new_empty(bias.shape))
+
+
+def _attention_setup(ctx, inputs, output) -> None:
+    q, k, v, bias, ptr, mask, *ctx.sizes = inputs
+    ctx.save_for_backward(q, k, v, bias, *output, ptr, mask)
+
+
+def _attention_grads(ctx, grad, grad_rest, grad_lse):
+    q, k, v, bias, out, rest, lse, ptr, mask = ctx.saved_tensors
+    _nat.no_tangents("window_attention backward", grad, q, k, v, bias)
+    *grads, dbias = torch.ops.geoembodied.window_attention_backward(
+        grad, out, out.new_empty(0) if rest is None else rest, lse, q, k, v, bias, ptr, mask, *ctx.sizes)
+    return (*grads, None if bias is None else dbias, None, None, None, None, None, None, None)
+
+
+_attention_op.register_autograd(_attention_grads, setup_context=_attention_setup)
+
+
+@torch.library.custom_op("geoembodied::window_attention_step", mutates_args=("k_cache", "v_cache"))
+def _step_op(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, positions: Tensor, bias: Optional[Tensor],
+             sinks: int, max_distance: int, scale: float) -> Tensor:
+    return window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale, bias,
+                                     _plan(bias, max_distance, False), lambda n: _nat.workspace(n, q.device) if n else None)
+
+
+@_step_op.register_fake
+def _(q, k, v, k_cache, v_cache, positions, bias, sinks, max_distance, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("geoembodied::window_cache_fill", mutates_args=("k_cache", "v_cache"))
+def _fill_op(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, sinks: int, ptr: Optional[Tensor],
+             start: Optional[Tensor]) -> None:
+    window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start)
+
+
+@_fill_op.register_fake
+def _(k, v, k_cache, v_cache, sinks, ptr, start):
+    return None
+
+
 class _WindowAttention(torch.autograd.Function):
+    """Eager mode: the op's kernels called directly, without the custom-op layers."""
+
     @staticmethod
-    def forward(ctx, q, k, v, bias, plan, ptr, mask, left, right, sinks, scale):
+    def forward(ctx, q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
+        plan = _plan(bias, max_distance, right != 0)
         out, rest, lse = window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, True)
         ctx.save_for_backward(q, k, v, bias, out, rest, lse, ptr, mask)
-        ctx.rest = (plan, left, right, sinks, scale)
+        ctx.sizes, ctx.plan = (left, right, sinks, max_distance, scale), plan
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        if not _nat.plain_eager(grad):
+            return _attention_grads(ctx, grad, None, None)
         q, k, v, bias, out, rest, lse, ptr, mask = ctx.saved_tensors
-        plan, left, right, sinks, scale = ctx.rest
-        dq, dk, dv, dbias = window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr,
-                                                          mask, bias, plan)
-        return dq, dk, dv, dbias, None, None, None, None, None, None, None
+        left, right, sinks, _, scale = ctx.sizes
+        grads = window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, ctx.plan)
+        return (*grads, None, None, None, None, None, None, None)
 
 
 def _reach(name: str, n: Optional[int]) -> int:
@@ -105,19 +190,23 @@ def window_attention(
     d = q.shape[2]
     if not 1 <= d <= 128:
         raise ValueError(f"window_attention: head size {d} (from 1 to 128)")
-    plan = None
-    if bias is not None:
-        if bias.dim() != 2 or bias.shape[1] != q.shape[1]:
-            raise ValueError(f"window_attention: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
-        plan = bucket_plan(bias.shape[0], int(max_distance), right != 0, q.device) + (int(max_distance),)
+    if bias is not None and (bias.dim() != 2 or bias.shape[1] != q.shape[1]):
+        raise ValueError(f"window_attention: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if d % 8:  # rows are read in pieces of 8 values: zeros beyond D change no score and no gradient
         q, k, v = (torch.nn.functional.pad(x, (0, 8 - d % 8)) for x in (q, k, v))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
-        out = _WindowAttention.apply(q, k, v, bias, plan, ptr, mask, left, right, int(sinks), scale)
+    sizes = left, right, int(sinks), int(max_distance), scale
+    if not _nat.plain_call(q, k, v, bias, ptr, mask):
+        _nat.no_tangents("window_attention", q, k, v, bias)
+        if bias is not None:
+            check_buckets(bias.shape[0], sizes[3], right != 0)
+        out, _, _ = torch.ops.geoembodied.window_attention(q, k, v, bias, ptr, mask, *sizes)
+    elif torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                      or (bias is not None and bias.requires_grad)):
+        out = _WindowAttention.apply(q, k, v, bias, ptr, mask, *sizes)
     else:
-        out, _, _ = window_attention_forward_hip(q, k, v, left, right, int(sinks), scale, ptr, mask, bias, plan, False)
+        out, _, _ = window_attention_forward_hip(q, k, v, left, right, sizes[2], scale, ptr, mask, bias,
+                                                 _plan(bias, sizes[3], right != 0), False)
     return out[..., :d] if d % 8 else out
 
 
@@ -139,8 +228,8 @@ class WindowCache:
             raise ValueError(f"WindowCache: head size {k.shape[3]} (a multiple of 8 up to 128)")
         for t in (k, v):
             size = t.element_size()
-            if t.stride(3) != 1 or t.stride(2) != t.shape[3] or any(x % 16 for x in (
-                    t.data_ptr(), t.stride(0) * size, t.stride(1) * size)):
+            at = t.data_ptr() if _nat.plain_eager(t) else 0  # traced: looked at when the program runs
+            if t.stride(3) != 1 or t.stride(2) != t.shape[3] or any(x % 16 for x in (at, t.stride(0) * size, t.stride(1) * size)):
                 raise ValueError("WindowCache: a head's slots must adjoin, on multiples of 16 bytes")
         self.k, self.v, self.sinks = k, v, int(sinks)
         self.left = k.shape[2] - self.sinks - 1
@@ -165,7 +254,11 @@ class WindowCache:
             raise ValueError(f"WindowCache.fill: ptr [{batch + 1}] of {batch} streams")
         if start is not None and start.shape != (batch,):
             raise ValueError(f"WindowCache.fill: start [{batch}], got {tuple(start.shape)}")
-        window_cache_fill_hip(k, v, self.k, self.v, self.sinks, ptr, start)
+        if _nat.plain_call(k, v, self.k, self.v, ptr, start):
+            window_cache_fill_hip(k, v, self.k, self.v, self.sinks, ptr, start)
+        else:
+            _nat.no_tangents("WindowCache.fill", k, v)
+            torch.ops.geoembodied.window_cache_fill(k, v, self.k, self.v, self.sinks, ptr, start)
 
     def _workspace(self, nbytes: int) -> Optional[Tensor]:
         if nbytes and (self._scratch is None or self._scratch.numel() < nbytes):
@@ -199,13 +292,17 @@ def window_attention_step(
         raise ValueError(f"window_attention_step: {q.shape[1]} heads are no multiple of {hk} key heads")
     if positions.shape != (batch,) or positions.dtype.is_floating_point:
         raise ValueError(f"window_attention_step: positions int64 [{batch}], got {positions.dtype} {tuple(positions.shape)}")
-    plan = None
-    if bias is not None:
-        if bias.dim() != 2 or bias.shape[1] != q.shape[1]:
-            raise ValueError(f"window_attention_step: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
-        plan = bucket_plan(bias.shape[0], int(max_distance), False, q.device) + (int(max_distance),)
+    if bias is not None and (bias.dim() != 2 or bias.shape[1] != q.shape[1]):
+        raise ValueError(f"window_attention_step: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias is not None and bias.requires_grad)):
         raise RuntimeError("window_attention_step has no backward: call it under torch.no_grad()")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    return window_attention_step_hip(q, k, v, cache.k, cache.v, cache.sinks, positions, scale, bias, plan, cache._workspace)
+    if _nat.plain_call(q, k, v, cache.k, cache.v, positions, bias):
+        return window_attention_step_hip(q, k, v, cache.k, cache.v, cache.sinks, positions, scale, bias,
+                                         _plan(bias, int(max_distance), False), cache._workspace)
+    _nat.no_tangents("window_attention_step", q, k, v, bias)
+    if bias is not None:
+        check_buckets(bias.shape[0], int(max_distance), False)
+    return torch.ops.geoembodied.window_attention_step(q, k, v, cache.k, cache.v, positions, bias, cache.sinks,
+                                                       int(max_distance), scale)

@@ -21,6 +21,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
+from gdl_amd import _native as _nat
 from gdl_amd.csrc import (
     gated_recurrence_backward_hip,
     gated_recurrence_forward_hip,
@@ -28,7 +29,73 @@ from gdl_amd.csrc import (
 )
 
 
+# ═══════════════════════════════════════════════════════════════════
+# Custom ops: what everything but plain eager execution uses (_native.plain_eager)
+# ═══════════════════════════════════════════════════════════════════
+
+
+@torch.library.custom_op("geoembodied::gated_recurrence", mutates_args=())
+def _recurrence_op(x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor, state: Optional[Tensor], ptr: Optional[Tensor],
+                   reverse: bool, rate: float) -> Tuple[Tensor, Tensor, Tensor]:
+    return gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate, True)
+
+
+def _carry_size(tokens, channels):
+    """geo_recurrence_carry_size (0 of no tokens or channels), of symbolic sizes too."""
+    return (tokens + 63) // 64 * ((channels + 3) // 4 * 4)
+
+
+@_recurrence_op.register_fake
+def _(x, gate_a, gate_x, decay, state, ptr, reverse, rate):
+    T, C = x.shape
+    last = x.new_empty((1 if ptr is None else ptr.shape[0] - 1, C), dtype=torch.float32)
+    return x.new_empty(x.shape), last, x.new_empty(_carry_size(T, C), dtype=torch.float32)
+
+
+@torch.library.custom_op("geoembodied::gated_recurrence_backward", mutates_args=())
+def _recurrence_backward_op(dh: Optional[Tensor], dlast: Optional[Tensor], carry: Tensor, x: Tensor, gate_a: Tensor,
+                            gate_x: Tensor, decay: Tensor, state: Optional[Tensor], ptr: Optional[Tensor], reverse: bool,
+                            rate: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    *grads, dstate = gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr, state, reverse, rate)
+    return (*grads, carry.new_empty(0) if dstate is None else dstate)
+
+
+@_recurrence_backward_op.register_fake
+def _(dh, dlast, carry, x, gate_a, gate_x, decay, state, ptr, reverse, rate):
+    return (*(x.new_empty(x.shape) for _ in range(3)), carry.new_empty(decay.shape),
+            carry.new_empty(0 if state is None else state.shape))
+
+
+def _recurrence_setup(ctx, inputs, output) -> None:
+    x, gate_a, gate_x, decay, state, ptr, *ctx.rest = inputs
+    ctx.save_for_backward(x, gate_a, gate_x, decay, state, ptr, output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _recurrence_grads(ctx, dh, dlast, dcarry):
+    x, gate_a, gate_x, decay, state, ptr, carry = ctx.saved_tensors
+    _nat.no_tangents("gated_recurrence backward", dh, dlast, x, gate_a, gate_x, decay, state)
+    dx, dga, dgx, ddecay, dstate = torch.ops.geoembodied.gated_recurrence_backward(dh, dlast, carry, x, gate_a, gate_x, decay,
+                                                                                   state, ptr, *ctx.rest)
+    return (dx, dga, dgx, ddecay.to(decay.dtype), None if state is None else dstate.to(state.dtype), None, None, None)
+
+
+_recurrence_op.register_autograd(_recurrence_grads, setup_context=_recurrence_setup)
+
+
+@torch.library.custom_op("geoembodied::gated_recurrence_step", mutates_args=())
+def _step_op(x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor, state: Tensor, rate: float) -> Tuple[Tensor, Tensor]:
+    return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate)
+
+
+@_step_op.register_fake
+def _(x, gate_a, gate_x, decay, state, rate):
+    return x.new_empty(x.shape), state.new_empty(state.shape)
+
+
 class _GatedRecurrence(torch.autograd.Function):
+    """Eager mode: the op's kernels called directly, without the custom-op layers."""
+
     @staticmethod
     def forward(ctx, x, gate_a, gate_x, decay, state, ptr, reverse, rate):
         h, last, carry = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, reverse, rate, True)
@@ -41,10 +108,12 @@ class _GatedRecurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, dlast):
         x, gate_a, gate_x, decay, state, ptr, carry = ctx.saved_tensors
-        dx, dga, dgx, ddecay, dstate = gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr, state,
-                                                                     *ctx.rest)
-        return (dx, dga, dgx, ddecay.to(decay.dtype), None if dstate is None else dstate.to(state.dtype), None, None,
-                None)
+        if all(g is None or _nat.plain_eager(g) for g in (dh, dlast)):
+            dx, dga, dgx, ddecay, dstate = gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr,
+                                                                         state, *ctx.rest)
+            return (dx, dga, dgx, ddecay.to(decay.dtype), None if dstate is None else dstate.to(state.dtype), None, None,
+                    None)
+        return _recurrence_grads(ctx, dh, dlast, None)
 
 
 def _check(name: str, x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor) -> None:
@@ -90,9 +159,14 @@ def gated_recurrence(
     rate = float(rate)
     if not rate > 0:
         raise ValueError(f"gated_recurrence: rate {rate} must be positive")
+    tensors = x, gate_a, gate_x, decay, state, ptr
+    if not _nat.plain_call(*tensors):
+        _nat.no_tangents("gated_recurrence", *tensors)
+        h, last, _ = torch.ops.geoembodied.gated_recurrence(*tensors, bool(reverse), rate)
+        return h, last
     if torch.is_grad_enabled() and (x.requires_grad or gate_a.requires_grad or gate_x.requires_grad or decay.requires_grad
                                     or (state is not None and state.requires_grad)):
-        return _GatedRecurrence.apply(x, gate_a, gate_x, decay, state, ptr, bool(reverse), rate)
+        return _GatedRecurrence.apply(*tensors, bool(reverse), rate)
     h, last, _ = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, bool(reverse), rate, False)
     return h, last
 
@@ -116,4 +190,7 @@ def gated_recurrence_step(
     if torch.is_grad_enabled() and (x.requires_grad or gate_a.requires_grad or gate_x.requires_grad or decay.requires_grad
                                     or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad()")
-    return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, float(rate))
+    if _nat.plain_call(x, gate_a, gate_x, decay, state):
+        return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, float(rate))
+    _nat.no_tangents("gated_recurrence_step", x, gate_a, gate_x, decay, state)
+    return torch.ops.geoembodied.gated_recurrence_step(x, gate_a, gate_x, decay, state, float(rate))

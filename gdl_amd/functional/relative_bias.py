@@ -24,7 +24,7 @@ MAX_BUCKETS = 256
 MAX_DISTANCE = 1024
 
 
-def _check(buckets: int, max_distance: int, two_sided: bool) -> None:
+def check_buckets(buckets: int, max_distance: int, two_sided: bool) -> None:
     least = 4 if two_sided else 2
     if not least <= buckets <= MAX_BUCKETS or (two_sided and buckets % 2):
         raise ValueError(f"relative bias: {buckets} buckets (from {least} to {MAX_BUCKETS}, an even number "
@@ -39,7 +39,7 @@ def _check(buckets: int, max_distance: int, two_sided: bool) -> None:
 def _table(buckets: int, max_distance: int, two_sided: bool) -> Tuple[Tuple[int, ...], Tuple[Tuple[int, int], ...]]:
     """The bucket of each distance -max_distance .. max_distance, and for each bucket the places
     first <= x < end of that list which hold it."""
-    _check(buckets, max_distance, two_sided)
+    check_buckets(buckets, max_distance, two_sided)
     half = buckets // 2 if two_sided else buckets
     exact = half // 2
     power = half - exact
