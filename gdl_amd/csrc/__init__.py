@@ -719,9 +719,9 @@ def gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, pt
     return dx, dga, dgx, ddecay, dstate
 
 
-def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate):
-    """(h [B, C], new state float32 [B, C]) of one token per stream."""
-    args, _held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, None, state, False, rate,
+def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, positions, rate):
+    """(h [B, C], new state float32 [B, C]) of one token per stream, at ``positions`` [B] (None: none begins)."""
+    args, _held, dev, _ = _recurrence_args("gated_recurrence_step", x, gate_a, gate_x, decay, positions, state, False, rate,
                                            x.shape[0])
     h, new = _like(x), _like(state)
     if x.numel():

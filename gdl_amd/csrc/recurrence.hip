@@ -670,7 +670,7 @@ __global__ __launch_bounds__(kCarryChannels * kRuns) void scan_bwd_decay(const f
   out[at] = x * ratio;
 }
 
-// One token of each of B streams, a thread for each lane's channels: 256 streams of 1024 channels in
+// One token of each of B streams (s.ptr: their positions, or null), a thread for each lane's channels: 256 streams of 1024 channels in
 // bfloat16 4.4 us, as long as a launch whose loads wait for one another once.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict__ state_out, T* __restrict__ h) {
@@ -679,13 +679,23 @@ __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict
   const int64_t b = n / per, at = n % per * V;
   using Raw = typename Pack<T, V>::Raw;
   float xf[V], af[V], gf[V], H[V];
+  const int64_t position = s.ptr ? s.ptr[b] : 1;
+  if (position < 0) {  // no token
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      H[v] = 0.f;
+      state_out[b * s.C + at + v] = s.state[b * s.C + at + v];
+    }
+    *reinterpret_cast<Raw*>(h + b * s.C + at) = pack<T, V>(H);
+    return;
+  }
   unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.x) + b * s.x_st + at), xf);
   unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.ga) + b * s.ga_st + at), af);
   unpack<T, V>(*reinterpret_cast<const Raw*>(static_cast<const T*>(s.gx) + b * s.gx_st + at), gf);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const Gates g = gates(af[v], gf[v], log_rate(s.decay[at + v], s.rate));
-    H[v] = fmaf(g.a, s.state[b * s.C + at + v], g.m * g.z * xf[v]);
+    H[v] = fmaf(g.a, position ? s.state[b * s.C + at + v] : 0.f, g.m * g.z * xf[v]);
     state_out[b * s.C + at + v] = H[v];
   }
   *reinterpret_cast<Raw*>(h + b * s.C + at) = pack<T, V>(H);

@@ -84,12 +84,13 @@ _recurrence_op.register_autograd(_recurrence_grads, setup_context=_recurrence_se
 
 
 @torch.library.custom_op("geoembodied::gated_recurrence_step", mutates_args=())
-def _step_op(x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor, state: Tensor, rate: float) -> Tuple[Tensor, Tensor]:
-    return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, rate)
+def _step_op(x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor, state: Tensor, positions: Optional[Tensor],
+             rate: float) -> Tuple[Tensor, Tensor]:
+    return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, positions, rate)
 
 
 @_step_op.register_fake
-def _(x, gate_a, gate_x, decay, state, rate):
+def _(x, gate_a, gate_x, decay, state, positions, rate):
     return x.new_empty(x.shape), state.new_empty(state.shape)
 
 
@@ -178,19 +179,26 @@ def gated_recurrence_step(
     decay: Tensor,
     state: Tensor,
     *,
+    positions: Optional[Tensor] = None,
     rate: float = 8.0,
 ) -> Tuple[Tensor, Tensor]:
     """One token of each stream: x, gates [B, C] and the streams' float32 states [B, C] to
-    (h [B, C] of x's type, new states float32 [B, C]).  No gradients."""
+    (h [B, C] of x's type, new states float32 [B, C]).  No gradients.
+
+    With ``positions`` (int64 [B], as ``window_attention_step`` takes them) a stream at position 0 begins
+    from 0 whatever its state holds, and one at a negative position keeps its state and gives 0.
+    """
     _check("gated_recurrence_step", x, gate_a, gate_x, decay)
     if state.shape != x.shape or state.dtype is not torch.float32:
         raise ValueError(f"gated_recurrence_step: state must be float32 {tuple(x.shape)}, got {state.dtype} {tuple(state.shape)}")
+    if positions is not None and (positions.shape != x.shape[:1] or positions.dtype.is_floating_point):
+        raise ValueError(f"gated_recurrence_step: positions int64 [{x.shape[0]}], got {positions.dtype} {tuple(positions.shape)}")
     if not rate > 0:
         raise ValueError(f"gated_recurrence_step: rate {rate} must be positive")
     if torch.is_grad_enabled() and (x.requires_grad or gate_a.requires_grad or gate_x.requires_grad or decay.requires_grad
                                     or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no backward: call it under torch.no_grad()")
-    if _nat.plain_call(x, gate_a, gate_x, decay, state):
-        return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, float(rate))
+    if _nat.plain_call(x, gate_a, gate_x, decay, state, positions):
+        return gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, positions, float(rate))
     _nat.no_tangents("gated_recurrence_step", x, gate_a, gate_x, decay, state)
-    return torch.ops.geoembodied.gated_recurrence_step(x, gate_a, gate_x, decay, state, float(rate))
+    return torch.ops.geoembodied.gated_recurrence_step(x, gate_a, gate_x, decay, state, positions, float(rate))

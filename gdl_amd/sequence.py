@@ -109,9 +109,11 @@ class PointSequenceBlock(nn.Module):
     @torch.no_grad()
     def step(self, x: Tensor, positions: Tensor, cache: BlockCache) -> Tensor:
         """One token x [B, channels] of each stream at ``positions`` (int64 [B], from 0), which ``cache``
-        then holds; the forward's row for it."""
+        then holds; the forward's row for it.  A stream at position 0 begins anew; one at a negative
+        position has no token: the cache keeps what it holds of it, and its row means nothing."""
         parts = self.scan_in(self.scan_norm(x)).split(self.channels, 1)
-        h, cache.state = gated_recurrence_step(*parts, self.decay, cache.state)
+        h, state = gated_recurrence_step(*parts, self.decay, cache.state, positions=positions)
         x = x + self.scan_out(h)
         out = window_attention_step(*self._split(x), cache.window, positions, bias=self.bias, max_distance=self.max_distance)
+        cache.state = state  # a call that is refused above leaves the cache as it was
         return x + self.attend_out(out.flatten(1))

@@ -714,7 +714,8 @@ int geo_recurrence_bwd(const geo_recurrence_t* args, const float* carry, const v
                        const float* dlast, void* dx, void* dgate_a, void* dgate_x, float* ddecay,
                        float* dstate, void* workspace, size_t workspace_bytes, void* stream);
 /* One token of each of `sequences` = `tokens` streams: x, gates and h [streams, channels], state read,
- * state_out written (they may be one tensor). */
+ * state_out written (they may be one tensor).  ptr holds the tokens' positions [streams], or is NULL: the
+ * state ahead of position 0 is 0, and a stream at a negative position keeps its state and gives 0. */
 int geo_recurrence_step(const geo_recurrence_t* args, float* state_out, void* h, void* stream);
 
 #ifdef __cplusplus
