@@ -87,8 +87,14 @@ class PointSequenceBlock(nn.Module):
         return y.split((self.heads, self.kv_heads, self.kv_heads), 1)
 
     def forward(self, x: Tensor, ptr: Optional[Tensor] = None, mask: Optional[Tensor] = None) -> Tensor:
-        """x [T, channels] of sequences ``ptr``; keys whose ``mask`` is False are not attended to."""
+        """x [T, channels] of sequences ``ptr``.  Points whose ``mask`` (bool [T]) is False count for
+        nothing: no other point's row depends on them, whatever they hold, and their own mean nothing."""
+        if mask is not None:
+            hidden = ~mask.unsqueeze(1)
+            x = x.masked_fill(hidden, 0.0)  # NaN among them would reach the weights' gradients
         parts = self.scan_in(self.scan_norm(x)).split(self.channels, 1)
+        if mask is not None:  # a closed gate hands the state on as it is
+            parts = parts[0], parts[1].masked_fill(hidden, -torch.inf), parts[2]
         h, _ = gated_recurrence(*parts, self.decay, ptr=ptr)
         if not self.causal:
             h = h + gated_recurrence(*parts, self.decay, ptr=ptr, reverse=True)[0]
