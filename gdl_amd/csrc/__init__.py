@@ -605,9 +605,8 @@ def window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, si
     return dq, dk, dv, dbias
 
 
-def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale, bias, plan, workspace):
-    """[B, H, D] of the tokens at ``positions``, whose k and v go into the caches [B, Hk, slots, D];
-    ``workspace(bytes)`` gives the scratch."""
+def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale, bias, plan):
+    """[B, H, D] of the tokens at ``positions``, whose k and v go into the caches [B, Hk, slots, D]."""
     name = "window_attention_step"
     dev = _sequence_device(name, q, k, v, k_cache, v_cache, positions, bias)
     code = _sequence_code(name, q, k, v, k_cache, v_cache)
@@ -631,9 +630,11 @@ def window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale
     out = _like(q)
     L = _nat.lib()
     with _nat.on_device(dev):
-        ws = workspace(L.geo_window_attention_step_workspace_bytes(B, H, Hk, slots, D))
-        _nat.check(L.geo_window_attention_step(args, out.data_ptr(), _nat.ptr(ws), 0 if ws is None else ws.numel(),
-                                               _nat.stream_of(dev)), "geo_window_attention_step")
+        ws_bytes = L.geo_window_attention_step_workspace_bytes(B, H, Hk, slots, D)
+        # from the allocator, which keeps what a captured call was given for the graph's replays
+        ws = _nat.workspace(ws_bytes, dev) if ws_bytes else None
+        _nat.check(L.geo_window_attention_step(args, out.data_ptr(), _nat.ptr(ws), ws_bytes, _nat.stream_of(dev)),
+                   "geo_window_attention_step")
     return out
 
 

@@ -99,7 +99,7 @@ _attention_op.register_autograd(_attention_grads, setup_context=_attention_setup
 def _step_op(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, positions: Tensor, bias: Optional[Tensor],
              sinks: int, max_distance: int, scale: float) -> Tensor:
     return window_attention_step_hip(q, k, v, k_cache, v_cache, sinks, positions, scale, bias,
-                                     _plan(bias, max_distance, False), lambda n: _nat.workspace(n, q.device) if n else None)
+                                     _plan(bias, max_distance, False))
 
 
 @_step_op.register_fake
@@ -215,8 +215,7 @@ class WindowCache:
 
     Token ``j`` of a stream lies in slot ``j`` for ``j < sinks``, else in slot
     ``sinks + (j - sinks) % ring``, ``ring`` = left + 1 tokens of the window.  The object holds the two
-    tensors (given ones are used as they are) and the scratch of the steps; calls on it are ordered by
-    the caller's stream.
+    tensors (given ones are used as they are); calls on it are ordered by the caller's stream.
     """
 
     def __init__(self, k: Tensor, v: Tensor, *, sinks: int = 0):
@@ -233,7 +232,6 @@ class WindowCache:
                 raise ValueError("WindowCache: a head's slots must adjoin, on multiples of 16 bytes")
         self.k, self.v, self.sinks = k, v, int(sinks)
         self.left = k.shape[2] - self.sinks - 1
-        self._scratch: Optional[Tensor] = None
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, head_dim: int, left: int, *, sinks: int = 0,
@@ -259,11 +257,6 @@ class WindowCache:
         else:
             _nat.no_tangents("WindowCache.fill", k, v)
             torch.ops.geoembodied.window_cache_fill(k, v, self.k, self.v, self.sinks, ptr, start)
-
-    def _workspace(self, nbytes: int) -> Optional[Tensor]:
-        if nbytes and (self._scratch is None or self._scratch.numel() < nbytes):
-            self._scratch = _nat.workspace(nbytes, self.k.device)
-        return self._scratch if nbytes else None
 
 
 def window_attention_step(
@@ -300,7 +293,7 @@ def window_attention_step(
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if _nat.plain_call(q, k, v, cache.k, cache.v, positions, bias):
         return window_attention_step_hip(q, k, v, cache.k, cache.v, cache.sinks, positions, scale, bias,
-                                         _plan(bias, int(max_distance), False), cache._workspace)
+                                         _plan(bias, int(max_distance), False))
     _nat.no_tangents("window_attention_step", q, k, v, bias)
     if bias is not None:
         check_buckets(bias.shape[0], int(max_distance), False)
