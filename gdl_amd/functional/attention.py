@@ -174,7 +174,8 @@ def window_attention(
             Tokens outside ``ptr[0] .. ptr[B]`` see nothing.
         mask: bool [T], False keys are seen by no one (and may hold anything).
         bias: [buckets, H] learned relative position bias, added to the scores (``relative_buckets``);
-            two-sided unless ``window`` has no right side.
+            two-sided unless ``window`` has no right side.  The first call with a number of buckets and
+            a ``max_distance`` copies their table to the device and cannot be captured into a graph.
         max_distance: where the bias's last bucket begins (at most 1024).
         scale: of the scores; ``D ** -0.5`` by default.
 

@@ -56,8 +56,11 @@ def _table(buckets: int, max_distance: int, two_sided: bool) -> Tuple[Tuple[int,
 @functools.lru_cache(maxsize=None)
 def bucket_plan(buckets: int, max_distance: int, two_sided: bool, device: torch.device) -> Tuple[Tensor, Tensor]:
     """(bucket of each distance int32 [2 max_distance + 1], spans int32 [buckets, 2]) on a device,
-    laid out once per configuration."""
+    laid out once per configuration, by a copy that the host waits for."""
     lut, spans = _table(buckets, max_distance, two_sided)
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"relative bias: a graph cannot capture the first call with {buckets} buckets up to distance "
+                           f"{max_distance} (its table is copied to the device): make one call before the capture")
     return (torch.tensor(lut, dtype=torch.int32, device=device),
             torch.tensor(spans, dtype=torch.int32, device=device))
 
