@@ -4,6 +4,8 @@
 // The cache of a stream and key head is [sinks + ring, D]: token j lies in slot j for j < sinks, else
 // in slot sinks + (j - sinks) mod ring.  The new token at position p is written to its slot and
 // attends to the tokens j <= p that are held: the first ones and the last `ring` up to p itself.
+#include <utility>
+
 #include "attention_tile.hpp"
 
 namespace geo {
@@ -282,6 +284,16 @@ __global__ __launch_bounds__(256) void cache_fill(const char* __restrict__ k, co
       *reinterpret_cast<const uint4*>(v + (t * v_st + h * v_sh) * SIZE + e);
 }
 
+// The heads of all streams lie apart, so that what is written to one is read from no other.
+inline bool apart(int64_t batch, int64_t stream, int64_t heads, int64_t head, int64_t block) {
+  if (batch > 1 && heads > 1 && stream < head) {  // heads outside
+    std::swap(batch, heads);
+    std::swap(stream, head);
+  }
+  if (heads > 1 && head < block) return false;
+  return batch <= 1 || stream >= (heads > 1 ? head * (heads - 1) : 0) + block;
+}
+
 inline int lanes_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : 16; }
 
 // Pieces of a stream's slots: sixteen workgroups for each of the 256 CUs where there is work, at least
@@ -366,6 +378,9 @@ extern "C" int geo_window_attention_step(const geo_window_step_t* g, void* out, 
                   in_pieces(g->v, g->v_stream, g->v_head) && in_pieces(g->k_cache, g->k_cache_stream, g->k_cache_head) &&
                   in_pieces(g->v_cache, g->v_cache_stream, g->v_cache_head),
               "window attention step: null tensor, or rows not on multiples of 16 bytes");
+  GEO_REQUIRE(attn::apart(g->batch, g->k_cache_stream, g->kv_heads, g->k_cache_head, g->slots * g->head_dim) &&
+                  attn::apart(g->batch, g->v_cache_stream, g->kv_heads, g->v_cache_head, g->slots * g->head_dim) && g->k_cache != g->v_cache,
+              "window attention step: heads or streams of a cache share memory");
   GEO_REQUIRE(out && g->positions, "window attention step: null output or positions");
   const size_t need = geo_window_attention_step_workspace_bytes(g->batch, g->heads, g->kv_heads, g->slots, g->head_dim);
   if (need && (!workspace || workspace_bytes < need))
@@ -404,6 +419,9 @@ extern "C" int geo_window_cache_fill(int dtype, const void* k, const void* v, in
   GEO_REQUIRE(in_pieces(k, k_token, k_head) && in_pieces(v, v_token, v_head) &&
                   in_pieces(k_cache, k_cache_stream, k_cache_head) && in_pieces(v_cache, v_cache_stream, v_cache_head),
               "window cache: null tensor, or rows not on multiples of 16 bytes");
+  GEO_REQUIRE(attn::apart(batch, k_cache_stream, kv_heads, k_cache_head, slots * head_dim) &&
+                  attn::apart(batch, v_cache_stream, kv_heads, v_cache_head, slots * head_dim) && k_cache != v_cache,
+              "window cache: heads or streams of a cache share memory");
   const int64_t blocks = ceil_div(tokens * kv_heads * (head_dim * size / 16), 256);
   GEO_REQUIRE(blocks < (int64_t(1) << 31), "window cache: too many workgroups");
   auto launch = [&](auto kernel) {

@@ -211,6 +211,16 @@ def window_attention(
     return out[..., :d] if d % 8 else out
 
 
+def _apart(t: Tensor) -> bool:
+    """No two heads of two streams of t [B, Hk, slots, D], each head's slots adjoining, share memory."""
+    reach = t.shape[2] * t.shape[3]
+    for stride, n in sorted((t.stride(n), t.shape[n]) for n in (0, 1) if t.shape[n] > 1):
+        if stride < reach:
+            return False
+        reach += stride * (n - 1)
+    return True
+
+
 class WindowCache:
     """Keys and values of streams that a causal window reaches: ``k, v [B, Hk, sinks + ring, D]``.
 
@@ -231,6 +241,10 @@ class WindowCache:
             at = t.data_ptr() if _nat.plain_eager(t) else 0  # traced: looked at when the program runs
             if t.stride(3) != 1 or t.stride(2) != t.shape[3] or any(x % 16 for x in (at, t.stride(0) * size, t.stride(1) * size)):
                 raise ValueError("WindowCache: a head's slots must adjoin, on multiples of 16 bytes")
+            if not _apart(t):
+                raise ValueError(f"WindowCache: streams or heads share memory (strides {t.stride()} of {tuple(t.shape)})")
+        if k.numel() and _nat.plain_eager(k) and _nat.plain_eager(v) and k.data_ptr() == v.data_ptr():
+            raise ValueError("WindowCache: k and v are the same memory")
         self.k, self.v, self.sinks = k, v, int(sinks)
         self.left = k.shape[2] - self.sinks - 1
 

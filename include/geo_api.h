@@ -659,7 +659,7 @@ int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out
  */
 typedef struct {
   const void *q, *k, *v;       /* [batch, heads or kv_heads, head_dim] */
-  void *k_cache, *v_cache;     /* [batch, kv_heads, slots, head_dim], rows of a head adjoining */
+  void *k_cache, *v_cache;     /* [batch, kv_heads, slots, head_dim], rows of a head adjoining, heads apart */
   int64_t q_stream, q_head, k_stream, k_head, v_stream, v_head; /* strides in elements */
   int64_t k_cache_stream, k_cache_head, v_cache_stream, v_cache_head;
   const int64_t* positions;    /* [batch] */
