@@ -514,13 +514,12 @@ def _sequence_code(name: str, *tensors: Tensor) -> int:
 
 def _sequence_device(name: str, *tensors: Optional[Tensor]) -> torch.device:
     """The GPU that holds all of an operator's tensors."""
-    dev = tensors[0].device
+    dev, index = tensors[0].device, tensors[0].get_device()
     for t in tensors:
-        if t is not None:
+        if t is not None and (index < 0 or t.get_device() != index):  # a number: cheaper than devices
             if not t.is_cuda:
                 _require_gpu(name, t)
-            if t.device != dev:
-                raise ValueError(f"{name}: tensors on different devices")
+            raise ValueError(f"{name}: tensors on different devices")
     return dev
 
 
@@ -585,20 +584,22 @@ def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, 
     return out, rest, lse
 
 
-def window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan):
-    """(dq, dk, dv, dbias or None), contiguous and of the inputs' types."""
+def window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan,
+                                  need_q=True, need_kv=True, need_bias=True):
+    """(dq, dk, dv, dbias), contiguous and of the inputs' types; None for what is not needed."""
     name = "window_attention backward"
     args, _held, dev = _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
     grad = _in_pieces(grad.to(out.dtype).contiguous())
-    dq, dk, dv = _like(q), _like(k), _like(v)
-    dbias = None if bias is None else _like(bias)
+    dq = _like(q) if need_q else None
+    dk, dv = (_like(k), _like(v)) if need_kv else (None, None)
+    dbias = _like(bias) if bias is not None and need_bias else None
     L = _nat.lib()
     with _nat.on_device(dev):
         ws_bytes = L.geo_window_attention_bwd_workspace_bytes(args)
         ws = _nat.workspace(ws_bytes, dev)
         _nat.check(L.geo_window_attention_bwd(
-            args, out.data_ptr(), _nat.ptr(rest), grad.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            dv.data_ptr(), None if bias is None else plan[1].data_ptr(), _nat.ptr(dbias), ws.data_ptr(), ws_bytes,
+            args, out.data_ptr(), _nat.ptr(rest), grad.data_ptr(), lse.data_ptr(), _nat.ptr(dq), _nat.ptr(dk), _nat.ptr(dv),
+            None if dbias is None else plan[1].data_ptr(), _nat.ptr(dbias), ws.data_ptr(), ws_bytes,
             _nat.stream_of(dev)), "geo_window_attention_bwd")
     if dbias is not None and q.shape[0] == 0:
         dbias.zero_()

@@ -119,6 +119,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
     dl = halves_sum(dl);
     if (real && half == 0) delta[static_cast<int64_t>(h) * a.seq.T + i] = dl;
   }
+  if (!dq && !(BIAS && range)) return;  // delta alone
   const float ls = real ? lse[static_cast<int64_t>(h) * a.seq.T + i] : kInf;
   if (BIAS && far_sum(ls)) {  // the factor of the row's weights, as one of what they are multiplied with
     const float norm = lse[static_cast<int64_t>(a.Hq + h) * a.seq.T + i];
@@ -226,8 +227,8 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, c
     }
     if (odd) add_wild<T, kMt, true>(kbase, a.k_st, j0, odd, vis, a.D, o);
   }
-  if (real) store_row<T>(dq + (static_cast<int64_t>(i) * a.Hq + h) * a.D, o, a.scale, a.D);
-  if (BIAS) {
+  if (real && dq) store_row<T>(dq + (static_cast<int64_t>(i) * a.Hq + h) * a.D, o, a.scale, a.D);
+  if (BIAS && range) {
     below = wave_sum(below);
     above = wave_sum(above);
     if (lane == 0) {
@@ -647,7 +648,7 @@ int launch_q(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream)
       a, static_cast<const T*>(g.out), static_cast<const T*>(g.rest), static_cast<const T*>(g.grad), g.lse, p.delta, static_cast<T*>(g.dq), g.range,
       p.part);
   GEO_LAUNCH_CHECK("attend_bwd_q");
-  if (BIAS) {
+  if (g.dbias) {
     attend_bwd_bias<<<dim3(a.bias.buckets * a.Hq), dim3(64), 0, stream>>>(p.part, p.q_blocks, a.bias.buckets, a.Hq,
                                                                           a.bias.dtype, g.dbias);
     GEO_LAUNCH_CHECK("attend_bwd_bias");
@@ -671,6 +672,7 @@ template <typename T, int DP, bool BIAS>
 int all_grads(const Attend& a, const Grads& g, const Plan& p, hipStream_t stream) {
   int rc = lone_wave(a, a.Hq, sizeof(T) == 4) ? launch_q<T, DP, 1, 32, BIAS>(a, g, p, stream)
                                               : launch_q<T, DP, 4, q_rows<DP>(), BIAS>(a, g, p, stream);
+  if (!g.dk) return rc;
   if (rc == GEO_OK && p.far.len)
     rc = launch_kv<T, DP, 1, 32, BIAS, true>(a, g, p, (p.pieces - 1) * ceil_div(a.sinks, 32) * a.Hq, stream);
   if (rc == GEO_OK)
@@ -715,11 +717,11 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
   geo::attn::Attend a;
   const int rc = geo::attn::attend_args(args, &a);
   if (rc != GEO_OK || args->tokens == 0) return rc;
-  GEO_REQUIRE(out && grad && lse && dq && dk && dv, "window attention backward: null tensor");
+  GEO_REQUIRE(out && grad && lse && !dk == !dv, "window attention backward: null tensor");
   GEO_REQUIRE(reinterpret_cast<uintptr_t>(grad) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(rest) % 16 == 0,
               "window attention backward: out, rest and grad must lie on multiples of 16 bytes");
-  GEO_REQUIRE(!args->bias || (bucket_range && dbias), "window attention backward: null bucket_range or dbias");
+  GEO_REQUIRE(!dbias || (args->bias && bucket_range), "window attention backward: null bias or bucket_range");
   geo::attn::Plan p;
   const size_t need = geo::attn::plan(*args, a, workspace, &p);
   if (!workspace || workspace_bytes < need)
@@ -727,7 +729,7 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
                           workspace ? workspace_bytes : size_t(0), need);
   GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks * 4 < (int64_t(1) << 31),
               "window attention backward: too many workgroups");
-  const geo::attn::Grads g{out, rest, grad, lse, dq, dk, dv, dbias, bucket_range};
+  const geo::attn::Grads g{out, rest, grad, lse, dq, dk, dv, dbias, dbias ? bucket_range : nullptr};
   const hipStream_t s = geo::as_stream(stream);
   if (args->dtype == GEO_F32) return geo::attn::choose_grads<float>(a, g, p, s);
   if (args->dtype == GEO_BF16) return geo::attn::choose_grads<__bf16>(a, g, p, s);

@@ -66,17 +66,18 @@ def _(q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
 @torch.library.custom_op("geoembodied::window_attention_backward", mutates_args=())
 def _attention_backward_op(grad: Tensor, out: Tensor, rest: Tensor, lse: Tensor, q: Tensor, k: Tensor, v: Tensor,
                            bias: Optional[Tensor], ptr: Optional[Tensor], mask: Optional[Tensor], left: int, right: int,
-                           sinks: int, max_distance: int, scale: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    dq, dk, dv, dbias = window_attention_backward_hip(
+                           sinks: int, max_distance: int, scale: float, need_q: bool, need_kv: bool,
+                           need_bias: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    grads = window_attention_backward_hip(
         grad, out, rest if rest.numel() else None, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias,
-        _plan(bias, max_distance, right != 0))
-    return dq, dk, dv, lse.new_empty(0) if dbias is None else dbias
+        _plan(bias, max_distance, right != 0), need_q, need_kv, need_bias)
+    return tuple(lse.new_empty(0) if g is None else g for g in grads)
 
 
 @_attention_backward_op.register_fake
-def _(grad, out, rest, lse, q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
-    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
-            lse.new_empty(0) if bias is None else bias.new_empty(bias.shape))
+def _(grad, out, rest, lse, q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale, need_q, need_kv, need_bias):
+    needs = need_q, need_kv, need_kv, need_bias and bias is not None
+    return tuple(t.new_empty(t.shape) if need else lse.new_empty(0) for t, need in zip((q, k, v, bias), needs))
 
 
 def _attention_setup(ctx, inputs, output) -> None:
@@ -84,12 +85,20 @@ def _attention_setup(ctx, inputs, output) -> None:
     ctx.save_for_backward(q, k, v, bias, *output, ptr, mask)
 
 
+def _needs(ctx):
+    """Whether the gradients of q, of k or v, and of the bias are needed."""
+    q, k, v, bias = ctx.needs_input_grad[:4]
+    return q, k or v, bias
+
+
 def _attention_grads(ctx, grad, grad_rest, grad_lse):
     q, k, v, bias, out, rest, lse, ptr, mask = ctx.saved_tensors
     _nat.no_tangents("window_attention backward", grad, q, k, v, bias)
-    *grads, dbias = torch.ops.geoembodied.window_attention_backward(
-        grad, out, out.new_empty(0) if rest is None else rest, lse, q, k, v, bias, ptr, mask, *ctx.sizes)
-    return (*grads, None if bias is None else dbias, None, None, None, None, None, None, None)
+    needs = _needs(ctx)
+    grads = torch.ops.geoembodied.window_attention_backward(
+        grad, out, out.new_empty(0) if rest is None else rest, lse, q, k, v, bias, ptr, mask, *ctx.sizes, *needs)
+    grads = (g if need else None for g, need in zip(grads, (needs[0], needs[1], needs[1], needs[2])))
+    return (*grads, None, None, None, None, None, None, None)
 
 
 _attention_op.register_autograd(_attention_grads, setup_context=_attention_setup)
@@ -136,7 +145,8 @@ class _WindowAttention(torch.autograd.Function):
             return _attention_grads(ctx, grad, None, None)
         q, k, v, bias, out, rest, lse, ptr, mask = ctx.saved_tensors
         left, right, sinks, _, scale = ctx.sizes
-        grads = window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, ctx.plan)
+        grads = window_attention_backward_hip(grad, out, rest, lse, q, k, v, left, right, sinks, scale, ptr, mask, bias, ctx.plan,
+                                              *_needs(ctx))
         return (*grads, None, None, None, None, None, None, None)
 
 

@@ -643,7 +643,8 @@ typedef struct {
 int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, void* rest, float* lse, void* stream);
 /* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out,
  * rest (may be NULL) and lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of
- * bias_lut that hold the bucket (each bucket's places are consecutive).  Sums have a fixed order. */
+ * bias_lut that hold the bucket (each bucket's places are consecutive).  Sums have a fixed order.  A
+ * gradient that is not wanted is NULL (dk and dv together). */
 size_t geo_window_attention_bwd_workspace_bytes(const geo_window_attention_t* args);
 int geo_window_attention_bwd(const geo_window_attention_t* args, const void* out, const void* rest,
                              const void* grad, const float* lse, void* dq, void* dk, void* dv, const int32_t* bucket_range,
