@@ -587,13 +587,16 @@ __global__ __launch_bounds__(64 * kJoinRuns) void attend_bwd_join(const Attend a
 
 // ---------------------------------------------------------------------- host ---
 
-// Pieces of the queries past a leading token's window: 256 tokens (64 pieces keep the sums of a
-// sequence of 16,384 small), longer where that would be more than 512 pieces.
-inline int far_len(int T, int left, int sinks) {
+// Pieces of the queries past a leading token's window: 256 tokens, longer where that would be more than
+// 512 pieces or their sums (`each` bytes a piece) more than kFarBytes.  131,072 tokens, 16 (4) heads of 128 in
+// bfloat16, window 511, backward in us at 16 | 64 | 256 MiB | no bound: 64 leading tokens 5996 | 4168 | 4147 |
+// 4350, 256 of them (2.7 GB without a bound) 19,920 | 6500 | 5640 | 6510; up to 64 MiB nothing changes.
+constexpr int64_t kFarBytes = int64_t(64) << 20;
+inline int far_len(int T, int left, int sinks, int64_t each) {
   if (sinks == 0 || T - 1 <= left) return 0;
   int len = 256;
-  while (ceil_div(T, len) > 512) len *= 2;
-  return (left / len + 1) * len < T ? len : 0;
+  while (len < T && (ceil_div(T, len) > 512 || ceil_div(T, len) * each > kFarBytes)) len *= 2;
+  return (left / len + 1) * static_cast<int64_t>(len) < T ? len : 0;
 }
 
 struct Plan {
@@ -608,7 +611,7 @@ inline size_t plan(const geo_window_attention_t& g, const Attend& a, void* works
   p->q_blocks = ceil_div(T, lone_wave(a, a.Hq, g.dtype == GEO_F32) ? 32 : 128);
   p->delta = c.take<float>(static_cast<size_t>(g.heads) * T);
   p->part = c.take<float>(g.bias ? static_cast<size_t>(p->q_blocks) * g.heads * g.buckets : 0);
-  p->far.len = far_len(T, a.left, sinks);
+  p->far.len = far_len(T, a.left, sinks, int64_t(g.heads + g.kv_heads) * sinks * 2 * g.head_dim * sizeof(float));
   p->pieces = p->far.len ? ceil_div(T, p->far.len) : 0;
   p->far.own = c.take<float>(static_cast<size_t>(p->pieces) * g.kv_heads * sinks * 2 * g.head_dim);
   p->far.part = c.take<float>(static_cast<size_t>(p->pieces) * g.heads * sinks * 2 * g.head_dim);
