@@ -44,6 +44,9 @@ int set_error(int code, const char* fmt, ...);
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+// A launch holds less than 2^32 threads.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (int64_t(1) << 32) / threads; }
+
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Carves aligned sub-buffers out of one caller-provided workspace.

@@ -715,7 +715,7 @@ inline int scan_args(const geo_recurrence_t* g, Scan* s) {
   *s = Scan{g->x, g->gate_a, g->gate_x, g->x_token, g->gate_a_token, g->gate_x_token, g->decay, g->ptr, g->state,
             g->tokens, g->channels, g->sequences, g->rate, g->reverse};
   GEO_REQUIRE(g->tokens == 0 || g->channels == 0 || (g->x && g->gate_a && g->gate_x && g->decay), "gated recurrence: null tensor");
-  GEO_REQUIRE(chunks_of(g->tokens) * ceil_div(g->channels, 64) < (int64_t(1) << 31), "gated recurrence: too many workgroups");
+  GEO_REQUIRE(grid_fits(chunks_of(g->tokens) * ceil_div(g->channels, 64), 64 * kWaves), "gated recurrence: too many workgroups");
   return GEO_OK;
 }
 
@@ -819,7 +819,7 @@ namespace rec {
 template <typename T, int V>
 int step(const Scan& s, float* state_out, void* h, hipStream_t stream) {
   const int64_t blocks = ceil_div(s.B * (s.C / V), 256);
-  GEO_REQUIRE(blocks < (int64_t(1) << 31), "gated recurrence step: too many workgroups");
+  GEO_REQUIRE(grid_fits(blocks, 256), "gated recurrence step: too many workgroups");
   scan_step<T, V><<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, stream>>>(s, state_out, static_cast<T*>(h));
   GEO_LAUNCH_CHECK("scan_step");
   return GEO_OK;

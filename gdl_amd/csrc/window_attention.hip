@@ -207,7 +207,7 @@ constexpr int fwd_waves() {
 template <typename T, int DP, int NW, int BN, bool BIAS>
 int launch_fwd(const Attend& a, void* out, void* rest, float* lse, hipStream_t stream) {
   const int64_t blocks = ceil_div(a.seq.T, 32 * NW) * a.Hq;
-  GEO_REQUIRE(blocks < (int64_t(1) << 31), "window attention: %lld workgroups", static_cast<long long>(blocks));
+  GEO_REQUIRE(grid_fits(blocks, 64 * NW), "window attention: too many workgroups (%lld)", static_cast<long long>(blocks));
   const size_t lds = 2 * Tile<T, DP, BN, 64 * NW>::kBytes +
                      (BIAS ? sizeof(float) * (32 * NW + BN + 2 * a.bias.maxd + 1) : 0);
   GEO_HIP_CHECK(allow_lds(reinterpret_cast<const void*>(attend_fwd<T, DP, NW, BN, BIAS, fwd_waves<T, DP, NW>()>), lds));

@@ -730,7 +730,9 @@ extern "C" int geo_window_attention_bwd(const geo_window_attention_t* args, cons
   if (!workspace || workspace_bytes < need)
     return geo::set_error(GEO_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes, %zu needed",
                           workspace ? workspace_bytes : size_t(0), need);
-  GEO_REQUIRE(p.q_blocks * a.Hq < (int64_t(1) << 31) && p.pieces * a.Hq * a.sinks * 4 < (int64_t(1) << 31),
+  const int64_t far = p.pieces * a.sinks;
+  GEO_REQUIRE(geo::grid_fits(geo::ceil_div(a.seq.T, 128) * a.Hq, 256) && geo::grid_fits(far * a.Hq, 64) &&
+                  geo::grid_fits(far * a.Hk * 4, 64 * geo::attn::kJoinRuns),
               "window attention backward: too many workgroups");
   const geo::attn::Grads g{out, rest, grad, lse, dq, dk, dv, dbias, dbias ? bucket_range : nullptr};
   const hipStream_t s = geo::as_stream(stream);

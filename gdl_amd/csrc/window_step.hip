@@ -311,7 +311,8 @@ int launch_step(const Step& a, void* out, float* part, hipStream_t stream) {
   const int group = a.Hq / a.Hk;
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * ceil_div(group, GB);
   const int pieces = step_pieces(rows, a.slots, a.D);
-  GEO_REQUIRE(rows * pieces < (int64_t(1) << 31), "window attention step: too many workgroups");
+  GEO_REQUIRE(grid_fits(rows * pieces, kStepThreads) && grid_fits(static_cast<int64_t>(a.B) * a.Hq, 8 * LW),
+              "window attention step: too many workgroups");
   const size_t lds = a.bias.table ? sizeof(float) * GB * (a.bias.maxd + 1) : 0;
   step_piece<T, LW, GB><<<dim3(static_cast<uint32_t>(rows * pieces)), dim3(kStepThreads), lds, stream>>>(a, pieces, part, static_cast<T*>(out));
   GEO_LAUNCH_CHECK("step_piece");
@@ -356,7 +357,7 @@ extern "C" int geo_window_attention_step(const geo_window_step_t* g, void* out, 
   GEO_REQUIRE(g, "window attention step: null arguments");
   GEO_REQUIRE(g->dtype == GEO_F32 || g->dtype == GEO_BF16 || g->dtype == GEO_F16, "window attention step: dtype code %d",
               static_cast<int>(g->dtype));
-  GEO_REQUIRE(g->batch >= 0 && g->kv_heads >= 1 && g->heads >= 1 && g->heads % g->kv_heads == 0,
+  GEO_REQUIRE(g->batch >= 0 && g->batch < (int64_t(1) << 31) && g->kv_heads >= 1 && g->heads >= 1 && g->heads % g->kv_heads == 0,
               "window attention step: %d heads are no multiple of %d key heads", g->heads, g->kv_heads);
   GEO_REQUIRE(g->head_dim >= 8 && g->head_dim <= 128 && g->head_dim % 8 == 0,
               "window attention step: head size %d (a multiple of 8 up to 128)", g->head_dim);
@@ -423,7 +424,7 @@ extern "C" int geo_window_cache_fill(int dtype, const void* k, const void* v, in
                   attn::apart(batch, v_cache_stream, kv_heads, v_cache_head, slots * head_dim) && k_cache != v_cache,
               "window cache: heads or streams of a cache share memory");
   const int64_t blocks = ceil_div(tokens * kv_heads * (head_dim * size / 16), 256);
-  GEO_REQUIRE(blocks < (int64_t(1) << 31), "window cache: too many workgroups");
+  GEO_REQUIRE(grid_fits(blocks, 256), "window cache: too many workgroups");
   auto launch = [&](auto kernel) {
     kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, as_stream(stream)>>>(
         static_cast<const char*>(k), static_cast<const char*>(v), k_token, k_head, v_token, v_head, ptr, start, tokens, batch,
