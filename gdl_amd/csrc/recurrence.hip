@@ -12,7 +12,7 @@
 //
 // The inputs are read twice in each direction, and still vector instructions bound the passes: 79 to 94%
 // of a SIMD's cycles, for two sigmoids, a decay, a root and 1 - a^2 of every element.  131,072 tokens of
-// 256 channels in bfloat16: pass 1 60 us, carry 9, pass 2 62; backward 34, 9 and 121, decay's sums 4.
+// 256 channels in bfloat16: pass 1 60 us, carry 9, pass 2 63; backward 34, 9 and 122, decay's sums 4.
 #include "common.hpp"
 
 namespace geo {
@@ -60,8 +60,9 @@ __device__ __forceinline__ float sigmoid(float x) {
   const float err = __builtin_amdgcn_fmed3f(fmaf(-x, kLog2e, -t), -1.f, 1.f);
   return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(t), fmaf(err, 0.6931471805599453f, 1.f), 1.f));
 }
-// 1 - exp(u) for u <= 0, relatively to 5e-7: near 0 the series of -expm1, since the difference would
-// cancel (its first term left out is u^5 / 720).
+// 1 - exp(u) for u <= 0: near 0 the series of -expm1, since the difference would cancel (its first term left
+// out is u^5 / 720 of it, 4e-8 at its end).  Just past it a unit of exp_u is 5e-7 of the difference; as
+// the square of a rounded exponential exp_u is off by up to three, m, its root, by half of that.
 __device__ __forceinline__ float one_minus_exp(float u, float exp_u) {
   float s = fmaf(u, 1.f / 120.f, 1.f / 24.f);
   s = fmaf(s, u, 1.f / 6.f);

@@ -18,10 +18,11 @@ namespace attn {
 // Which of a tile's keys a query sees is a 64-bit word per lane: the tile is skipped by a wave
 // whose words are all zero, and takes no select where all bits are set.
 //
-// Bound by vector instructions: per score a scale, a maximum, an exponential, a sum and half a
-// conversion against 4 D operations of the matrix units.  131,072 tokens, 8 heads of 64 in bfloat16,
-// window 512 to both sides: 428-446 us, 617-643 TFLOP/s (a large matrix product: 1122); of a SIMD's
-// cycles vector instructions are active in 64%, matrix instructions in 33%.
+// A wave forms a tile's scores, their softmax and the product with V one after the other, per score a scale, a
+// maximum, an exponential, a sum and half a conversion against 4 D operations of the matrix units.
+// 131,072 tokens, 8 heads of 64 in bfloat16, window 512 to both sides: 430-446 us, 615-639 TFLOP/s (a large
+// matrix product: 1122); vector instructions are active in 64% of a SIMD's cycles, matrix instructions in
+// 33%, so neither alone is the bound, but how little of the one runs beside the other.
 template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
 __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* __restrict__ out, T* __restrict__ rest,
                                                             float* __restrict__ lse) {

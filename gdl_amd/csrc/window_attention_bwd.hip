@@ -4,9 +4,9 @@
 //   dv_j = sum_i p_ij g_i,  ds_ij = p_ij (g_i.v_j - delta_i),
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dbias(d) = sum of ds_ij, j - i = d.
 // delta is formed from the output before its rounding (out + rest): the rounding would cost as much
-// again as the rounding of ds does.  The weights are formed again from the scores and the forward's log-sums, once for dq (and the
-// bias) and once for dk and dv: seven products instead of five, for sums that no two workgroups
-// share, so every gradient is the same from run to run.
+// again as the rounding of ds does.  The weights are formed again from the scores and the forward's
+// log-sums, once for dq (and the bias) and once for dk and dv: seven products instead of five, for sums
+// that no two workgroups share, so every gradient is the same from run to run.
 #include "attention_args.hpp"
 #include "attention_tile.hpp"
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ float sum_by_distance(const f32x16& x) {
 //
 // 32,768 tokens, 8 (2) heads of 128 in bfloat16, window 2047 back: 525 us, 767 TFLOP/s of its three
 // products; matrix instructions 41% of a SIMD's cycles, vector instructions 34%.  With the bias, 65,536
-// tokens, 8 heads of 32, window 128 to both sides: 140 us, vector instructions.
+// tokens, 8 heads of 32, window 128 to both sides: 145 us, vector instructions.
 template <typename T, int DP, int NW, int BN, bool BIAS, int WAVES>
 __global__ __launch_bounds__(64 * NW, WAVES) void attend_bwd_q(const Attend a, const T* __restrict__ out,
                                                         const T* __restrict__ rest,
@@ -625,7 +625,7 @@ struct Grads {
   const int32_t* range;
 };
 
-// Waves per SIMD that the registers are bounded for.  dk and dv with wide heads keep 128 registers of
+// Waves per SIMD that the registers are bounded for.  dk and dv with heads of 128 keep 128 registers of
 // sums and take a SIMD for themselves: two waves there spilled into the loop (1166 us against 1009 at
 // 32,768 tokens, 8 (2) heads of 128, window 2047).
 template <typename T, int DP, int NW>

@@ -251,7 +251,8 @@ __global__ __launch_bounds__(8 * LW) void step_join(int D, int Hq, int pieces, c
   if (e < D) out[static_cast<int64_t>(blockIdx.x) * D + e] = static_cast<T>(pos[blockIdx.x / Hq] < 0 ? 0.f : y / sum);
 }
 
-// Tokens into caches: one thread per 16 bytes of a token's and head's row, k and v.
+// Tokens into caches: one thread per 16 bytes of a token's and head's row, k and v.  131,072 tokens of 8 heads of
+// 64 in bfloat16: 100 us, 5.35 TB/s (a large copy: 5.19).
 template <int SIZE>
 __global__ __launch_bounds__(256) void cache_fill(const char* __restrict__ k, const char* __restrict__ v, int64_t k_st,
                                                   int64_t k_sh, int64_t v_st, int64_t v_sh, const int64_t* __restrict__ ptr,

@@ -109,7 +109,7 @@ class _GatedRecurrence(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, dlast):
         x, gate_a, gate_x, decay, state, ptr, carry = ctx.saved_tensors
-        if all(g is None or _nat.plain_eager(g) for g in (dh, dlast)):
+        if (dh is None or _nat.plain_eager(dh)) and (dlast is None or _nat.plain_eager(dlast)):
             dx, dga, dgx, ddecay, dstate = gated_recurrence_backward_hip(dh, dlast, carry, x, gate_a, gate_x, decay, ptr,
                                                                          state, *ctx.rest)
             return (dx, dga, dgx, ddecay.to(decay.dtype), None if dstate is None else dstate.to(state.dtype), None, None,
