@@ -570,14 +570,14 @@ def _attention_args(name, q, k, v, left, right, sinks, scale, ptr, mask, bias, p
 
 def window_attention_forward_hip(q, k, v, left, right, sinks, scale, ptr, mask, bias, plan, train):
     """(out [T, H, D], and for the backward, with ``train``: what its rounding took, for 16-bit types,
-    and the log-sums and their corrections float32 [2, H, T]); ``plan``: (bucket of each distance, spans, max_distance) of the
-    bias."""
+    and the log-sums float32 [1, H, T], with a bias and their corrections [2, H, T]); ``plan``: (bucket of
+    each distance, spans, max_distance) of the bias."""
     args, _held, dev = _attention_args("window_attention", q, k, v, left, right, sinks, scale, ptr, mask, bias, plan)
     out = _like(q)
     rest = lse = None
     if train:
         rest = _like(q) if q.dtype is not torch.float32 else None
-        lse = torch.empty(2, q.shape[1], q.shape[0], dtype=torch.float32, device=dev)
+        lse = torch.empty(1 if bias is None else 2, q.shape[1], q.shape[0], dtype=torch.float32, device=dev)
     with _nat.on_device(dev):
         _nat.check(_nat.lib().geo_window_attention_fwd(args, out.data_ptr(), _nat.ptr(rest), _nat.ptr(lse),
                                                        _nat.stream_of(dev)), "geo_window_attention_fwd")

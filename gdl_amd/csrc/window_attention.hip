@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
       const int64_t at = static_cast<int64_t>(h) * a.seq.T + i;
       const float sum = log2f(l), x = m + sum;
       lse[at] = l == 0.f ? kInf : x;
-      if (BIAS && far_sum(x)) lse[static_cast<int64_t>(a.Hq) * a.seq.T + at] = exp2_hw(x - m - sum);
+      if (BIAS) lse[static_cast<int64_t>(a.Hq) * a.seq.T + at] = far_sum(x) ? exp2_hw(x - m - sum) : 1.f;
     }
   }
 }

@@ -60,7 +60,7 @@ def _attention_op(q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], ptr: 
 @_attention_op.register_fake
 def _(q, k, v, bias, ptr, mask, left, right, sinks, max_distance, scale):
     rest = q.new_empty(0) if q.dtype is torch.float32 else q.new_empty(q.shape)
-    return q.new_empty(q.shape), rest, q.new_empty((2, q.shape[1], q.shape[0]), dtype=torch.float32)
+    return q.new_empty(q.shape), rest, q.new_empty((1 if bias is None else 2, q.shape[1], q.shape[0]), dtype=torch.float32)
 
 
 @torch.library.custom_op("geoembodied::window_attention_backward", mutates_args=())

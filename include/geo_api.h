@@ -637,9 +637,9 @@ typedef struct {
 } geo_window_attention_t;
 
 /* out [tokens, heads, head_dim]; for the backward (each may be NULL): rest, what the rounding of out
- * took from its values, of out's shape and type (16-bit types); lse [2, heads, tokens], log2 of the
- * softmax's sum, and with a bias, where that passes 4096 in magnitude, what its rounding left out, as a
- * factor (the other places of the second half are not written). */
+ * took from its values, of out's shape and type (16-bit types); lse [heads, tokens], log2 of the
+ * softmax's sum, with a bias [2, heads, tokens]: then what its rounding left out too, as a factor (1 where it
+ * is at most 4096 in magnitude). */
 int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, void* rest, float* lse, void* stream);
 /* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out,
  * rest (may be NULL) and lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of

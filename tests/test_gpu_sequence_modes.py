@@ -50,6 +50,39 @@ def test_compiled_gradients(dev, name, dtype):
     assert _equal(*results)
 
 
+OPS = {"window_attention": lambda a: (*a, 5, 0, 2, 9, 0.25), "gated_recurrence": lambda a: (*a, True, 8.0),
+       "window_attention_step": lambda a: (*a, 1, 9, 0.25), "window_cache_fill": lambda a: (*a[:4], 0, a[4], None),
+       "gated_recurrence_step": lambda a: (*a, None, 8.0)}
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("bias", [True, False])
+def test_the_ops_are_what_they_say(dev, name, bias):
+    """Schemas, registered gradients and shapes against what the ops do, all their outputs."""
+    args = _args(name, dev)
+    if not bias and name.startswith("window_attention"):
+        args[3 if name == "window_attention" else 6] = None
+    if name in ("window_attention", "gated_recurrence"):
+        args = [t.requires_grad_() if t is not None and t.is_floating_point() else t for t in args]
+    torch.library.opcheck(getattr(torch.ops.geoembodied, name).default, OPS[name](args))
+
+
+def test_batches(dev):
+    """vmap, and gradients of several vectors at once: a call each, or the same."""
+    from gdl_amd.functional import gated_recurrence, window_attention
+    torch.manual_seed(3)
+    q, k, v = (torch.randn(3, 20, 2, 16, device=dev) for _ in range(3))
+    out = torch.func.vmap(lambda a, b, c: window_attention(a, b, c, 4))(q, k, v)
+    assert torch.equal(out, torch.stack([window_attention(a, b, c, 4) for a, b, c in zip(q, k, v)]))
+    x = q[0].clone().requires_grad_()
+    g = torch.randn(3, 20, 2, 16, device=dev)
+    for f in (lambda y: window_attention(y, k[0], v[0], 4), lambda y: gated_recurrence(y[:, 0], k[0, :, 0], v[0, :, 0], v[0, 0, 0])[0]):
+        out = f(x)
+        rows = g if out.dim() == 3 else g[:, :, 0]
+        many, = torch.autograd.grad(out, x, rows, is_grads_batched=True, retain_graph=True)
+        assert torch.equal(many, torch.stack([torch.autograd.grad(out, x, r, retain_graph=True)[0] for r in rows]))
+
+
 @pytest.mark.parametrize("name", ["window_attention", "gated_recurrence"])
 def test_second_derivatives_are_refused(dev, name):
     call = CALLS[name][0]
