@@ -191,7 +191,10 @@ __global__ __launch_bounds__(64 * NW, WAVES) void attend_fwd(const Attend a, T* 
     // +inf where no key is seen: the backward's exp2(s - lse) is 0 there
     if (lse && half == 0) {
       const int64_t at = static_cast<int64_t>(h) * a.seq.T + i;
-      const float sum = log2f(l), x = m + sum;
+      const float sum = log2f(l);
+      float x = m + sum;
+      // a factor of at most 1: times what is near float16's largest value it has to stay one
+      if (BIAS && far_sum(x) && x - m > sum) x = nextafterf(x, -kInf);
       lse[at] = l == 0.f ? kInf : x;
       if (BIAS) lse[static_cast<int64_t>(a.Hq) * a.seq.T + at] = far_sum(x) ? exp2_hw(x - m - sum) : 1.f;
     }

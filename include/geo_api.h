@@ -638,8 +638,8 @@ typedef struct {
 
 /* out [tokens, heads, head_dim]; for the backward (each may be NULL): rest, what the rounding of out
  * took from its values, of out's shape and type (16-bit types); lse [heads, tokens], log2 of the
- * softmax's sum, with a bias [2, heads, tokens]: then what its rounding left out too, as a factor (1 where it
- * is at most 4096 in magnitude). */
+ * softmax's sum, with a bias [2, heads, tokens]: then what its rounding (down) left out too, as a factor (1
+ * where it is at most 4096 in magnitude). */
 int geo_window_attention_fwd(const geo_window_attention_t* args, void* out, void* rest, float* lse, void* stream);
 /* Gradients of q, k, v (contiguous, of the inputs' types) and of the bias, from the forward's out,
  * rest (may be NULL) and lse and the output's gradient (contiguous).  bucket_range [buckets][2]: the places x0 <= x < x1 of

@@ -58,3 +58,24 @@ def test_equal_weights(dev, dtype):
                             (dk, ds.transpose(1, 2) @ qd / D ** 0.5, size.transpose(1, 2) @ qd.abs() / D ** 0.5)):
         bound = (3 * u + 2.0 ** -16) * term + u * want.abs() + 2.0 ** -20
         assert ((got.detach().double().cpu().transpose(0, 1) - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("bias", [-2e7, 5e7, 1e8, -1.3e8])
+def test_many_keys_and_large_gradients(dev, dtype, bias):
+    """Log-sums whose units (4 to 16) are as large as log2 of the 4096 keys, output gradients of 4096: as above,
+    with the spacing of float16 below its normal numbers, 2^-24, in the gradient times the factor, for every key."""
+    from gdl_amd.functional import window_attention
+    T, H, D = 4096, 2, 32
+    gen = torch.Generator().manual_seed(2)
+    q, k, v, g = (torch.randn(T, H, D, generator=gen).to(dev, dtype) for _ in range(4))
+    g = (g.float() * 4096).to(dtype)
+    table = torch.full((8, H), bias, device=dev)
+    leaves = [x.requires_grad_() for x in (q, k, v, table)]
+    out = window_attention(*leaves[:3], (None, 0), bias=table, max_distance=9)
+    dv = torch.autograd.grad(out, leaves, g)[2]
+    assert torch.isfinite(dv).all()
+    dv, gd, u = dv.double(), g.double(), UNIT[dtype]
+    bound = (2 * u + 2.0 ** -14) * gd.abs().sum(0) + u * dv.abs().sum(0) + T * T * 2.0 ** -25
+    off = (dv.sum(0) - gd.sum(0)).abs()
+    assert (off <= bound).all(), (off / bound).max()
