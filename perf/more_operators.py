@@ -1,0 +1,375 @@
+"""The work of streams that keep their whole history, as cases that can be timed and checked: keys and
+values of every token in pages of a shared pool (in the tokens' type or in 8 bits with a scale for
+each token and head), written, read back, and attended to by one new token of each stream.
+
+``run`` computes a case in plain torch operations in 32 bits (``own`` false) or through the
+framework's entry points (``own`` true).  ``exact`` is written apart from both, from the definitions,
+in 64 bits.
+
+A pool of P pages holds ``k [P, Hk, page, D]`` and ``v [P, Hk, page / blk, D, blk]``, where blk tokens
+take 64 bytes, and in 8 bits ``k_scale, v_scale [P, Hk, page]``; token j of a stream lies in page
+``table[stream, j // page]``.  Streams have random pages, unequal ages and tables wider than they need.
+
+Kinds of case:
+
+* ``step``   one new token per stream, written to its page and attending to all tokens up to itself
+* ``write``  tokens of packed sequences into the pages; in 8 bits also read back, as values
+* ``read``   the tokens of packed sequences out of the pages
+"""
+
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+LARGEST = {"int8": 127.0, "float8_e4m3fn": 448.0}
+
+
+def listed():
+    return [
+        # one young stream in float32, answered token by token with the relative bias: latency counts
+        dict(name="young_step", kind="step", b=1, n=1000, hq=4, hk=4, d=32, page=64, buckets=32, maxd=128, store="float32",
+             dtype="float32"),
+        # one scanner's stream of 131,072 points: few rows, a long axis
+        dict(name="long_step", kind="step", b=1, n=131072, hq=8, hk=2, d=64, page=64, buckets=0, maxd=0, store="bfloat16",
+             dtype="bfloat16"),
+        # a handful of small streams of an odd head size
+        dict(name="small_step", kind="step", b=7, n=700, hq=6, hk=2, d=24, page=64, buckets=16, maxd=64, store="float16",
+             dtype="float16"),
+        # many streams served together, unequal ages, shared key heads
+        dict(name="serve_step", kind="step", b=64, n=16384, hq=16, hk=4, d=128, page=64, buckets=0, maxd=0, store="bfloat16",
+             dtype="bfloat16"),
+        # twice as many in the same memory: the history in 8 bits, the largest case
+        dict(name="serve_int8_step", kind="step", b=128, n=16384, hq=16, hk=4, d=128, page=64, buckets=32, maxd=128, store="int8",
+             dtype="bfloat16"),
+        # a key head for each query head, float16 models over an 8-bit float history, larger pages
+        dict(name="serve_e4m3_step", kind="step", b=96, n=6000, hq=8, hk=8, d=64, page=128, buckets=0, maxd=0,
+             store="float8_e4m3fn", dtype="float16"),
+        # packets of a scanner, some hundred points for each of 32 streams in mid-page
+        dict(name="packet_write", kind="write", b=32, n=384, hk=8, d=64, page=64, late=True, store="float8_e4m3fn",
+             dtype="bfloat16"),
+        # a prompt of one lidar frame, kept in its own type
+        dict(name="frame_write", kind="write", b=1, n=131072, hk=4, d=128, page=64, late=False, store="bfloat16",
+             dtype="bfloat16"),
+        # a batch of unequal clouds of a float32 model, kept in 8 bits
+        dict(name="batch_int8_write", kind="write", b=16, n=4096, hk=4, d=32, page=64, late=False, store="int8",
+             dtype="float32"),
+        # one young stream's history: latency counts
+        dict(name="young_read", kind="read", b=1, n=500, hk=2, d=64, page=64, late=False, store="float16", dtype="float16"),
+        # the histories of a batch, 8 bits to the model's type
+        dict(name="batch_int8_read", kind="read", b=16, n=8192, hk=4, d=128, page=64, late=False, store="int8",
+             dtype="bfloat16"),
+        # the later half of long histories, in float32
+        dict(name="late_e4m3_read", kind="read", b=4, n=16384, hk=8, d=64, page=256, late=True, store="float8_e4m3fn",
+             dtype="float32"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    most = {kind: max(work(c)["bytes"] for c in listed() if c["kind"] == kind) for kind in ("step", "write", "read")}
+    while True:
+        kind = rng.choice(["step", "step", "step", "write", "read"])
+        dtype = rng.choice(["float32", "bfloat16", "bfloat16", "float16"])
+        store = rng.choice([dtype, "int8", "float8_e4m3fn"])
+        hk = rng.choice([1, 2, 3, 4, 8])
+        d = rng.choice([16, 32, 48, 64, 80, 128] if store in LARGEST else [8, 16, 24, 32, 40, 64, 80, 128])
+        page = rng.choice([64, 64, 128, 256])
+        if kind == "step":
+            bias = rng.random() < 0.5
+            c = dict(kind=kind, b=_log(rng, 1, 300), n=_log(rng, 1, 131072), hq=hk * rng.choice([1, 2, 3, 4, 8, 20]), hk=hk, d=d,
+                     page=page, buckets=rng.choice([16, 32]) if bias else 0, maxd=rng.choice([64, 128, 400]) if bias else 0,
+                     store=store, dtype=dtype)
+            # the plain form holds all of it, and the scores, in float32
+            if work(c)["bytes"] < most[kind] and c["b"] * c["n"] * (hk * d + c["hq"]) < 1.2e9:
+                return c
+        else:
+            c = dict(kind=kind, b=_log(rng, 1, 100), n=_log(rng, 1, 131072), hk=hk, d=d, page=page, late=rng.random() < 0.5,
+                     store=store, dtype=dtype)
+            if work(c)["bytes"] < most[kind]:
+                return c
+
+
+def _lengths(case):
+    """Tokens of each stream (steps: the new one among them): n for a single one, else from n / 3 to n."""
+    b, n = case["b"], case["n"]
+    return [n] if b == 1 else [max(1, n - (n * ((i * 29 + 11) % 64)) // 96) for i in range(b)]
+
+
+def _starts(case):
+    """Position of each sequence's first token: late ones come behind as much history as they are long, in mid-page."""
+    return [n + 7 * i if case["late"] else 0 for i, n in enumerate(_lengths(case))]
+
+
+def _ends(case):
+    """Tokens that each stream's pages hold."""
+    return _lengths(case) if case["kind"] == "step" else [a + n for a, n in zip(_starts(case), _lengths(case))]
+
+
+def _block(store):
+    return 64 // getattr(torch, store).itemsize
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    dtype, store = getattr(torch, case["dtype"]), getattr(torch, case["store"])
+    b, hk, d, page = case["b"], case["hk"], case["d"], case["page"]
+
+    def normal(*shape):
+        return torch.randn(*shape, device=DEV, generator=g)
+
+    need = [-(-n // page) for n in _ends(case)]
+    pages = sum(need) + 3  # some that belong to nobody
+    order = torch.randperm(pages, device=DEV, generator=g).int()
+    # a table is as wide as the oldest stream needs and a little more; -1 where a stream has no page
+    column = torch.arange(max(need) + 2, device=DEV)
+    count = torch.tensor(need, device=DEV).unsqueeze(1)
+    at = torch.cumsum(count, 0) - count + column
+    table = torch.where(column < count, order[at.clamp(max=pages - 1)], -1).int()
+    s = {"case": case, "table": table, "k_scale": None, "v_scale": None}
+    blk = _block(case["store"])
+    if case["store"] in LARGEST:
+        for name in ("k", "v"):
+            x, scale = _quantise(normal(pages, hk, page, d).to(dtype), case["store"])
+            s[name], s[name + "_scale"] = x, scale
+    else:
+        s["k"], s["v"] = (torch.empty(pages, hk, page, d, device=DEV, dtype=store).normal_(generator=g) for _ in range(2))
+    v = s["v"].view(torch.uint8) if case["store"] in LARGEST else s["v"]
+    s["v"] = v.view(pages, hk, page // blk, blk, d).transpose(3, 4).contiguous().view(store)
+    if case["kind"] == "step":
+        x = normal(b, case["hq"] + 2 * hk, d).to(dtype)  # one projection's output
+        s["q"], s["k_new"], s["v_new"] = x.split((case["hq"], hk, hk), 1)
+        s["positions"] = torch.tensor(_lengths(case), device=DEV) - 1
+        s["bias"] = (0.5 * normal(case["buckets"], case["hq"])).to(dtype) if case["buckets"] else None
+        s["tokens"], s["begin"] = b, torch.arange(b + 1, device=DEV)
+    else:
+        s["ptr"] = torch.tensor([0] + _lengths(case), device=DEV).cumsum(0)
+        s["start"] = torch.tensor(_starts(case), device=DEV)
+        s["tokens"] = sum(_lengths(case))
+        if case["kind"] == "write":
+            s["k_new"], s["v_new"] = normal(s["tokens"], 2 * hk, d).to(dtype).split((hk, hk), 1)
+    return s
+
+
+def run(s):
+    case = s["case"]
+    if own:
+        return _own(s, case)
+    dtype = getattr(torch, case["dtype"])
+    if case["kind"] == "step":
+        stream = torch.arange(case["b"], device=DEV)
+        _put(s, case, stream, s["positions"])
+        out = _attend(s, case)
+        if case["store"] not in LARGEST:
+            return {"out": out, "k": s["k"], "v": s["v"]}
+        k, v = _get(s, case, stream, s["positions"])
+        return {"out": out, "k": k.to(dtype), "v": v.to(dtype)}
+    t = torch.arange(s["tokens"], device=DEV)
+    stream = torch.searchsorted(s["ptr"][1:].contiguous(), t, right=True)
+    position = s["start"][stream] + t - s["ptr"][stream]
+    if case["kind"] == "write":
+        _put(s, case, stream, position)
+        if case["store"] not in LARGEST:
+            return {"k": s["k"], "v": s["v"]}
+    k, v = _get(s, case, stream, position)
+    return {"k": k.to(dtype), "v": v.to(dtype)}
+
+
+def _own(s, case):
+    from gdl_amd import functional as F
+
+    if "cache" not in s:  # the handle that a serving program keeps beside its tensors
+        s["cache"] = F.PagedCache(s["k"], s["v"], s["k_scale"], s["v_scale"])
+    cache, dtype, narrow = s["cache"], getattr(torch, case["dtype"]), case["store"] in LARGEST
+    if case["kind"] == "step":
+        out = F.paged_attention_step(s["q"], s["k_new"], s["v_new"], cache, s["table"], s["positions"], bias=s["bias"],
+                                     max_distance=case["maxd"] or 128)
+        if not narrow:
+            return {"out": out, "k": s["k"], "v": s["v"]}
+        k, v = cache.read(s["table"], s["begin"], s["tokens"], start=s["positions"], dtype=dtype)
+        return {"out": out, "k": k, "v": v}
+    if case["kind"] == "write":
+        cache.write(s["k_new"], s["v_new"], s["table"], s["ptr"], s["start"])
+        if not narrow:
+            return {"k": s["k"], "v": s["v"]}
+    k, v = cache.read(s["table"], s["ptr"], s["tokens"], start=s["start"], dtype=dtype)
+    return {"k": k, "v": v}
+
+
+# ------------------------------------------------------------------ plain forms, 32 bits ---
+
+def _quantise(x, store):
+    """(codes, scales) of rows x [..., D].  Products with the rate in 64 bits: with few bits in the inputs' types many lie
+    on a border between two codes, or next to one."""
+    largest = x.float().abs().amax(-1, keepdim=True)
+    kept = largest >= 2.0 ** -100
+    most = torch.full_like(largest, LARGEST[store]).double()  # a quotient in 64 bits, rounded to 32, is the 32-bit one
+    scale = torch.where(torch.isfinite(largest), torch.where(kept, (largest / most).float(), 0.0), math.nan)
+    rate = torch.where(kept & torch.isfinite(largest), (most / largest).float(), 0.0)
+    y = torch.where(rate > 0, x.double() * rate.double(), 0.0)
+    if store == "int8":
+        return y.round().to(torch.int8), scale.squeeze(-1)
+    # a step is an eighth of the power of two below a value, the least one 2^-9
+    step = torch.exp2(torch.frexp(y)[1].clamp(min=-5).double() - 4)
+    return ((y / step).round() * step).float().to(torch.float8_e4m3fn), scale.squeeze(-1)
+
+
+def _place(s, case, stream, position):
+    """Page and slot of tokens."""
+    return s["table"][stream, position // case["page"]].long(), position % case["page"]
+
+
+def _bits(t):
+    """8-bit floats as bytes, for indexing."""
+    return t.view(torch.uint8) if t.dtype is torch.float8_e4m3fn else t
+
+
+def _put(s, case, stream, position):
+    page, slot = _place(s, case, stream, position)
+    blk = _block(case["store"])
+    for name in ("k", "v"):
+        x = s[name + "_new"]
+        if case["store"] in LARGEST:
+            x, scale = _quantise(x, case["store"])
+            s[name + "_scale"][page, :, slot] = scale
+        if name == "k":
+            _bits(s["k"])[page, :, slot] = _bits(x)
+        else:
+            _bits(s["v"])[page, :, slot // blk, :, slot % blk] = _bits(x)
+
+
+def _get(s, case, stream, position):
+    """Values [T, Hk, D] of tokens, float32."""
+    page, slot = _place(s, case, stream, position)
+    blk = _block(case["store"])
+    k = _bits(s["k"])[page, :, slot].view(s["k"].dtype).float()
+    v = _bits(s["v"])[page, :, slot // blk, :, slot % blk].view(s["v"].dtype).float()
+    if case["store"] in LARGEST:
+        k, v = k * s["k_scale"][page, :, slot].unsqueeze(-1), v * s["v_scale"][page, :, slot].unsqueeze(-1)
+    return k, v
+
+
+_edges = {}
+
+
+def _bucket(back, buckets, maxd):
+    """Bucket of a distance back: one each for the nearest, then logarithmically wider ones up to maxd.  The buckets'
+    first distances come from the configuration alone."""
+    first, key = buckets // 2, (buckets, maxd, str(back.device))
+    if key not in _edges:
+        m = buckets - first
+        at, n = [], first
+        for k in range(1, m):
+            while n ** m < first ** (m - k) * maxd ** k:
+                n += 1
+            at.append(n)
+        _edges[key] = torch.tensor(at, device=back.device)
+    return torch.where(back < first, back, first + torch.searchsorted(_edges[key], back, right=True))
+
+
+def _attend(s, case):
+    q, b, hk, d = s["q"], case["b"], case["hk"], case["d"]
+    at = s["table"].clamp(min=0).long()
+    n = at.shape[1] * case["page"]
+    k = _bits(s["k"])[at].view(s["k"].dtype).float().transpose(1, 2).reshape(b, hk, n, d)
+    v = _bits(s["v"])[at].view(s["v"].dtype).float().permute(0, 2, 1, 3, 5, 4).reshape(b, hk, n, d)
+    if case["store"] in LARGEST:
+        k = k * s["k_scale"][at].transpose(1, 2).reshape(b, hk, n, 1)
+        v = v * s["v_scale"][at].transpose(1, 2).reshape(b, hk, n, 1)
+    score = torch.matmul(q.float().reshape(b, hk, -1, d), k.transpose(2, 3).contiguous()) * (1 / math.sqrt(d))
+    back = s["positions"].unsqueeze(1) - torch.arange(n, device=DEV)
+    if s["bias"] is not None:
+        bias = s["bias"].float()[_bucket(back.clamp(min=0), case["buckets"], case["maxd"])]
+        score = score + bias.transpose(1, 2).reshape(score.shape)
+    score = score.masked_fill((back < 0).view(b, 1, 1, n), -math.inf)
+    w = torch.exp(score - score.amax(-1, keepdim=True))
+    o = torch.matmul(w / w.sum(-1, keepdim=True), v)
+    return o.view(b, case["hq"], d).to(q.dtype)
+
+
+# ------------------------------------------------------------- what a pass cannot do without ---
+
+def work(case):
+    size, stored = getattr(torch, case["dtype"]).itemsize, getattr(torch, case["store"]).itemsize
+    narrow = case["store"] in LARGEST
+    t, hk, d = sum(_lengths(case)), case["hk"], case["d"]
+    row = hk * (2 * d * stored + (8 if narrow else 0))  # a token's keys and values in the pool
+    if case["kind"] == "step":
+        new = case["b"] * (2 * hk * d * size + row)
+        return {"bytes": t * row + 2 * case["b"] * case["hq"] * d * size + new, "flops": 4 * t * case["hq"] * d}
+    values = 2 * t * hk * d * size
+    if case["kind"] == "read":
+        return {"bytes": t * row + values, "flops": 0}
+    return {"bytes": values + t * row + (values if narrow else 0), "flops": 0}
+
+
+# ----------------------------------------------------------------- the definitions, 64 bits ---
+
+def _stored(x, store):
+    """Rows as the cache holds them, float64: codes are the products with float32(largest code / largest value), rounded
+    to even, values the codes' products with float32(largest value / largest code)."""
+    x = x.double()
+    if store not in LARGEST:
+        return x
+    top = x.abs().amax(-1, keepdim=True)
+    most = torch.full_like(top, LARGEST[store])
+    y = x * (most / top).float()
+    if store == "int8":
+        code = torch.round(y)
+    else:
+        least = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+        code = torch.round(y / least) * least
+    return torch.where(top < 2.0 ** -100, 0.0, code * (top / most).float())
+
+
+def _history(s, case, i, first, end):
+    """Values float64 [end - first, Hk, D] of stream i's tokens, from the pool."""
+    page, blk = case["page"], _block(case["store"])
+    at = s["table"][i, first // page:(end + page - 1) // page].long()
+    k = _bits(s["k"])[at].view(s["k"].dtype).double().permute(0, 2, 1, 3).flatten(0, 1)
+    v = _bits(s["v"])[at].view(s["v"].dtype).double().permute(0, 2, 4, 1, 3).flatten(0, 2)
+    if case["store"] in LARGEST:
+        k, v = (x * s[n + "_scale"][at].double().transpose(1, 2).flatten(0, 1).unsqueeze(-1) for x, n in ((k, "k"), (v, "v")))
+    skip = first // page * page
+    return k[first - skip:end - skip], v[first - skip:end - skip]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["kind"] == "read":
+        parts = [_history(s, case, i, a, a + n) for i, (a, n) in enumerate(zip(_starts(case), _lengths(case)))]
+        return {"k": torch.cat([p[0] for p in parts]), "v": torch.cat([p[1] for p in parts])}
+    k, v = _stored(s["k_new"], case["store"]), _stored(s["v_new"], case["store"])
+    if case["store"] in LARGEST:
+        kept = {"k": k, "v": v}
+    else:
+        kept = {"k": s["k"].clone(), "v": s["v"].clone()}
+        blk, t = _block(case["store"]), 0
+        first = [n - 1 for n in _lengths(case)] if case["kind"] == "step" else _starts(case)
+        for i, (a, n) in enumerate(zip(first, _lengths(case) if case["kind"] == "write" else [1] * case["b"])):
+            at = torch.arange(a, a + n, device=DEV)
+            page, slot = s["table"][i][at // case["page"]].long(), at % case["page"]
+            kept["k"][page, :, slot] = s["k_new"][t:t + n]
+            kept["v"][page, :, slot // blk, :, slot % blk] = s["v_new"][t:t + n]
+            t += n
+    if case["kind"] == "write":
+        return kept
+    out = torch.empty(case["b"], case["hq"], case["d"], device=DEV, dtype=torch.float64)
+    group = case["hq"] // case["hk"]
+    for i, n in enumerate(_lengths(case)):
+        ks, vs = (torch.cat([x, y[i:i + 1]]) for x, y in zip(_history(s, case, i, 0, n - 1), (k, v)))
+        score = torch.einsum("hgd,nhd->hgn", s["q"][i].double().view(case["hk"], group, -1), ks) / math.sqrt(case["d"])
+        if s["bias"] is not None:
+            half, far = case["buckets"] // 2, case["maxd"]
+            lut = [x if x < half else half + sum(x ** (case["buckets"] - half) >= half ** (case["buckets"] - half - m) * far ** m
+                                                 for m in range(1, case["buckets"] - half)) for x in range(far + 1)]
+            back = (n - 1 - torch.arange(n, device=DEV)).clamp(max=far)
+            score = score + s["bias"].double()[torch.tensor(lut, device=DEV)[back]].t().view(case["hk"], group, n)
+        out[i] = torch.einsum("hgn,nhd->hgd", score.softmax(-1), vs).reshape(case["hq"], -1)
+    return {"out": out, **kept}
