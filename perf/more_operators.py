@@ -13,6 +13,8 @@ take 64 bytes, and in 8 bits ``k_scale, v_scale [P, Hk, page]``; token j of a st
 Kinds of case:
 
 * ``step``   one new token per stream, written to its page and attending to all tokens up to itself
+* ``prompt``  several new tokens per stream, which the pages hold already, each attending to all tokens
+  up to itself
 * ``write``  tokens of packed sequences into the pages; in 8 bits also read back, as values
 * ``read``   the tokens of packed sequences out of the pages
 """
@@ -35,35 +37,33 @@ def listed():
         # one scanner's stream of 131,072 points: few rows, a long axis
         dict(name="long_step", kind="step", b=1, n=131072, hq=8, hk=2, d=64, page=64, buckets=0, maxd=0, store="bfloat16",
              dtype="bfloat16"),
-        # a handful of small streams of an odd head size
-        dict(name="small_step", kind="step", b=7, n=700, hq=6, hk=2, d=24, page=64, buckets=16, maxd=64, store="float16",
-             dtype="float16"),
         # many streams served together, unequal ages, shared key heads
         dict(name="serve_step", kind="step", b=64, n=16384, hq=16, hk=4, d=128, page=64, buckets=0, maxd=0, store="bfloat16",
              dtype="bfloat16"),
-        # twice as many in the same memory: the history in 8 bits, the largest case
+        # twice as many in the same memory: the history in 8 bits
         dict(name="serve_int8_step", kind="step", b=128, n=16384, hq=16, hk=4, d=128, page=64, buckets=32, maxd=128, store="int8",
              dtype="bfloat16"),
         # a key head for each query head, float16 models over an 8-bit float history, larger pages
         dict(name="serve_e4m3_step", kind="step", b=96, n=6000, hq=8, hk=8, d=64, page=128, buckets=0, maxd=0,
              store="float8_e4m3fn", dtype="float16"),
-        # packets of a scanner, some hundred points for each of 32 streams in mid-page
-        dict(name="packet_write", kind="write", b=32, n=384, hk=8, d=64, page=64, late=True, store="float8_e4m3fn",
+        # one small object's tokens in float32 with the relative bias: latency counts
+        dict(name="object_prompt", kind="prompt", b=1, n=300, past=0, hq=4, hk=4, d=32, page=64, buckets=32, maxd=128,
+             store="float32", dtype="float32"),
+        # packets of a scanner, some hundred points for each of 32 streams behind some thousand
+        dict(name="packet_prompt", kind="prompt", b=32, n=384, past=4000, hq=8, hk=2, d=64, page=64, buckets=0, maxd=0,
+             store="float8_e4m3fn", dtype="bfloat16"),
+        # long prompts in pieces: 2048 tokens of a piece behind 8192, the largest case
+        dict(name="piece_prompt", kind="prompt", b=8, n=2048, past=8192, hq=16, hk=4, d=128, page=64, buckets=0, maxd=0,
+             store="bfloat16", dtype="bfloat16"),
+        # those packets' keys and values into the pages, in mid-page
+        dict(name="packet_write", kind="write", b=32, n=384, past=4000, hk=8, d=64, page=64, store="float8_e4m3fn",
              dtype="bfloat16"),
-        # a prompt of one lidar frame, kept in its own type
-        dict(name="frame_write", kind="write", b=1, n=131072, hk=4, d=128, page=64, late=False, store="bfloat16",
-             dtype="bfloat16"),
-        # a batch of unequal clouds of a float32 model, kept in 8 bits
-        dict(name="batch_int8_write", kind="write", b=16, n=4096, hk=4, d=32, page=64, late=False, store="int8",
-             dtype="float32"),
+        # one lidar frame, kept in its own type
+        dict(name="frame_write", kind="write", b=1, n=131072, past=0, hk=4, d=128, page=64, store="bfloat16", dtype="bfloat16"),
         # one young stream's history: latency counts
-        dict(name="young_read", kind="read", b=1, n=500, hk=2, d=64, page=64, late=False, store="float16", dtype="float16"),
+        dict(name="young_read", kind="read", b=1, n=500, past=0, hk=2, d=64, page=64, store="float16", dtype="float16"),
         # the histories of a batch, 8 bits to the model's type
-        dict(name="batch_int8_read", kind="read", b=16, n=8192, hk=4, d=128, page=64, late=False, store="int8",
-             dtype="bfloat16"),
-        # the later half of long histories, in float32
-        dict(name="late_e4m3_read", kind="read", b=4, n=16384, hk=8, d=64, page=256, late=True, store="float8_e4m3fn",
-             dtype="float32"),
+        dict(name="batch_int8_read", kind="read", b=16, n=8192, past=0, hk=4, d=128, page=256, store="int8", dtype="bfloat16"),
     ]
 
 
@@ -72,27 +72,32 @@ def _log(rng, lo, hi):
 
 
 def draw(rng):
-    most = {kind: max(work(c)["bytes"] for c in listed() if c["kind"] == kind) for kind in ("step", "write", "read")}
+    top = {c["name"]: work(c) for c in listed()}
+    most = {"step": top["serve_int8_step"]["bytes"], "write": top["frame_write"]["bytes"], "read": top["batch_int8_read"]["bytes"]}
     while True:
-        kind = rng.choice(["step", "step", "step", "write", "read"])
+        kind = rng.choice(["step", "step", "step", "prompt", "prompt", "write", "read"])
         dtype = rng.choice(["float32", "bfloat16", "bfloat16", "float16"])
         store = rng.choice([dtype, "int8", "float8_e4m3fn"])
-        hk = rng.choice([1, 2, 3, 4, 8])
-        d = rng.choice([16, 32, 48, 64, 80, 128] if store in LARGEST else [8, 16, 24, 32, 40, 64, 80, 128])
-        page = rng.choice([64, 64, 128, 256])
+        hk, bias = rng.choice([1, 2, 3, 4, 8]), kind in ("step", "prompt") and rng.random() < 0.5
+        c = dict(kind=kind, b=_log(rng, 1, 300 if kind == "step" else 60), n=_log(rng, 1, 4096 if kind == "prompt" else 131072), hk=hk,
+                 d=rng.choice([16, 32, 48, 64, 80, 128] if store in LARGEST else [8, 16, 24, 32, 40, 64, 80, 128]),
+                 page=rng.choice([64, 64, 128, 256]), store=store, dtype=dtype)
+        if kind != "step":
+            c.update(past=rng.choice([0, _log(rng, 1, 16384)]))
+        if kind in ("step", "prompt"):
+            c.update(hq=hk * rng.choice([1, 2, 3, 4, 8, 20]), buckets=rng.choice([16, 32]) if bias else 0,
+                     maxd=rng.choice([64, 128, 400]) if bias else 0)
+        # the plain form holds histories and scores in float32; products in float32 run at an eighth of the rate
+        held = max(_ends(c))
         if kind == "step":
-            bias = rng.random() < 0.5
-            c = dict(kind=kind, b=_log(rng, 1, 300), n=_log(rng, 1, 131072), hq=hk * rng.choice([1, 2, 3, 4, 8, 20]), hk=hk, d=d,
-                     page=page, buckets=rng.choice([16, 32]) if bias else 0, maxd=rng.choice([64, 128, 400]) if bias else 0,
-                     store=store, dtype=dtype)
-            # the plain form holds all of it, and the scores, in float32
-            if work(c)["bytes"] < most[kind] and c["b"] * c["n"] * (hk * d + c["hq"]) < 1.2e9:
+            if work(c)["bytes"] < most[kind] and c["b"] * held * (hk * c["d"] + c["hq"]) < 1.2e9:
                 return c
-        else:
-            c = dict(kind=kind, b=_log(rng, 1, 100), n=_log(rng, 1, 131072), hk=hk, d=d, page=page, late=rng.random() < 0.5,
-                     store=store, dtype=dtype)
-            if work(c)["bytes"] < most[kind]:
+        elif kind == "prompt":
+            room = top["piece_prompt"]["flops"] / (8 if dtype == "float32" else 1)
+            if work(c)["flops"] < room and c["b"] * held * (hk * c["d"] + c["n"] * c["hq"]) < 2.8e9:
                 return c
+        elif work(c)["bytes"] < most[kind]:
+            return c
 
 
 def _lengths(case):
@@ -102,8 +107,8 @@ def _lengths(case):
 
 
 def _starts(case):
-    """Position of each sequence's first token: late ones come behind as much history as they are long, in mid-page."""
-    return [n + 7 * i if case["late"] else 0 for i, n in enumerate(_lengths(case))]
+    """Position of each sequence's first token: behind a history, in mid-page."""
+    return [case["past"] + 7 * i if case["past"] else 0 for i in range(case["b"])]
 
 
 def _ends(case):
@@ -146,7 +151,6 @@ def prepare(case, seed):
         x = normal(b, case["hq"] + 2 * hk, d).to(dtype)  # one projection's output
         s["q"], s["k_new"], s["v_new"] = x.split((case["hq"], hk, hk), 1)
         s["positions"] = torch.tensor(_lengths(case), device=DEV) - 1
-        s["bias"] = (0.5 * normal(case["buckets"], case["hq"])).to(dtype) if case["buckets"] else None
         s["tokens"], s["begin"] = b, torch.arange(b + 1, device=DEV)
     else:
         s["ptr"] = torch.tensor([0] + _lengths(case), device=DEV).cumsum(0)
@@ -154,6 +158,10 @@ def prepare(case, seed):
         s["tokens"] = sum(_lengths(case))
         if case["kind"] == "write":
             s["k_new"], s["v_new"] = normal(s["tokens"], 2 * hk, d).to(dtype).split((hk, hk), 1)
+        elif case["kind"] == "prompt":
+            s["q"] = normal(s["tokens"], case["hq"] + 2 * hk, d).to(dtype)[:, :case["hq"]]  # of one projection's output
+    if case.get("hq"):
+        s["bias"] = (0.5 * normal(case["buckets"], case["hq"])).to(dtype) if case["buckets"] else None
     return s
 
 
@@ -165,7 +173,7 @@ def run(s):
     if case["kind"] == "step":
         stream = torch.arange(case["b"], device=DEV)
         _put(s, case, stream, s["positions"])
-        out = _attend(s, case)
+        out = _attend(s, case, s["q"].unsqueeze(1), s["positions"].unsqueeze(1)).squeeze(1)
         if case["store"] not in LARGEST:
             return {"out": out, "k": s["k"], "v": s["v"]}
         k, v = _get(s, case, stream, s["positions"])
@@ -173,6 +181,12 @@ def run(s):
     t = torch.arange(s["tokens"], device=DEV)
     stream = torch.searchsorted(s["ptr"][1:].contiguous(), t, right=True)
     position = s["start"][stream] + t - s["ptr"][stream]
+    if case["kind"] == "prompt":
+        row = t - s["ptr"][stream]
+        q = torch.zeros(case["b"], max(_lengths(case)), *s["q"].shape[1:], device=DEV, dtype=dtype)
+        at = torch.zeros(q.shape[:2], device=DEV, dtype=torch.long)
+        q[stream, row], at[stream, row] = s["q"], position
+        return {"out": _attend(s, case, q, at)[stream, row]}
     if case["kind"] == "write":
         _put(s, case, stream, position)
         if case["store"] not in LARGEST:
@@ -194,6 +208,9 @@ def _own(s, case):
             return {"out": out, "k": s["k"], "v": s["v"]}
         k, v = cache.read(s["table"], s["begin"], s["tokens"], start=s["positions"], dtype=dtype)
         return {"out": out, "k": k, "v": v}
+    if case["kind"] == "prompt":
+        return {"out": F.paged_attention(s["q"], cache, s["table"], s["ptr"], s["start"], bias=s["bias"],
+                                         max_distance=case["maxd"] or 128)}
     if case["kind"] == "write":
         cache.write(s["k_new"], s["v_new"], s["table"], s["ptr"], s["start"])
         if not narrow:
@@ -273,24 +290,26 @@ def _bucket(back, buckets, maxd):
     return torch.where(back < first, back, first + torch.searchsorted(_edges[key], back, right=True))
 
 
-def _attend(s, case):
-    q, b, hk, d = s["q"], case["b"], case["hk"], case["d"]
-    at = s["table"].clamp(min=0).long()
+def _attend(s, case, q, position):
+    """q [b, m, Hq, D] at positions [b, m] over the streams' pages."""
+    b, m, hq, d = q.shape
+    hk, at = case["hk"], s["table"].clamp(min=0).long()
     n = at.shape[1] * case["page"]
     k = _bits(s["k"])[at].view(s["k"].dtype).float().transpose(1, 2).reshape(b, hk, n, d)
     v = _bits(s["v"])[at].view(s["v"].dtype).float().permute(0, 2, 1, 3, 5, 4).reshape(b, hk, n, d)
     if case["store"] in LARGEST:
         k = k * s["k_scale"][at].transpose(1, 2).reshape(b, hk, n, 1)
         v = v * s["v_scale"][at].transpose(1, 2).reshape(b, hk, n, 1)
-    score = torch.matmul(q.float().reshape(b, hk, -1, d), k.transpose(2, 3).contiguous()) * (1 / math.sqrt(d))
-    back = s["positions"].unsqueeze(1) - torch.arange(n, device=DEV)
+    rows = q.float().view(b, m, hk, hq // hk, d).permute(0, 2, 3, 1, 4).reshape(b, hk, -1, d)
+    score = torch.matmul(rows, k.transpose(2, 3).contiguous()).view(b, hk, hq // hk, m, n) * (1 / math.sqrt(d))
+    back = position.unsqueeze(2) - torch.arange(n, device=DEV)
     if s["bias"] is not None:
-        bias = s["bias"].float()[_bucket(back.clamp(min=0), case["buckets"], case["maxd"])]
-        score = score + bias.transpose(1, 2).reshape(score.shape)
-    score = score.masked_fill((back < 0).view(b, 1, 1, n), -math.inf)
+        bias = s["bias"].float().t().reshape(hk, hq // hk, -1)[:, :, _bucket(back.clamp(min=0), case["buckets"], case["maxd"])]
+        score = score + bias.permute(2, 0, 1, 3, 4)
+    score = score.masked_fill((back < 0).view(b, 1, 1, m, n), -math.inf)
     w = torch.exp(score - score.amax(-1, keepdim=True))
-    o = torch.matmul(w / w.sum(-1, keepdim=True), v)
-    return o.view(b, case["hq"], d).to(q.dtype)
+    o = torch.matmul((w / w.sum(-1, keepdim=True)).view(b, hk, -1, n), v)
+    return o.view(b, hk, hq // hk, m, d).permute(0, 3, 1, 2, 4).reshape(b, m, hq, d).to(q.dtype)
 
 
 # ------------------------------------------------------------- what a pass cannot do without ---
@@ -303,6 +322,9 @@ def work(case):
     if case["kind"] == "step":
         new = case["b"] * (2 * hk * d * size + row)
         return {"bytes": t * row + 2 * case["b"] * case["hq"] * d * size + new, "flops": 4 * t * case["hq"] * d}
+    if case["kind"] == "prompt":
+        pairs = sum(n * a + n * (n + 1) // 2 for a, n in zip(_starts(case), _lengths(case)))
+        return {"bytes": sum(_ends(case)) * row + 2 * t * case["hq"] * d * size, "flops": 4 * pairs * case["hq"] * d}
     values = 2 * t * hk * d * size
     if case["kind"] == "read":
         return {"bytes": t * row + values, "flops": 0}
@@ -340,19 +362,35 @@ def _history(s, case, i, first, end):
     return k[first - skip:end - skip], v[first - skip:end - skip]
 
 
+def _softmax_rows(s, case, q, k, v, first):
+    """Queries float64 [m, Hq, D] at positions first .. over the values k, v [n, Hk, D]."""
+    m, n, hk = len(q), len(k), case["hk"]
+    score = torch.einsum("mhgd,nhd->hgmn", q.view(m, hk, -1, case["d"]), k) / math.sqrt(case["d"])
+    back = first + torch.arange(m, device=DEV).unsqueeze(1) - torch.arange(n, device=DEV)
+    if s["bias"] is not None:
+        half, far = case["buckets"] // 2, case["maxd"]
+        lut = [x if x < half else half + sum(x ** (case["buckets"] - half) >= half ** (case["buckets"] - half - j) * far ** j
+                                             for j in range(1, case["buckets"] - half)) for x in range(far + 1)]
+        bucket = torch.tensor(lut, device=DEV)[back.clamp(0, far)]
+        score = score + s["bias"].double()[bucket].permute(2, 0, 1).view(score.shape)
+    score = score.masked_fill(back < 0, -math.inf).softmax(-1)
+    return torch.einsum("hgmn,nhd->mhgd", score, v).reshape(m, -1, case["d"])
+
+
 def exact(case, seed):
     s = prepare(case, seed)
+    spans = list(zip(_starts(case), _lengths(case))) if case["kind"] != "step" else [(n - 1, 1) for n in _lengths(case)]
     if case["kind"] == "read":
-        parts = [_history(s, case, i, a, a + n) for i, (a, n) in enumerate(zip(_starts(case), _lengths(case)))]
+        parts = [_history(s, case, i, a, a + n) for i, (a, n) in enumerate(spans)]
         return {"k": torch.cat([p[0] for p in parts]), "v": torch.cat([p[1] for p in parts])}
-    k, v = _stored(s["k_new"], case["store"]), _stored(s["v_new"], case["store"])
-    if case["store"] in LARGEST:
+    kept = {}
+    if case["kind"] != "prompt":
+        k, v = _stored(s["k_new"], case["store"]), _stored(s["v_new"], case["store"])
         kept = {"k": k, "v": v}
-    else:
+    if kept and case["store"] not in LARGEST:
         kept = {"k": s["k"].clone(), "v": s["v"].clone()}
         blk, t = _block(case["store"]), 0
-        first = [n - 1 for n in _lengths(case)] if case["kind"] == "step" else _starts(case)
-        for i, (a, n) in enumerate(zip(first, _lengths(case) if case["kind"] == "write" else [1] * case["b"])):
+        for i, (a, n) in enumerate(spans):
             at = torch.arange(a, a + n, device=DEV)
             page, slot = s["table"][i][at // case["page"]].long(), at % case["page"]
             kept["k"][page, :, slot] = s["k_new"][t:t + n]
@@ -360,16 +398,14 @@ def exact(case, seed):
             t += n
     if case["kind"] == "write":
         return kept
-    out = torch.empty(case["b"], case["hq"], case["d"], device=DEV, dtype=torch.float64)
-    group = case["hq"] // case["hk"]
-    for i, n in enumerate(_lengths(case)):
-        ks, vs = (torch.cat([x, y[i:i + 1]]) for x, y in zip(_history(s, case, i, 0, n - 1), (k, v)))
-        score = torch.einsum("hgd,nhd->hgn", s["q"][i].double().view(case["hk"], group, -1), ks) / math.sqrt(case["d"])
-        if s["bias"] is not None:
-            half, far = case["buckets"] // 2, case["maxd"]
-            lut = [x if x < half else half + sum(x ** (case["buckets"] - half) >= half ** (case["buckets"] - half - m) * far ** m
-                                                 for m in range(1, case["buckets"] - half)) for x in range(far + 1)]
-            back = (n - 1 - torch.arange(n, device=DEV)).clamp(max=far)
-            score = score + s["bias"].double()[torch.tensor(lut, device=DEV)[back]].t().view(case["hk"], group, n)
-        out[i] = torch.einsum("hgn,nhd->hgd", score.softmax(-1), vs).reshape(case["hq"], -1)
-    return {"out": out, **kept}
+    out, t = [], 0
+    for i, (a, n) in enumerate(spans):
+        if case["kind"] == "step":
+            ks, vs = (torch.cat([x, y[i:i + 1]]) for x, y in zip(_history(s, case, i, 0, a), (k, v)))
+        else:
+            ks, vs = _history(s, case, i, 0, a + n)
+        for at in range(0, n, 512):
+            end = min(at + 512, n)
+            out.append(_softmax_rows(s, case, s["q"][t + at:t + end].double(), ks[:a + end], vs[:a + end], a + at))
+        t += n
+    return {"out": torch.cat(out), **kept}
