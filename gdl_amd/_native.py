@@ -37,6 +37,10 @@ pack_window_attention = struct.Struct("=3Q6q4Q5q7if").pack
 pack_window_step = struct.Struct("=5Q10q3Q3q7if").pack
 # geo_recurrence_t: 3 tensors, 3 strides, decay, ptr, state, 3 sizes, 2 codes, rate, 4 bytes to the end
 pack_recurrence = struct.Struct("=3Q3q3Q3q2if4x").pack
+# geo_paged_t: 5 tensors, table stride, 2 sizes, 4 codes; geo_paged_step_t: that, 3 tensors, 6 strides, positions, bias,
+# bias_lut, batch, 5 codes, scale
+pack_paged = struct.Struct("=5Q3q4i").pack
+pack_paged_step = struct.Struct("=80s3Q6q3Qq5if").pack
 
 
 def at(t: torch.Tensor | None) -> int:
@@ -155,6 +159,10 @@ _SIGNATURES = {
     "geo_window_attention_step": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
     "geo_window_cache_fill": (c_int, [c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
                                       c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "geo_paged_write": (c_int, [c_bytes, c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp]),
+    "geo_paged_read": (c_int, [c_bytes, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "geo_paged_attention_step_workspace_bytes": (c_size, [c_bytes]),
+    "geo_paged_attention_step": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_carry_size": (c_i64, [c_i64, c_i64]),
     "geo_recurrence_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_bwd_workspace_bytes": (c_size, [c_i64, c_i64]),
@@ -169,6 +177,8 @@ GEO_F32, GEO_BF16, GEO_F64 = 0, 1, 2
 GEO_F16 = 3
 # element types of the sequence operators
 SEQUENCE_DTYPES = {torch.float32: GEO_F32, torch.bfloat16: GEO_BF16, torch.float16: GEO_F16}
+# element types of paged caches
+PAGED_DTYPES = {**SEQUENCE_DTYPES, torch.int8: 4, torch.float8_e4m3fn: 5}
 REDUCE_CODES = {"sum": 0, "mean": 1, "max": 2}
 DTYPE_CODES = {torch.float32: GEO_F32, torch.bfloat16: GEO_BF16, torch.float64: GEO_F64}
 

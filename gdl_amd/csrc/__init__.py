@@ -655,6 +655,80 @@ def window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start):
             _nat.stream_of(dev)), "geo_window_cache_fill")
 
 
+def _paged_args(k, v, k_scale, v_scale, table):
+    """geo_paged_t of a pool (packed), and the table that it points into."""
+    if table.stride(1) != 1 and table.shape[1] > 1:
+        table = table.contiguous()
+    at = _nat.at
+    pages, heads, page, d = k.shape
+    return _nat.pack_paged(k.data_ptr(), v.data_ptr(), at(k_scale), at(v_scale), table.data_ptr(), table.stride(0), pages,
+                           table.shape[1], _nat.PAGED_DTYPES[k.dtype], heads, d, page), table
+
+
+def _paged_spans(dev, ptr, start):
+    return None if ptr is None else _i64(ptr, dev), None if start is None else _i64(start, dev)
+
+
+def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start):
+    """Tokens k, v [T, Hk, D] of packed sequences into the pages that ``table`` gives their streams."""
+    name = "PagedCache.write"
+    dev = _sequence_device(name, k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
+    code = _sequence_code(name, k, v)
+    k, v = _in_pieces(k), _in_pieces(v)
+    ptr, start = _paged_spans(dev, ptr, start)
+    cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
+    with _nat.on_device(dev):
+        _nat.check(_nat.lib().geo_paged_write(
+            cache, code, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _nat.ptr(ptr),
+            _nat.ptr(start), k.shape[0], table.shape[0], _nat.stream_of(dev)), "geo_paged_write")
+
+
+def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens, dtype):
+    """(k, v) [tokens, Hk, D]: the values of packed sequences' tokens out of the pages."""
+    dev = _sequence_device("PagedCache.read", k_pages, v_pages, k_scale, v_scale, table, ptr, start)
+    ptr, start = _paged_spans(dev, ptr, start)
+    cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
+    k, v = (torch.empty(tokens, k_pages.shape[1], k_pages.shape[3], dtype=dtype, device=dev) for _ in range(2))
+    with _nat.on_device(dev):
+        _nat.check(_nat.lib().geo_paged_read(
+            cache, _nat.SEQUENCE_DTYPES[dtype], _nat.ptr(ptr), _nat.ptr(start), tokens, table.shape[0], k.data_ptr(),
+            v.data_ptr(), _nat.stream_of(dev)), "geo_paged_read")
+    return k, v
+
+
+def _paged_bias(name, bias, plan):
+    """(bias, lut, type code, max_distance, buckets) as the packed structures take them."""
+    if bias is None:
+        return None, None, 0, 0, 0
+    lut, _, maxd = plan
+    return bias.contiguous(), lut, _sequence_code(f"{name} bias", bias), maxd, bias.shape[0]
+
+
+def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, scale, bias, plan):
+    """[B, H, D] of the tokens at ``positions``, whose k and v go into the streams' pages."""
+    name = "paged_attention_step"
+    dev = _sequence_device(name, q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, bias)
+    code = _sequence_code(name, q, k, v)
+    q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
+    positions = _i64(positions, dev)
+    B, H, _ = q.shape
+    cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
+    bias, lut, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
+    (qs, qh, _), (ks, kh, _), (vs, vh, _) = q.stride(), k.stride(), v.stride()
+    at = _nat.at
+    args = _nat.pack_paged_step(cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, qh, ks, kh, vs, vh, positions.data_ptr(),
+                                at(bias), at(lut), B, code, bias_code, H, buckets, maxd, scale)
+    out = _like(q)
+    L = _nat.lib()
+    with _nat.on_device(dev):
+        ws_bytes = L.geo_paged_attention_step_workspace_bytes(args)
+        # from the allocator, which keeps what a captured call was given for the graph's replays
+        ws = _nat.workspace(ws_bytes, dev) if ws_bytes else None
+        _nat.check(L.geo_paged_attention_step(args, out.data_ptr(), _nat.ptr(ws), ws_bytes, _nat.stream_of(dev)),
+                   "geo_paged_attention_step")
+    return out
+
+
 def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate, streams=None):
     """geo_recurrence_t of the call (packed), the tensors that it points into, the device and the
     number of sequences (``streams``: that many of one token each)."""
@@ -1105,7 +1179,7 @@ __all__ = [
     "graph_avg_degree_hip",
     "segment_reduce_forward_hip", "segment_reduce_backward_hip",
     "window_attention_forward_hip", "window_attention_backward_hip", "window_attention_step_hip",
-    "window_cache_fill_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
+    "window_cache_fill_hip", "paged_write_hip", "paged_read_hip", "paged_attention_step_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
     "gated_recurrence_step_hip",
     "knn_available", "knn_cuda", "knn_self_cuda",
     "fps_available", "fps_cuda", "fps_uniform_hip",

@@ -1,0 +1,156 @@
+// paged.hpp — keys and values of streams in pages of a shared pool: the layout, the 8-bit codes, and
+// where the tokens of packed sequences lie.
+//
+// k [pages, Hk, page, D] row by row; v [pages, Hk, page / blk, D, blk], blk tokens to 64 bytes: a matrix
+// instruction's operand of the values is 16 bytes of one dimension's tokens, so a wave's read of 16
+// dimensions is one contiguous KiB and nothing is turned on the way.  Both take 64 D bytes for blk
+// tokens, so a token block begins at the same offset in either.
+#pragma once
+
+#include "attention_tile.hpp"
+
+namespace geo {
+namespace paged {
+
+using attn::kInf;
+using attn::exp2_hw;
+using attn::kLog2e;
+
+// Element types of 8-bit pools: whole numbers and e4m3 floats, each token and head with a scale.
+struct I8 { uint8_t bits; };
+struct E4 { uint8_t bits; };
+
+template <typename C> struct Code { static constexpr bool kNarrow = false; };
+template <> struct Code<I8> {
+  static constexpr bool kNarrow = true;
+  static constexpr float kMost = 127.f;
+  // The product x rate, rounded once: the sum with 1.5 * 2^23 has steps of 1 (to even).
+  static __device__ __forceinline__ float round(float x, float rate) {
+    constexpr float kStep1 = 12582912.f;
+    return fmaf(x, rate, kStep1) - kStep1;
+  }
+  static __device__ __forceinline__ uint8_t bits(float y) { return static_cast<uint8_t>(static_cast<int>(y)); }
+  static __device__ __forceinline__ float value(uint8_t b) { return static_cast<float>(static_cast<int8_t>(b)); }
+};
+template <> struct Code<E4> {
+  static constexpr bool kNarrow = true;
+  static constexpr float kMost = 448.f;
+  // The same with steps of an eighth of the product's power of two, at least 2^-9.
+  static __device__ __forceinline__ float round(float x, float rate) {
+    const uint32_t power = max(__float_as_uint(x * rate) & 0x7f800000u, 0x3c800000u);
+    const float big = __uint_as_float((power + (20u << 23)) | 0x400000u);
+    return fmaf(x, rate, big) - big;
+  }
+  static __device__ __forceinline__ uint8_t bits(float y) {
+    return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false));
+  }
+  static __device__ __forceinline__ float value(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8(b, 0); }
+};
+
+// How a row of largest magnitude a (its bits, so that NaN counts as most) is kept: values are code * scale,
+// codes the exact products x * rate rounded once.  Rows below 2^-100 are kept as zeros; one with an
+// infinity or a NaN has a scale of NaN and reads back so.
+struct RowScale { float scale, rate; };
+template <typename C>
+__device__ __forceinline__ RowScale row_scale(uint32_t most_bits) {
+  const float a = __uint_as_float(most_bits);
+  if (most_bits >= 0x7f800000u) return {__builtin_nanf(""), 0.f};
+  if (a < 0x1p-100f) return {0.f, 0.f};
+  return {a / Code<C>::kMost, Code<C>::kMost / a};
+}
+template <typename C>
+__device__ __forceinline__ float encode(float x, float rate) { return rate > 0.f ? Code<C>::round(x, rate) : 0.f; }
+
+// Largest of unsigned numbers over a group of LW = 4, 8 or 16 lanes, in all of them.
+template <int LW>
+__device__ __forceinline__ uint32_t group_most(uint32_t x) {
+  x = max(x, dpp_u32<kDppXor1>(x));
+  x = max(x, dpp_u32<kDppXor2>(x));
+  if constexpr (LW >= 8) x = max(x, dpp_u32<kDppHalfMirror>(x));
+  if constexpr (LW >= 16) x = max(x, dpp_u32<kDppMirror>(x));
+  return x;
+}
+
+struct Pool {
+  char *k, *v;
+  float *ks, *vs;        // [pages, Hk, page], of 8-bit pools
+  const int32_t* table;  // [streams, columns]: page of each `page` tokens
+  int64_t table_st;
+  int pages, columns, page, Hk, D;
+};
+
+template <typename C>
+constexpr int block_tokens() { return 64 / static_cast<int>(sizeof(C)); }
+
+// The packed sequences cut into tiles of U tokens' positions, at multiples of U.  Sequence b has at most
+// n / U + 2 of them, so its tiles are numbered from ptr[b] / U + 2 b on; numbers without a tile are idle.
+inline int64_t tiles_of(int64_t tokens, int64_t batch, int unit) { return tokens / unit + 2 * batch; }
+
+struct Span {
+  int64_t first, start;  // row of the sequence's first token, and its position
+  int64_t tile0;         // the tile's first position
+  int b, lo, hi;         // the sequence; the tile's places that have tokens, lo .. hi - 1 (none: lo >= hi)
+};
+// Wave-wide: 64 sequences are looked at together.
+template <int U>
+__device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile) {
+  const int lane = threadIdx.x & 63;
+  auto offset = [&](int b) { return ptr ? min(max(ptr[b], int64_t(0)), T) : b ? T : int64_t(0); };
+  int lo = 0, len = B;
+  bool some = true;
+  do {
+    const int step = (len + 63) / 64, at = lo + lane * step;
+    const bool ok = at < lo + len && offset(at) / U + 2 * static_cast<int64_t>(at) <= tile;
+    const int n = __popcll(__ballot(ok));
+    some = some && n > 0;
+    const int next = lo + max(n - 1, 0) * step;
+    len = min(step, lo + len - next);
+    lo = next;
+  } while (len > 1);
+  const int b = __builtin_amdgcn_readfirstlane(lo);
+  Span s{offset(b), start ? start[b] : 0, 0, b, 0, 0};
+  const int64_t n = offset(b + 1) - s.first, from = max(s.start, int64_t(0)), end = s.start + n;
+  s.tile0 = (from / U + tile - (s.first / U + 2 * static_cast<int64_t>(b))) * U;
+  if (!some || s.tile0 >= end) return s;
+  s.lo = static_cast<int>(max(from - s.tile0, int64_t(0)));
+  s.hi = static_cast<int>(min(end - s.tile0, int64_t(U)));
+  return s;
+}
+
+// The page of a stream's column, or -1 where the table or the pool has none.
+__device__ __forceinline__ int page_of(const Pool& p, int b, int64_t column) {
+  if (column >= p.columns) return -1;
+  const int n = p.table[b * p.table_st + column];
+  return static_cast<uint32_t>(n) < static_cast<uint32_t>(p.pages) ? n : -1;
+}
+
+// Checks on the host; fills *pool.
+inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool) {
+  GEO_REQUIRE(g, "%s: null arguments", name);
+  const bool narrow = g->stored == GEO_I8 || g->stored == GEO_E4M3;
+  GEO_REQUIRE(narrow || g->stored == GEO_F32 || g->stored == GEO_BF16 || g->stored == GEO_F16, "%s: pool type code %d", name,
+              static_cast<int>(g->stored));
+  GEO_REQUIRE(g->kv_heads >= 1 && g->kv_heads < (1 << 16), "%s: %d key heads", name, g->kv_heads);
+  GEO_REQUIRE(g->head_dim >= 8 && g->head_dim <= 128 && g->head_dim % (narrow ? 16 : 8) == 0,
+              "%s: head size %d (a multiple of %d up to 128)", name, g->head_dim, narrow ? 16 : 8);
+  GEO_REQUIRE(g->page >= 64 && g->page % 64 == 0 && g->page <= (1 << 20), "%s: pages of %d tokens (a multiple of 64 up to 2^20)",
+              name, g->page);
+  GEO_REQUIRE(g->pages >= 1 && g->pages < (int64_t(1) << 31), "%s: %lld pages", name, static_cast<long long>(g->pages));
+  GEO_REQUIRE(g->columns >= 1 && g->columns * g->page < (int64_t(1) << 30), "%s: a table of %lld columns of %d tokens (below 2^30)",
+              name, static_cast<long long>(g->columns), g->page);
+  auto aligned = [](const void* p) { return p && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  GEO_REQUIRE(aligned(g->k) && aligned(g->v) && g->k != g->v, "%s: null pool, not on 16 bytes, or one for both", name);
+  GEO_REQUIRE(!narrow || (aligned(g->k_scale) && aligned(g->v_scale) && g->k_scale != g->v_scale),
+              "%s: an 8-bit pool needs scales, on 16 bytes", name);
+  GEO_REQUIRE(g->table, "%s: null table", name);
+  *pool = Pool{static_cast<char*>(g->k), static_cast<char*>(g->v), g->k_scale, g->v_scale, g->table, g->table_stream,
+               static_cast<int>(g->pages), static_cast<int>(g->columns), g->page, g->kv_heads, g->head_dim};
+  return GEO_OK;
+}
+inline bool type_ok(int dtype, int stored) {
+  return (dtype == GEO_F32 || dtype == GEO_BF16 || dtype == GEO_F16) &&
+         (stored == dtype || stored == GEO_I8 || stored == GEO_E4M3);
+}
+
+}  // namespace paged
+}  // namespace geo

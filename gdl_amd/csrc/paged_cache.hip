@@ -1,0 +1,278 @@
+// paged_cache.hip — tokens of packed sequences into the pages of a pool and out of them.
+//
+// A workgroup takes 64 positions of one sequence, at a multiple of 64, and one key head: a part of one
+// page.  Keys are rows on both sides.  Values are turned in LDS, so that reads and writes of memory are
+// contiguous on both sides.  An 8-bit row's largest magnitude is found by the lanes that hold it.
+#include "paged.hpp"
+
+namespace geo {
+namespace paged {
+
+constexpr int kTile = 64, kThreads = 256;
+
+// Eight values of a row of type T in float32.
+template <typename T>
+struct Eight {
+  union { uint4 u[sizeof(T) / 2]; T t[8]; };
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) u[n] = reinterpret_cast<const uint4*>(p)[n];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) reinterpret_cast<uint4*>(p)[n] = u[n];
+  }
+};
+template <typename T, typename C>
+struct Kept {  // eight values as the pool holds them
+  union { uint4 w[sizeof(C) * 8 > 16 ? 2 : 1]; uint2 n; C c[8]; };
+  float scale;
+  // from the row's values, by the LW lanes that share the row
+  template <int LW>
+  __device__ __forceinline__ void from(const Eight<T>& x) {
+    if constexpr (Code<C>::kNarrow) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(static_cast<float>(x.t[e])) & 0x7fffffffu);
+      const RowScale s = row_scale<C>(group_most<LW>(most));
+      scale = s.scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e].bits = Code<C>::bits(encode<C>(static_cast<float>(x.t[e]), s.rate));
+    } else {
+#pragma unroll
+      for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) w[n] = x.u[n];
+    }
+  }
+  __device__ __forceinline__ void to(Eight<T>& x) const {
+    if constexpr (Code<C>::kNarrow) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.t[e] = static_cast<T>(Code<C>::value(c[e].bits) * scale);
+    } else {
+#pragma unroll
+      for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) x.u[n] = w[n];
+    }
+  }
+  __device__ __forceinline__ void load(const C* p) {
+    if constexpr (sizeof(C) == 1) {
+      n = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(C) / 2); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+  }
+  __device__ __forceinline__ void store(C* p) const {
+    if constexpr (sizeof(C) == 1) {
+      *reinterpret_cast<uint2*>(p) = n;
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(C) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    }
+  }
+};
+
+// LDS rows of a tile's values: 16 bytes (8 of 8-bit types) more than the row, so that rows begin in other banks.
+template <typename C, int LW>
+constexpr int lds_row() { return 8 * LW + (sizeof(C) == 1 ? 8 : 16 / static_cast<int>(sizeof(C))); }
+
+template <typename T, typename C, int LW>
+__global__ __launch_bounds__(kThreads) void paged_write(const Pool p, const T* __restrict__ k, const T* __restrict__ v, int64_t k_st,
+                                                        int64_t k_sh, int64_t v_st, int64_t v_sh, const int64_t* __restrict__ ptr,
+                                                        const int64_t* __restrict__ start, int64_t T_all, int B) {
+  constexpr int kRow = lds_row<C, LW>(), kGroups = kThreads / LW, kBlk = block_tokens<C>(), kPer = 16 / sizeof(C);
+  __shared__ __attribute__((aligned(16))) C turned[kTile * kRow];
+  const int h = static_cast<int>(blockIdx.x % p.Hk);
+  const Span s = span_of<kTile>(ptr, start, B, T_all, blockIdx.x / p.Hk);
+  if (s.lo >= s.hi) return;
+  const int page = page_of(p, s.b, s.tile0 / p.page), off = static_cast<int>(s.tile0 % p.page);
+  if (page < 0) return;
+  const int64_t slot0 = (static_cast<int64_t>(page) * p.Hk + h) * p.page + off;
+  C* const kp = reinterpret_cast<C*>(p.k) + slot0 * p.D;
+  C* const vp = reinterpret_cast<C*>(p.v) + slot0 * p.D;
+  const int lane = threadIdx.x % LW, g = threadIdx.x / LW, d = 8 * lane;
+  const int64_t t0 = s.first + s.tile0 - s.start;
+  Eight<T> kx[kTile / kGroups], vx[kTile / kGroups];
+#pragma unroll
+  for (int n = 0; n < kTile / kGroups; ++n) {
+    const int r = g + n * kGroups;
+    kx[n] = vx[n] = Eight<T>{};
+    if (r >= s.lo && r < s.hi && d < p.D) {
+      kx[n].load(k + (t0 + r) * k_st + h * k_sh + d);
+      vx[n].load(v + (t0 + r) * v_st + h * v_sh + d);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kTile / kGroups; ++n) {
+    const int r = g + n * kGroups;
+    const bool in = r >= s.lo && r < s.hi;
+    Kept<T, C> ck, cv;
+    ck.template from<LW>(kx[n]);
+    cv.template from<LW>(vx[n]);
+    if (in && d < p.D) ck.store(kp + r * p.D + d);
+    if constexpr (Code<C>::kNarrow) {
+      if (in && lane == 0) {
+        p.ks[slot0 + r] = ck.scale;
+        p.vs[slot0 + r] = cv.scale;
+      }
+    }
+    cv.store(turned + r * kRow + d);
+  }
+  __syncthreads();
+  const int pieces = kTile * p.D / kPer;
+  for (int x = threadIdx.x; x < pieces; x += kThreads) {
+    const int row = x / (kBlk / kPer), e = row % p.D, r0 = row / p.D * kBlk + x % (kBlk / kPer) * kPer;
+    if (r0 >= s.hi || r0 + kPer <= s.lo) continue;
+    union { uint4 u; C c[kPer]; } y;
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) y.c[n] = turned[(r0 + n) * kRow + e];
+    if (r0 >= s.lo && r0 + kPer <= s.hi) {
+      reinterpret_cast<uint4*>(vp)[x] = y.u;
+    } else {
+      for (int n = max(s.lo - r0, 0); n < min(s.hi - r0, kPer); ++n) vp[x * kPer + n] = turned[(r0 + n) * kRow + e];
+    }
+  }
+}
+
+template <typename T, typename C, int LW>
+__global__ __launch_bounds__(kThreads) void paged_read(const Pool p, T* __restrict__ k, T* __restrict__ v,
+                                                       const int64_t* __restrict__ ptr, const int64_t* __restrict__ start,
+                                                       int64_t T_all, int B) {
+  constexpr int kRow = lds_row<C, LW>(), kGroups = kThreads / LW, kBlk = block_tokens<C>(), kPer = 16 / sizeof(C);
+  __shared__ __attribute__((aligned(16))) C turned[kTile * kRow];
+  const int h = static_cast<int>(blockIdx.x % p.Hk);
+  const int64_t tile = blockIdx.x / p.Hk;
+  const int lane = threadIdx.x % LW, g = threadIdx.x / LW, d = 8 * lane;
+  auto fill = [&](int64_t t, float x) {
+    Eight<T> y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.t[e] = static_cast<T>(x);
+    if (d < p.D) {
+      y.store(k + (t * p.Hk + h) * p.D + d);
+      y.store(v + (t * p.Hk + h) * p.D + d);
+    }
+  };
+  if (ptr) {  // rows of no sequence, by the workgroups of the same number
+    const int64_t first = ptr[0], end = ptr[B];
+    for (int r = g; r < kTile; r += kGroups) {
+      const int64_t t = tile * kTile + r;
+      if (t < T_all && (t < first || t >= end)) fill(t, 0.f);
+    }
+  }
+  const Span s = span_of<kTile>(ptr, start, B, T_all, tile);
+  const int64_t t0 = s.first + s.tile0 - s.start;
+  if (s.start < 0 && tile == s.first / kTile + 2 * static_cast<int64_t>(s.b)) {  // positions before the stream's first
+    const int64_t n = min(-s.start, (ptr ? min(max(ptr[s.b + 1], int64_t(0)), T_all) : T_all) - s.first);
+    for (int64_t r = g; r < n; r += kGroups) fill(s.first + r, __builtin_nanf(""));
+  }
+  if (s.lo >= s.hi) return;
+  const int page = page_of(p, s.b, s.tile0 / p.page), off = static_cast<int>(s.tile0 % p.page);
+  if (page < 0) {
+    for (int r = g; r < kTile; r += kGroups)
+      if (r >= s.lo && r < s.hi) fill(t0 + r, __builtin_nanf(""));
+    return;
+  }
+  const int64_t slot0 = (static_cast<int64_t>(page) * p.Hk + h) * p.page + off;
+  const C* const kp = reinterpret_cast<const C*>(p.k) + slot0 * p.D;
+  const C* const vp = reinterpret_cast<const C*>(p.v) + slot0 * p.D;
+  Kept<T, C> kx[kTile / kGroups];
+#pragma unroll
+  for (int n = 0; n < kTile / kGroups; ++n) {
+    const int r = g + n * kGroups;
+    if (r >= s.lo && r < s.hi && d < p.D) {
+      kx[n].load(kp + r * p.D + d);
+      if constexpr (Code<C>::kNarrow) kx[n].scale = p.ks[slot0 + r];
+    }
+  }
+  const int pieces = kTile * p.D / kPer;
+  for (int x = threadIdx.x; x < pieces; x += kThreads) {
+    const int row = x / (kBlk / kPer), e = row % p.D, r0 = row / p.D * kBlk + x % (kBlk / kPer) * kPer;
+    if (r0 >= s.hi || r0 + kPer <= s.lo) continue;
+    union { uint4 u; C c[kPer]; } y;
+    y.u = reinterpret_cast<const uint4*>(vp)[x];
+#pragma unroll
+    for (int n = 0; n < kPer; ++n) turned[(r0 + n) * kRow + e] = y.c[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kTile / kGroups; ++n) {
+    const int r = g + n * kGroups;
+    if (r >= s.lo && r < s.hi && d < p.D) {
+      Eight<T> x;
+      kx[n].to(x);
+      x.store(k + ((t0 + r) * p.Hk + h) * p.D + d);
+      Kept<T, C> cv;
+      cv.load(turned + r * kRow + d);
+      if constexpr (Code<C>::kNarrow) cv.scale = p.vs[slot0 + r];
+      cv.to(x);
+      x.store(v + ((t0 + r) * p.Hk + h) * p.D + d);
+    }
+  }
+}
+
+struct Move {  // arguments of either direction
+  const void *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  const int64_t *ptr, *start;
+  int64_t T, B;
+  bool write;
+};
+template <typename T, typename C, int LW>
+int launch_move(const Pool& p, const Move& m, hipStream_t stream) {
+  const int64_t blocks = tiles_of(m.T, m.B, kTile) * p.Hk;
+  GEO_REQUIRE(grid_fits(blocks, kThreads), "paged cache: too many workgroups");
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  if (m.write)
+    paged_write<T, C, LW><<<grid, dim3(kThreads), 0, stream>>>(p, static_cast<const T*>(m.k), static_cast<const T*>(m.v), m.k_st,
+                                                              m.k_sh, m.v_st, m.v_sh, m.ptr, m.start, m.T, static_cast<int>(m.B));
+  else
+    paged_read<T, C, LW><<<grid, dim3(kThreads), 0, stream>>>(p, static_cast<T*>(const_cast<void*>(m.k)),
+                                                             static_cast<T*>(const_cast<void*>(m.v)), m.ptr, m.start, m.T,
+                                                             static_cast<int>(m.B));
+  GEO_LAUNCH_CHECK(m.write ? "paged_write" : "paged_read");
+  return GEO_OK;
+}
+template <typename T, typename C>
+int choose_lanes(const Pool& p, const Move& m, hipStream_t stream) {
+  if (p.D <= 32) return launch_move<T, C, 4>(p, m, stream);
+  return p.D <= 64 ? launch_move<T, C, 8>(p, m, stream) : launch_move<T, C, 16>(p, m, stream);
+}
+template <typename T>
+int choose_stored(int stored, const Pool& p, const Move& m, hipStream_t stream) {
+  if (stored == GEO_I8) return choose_lanes<T, I8>(p, m, stream);
+  return stored == GEO_E4M3 ? choose_lanes<T, E4>(p, m, stream) : choose_lanes<T, T>(p, m, stream);
+}
+
+int move(const char* name, const geo_paged_t* cache, int dtype, const Move& m, void* stream) {
+  Pool p;
+  if (const int rc = pool_args(name, cache, &p)) return rc;
+  GEO_REQUIRE(type_ok(dtype, cache->stored), "%s: tokens of type code %d, a pool of %d", name, dtype, static_cast<int>(cache->stored));
+  GEO_REQUIRE(m.T >= 0 && m.T < (int64_t(1) << 31) - 64 && m.B >= 0 && m.B < (int64_t(1) << 30) && (m.ptr || m.B <= 1),
+              "%s: %lld tokens of %lld sequences%s", name, static_cast<long long>(m.T), static_cast<long long>(m.B),
+              m.ptr ? "" : " without ptr");
+  if (m.T == 0) return GEO_OK;
+  GEO_REQUIRE(m.B >= 1, "%s: tokens of no sequence", name);
+  const int size = dtype == GEO_F32 ? 4 : 2;
+  auto in_pieces = [size](const void* x, int64_t st, int64_t sh) {
+    return x && reinterpret_cast<uintptr_t>(x) % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+  };
+  GEO_REQUIRE(in_pieces(m.k, m.k_st, m.k_sh) && in_pieces(m.v, m.v_st, m.v_sh),
+              "%s: null k or v, or rows not on multiples of 16 bytes", name);
+  if (dtype == GEO_F32) return choose_stored<float>(cache->stored, p, m, as_stream(stream));
+  if (dtype == GEO_BF16) return choose_stored<__bf16>(cache->stored, p, m, as_stream(stream));
+  return choose_stored<_Float16>(cache->stored, p, m, as_stream(stream));
+}
+
+}  // namespace paged
+}  // namespace geo
+
+extern "C" int geo_paged_write(const geo_paged_t* cache, int dtype, const void* k, const void* v, int64_t k_token, int64_t k_head,
+                               int64_t v_token, int64_t v_head, const int64_t* ptr, const int64_t* start, int64_t tokens,
+                               int64_t batch, void* stream) {
+  return geo::paged::move("paged write", cache, dtype,
+                          {k, v, k_token, k_head, v_token, v_head, ptr, start, tokens, batch, true}, stream);
+}
+
+extern "C" int geo_paged_read(const geo_paged_t* cache, int dtype, const int64_t* ptr, const int64_t* start, int64_t tokens,
+                              int64_t batch, void* k, void* v, void* stream) {
+  GEO_REQUIRE(tokens == 0 || k != v, "paged read: one output for keys and values");
+  return geo::paged::move("paged read", cache, dtype, {k, v, 0, 0, 0, 0, ptr, start, tokens, batch, false}, stream);
+}

@@ -1,0 +1,635 @@
+// paged_step.hip — attention of one new token per stream over its pages, split over the stream's
+// length and joined.
+//
+// Sᵀ = K Qᵀ and Oᵀ = Vᵀ Pᵀ on 16x16 matrix instructions, 16 query heads of a key head as the columns.  A
+// lane holds column lane % 16 and, of every product's inner dimension, the part of its group lane / 16.
+// A block is the blk tokens that 64 bytes hold; a group owns a quarter of them, 16 bytes of each row of Vᵀ.
+// The rows of Sᵀ are dealt out so that a group's results are just its own tokens: weights become the second
+// product's operand without leaving their lane, and both operands from memory are read 16 bytes a lane,
+// straight into the registers that the instructions take.  Nothing goes through LDS but the join.
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace geo {
+namespace paged {
+
+using bf16x8 = attn::bf16x8;
+using f16x8 = attn::f16x8;
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
+struct Step {
+  Pool pool;
+  const void *q, *k, *v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  const int64_t* pos;
+  attn::Bias bias;
+  int B, Hq;
+  float scale;
+};
+
+constexpr int kThreads = 256, kWaves = 4, kCols = 16;
+constexpr float kLazy = 8.f;  // how far scores (in units of log 2) may exceed the maximum that weights refer to
+
+// --- operands ---
+
+union Bytes16 {
+  uint4 u;
+  uint32_t w[4];
+  float f[4];
+  bf16x8 b;
+  f16x8 h;
+};
+
+// Eight codes (two words) as bf16, which holds them exactly.
+template <typename C>
+__device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
+  Bytes16 y;
+  if constexpr (__is_same(C, I8)) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const uint32_t x = n < 2 ? lo : hi;
+      const float a = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1))));
+      const float b = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1) + 8)));
+      y.w[n] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // their upper halves
+    }
+  } else {
+    y.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    y.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    y.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    y.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  }
+  return y.b;
+}
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Eight float32 values as the sum of PARTS bf16 operands: 8, 16 or all 24 bits of them.  Codes are exact in
+// bf16, so products of 8-bit pools keep what the queries' type holds: one part for bfloat16, two for
+// float16, three for float32.
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&y)[PARTS]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float r = x[e];
+#pragma unroll
+    for (int n = 0; n < PARTS; ++n) {
+      y[n][e] = static_cast<__bf16>(r);
+      if (n + 1 < PARTS) r -= static_cast<float>(y[n][e]);
+    }
+  }
+}
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1; }
+
+// The queries of a column in operand order: LOADS pieces of the 64 bytes of a pool row each.
+template <typename T, typename C, int LOADS>
+struct Query {  // pools in the queries' type: the pieces themselves
+  Bytes16 x[LOADS];
+  __device__ __forceinline__ void load(const T* q, int g, int D) {
+#pragma unroll
+    for (int c = 0; c < LOADS; ++c) {
+      const int d = (c * 64 + g * 16) / static_cast<int>(sizeof(T));
+      x[c].u = d < D ? *reinterpret_cast<const uint4*>(q + d) : uint4{};
+    }
+  }
+  __device__ __forceinline__ f32x4 times(int c, const Bytes16& k, f32x4 s) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = mma(k.f[e], x[c].f[e], s);
+    } else if constexpr (__is_same(T, __bf16)) {
+      s = mma(k.b, x[c].b, s);
+    } else {
+      s = mma(k.h, x[c].h, s);
+    }
+    return s;
+  }
+};
+template <typename T, typename C, int LOADS>
+struct NarrowQuery {  // 8-bit pools
+  static constexpr int kParts = parts_of<T>();
+  bf16x8 x[LOADS][2][kParts];
+  __device__ __forceinline__ void load(const T* q, int g, int D) {
+#pragma unroll
+    for (int c = 0; c < LOADS; ++c) {
+      const int d = c * 64 + g * 16;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float y[8] = {};
+        if (d < D) {
+          union { uint4 u[sizeof(T) / 2]; T t[8]; } in;
+#pragma unroll
+          for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) in.u[n] = reinterpret_cast<const uint4*>(q + d + 8 * half)[n];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(in.t[e]);
+        }
+        split8<kParts>(y, x[c][half]);
+      }
+    }
+  }
+  __device__ __forceinline__ f32x4 times(int c, const Bytes16& k, f32x4 s) const {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bf16x8 a = decode8<C>(k.w[2 * half], k.w[2 * half + 1]);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) s = mma(a, x[c][half][n], s);
+    }
+    return s;
+  }
+};
+
+// The weights of a group's tokens as the second product's operand.
+template <typename T, typename C>
+struct Weights {
+  union { bf16x8 b; f16x8 h; float f[4]; } x;
+  __device__ __forceinline__ void from(const float* p) {
+#pragma unroll
+    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
+      if constexpr (sizeof(T) == 4) x.f[e] = p[e];
+      else if constexpr (__is_same(T, __bf16)) x.b[e] = static_cast<__bf16>(p[e]);
+      else x.h[e] = static_cast<_Float16>(p[e]);
+    }
+  }
+  __device__ __forceinline__ f32x4 times(const Bytes16& v, f32x4 o) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o = mma(v.f[e], x.f[e], o);
+    } else if constexpr (__is_same(T, __bf16)) {
+      o = mma(v.b, x.b, o);
+    } else {
+      o = mma(v.h, x.h, o);
+    }
+    return o;
+  }
+};
+template <typename T, typename C>
+struct NarrowWeights {
+  static constexpr int kParts = parts_of<T>();
+  bf16x8 x[2][kParts];
+  __device__ __forceinline__ void from(const float* p) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = p[8 * half + e];
+      split8<kParts>(y, x[half]);
+    }
+  }
+  __device__ __forceinline__ f32x4 times(const Bytes16& v, f32x4 o) const {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const bf16x8 a = decode8<C>(v.w[2 * half], v.w[2 * half + 1]);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) o = mma(a, x[half][n], o);
+    }
+    return o;
+  }
+};
+
+// x times log2 e for a key `back` tokens behind, of head h.
+__device__ __forceinline__ float bias_at(const attn::Bias& b, int Hq, int h, int64_t back) {
+  const int n = static_cast<int>(min(back, static_cast<int64_t>(b.maxd)));
+  return attn::bias_value(b, static_cast<int64_t>(b.lut[b.maxd - n]) * Hq + h);
+}
+
+template <int LW>
+__device__ __forceinline__ float group_sum(float x) {
+  x += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(x)));
+  x += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(x)));
+  return x + __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(x)));
+}
+
+// Lane values of a row of DP values, 16 lanes to a row, as the pool keeps them; `bits` to be stored.
+template <typename T, typename C, int DP>
+struct NewRow {
+  float value[DP / 16];
+  C code[DP / 16];
+  float scale;
+  __device__ __forceinline__ void load(const T* row, int lane, int D) {
+    uint32_t most = 0;
+    T x[DP / 16];
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+      const int d = lane + 16 * n;
+      x[n] = d < D ? row[d] : T(0);
+      value[n] = static_cast<float>(x[n]);
+      most = max(most, __float_as_uint(value[n]) & 0x7fffffffu);
+    }
+    scale = 1.f;
+    if constexpr (Code<C>::kNarrow) {
+      const RowScale s = row_scale<C>(group_most<16>(most));
+      scale = s.scale;
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        code[n].bits = Code<C>::bits(encode<C>(value[n], s.rate));
+        value[n] = Code<C>::value(code[n].bits) * s.scale;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) code[n] = x[n];
+    }
+  }
+};
+
+// One workgroup: `per` tokens of one stream, for up to 16 query heads of one key head, a quarter of them
+// to each wave.  The new token is no part of that: the first piece's workgroup forms its row as the pool
+// keeps it, writes it, and adds it to the join, so that no read waits for the write.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces, int per, float* __restrict__ part, T* __restrict__ out) {
+  constexpr bool kNarrow = Code<C>::kNarrow;
+  constexpr int kSize = sizeof(C), kBlk = block_tokens<C>(), kOwn = kBlk / 4, kTiles = kBlk / 16;
+  constexpr int kLoads = DP * kSize / 64, kRows = DP / 16, kLds = DP + 4;
+  using Q = typename std::conditional<kNarrow, NarrowQuery<T, C, kLoads>, Query<T, C, kLoads>>::type;
+  using W = typename std::conditional<kNarrow, NarrowWeights<T, C>, Weights<T, C>>::type;
+  __shared__ float sm[kWaves + 1][kCols], sl[kWaves + 1][kCols], fresh[DP];
+  __shared__ __attribute__((aligned(16))) float so[kWaves][kCols][kLds];
+  const Pool& pool = a.pool;
+  const int D = pool.D, group = a.Hq / pool.Hk, chunks = (group + kCols - 1) / kCols;
+  uint32_t w = blockIdx.x;
+  const int piece = static_cast<int>(w % pieces); w /= pieces;
+  const int gc = static_cast<int>(w % chunks); w /= chunks;
+  const int hk = static_cast<int>(w % pool.Hk);
+  const int b = static_cast<int>(w / pool.Hk);
+  const int heads = min(kCols, group - gc * kCols), h0 = hk * group + gc * kCols;
+  const int64_t p = a.pos[b];
+  const int held = static_cast<int>(min(max(p, int64_t(0)), static_cast<int64_t>(pool.columns) * pool.page));  // tokens before the new one
+  const int s0 = piece * per, s1 = min(held, s0 + per);
+  if (piece > 0 && s0 >= s1) return;
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = ((s1 - s0 + kWaves - 1) / kWaves + kBlk - 1) / kBlk * kBlk;
+  const int w0 = s0 + wave * share, w1 = min(s1, w0 + share);
+  const int head = h0 + min(col, heads - 1);
+
+  Q q;
+  q.load(static_cast<const T*>(a.q) + b * a.q_st + head * a.q_sh, g, D);
+
+  // where the wave reads: a column of the table and a place in its page
+  const int32_t* const row = pool.table + b * pool.table_st;
+  int column = w0 / pool.page, off = w0 % pool.page;
+  bool bad = false;
+  int at = 0;
+  auto page_here = [&]() {
+    at = w0 < w1 ? row[column] : 0;
+    if (static_cast<uint32_t>(at) >= static_cast<uint32_t>(pool.pages)) {
+      bad = true;
+      at = 0;
+    }
+    at = __builtin_amdgcn_readfirstlane(at);
+  };
+  page_here();
+
+  // this lane's places in a block: row 4 g' + i of tile n is token g' kOwn + 4 n + i
+  uint32_t kat[kTiles][kLoads];
+  bool idle[kLoads];
+#pragma unroll
+  for (int c = 0; c < kLoads; ++c) {
+    const int d = (c * 64 + g * 16) / kSize;
+    idle[c] = d >= D;  // past the head: read the row's first values instead and count them as zeros
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+      kat[n][c] = ((col >> 2) * kOwn + 4 * n + (col & 3)) * D * kSize + (idle[c] ? 0 : d * kSize);
+  }
+  const bool some_idle = D < DP;
+  Bytes16 kx[kTiles][kLoads], vx[kRows];
+  f32x4 ksx[kNarrow ? kTiles : 1], vsx[kNarrow ? kTiles : 1];
+  auto load_k = [&](int page, int place) {
+    const int64_t slot0 = (static_cast<int64_t>(page) * pool.Hk + hk) * pool.page + place;
+    const char* const base = pool.k + slot0 * D * kSize;
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) kx[n][c].u = *reinterpret_cast<const uint4*>(base + kat[n][c]);
+    if constexpr (kNarrow) {
+      const f32x4* const scales = reinterpret_cast<const f32x4*>(pool.ks + slot0 + g * kOwn);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) ksx[n] = scales[n];
+    }
+  };
+  auto load_v = [&](int page, int place) {
+    const int64_t slot0 = (static_cast<int64_t>(page) * pool.Hk + hk) * pool.page + place;
+    const char* const base = pool.v + slot0 * D * kSize;
+#pragma unroll
+    for (int m = 0; m < kRows; ++m)  // rows past the head are not kept: any row does
+      vx[m].u = *reinterpret_cast<const uint4*>(base + min(16 * m + col, D - 1) * 64 + g * 16);
+    if constexpr (kNarrow) {
+      const f32x4* const scales = reinterpret_cast<const f32x4*>(pool.vs + slot0 + g * kOwn);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) vsx[n] = scales[n];
+    }
+  };
+  if (w0 < w1) {
+    load_k(at, off);
+    load_v(at, off);
+  }
+
+  if (piece == 0 && p >= 0) {
+    const int cell = threadIdx.x >> 4, e = threadIdx.x & 15;  // 16 lanes to a head
+    NewRow<T, C, DP> nk, nv;
+    nk.load(static_cast<const T*>(a.k) + b * a.k_st + hk * a.k_sh, e, D);
+    nv.load(static_cast<const T*>(a.v) + b * a.v_st + hk * a.v_sh, e, D);
+    const T* const qr = static_cast<const T*>(a.q) + b * a.q_st + (h0 + min(cell, heads - 1)) * a.q_sh;
+    float s = 0.f;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+      const int d = e + 16 * n;
+      if (d < D) s = fmaf(static_cast<float>(qr[d]), nk.value[n], s);
+    }
+    s = group_sum<16>(s) * (a.scale * kLog2e);
+    if (a.bias.table) s += bias_at(a.bias, a.Hq, h0 + min(cell, heads - 1), 0);
+    const int page = page_of(pool, b, p / pool.page), place = static_cast<int>(p % pool.page);
+    if (e == 0) {
+      sm[kWaves][cell] = s;
+      sl[kWaves][cell] = page < 0 ? __builtin_nanf("") : 1.f;
+    }
+    if (cell == 0) {
+      const int64_t slot0 = (static_cast<int64_t>(max(page, 0)) * pool.Hk + hk) * pool.page;
+      C* const kp = reinterpret_cast<C*>(pool.k) + (slot0 + place) * D;
+      C* const vp = reinterpret_cast<C*>(pool.v) + slot0 * D + place / kBlk * (kBlk * D) + place % kBlk;
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        const int d = e + 16 * n;
+        fresh[d] = nv.value[n];
+        if (gc == 0 && page >= 0 && d < D) {
+          kp[d] = nk.code[n];
+          vp[d * kBlk] = nv.code[n];
+        }
+      }
+      if constexpr (kNarrow) {
+        if (gc == 0 && page >= 0 && e == 0) {
+          pool.ks[slot0 + place] = nk.scale;
+          pool.vs[slot0 + place] = nv.scale;
+        }
+      }
+    }
+  }
+
+  f32x4 o[kRows];
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) o[m] = f32x4{};
+  float top = -kInf, sum = 0.f;
+  const float scale2 = a.scale * kLog2e;
+  const float far = a.bias.table ? bias_at(a.bias, a.Hq, head, a.bias.maxd) : 0.f;
+
+  for (int t = w0; t < w1; t += kBlk) {
+    if (some_idle) {
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c)
+        if (idle[c]) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) kx[n][c].u = uint4{};
+        }
+    }
+    float x[kOwn];
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n) {
+      f32x4 s = {};
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c) s = q.times(c, kx[n][c], s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[4 * n + i] = s[i] * scale2;
+        if constexpr (kNarrow) x[4 * n + i] *= ksx[n][i];
+      }
+    }
+    // the next block's keys are on their way while this one's weights are formed
+    const bool more = t + kBlk < w1;
+    if (more) {
+      off += kBlk;
+      if (off == pool.page) {
+        off = 0;
+        ++column;
+        page_here();
+      }
+      load_k(at, off);
+    }
+    if (a.bias.table) {
+      if (p - (t + kBlk - 1) < a.bias.maxd) {
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) x[n] += bias_at(a.bias, a.Hq, head, max(p - (t + g * kOwn + n), int64_t(0)));
+      } else {
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) x[n] += far;
+      }
+    }
+    if (t + kBlk > s1) {  // the block behind the last token: what it holds may be anything
+      const int in = s1 - (t + g * kOwn);
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n)
+        if (n >= in) x[n] = -kInf;
+      uint32_t keep[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int bits = 8 * kSize * in - 32 * n;
+        keep[n] = bits >= 32 ? ~0u : bits <= 0 ? 0u : (1u << bits) - 1;
+      }
+#pragma unroll
+      for (int m = 0; m < kRows; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) vx[m].w[n] &= keep[n];
+      if constexpr (kNarrow) {
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n)
+          if (n >= in) vsx[n / 4][n % 4] = 0.f;
+      }
+    }
+    float most = x[0];
+#pragma unroll
+    for (int n = 1; n < kOwn; ++n) most = fmaxf(most, x[n]);
+    if (__any(most > top + kLazy)) {
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(fmaxf(most, __shfl_xor(most, 32, 64)), top);
+      const float keep = top == -kInf ? 0.f : exp2_hw(top - most);
+      if (top != -kInf) {
+#pragma unroll
+        for (int m = 0; m < kRows; ++m) o[m] *= keep;
+        sum *= keep;
+      }
+      top = most;
+    }
+    const float shift = top == -kInf ? 0.f : top;
+#pragma unroll
+    for (int n = 0; n < kOwn; ++n) {
+      x[n] = exp2_hw(x[n] - shift);
+      sum += x[n];
+      if constexpr (kNarrow) x[n] *= vsx[n / 4][n % 4];
+    }
+    W weights;
+    weights.from(x);
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) o[m] = weights.times(vx[m], o[m]);
+    if (more) load_v(at, off);
+  }
+
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  if (g == 0) {
+    sm[wave][col] = top;
+    sl[wave][col] = bad ? __builtin_nanf("") : sum;
+  }
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) *reinterpret_cast<f32x4*>(&so[wave][col][16 * m + 4 * g]) = o[m];
+  __syncthreads();
+  const int sources = piece == 0 && p >= 0 ? kWaves + 1 : kWaves;
+  for (int x = threadIdx.x; x < heads * DP; x += kThreads) {
+    const int c = x / DP, d = x % DP;
+    float m = sm[0][c];
+    for (int n = 1; n < sources; ++n) m = fmaxf(m, sm[n][c]);
+    float l = 0.f, y = 0.f;
+    for (int n = 0; n < sources; ++n) {
+      const float keep = sm[n][c] == -kInf ? 0.f : exp2_hw(sm[n][c] - m);
+      // no page: its sum is NaN whatever the maximum; weights of nothing but -inf: 0 / 0 at the end
+      l += sl[n][c] == sl[n][c] ? sl[n][c] * keep : sl[n][c];
+      y += (n < kWaves ? so[n][c][d] : fresh[d]) * keep;
+    }
+    if (pieces == 1) {
+      if (d < D) out[(static_cast<int64_t>(b) * a.Hq + h0 + c) * D + d] = static_cast<T>(p < 0 ? 0.f : y / l);
+    } else {
+      float* const to = part + ((static_cast<int64_t>(b) * a.Hq + h0 + c) * pieces + piece) * (DP + 2);
+      to[2 + d] = y;
+      if (d == 0) {
+        to[0] = m;
+        to[1] = l;
+      }
+    }
+  }
+}
+
+// One workgroup: the pieces of a stream and head.
+constexpr int kMostPieces = 1024;
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void paged_join(int D, int Hq, int pieces, int per, int most, const int64_t* __restrict__ pos,
+                                                       const float* __restrict__ part, T* __restrict__ out) {
+  constexpr int kRow = DP + 2, kSets = kThreads / DP;
+  __shared__ float weight[kMostPieces], wave_top[kWaves], wave_sum[kWaves], acc[kSets][DP];
+  const int64_t at = blockIdx.x, p = pos[at / Hq];
+  const int used = p < 0 ? 0 : max(1, static_cast<int>((min(p, static_cast<int64_t>(most)) + per - 1) / per));
+  const float* const row = part + at * pieces * kRow;
+  float top = -kInf;
+  for (int n = threadIdx.x; n < used; n += kThreads) top = fmaxf(top, row[n * kRow]);
+#pragma unroll
+  for (int n = 1; n < 64; n *= 2) top = fmaxf(top, __shfl_xor(top, n, 64));
+  if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+  float sum = 0.f;
+  for (int n = threadIdx.x; n < used; n += kThreads) {
+    const float m = row[n * kRow], l = row[n * kRow + 1], keep = m == -kInf ? 0.f : exp2_hw(m - top);
+    weight[n] = keep;
+    sum += l == l ? l * keep : l;
+  }
+#pragma unroll
+  for (int n = 1; n < 64; n *= 2) sum += __shfl_xor(sum, n, 64);
+  if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+  const int d = threadIdx.x % DP, set = threadIdx.x / DP;
+  float y = 0.f;
+  for (int n = set; n < used; n += kSets) y = fmaf(row[n * kRow + 2 + d], weight[n], y);
+  acc[set][d] = y;
+  __syncthreads();
+  if (threadIdx.x < D) {
+#pragma unroll
+    for (int n = 1; n < kSets; ++n) y += acc[n][d];
+    out[at * D + d] = static_cast<T>(p < 0 ? 0.f : y / sum);
+  }
+}
+
+// How many tokens a workgroup takes, and how many workgroups that makes of the longest stream that the
+// table has room for (the lengths themselves are on the device): at least 256, more where the rows fill the
+// card anyway, and never more pieces than the join holds.
+struct Split { int per, pieces; };
+inline Split split_of(int64_t rows, int64_t most) {
+  int64_t per = 256;
+  while (per < most && (ceil_div(most, per) * rows > 4096 || ceil_div(most, per) > kMostPieces)) per *= 2;
+  return {static_cast<int>(per), static_cast<int>(ceil_div(most, per))};
+}
+inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64 ? 64 : 128; }
+inline Split split_for(const geo_paged_step_t* g) {
+  const int64_t chunks = ceil_div(static_cast<int64_t>(g->heads / g->cache.kv_heads), static_cast<int64_t>(kCols));
+  return split_of(g->batch * g->cache.kv_heads * chunks, g->cache.columns * g->cache.page);
+}
+
+template <typename T, typename C, int DP>
+int launch_step(const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
+  const int64_t chunks = ceil_div(static_cast<int64_t>(a.Hq / a.pool.Hk), static_cast<int64_t>(kCols));
+  const int64_t blocks = static_cast<int64_t>(a.B) * a.pool.Hk * chunks * s.pieces;
+  GEO_REQUIRE(grid_fits(blocks, kThreads) && grid_fits(static_cast<int64_t>(a.B) * a.Hq, kThreads),
+              "paged attention step: too many workgroups");
+  paged_step<T, C, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(a, s.pieces, s.per, part, static_cast<T*>(out));
+  GEO_LAUNCH_CHECK("paged_step");
+  if (s.pieces > 1) {
+    paged_join<T, DP><<<dim3(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.Hq)), dim3(kThreads), 0, stream>>>(
+        a.pool.D, a.Hq, s.pieces, s.per, a.pool.columns * a.pool.page, a.pos, part, static_cast<T*>(out));
+    GEO_LAUNCH_CHECK("paged_join");
+  }
+  return GEO_OK;
+}
+template <typename T, typename C>
+int choose_head(const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
+  switch (padded(a.pool.D, Code<C>::kNarrow)) {
+    case 32:
+      if constexpr (!Code<C>::kNarrow) return launch_step<T, C, 32>(a, s, out, part, stream);
+      [[fallthrough]];
+    case 64: return launch_step<T, C, 64>(a, s, out, part, stream);
+    default: return launch_step<T, C, 128>(a, s, out, part, stream);
+  }
+}
+template <typename T>
+int choose_stored(int stored, const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
+  if (stored == GEO_I8) return choose_head<T, I8>(a, s, out, part, stream);
+  return stored == GEO_E4M3 ? choose_head<T, E4>(a, s, out, part, stream) : choose_head<T, T>(a, s, out, part, stream);
+}
+
+}  // namespace paged
+}  // namespace geo
+
+extern "C" size_t geo_paged_attention_step_workspace_bytes(const geo_paged_step_t* g) {
+  using namespace geo::paged;
+  if (!g || g->batch < 1 || g->cache.kv_heads < 1 || g->heads < g->cache.kv_heads || g->cache.columns < 1 || g->cache.page < 1) return 0;
+  const Split s = split_for(g);
+  const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
+  return s.pieces == 1 ? 0 : static_cast<size_t>(g->batch) * g->heads * s.pieces * (padded(g->cache.head_dim, narrow) + 2) * sizeof(float);
+}
+
+extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace geo;
+  const char* const name = "paged attention step";
+  GEO_REQUIRE(g, "%s: null arguments", name);
+  paged::Step a;
+  if (const int rc = paged::pool_args(name, &g->cache, &a.pool)) return rc;
+  GEO_REQUIRE(paged::type_ok(g->dtype, g->cache.stored), "%s: tokens of type code %d, a pool of %d", name,
+              static_cast<int>(g->dtype), static_cast<int>(g->cache.stored));
+  GEO_REQUIRE(g->batch >= 0 && g->batch < (int64_t(1) << 31) && g->heads >= 1 && g->heads % g->cache.kv_heads == 0,
+              "%s: %d heads are no multiple of %d key heads", name, g->heads, g->cache.kv_heads);
+  if (g->bias) {
+    GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16, "%s: bias dtype code %d", name,
+                static_cast<int>(g->bias_dtype));
+    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->max_distance >= 1 && g->max_distance <= 1024,
+                "%s: bias of %d buckets up to distance %d (at most 1024)", name, g->buckets, g->max_distance);
+  }
+  if (g->batch == 0) return GEO_OK;
+  const int size = g->dtype == GEO_F32 ? 4 : 2;
+  auto in_pieces = [size](const void* p, int64_t st, int64_t sh) {
+    return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+  };
+  GEO_REQUIRE(in_pieces(g->q, g->q_stream, g->q_head) && in_pieces(g->k, g->k_stream, g->k_head) &&
+                  in_pieces(g->v, g->v_stream, g->v_head),
+              "%s: null q, k or v, or rows not on multiples of 16 bytes", name);
+  GEO_REQUIRE(out && g->positions, "%s: null output or positions", name);
+  const size_t need = geo_paged_attention_step_workspace_bytes(g);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(GEO_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace ? workspace_bytes : size_t(0), need);
+  a.q = g->q, a.k = g->k, a.v = g->v;
+  a.q_st = g->q_stream, a.q_sh = g->q_head, a.k_st = g->k_stream, a.k_sh = g->k_head, a.v_st = g->v_stream, a.v_sh = g->v_head;
+  a.pos = g->positions;
+  a.bias = {g->bias, g->bias_lut, g->bias_dtype, g->buckets, g->max_distance};
+  a.B = static_cast<int>(g->batch), a.Hq = g->heads, a.scale = g->scale;
+  const paged::Split s = paged::split_for(g);
+  float* const part = static_cast<float*>(workspace);
+  const hipStream_t on = as_stream(stream);
+  if (g->dtype == GEO_F32) return paged::choose_stored<float>(g->cache.stored, a, s, out, part, on);
+  if (g->dtype == GEO_BF16) return paged::choose_stored<__bf16>(g->cache.stored, a, s, out, part, on);
+  return paged::choose_stored<_Float16>(g->cache.stored, a, s, out, part, on);
+}

@@ -25,6 +25,7 @@ _ALIASES = (
     "functional.fps",
     "functional.gather",
     "functional.knn",
+    "functional.paged",
     "functional.radius_graph",
     "functional.recurrence",
     "functional.relative_bias",

@@ -41,6 +41,8 @@ extern "C" {
 #define GEO_BF16 1
 #define GEO_F64 2
 #define GEO_F16 3 /* the sequence operators only */
+#define GEO_I8 4  /* pools of paged caches only: whole numbers and e4m3 floats with scales */
+#define GEO_E4M3 5
 
 /* reduction codes for segment reduce */
 #define GEO_REDUCE_SUM 0
@@ -683,6 +685,59 @@ int geo_window_cache_fill(int dtype, const void* k, const void* v, int64_t k_tok
                           void* k_cache, void* v_cache, int64_t k_cache_stream, int64_t k_cache_head,
                           int64_t v_cache_stream, int64_t v_cache_head, int64_t slots, int64_t sinks,
                           void* stream);
+
+/*
+ * Keys and values of streams of any length in pages of a shared pool.  Token j of stream b lies in
+ * page table[b, j / page], slot j % page.  k [pages, kv_heads, page, head_dim];
+ * v [pages, kv_heads, page / blk, head_dim, blk] with blk tokens to 64 bytes (16 in float32, 32 in
+ * 16 bits, 64 in 8 bits).  stored: GEO_F32/BF16/F16, or GEO_I8/GEO_E4M3 with
+ * k_scale, v_scale [pages, kv_heads, page]: a row (token, head) of largest magnitude a is kept as
+ * codes round(x * fl(M / a)) of the exact product, to even, with the scale fl(a / M), M = 127 or 448;
+ * as zeros where a < 2^-100, and with a scale of NaN where a is not finite.  Entries of the table
+ * outside [0, pages) are no page.  Rows of k, v, q and outputs contiguous, 16-byte aligned.
+ */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;      /* NULL unless 8 bits */
+  const int32_t* table;          /* [streams, columns] */
+  int64_t table_stream;          /* elements from stream to stream */
+  int64_t pages, columns;
+  int32_t stored, kv_heads, head_dim, page;
+} geo_paged_t;
+
+/* Tokens of packed sequences into their pages: token t of sequence b, [ptr[b], ptr[b+1]), has the
+ * position start[b] + t - ptr[b] (ptr NULL: one sequence; start NULL: from 0).  Tokens without a
+ * page, or at negative positions, are left out.  k, v [tokens, kv_heads, head_dim] by strides, of
+ * `dtype`: the pool's, or any of float32, bfloat16 and float16 for 8 bits. */
+int geo_paged_write(const geo_paged_t* cache, int dtype, const void* k, const void* v, int64_t k_token,
+                    int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* ptr, const int64_t* start,
+                    int64_t tokens, int64_t batch, void* stream);
+/* The reverse, as values: k, v [tokens, kv_heads, head_dim], contiguous.  NaN for tokens without a page or
+ * at negative positions, 0 for tokens of no sequence. */
+int geo_paged_read(const geo_paged_t* cache, int dtype, const int64_t* ptr, const int64_t* start,
+                   int64_t tokens, int64_t batch, void* k, void* v, void* stream);
+
+/*
+ * One new token for each of `batch` streams: its k and v are written to positions[b] (from 0) of
+ * the stream's pages, and q attends to the tokens 0 .. positions[b] as the pool holds them, the new
+ * one among them.  A negative position leaves the stream alone and gives 0.  NaN where one of these
+ * tokens has no page (the new one is written where it has one).  bias by distance as above,
+ * max_distance the last one with a place of its own.
+ */
+typedef struct {
+  geo_paged_t cache;
+  const void *q, *k, *v;         /* [batch, heads or kv_heads, head_dim] */
+  int64_t q_stream, q_head, k_stream, k_head, v_stream, v_head; /* strides in elements */
+  const int64_t* positions;      /* [batch] */
+  const void* bias;              /* [buckets, heads], or NULL */
+  const int32_t* bias_lut;
+  int64_t batch;
+  int32_t dtype, bias_dtype, heads, buckets, max_distance;
+  float scale;
+} geo_paged_step_t;
+size_t geo_paged_attention_step_workspace_bytes(const geo_paged_step_t* args);
+int geo_paged_attention_step(const geo_paged_step_t* args, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /*
  * Gated linear recurrence over packed sequences, in float32: with r = sigmoid(gate_a),
