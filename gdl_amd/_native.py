@@ -41,6 +41,8 @@ pack_recurrence = struct.Struct("=3Q3q3Q3q2if4x").pack
 # bias_lut, batch, 5 codes, scale
 pack_paged = struct.Struct("=5Q3q4i").pack
 pack_paged_step = struct.Struct("=80s3Q6q3Qq5if").pack
+# geo_paged_prompt_t: that, queries, 2 strides, ptr, start, bias, bias_lut, 2 sizes, 5 codes, scale
+pack_paged_prompt = struct.Struct("=80sQ2q4Q2q5if").pack
 
 
 def at(t: torch.Tensor | None) -> int:
@@ -163,6 +165,8 @@ _SIGNATURES = {
     "geo_paged_read": (c_int, [c_bytes, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "geo_paged_attention_step_workspace_bytes": (c_size, [c_bytes]),
     "geo_paged_attention_step": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
+    "geo_paged_attention_workspace_bytes": (c_size, [c_bytes]),
+    "geo_paged_attention": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_carry_size": (c_i64, [c_i64, c_i64]),
     "geo_recurrence_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_bwd_workspace_bytes": (c_size, [c_i64, c_i64]),

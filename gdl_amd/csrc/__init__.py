@@ -729,6 +729,29 @@ def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table,
     return out
 
 
+def paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, scale, bias, plan):
+    """[T, H, D] of packed queries over the pages that ``table`` gives their streams."""
+    name = "paged_attention"
+    dev = _sequence_device(name, q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias)
+    code = _sequence_code(name, q)
+    q = _in_pieces(q)
+    ptr, start = _paged_spans(dev, ptr, start)
+    T, H, _ = q.shape
+    cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
+    bias, lut, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
+    qs, qh, _ = q.stride()
+    at = _nat.at
+    args = _nat.pack_paged_prompt(cache, q.data_ptr(), qs, qh, at(ptr), at(start), at(bias), at(lut), T, table.shape[0], code,
+                                  bias_code, H, buckets, maxd, scale)
+    out = _like(q)
+    L = _nat.lib()
+    with _nat.on_device(dev):
+        ws_bytes = L.geo_paged_attention_workspace_bytes(args)
+        ws = _nat.workspace(ws_bytes, dev) if ws_bytes else None
+        _nat.check(L.geo_paged_attention(args, out.data_ptr(), _nat.ptr(ws), ws_bytes, _nat.stream_of(dev)), "geo_paged_attention")
+    return out
+
+
 def _recurrence_args(name, x, gate_a, gate_x, decay, ptr, state, reverse, rate, streams=None):
     """geo_recurrence_t of the call (packed), the tensors that it points into, the device and the
     number of sequences (``streams``: that many of one token each)."""
@@ -1179,7 +1202,8 @@ __all__ = [
     "graph_avg_degree_hip",
     "segment_reduce_forward_hip", "segment_reduce_backward_hip",
     "window_attention_forward_hip", "window_attention_backward_hip", "window_attention_step_hip",
-    "window_cache_fill_hip", "paged_write_hip", "paged_read_hip", "paged_attention_step_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
+    "window_cache_fill_hip", "paged_write_hip", "paged_read_hip", "paged_attention_step_hip",
+    "paged_attention_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
     "gated_recurrence_step_hip",
     "knn_available", "knn_cuda", "knn_self_cuda",
     "fps_available", "fps_cuda", "fps_uniform_hip",

@@ -7,7 +7,7 @@
 // tokens, so a token block begins at the same offset in either.
 #pragma once
 
-#include "attention_tile.hpp"
+#include "attention_args.hpp"
 
 namespace geo {
 namespace paged {
@@ -47,6 +47,70 @@ template <> struct Code<E4> {
   static __device__ __forceinline__ float value(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8(b, 0); }
 };
 
+using attn::bf16x8;
+using attn::f16x8;
+union Bytes16 {
+  uint4 u;
+  uint32_t w[4];
+  float f[4];
+  bf16x8 b;
+  f16x8 h;
+};
+// Eight codes (two words) as bf16 or float16, which hold them exactly.
+template <typename C>
+__device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
+  Bytes16 y;
+  if constexpr (__is_same(C, I8)) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const uint32_t x = n < 2 ? lo : hi;
+      const float a = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1))));
+      const float b = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1) + 8)));
+      y.w[n] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // their upper halves
+    }
+  } else {
+    y.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    y.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    y.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    y.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  }
+  return y.b;
+}
+template <typename C>
+__device__ __forceinline__ f16x8 decode8_f16(uint32_t lo, uint32_t hi) {
+  Bytes16 y;
+  if constexpr (__is_same(C, I8)) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+      y.h[n] = static_cast<_Float16>(static_cast<float>(static_cast<int8_t>((n < 4 ? lo : hi) >> (8 * (n & 3)))));
+  } else {
+    y.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+    y.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+    y.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+    y.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+  }
+  return y.h;
+}
+
+// Eight float32 values as the sum of PARTS bf16 operands: 8, 16 or all 24 bits of them.  Codes are exact in
+// bf16, so products of 8-bit pools keep what the queries' type holds: one part for bfloat16, two for
+// float16, three for float32.
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&y)[PARTS]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float r = x[e];
+#pragma unroll
+    for (int n = 0; n < PARTS; ++n) {
+      y[n][e] = static_cast<__bf16>(r);
+      if (n + 1 < PARTS) r -= static_cast<float>(y[n][e]);
+    }
+  }
+}
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1; }
+
+constexpr float kLazy = 8.f;  // how far scores (in units of log 2) may exceed the maximum that weights refer to
+
 // How a row of largest magnitude a (its bits, so that NaN counts as most) is kept: values are code * scale,
 // codes the exact products x * rate rounded once.  Rows below 2^-100 are kept as zeros; one with an
 // infinity or a NaN has a scale of NaN and reads back so.
@@ -82,25 +146,25 @@ struct Pool {
 template <typename C>
 constexpr int block_tokens() { return 64 / static_cast<int>(sizeof(C)); }
 
-// The packed sequences cut into tiles of U tokens' positions, at multiples of U.  Sequence b has at most
+// The packed sequences cut into tiles of U = 2^unit positions, at multiples of U.  Sequence b has at most
 // n / U + 2 of them, so its tiles are numbered from ptr[b] / U + 2 b on; numbers without a tile are idle.
-inline int64_t tiles_of(int64_t tokens, int64_t batch, int unit) { return tokens / unit + 2 * batch; }
+inline int64_t tiles_of(int64_t tokens, int64_t batch, int unit) { return (tokens >> unit) + 2 * batch; }
 
 struct Span {
   int64_t first, start;  // row of the sequence's first token, and its position
   int64_t tile0;         // the tile's first position
   int b, lo, hi;         // the sequence; the tile's places that have tokens, lo .. hi - 1 (none: lo >= hi)
+  int64_t before;        // on a sequence's first tile: how many of its tokens have negative positions
 };
 // Wave-wide: 64 sequences are looked at together.
-template <int U>
-__device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile) {
+__device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile, int unit) {
   const int lane = threadIdx.x & 63;
   auto offset = [&](int b) { return ptr ? min(max(ptr[b], int64_t(0)), T) : b ? T : int64_t(0); };
   int lo = 0, len = B;
   bool some = true;
   do {
     const int step = (len + 63) / 64, at = lo + lane * step;
-    const bool ok = at < lo + len && offset(at) / U + 2 * static_cast<int64_t>(at) <= tile;
+    const bool ok = at < lo + len && (offset(at) >> unit) + 2 * static_cast<int64_t>(at) <= tile;
     const int n = __popcll(__ballot(ok));
     some = some && n > 0;
     const int next = lo + max(n - 1, 0) * step;
@@ -108,12 +172,14 @@ __device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start
     lo = next;
   } while (len > 1);
   const int b = __builtin_amdgcn_readfirstlane(lo);
-  Span s{offset(b), start ? start[b] : 0, 0, b, 0, 0};
+  Span s{offset(b), start ? start[b] : 0, 0, b, 0, 0, 0};
   const int64_t n = offset(b + 1) - s.first, from = max(s.start, int64_t(0)), end = s.start + n;
-  s.tile0 = (from / U + tile - (s.first / U + 2 * static_cast<int64_t>(b))) * U;
-  if (!some || s.tile0 >= end) return s;
+  const int64_t turn = tile - ((s.first >> unit) + 2 * static_cast<int64_t>(b));
+  s.tile0 = ((from >> unit) + turn) << unit;
+  if (some && turn == 0 && s.start < 0 && n > 0) s.before = s.start < -n ? n : -s.start;
+  if (!some || n <= 0 || s.tile0 >= end) return s;
   s.lo = static_cast<int>(max(from - s.tile0, int64_t(0)));
-  s.hi = static_cast<int>(min(end - s.tile0, int64_t(U)));
+  s.hi = static_cast<int>(min(end - s.tile0, int64_t(1) << unit));
   return s;
 }
 

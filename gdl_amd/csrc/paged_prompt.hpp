@@ -1,0 +1,511 @@
+// paged_prompt.hpp — attention of several new tokens per stream, which its pages hold already, over all
+// the stream's tokens up to each: a prompt, or a piece of one behind a history.
+//
+// Sᵀ = K Qᵀ and Oᵀ = Vᵀ Pᵀ on 32x32x16 products, a query to a lane (and its twin in the other half), as in the
+// window's attention.  Four waves of 32 queries share tiles of keys and values in LDS, which are filled
+// through registers one tile ahead: 8-bit codes are decoded once there, for four waves.  Query heads that
+// share a key head go to one workgroup where they can.  Values come in columns (one dimension's tokens
+// adjoin), as the second product takes them; the rows of Sᵀ are read in the order that leaves each lane the
+// weights of eight adjoining tokens.
+#pragma once
+
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace geo {
+namespace paged {
+
+using attn::f32x16;
+using attn::halves_max;
+using attn::halves_sum;
+using attn::Type;
+
+struct Prompt {
+  Pool pool;
+  const void* q;
+  int64_t q_st, q_sh;
+  const int64_t *ptr, *start;
+  attn::Bias bias;
+  int64_t T;
+  int B, Hq, heads;  // heads: of a key head's that a workgroup takes (1, 2 or 4), with 128 / heads tokens each
+  float scale;
+};
+
+constexpr int kPromptThreads = 256;
+
+// How a pool of C meets queries of T: key tiles of type K, value tiles of type V.  Codes stay codes where a
+// 16-bit type holds them (float16 weights times a scale could leave its range, so those meet bf16 values in two
+// parts) and are multiplied out for float32.
+template <typename T, typename C>
+struct Meet {
+  static constexpr bool kNarrow = Code<C>::kNarrow, kFloat = sizeof(T) == 4;
+  static constexpr bool kScaled = kNarrow && !kFloat;  // scales meet scores and weights, not the tiles
+  using K = T;
+  using V = typename std::conditional<kScaled, __bf16, T>::type;
+  static constexpr int kParts = kScaled ? parts_of<T>() : 1;
+  static constexpr int kKeys = kFloat ? 32 : 64;
+};
+
+template <typename T, typename C, int DP>
+struct PromptLds {
+  using M = Meet<T, C>;
+  static constexpr int kKRow = DP * sizeof(T) + 16, kVRow = M::kKeys * sizeof(typename M::V) + 16;  // bytes: rows in other banks
+  static constexpr int kK = M::kKeys * kKRow, kV = DP * kVRow, kS = M::kScaled ? 2 * M::kKeys * 4 : 0;
+  static constexpr int kBuffer = kK + kV + kS;
+};
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
+                                                                  float* __restrict__ part, T* __restrict__ out) {
+  using M = Meet<T, C>;
+  using L = PromptLds<T, C, DP>;
+  using TK = typename M::K;
+  using TV = typename M::V;
+  using KFrag = typename Type<TK>::Frag;
+  using VFrag = typename Type<TV>::Frag;
+  typedef KFrag KLds __attribute__((aligned(16)));  // as LDS holds them
+  typedef VFrag VLds __attribute__((aligned(16)));
+  constexpr int kSize = sizeof(C), kKeys = M::kKeys, kBlk = block_tokens<C>(), kPer = 16 / kSize;
+  constexpr int kSub = kKeys / 32, kKc = DP / 16, kMt = DP / 32;
+  constexpr int kLoads = (kKeys * DP * kSize + 16 * kPromptThreads - 1) / (16 * kPromptThreads);
+  constexpr int kSpan = kKeys < kBlk ? kKeys : kBlk, kCpb = kSpan * kSize / 16;  // tokens and pieces of a dimension in a block
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // rows of a tile's values that hold infinities or NaN, which are taken out: tile n's in wild[n % 3], cleared while tile
+  // n - 2 is worked on, filled during n - 1, read during n
+  __shared__ uint32_t wild[3][2];
+  float* const sbias = reinterpret_cast<float*>(lds + 2 * L::kBuffer);
+  const Pool& pool = a.pool;
+  const int D = pool.D, group = a.Hq / pool.Hk, sets = group / a.heads;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // one XCD works through one key head's sequences, so that their pages stay in its L2
+  int64_t w = xcd_block();
+  const int64_t tile = tiles - 1 - w % tiles;  // the longest first
+  w /= tiles;
+  const int piece = static_cast<int>(w % pieces);
+  w /= pieces;
+  const int set = static_cast<int>(w % sets), hk = static_cast<int>(w / sets);
+  const int head = hk * group + set * a.heads + wave % a.heads;
+  const int64_t rows = a.T * a.Hq;  // of a piece's partial results
+
+  // rows that see nothing: outside all sequences, or at negative positions
+  auto nothing = [&](int64_t t) {
+    if (pieces == 1) {
+      T* const row = out + (t * a.Hq + head) * D;
+      for (int d = lane & 31; d < D; d += 32) row[d] = static_cast<T>(0.f);
+    } else if ((lane & 31) == 0) {
+      float* const row = part + (piece * rows + t * a.Hq + head) * (DP + 4);
+      row[0] = -kInf;
+      row[1] = -1.f;
+    }
+  };
+  const int lanes32 = (wave / a.heads) * 2 + half, sets32 = 8 / a.heads;  // half waves of this head
+  if (a.ptr) {
+    const int64_t first = a.ptr[0], end = a.ptr[a.B];
+    for (int r = lanes32; r < 1 << unit; r += sets32) {
+      const int64_t t = (tile << unit) + r;
+      if (t < a.T && (t < first || t >= end)) nothing(t);
+    }
+  }
+  const Span s = span_of(a.ptr, a.start, a.B, a.T, tile, unit);
+  for (int64_t r = lanes32; r < s.before; r += sets32) nothing(s.first + r);
+  if (s.lo >= s.hi) return;
+
+  const int room = pool.columns * pool.page;  // tokens that the table has a place for
+  auto held = [&](int64_t p) { return static_cast<int>(min(p, static_cast<int64_t>(room))); };
+  const int place = (wave / a.heads) * 32 + (lane & 31);  // the lane's query in the tile
+  const int p = held(s.tile0 + place);                    // its position; `room`: beyond the table
+  const int wave_first = held(s.tile0 + (wave / a.heads) * 32), wave_last = held(s.tile0 + (wave / a.heads) * 32 + 31);
+  const int first_query = held(s.tile0 + s.lo), end = held(s.tile0 + s.hi);  // keys that someone here sees end there
+  const int k0 = piece * per, k1 = min(end, k0 + per);
+  const int64_t token = s.first + s.tile0 - s.start + place;
+  const bool real = place >= s.lo && place < s.hi;
+
+  KFrag q[kKc];
+  {
+    const int64_t t = s.first + s.tile0 - s.start + min(max(place, s.lo), s.hi - 1);
+    const T* const row = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
+#pragma unroll
+    for (int c = 0; c < kKc; ++c) {
+      const int d = 16 * c + 8 * half;
+      union { uint4 u[sizeof(T) / 2]; KFrag f; } x = {};
+      if (d < D) {
+#pragma unroll
+        for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) x.u[n] = reinterpret_cast<const uint4*>(row + d)[n];
+      }
+      q[c] = x.f;
+    }
+  }
+  const float scale2 = a.scale * kLog2e;
+  float far = 0.f;
+  const float* const near = sbias + (wave % a.heads) * (a.bias.maxd + 1);
+  if (a.bias.table) {
+    for (int x = threadIdx.x; x < a.heads * (a.bias.maxd + 1); x += kPromptThreads) {
+      const int h = x / (a.bias.maxd + 1), back = x % (a.bias.maxd + 1);
+      sbias[x] = attn::bias_value(a.bias, static_cast<int64_t>(a.bias.lut[a.bias.maxd - back]) * a.Hq + hk * group + set * a.heads + h);
+    }
+  }
+  if (threadIdx.x < 6) wild[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+  if (D < DP)  // keys' values past the head count as zeros
+    for (int x = threadIdx.x; x < 2 * kKeys * (DP - D); x += kPromptThreads) {
+      const int r = x / (DP - D);
+      reinterpret_cast<TK*>(lds + (r / kKeys) * L::kBuffer + (r % kKeys) * L::kKRow)[D + x % (DP - D)] = static_cast<TK>(0.f);
+    }
+
+  // this thread's pieces of a tile: 16 bytes each, from where and to where
+  const int pieces_of_tile = kKeys * D / kPer;
+  uint32_t kto[kLoads], vfrom[kLoads], vto[kLoads];
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    const int x = threadIdx.x + n * kPromptThreads, per_row = D / kPer;
+    kto[n] = x / per_row * L::kKRow + x % per_row * kPer * static_cast<int>(sizeof(TK));
+    const int blk = x / (kCpb * D), d = x / kCpb % D, at = x % kCpb;
+    vfrom[n] = blk * 64 * D + d * 64 + at * 16;
+    vto[n] = d * L::kVRow + (blk * kSpan + at * kPer) * static_cast<int>(sizeof(TV));
+  }
+  Bytes16 kx[kLoads], vx[kLoads];
+  float ksx = 0.f, vsx = 0.f;
+  int at = -1;  // the fetched tile's page
+  auto fetch = [&](int t) {
+    const int column = t / pool.page, off = t - column * pool.page;
+    at = __builtin_amdgcn_readfirstlane(pool.table[s.b * pool.table_st + column]);
+    if (static_cast<uint32_t>(at) >= static_cast<uint32_t>(pool.pages)) at = -1;
+    const int64_t slot0 = (static_cast<int64_t>(max(at, 0)) * pool.Hk + hk) * pool.page + off;
+    const char* const kb = pool.k + slot0 * D * kSize;
+    const char* const vb = pool.v + (slot0 / kBlk * kBlk) * D * kSize + slot0 % kBlk * kSize;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int x = threadIdx.x + n * kPromptThreads;
+      if (x < pieces_of_tile) {
+        kx[n].u = *reinterpret_cast<const uint4*>(kb + x * 16);
+        vx[n].u = *reinterpret_cast<const uint4*>(vb + vfrom[n]);
+      }
+    }
+    if constexpr (M::kScaled) {
+      if (threadIdx.x < kKeys) {
+        ksx = pool.ks[slot0 + threadIdx.x];
+        vsx = pool.vs[slot0 + threadIdx.x];
+      }
+    }
+  };
+  // `edge`: a tile whose later keys some query does not see.  Values there must not reach it through a
+  // weight of 0: what lies behind the last token becomes 0, and infinities and NaN are taken out, noted, and
+  // given back to those that do see them.
+  auto store = [&](int t, char* to, uint32_t* note) {
+    const bool edge = t + kKeys - 1 > first_query;
+    const int page = at;
+    int64_t slot0 = 0;
+    if constexpr (M::kNarrow && M::kFloat) {
+      const int column = t / pool.page;
+      slot0 = (static_cast<int64_t>(max(page, 0)) * pool.Hk + hk) * pool.page + (t - column * pool.page);
+    }
+    char *const kt = to, *const vt = to + L::kK;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int x = threadIdx.x + n * kPromptThreads;
+      if (x >= pieces_of_tile) break;
+      const int key0 = x / (kCpb * D) * kSpan + x % kCpb * kPer;  // first of the values' tokens
+      if constexpr (!M::kNarrow) {
+        *reinterpret_cast<uint4*>(kt + kto[n]) = kx[n].u;
+        if (edge) {
+          union { uint4 u; C c[kPer]; } y;
+          y.u = vx[n].u;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const bool in = t + key0 + e < end, fine = fabsf(static_cast<float>(y.c[e])) < kInf;
+            if (in && !fine) atomicOr(&note[(key0 + e) >> 5], 1u << ((key0 + e) & 31));
+            if (!in || !fine) y.c[e] = static_cast<C>(0.f);
+          }
+          vx[n].u = y.u;
+        }
+        *reinterpret_cast<uint4*>(vt + vto[n]) = vx[n].u;
+      } else if constexpr (M::kFloat) {
+        const float ks = pool.ks[slot0 + x / (D / kPer)];
+        union { uint4 u; uint8_t c[16]; } y, z;
+        y.u = kx[n].u;
+        z.u = vx[n].u;
+        float* const kr = reinterpret_cast<float*>(kt + kto[n]);
+        float* const vr = reinterpret_cast<float*>(vt + vto[n]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          kr[e] = Code<C>::value(y.c[e]) * ks;
+          float v = Code<C>::value(z.c[e]) * pool.vs[slot0 + key0 + e];
+          if (edge) {
+            const bool in = t + key0 + e < end, fine = fabsf(v) < kInf;
+            if (in && !fine) atomicOr(&note[(key0 + e) >> 5], 1u << ((key0 + e) & 31));
+            if (!in || !fine) v = 0.f;
+          }
+          vr[e] = v;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (__is_same(T, _Float16)) reinterpret_cast<f16x8*>(kt + kto[n])[h] = decode8_f16<C>(kx[n].w[2 * h], kx[n].w[2 * h + 1]);
+          else reinterpret_cast<bf16x8*>(kt + kto[n])[h] = decode8<C>(kx[n].w[2 * h], kx[n].w[2 * h + 1]);
+          Bytes16 v;
+          v.b = decode8<C>(vx[n].w[2 * h], vx[n].w[2 * h + 1]);
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = key0 + 8 * h + e;
+              const bool in = t + key < end, fine = fabsf(static_cast<float>(v.b[e])) < kInf;
+              if (in && !fine) atomicOr(&note[key >> 5], 1u << (key & 31));
+              if (!in || !fine) v.b[e] = static_cast<__bf16>(0.f);
+            }
+          }
+          reinterpret_cast<bf16x8*>(vt + vto[n])[h] = v.b;
+        }
+      }
+    }
+    if constexpr (M::kScaled) {
+      if (threadIdx.x < kKeys) {
+        float* const scales = reinterpret_cast<float*>(to + L::kK + L::kV);
+        scales[threadIdx.x] = ksx * scale2;
+        scales[kKeys + threadIdx.x] = vsx;
+      }
+    }
+  };
+
+  f32x16 o[kMt];
+#pragma unroll
+  for (int m = 0; m < kMt; ++m) o[m] = f32x16{};
+  float top = -kInf, sum = 0.f;
+  bool lost = p >= room;
+
+  __syncthreads();  // zeros past the head, biases, notes
+  if (a.bias.table) far = near[a.bias.maxd];
+  int page_now = -1;
+  if (k0 < k1) {
+    fetch(k0);
+    page_now = at;
+    store(k0, lds, wild[0]);
+  }
+  int buf = 0, turn = 0;
+  for (int t = k0; t < k1; t += kKeys, buf ^= 1, turn = turn == 2 ? 0 : turn + 1) {
+    __syncthreads();
+    if (threadIdx.x < 2) wild[turn == 0 ? 2 : turn - 1][threadIdx.x] = 0;
+    const char *const kt = lds + buf * L::kBuffer, *const vt = kt + L::kK;
+    const bool more = t + kKeys < k1;
+    if (more) fetch(t + kKeys);
+    const int page_next = at;
+    if (t <= wave_last) {
+      const bool whole = t + kKeys - 1 <= wave_first;
+      f32x16 x[kSub];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        x[u] = f32x16{};
+        // row 16 c + 8 a + 4 h + i of the product is token 16 c + 8 h + 4 a + i
+        const int r = lane & 31, key = 32 * u + ((r & 19) | (r >> 2 & 1) << 3 | (r >> 3 & 1) << 2);
+        const char* const row = kt + key * L::kKRow + half * 8 * static_cast<int>(sizeof(TK));
+#pragma unroll
+        for (int c = 0; c < kKc; ++c)
+          x[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], x[u]);
+      }
+      // register 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j
+      if constexpr (M::kScaled) {
+        const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 8 * half;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[u][r] *= scales[32 * u + 16 * (r >> 3) + (r & 7)];
+      } else {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) x[u] *= scale2;
+      }
+      if (a.bias.table) {
+        if (wave_first - (t + kKeys - 1) < a.bias.maxd) {
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              x[u][r] += near[min(max(p - (t + 32 * u + 16 * (r >> 3) + 8 * half + (r & 7)), 0), a.bias.maxd)];
+        } else {
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) x[u] += far;
+        }
+      }
+      const int seen = p - t - 8 * half;  // a lane's tokens 32 u + 16 c + j up to this one
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * u + 16 * (r >> 3) + (r & 7) > seen) x[u][r] = -kInf;
+      }
+      float most = x[0][0];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, x[u][r]);
+      most = halves_max(most);
+      const bool up = most > top + kLazy;
+      if (__any(up)) {
+        const float keep = up ? exp2_hw(top - most) : 1.f;
+        top = up ? most : top;
+        sum *= keep;
+#pragma unroll
+        for (int m = 0; m < kMt; ++m) o[m] *= keep;
+      }
+      const float shift = top == -kInf ? 0.f : top;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          x[u][r] = exp2_hw(x[u][r] - shift);
+          sum += x[u][r];
+        }
+      if constexpr (M::kScaled) {
+        const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + kKeys + 8 * half;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float y = x[u][r] * scales[32 * u + 16 * (r >> 3) + (r & 7)];
+            x[u][r] = whole || 32 * u + 16 * (r >> 3) + (r & 7) <= seen ? y : 0.f;  // an unseen scale may be NaN
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          VFrag w[M::kParts];
+          if constexpr (M::kScaled) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
+            split8<M::kParts>(y, w);
+          } else {
+            w[0] = attn::frag_of<TV>(x[u], c);
+          }
+          const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
+#pragma unroll
+          for (int m = 0; m < kMt; ++m) {
+            const VFrag v = *reinterpret_cast<const VLds*>(col + 32 * m * L::kVRow);
+#pragma unroll
+            for (int n = 0; n < M::kParts; ++n) o[m] = Type<TV>::mma(v, w[n], o[m]);
+          }
+        }
+      for (int u = 0; u < kSub; ++u) {
+        uint32_t rest = wild[turn][u];
+        while (rest) {  // rare: the queries that see an infinity or NaN have one in its dimension
+          const int key = 32 * u + __builtin_ctz(rest);
+          rest &= rest - 1;
+          const int slot = (t % pool.page) + key;
+          const int64_t slot0 = (static_cast<int64_t>(max(page_now, 0)) * pool.Hk + hk) * pool.page;
+          const C* const col = reinterpret_cast<const C*>(pool.v) + slot0 * D + static_cast<int64_t>(slot / kBlk) * kBlk * D + slot % kBlk;
+#pragma unroll
+          for (int m = 0; m < kMt; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int d = 32 * m + 8 * (r >> 2) + 4 * half + (r & 3);
+              if (d < D && p >= t + key) {
+                float v;
+                if constexpr (M::kNarrow) v = Code<C>::value(col[d * kBlk].bits) * pool.vs[slot0 + slot];
+                else v = static_cast<float>(col[d * kBlk]);
+                if (!(fabsf(v) < kInf)) o[m][r] = __builtin_nanf("");
+              }
+            }
+        }
+      }
+      if (page_now < 0 && p >= t) lost = true;
+    }
+    if (more) store(t + kKeys, lds + (buf ^ 1) * L::kBuffer, wild[turn == 2 ? 0 : turn + 1]);
+    page_now = page_next;
+  }
+  sum = halves_sum(sum);
+  if (lost) sum = __builtin_nanf("");
+  if (!real) return;
+  if (pieces == 1) {
+    attn::store_row<T>(out + (token * a.Hq + head) * D, o, 1.f / sum, D);  // weights of nothing but -inf: 0 times infinity
+  } else {
+    float* const row = part + (piece * rows + token * a.Hq + head) * (DP + 4);
+    if (half == 0) {
+      row[0] = top;
+      row[1] = sum;
+    }
+    attn::store_row<float>(row + 4, o, 1.f, DP);
+  }
+}
+
+// The pieces of a row joined: DP / 4 threads to a row.
+template <typename T, int DP>
+__global__ __launch_bounds__(kPromptThreads) void paged_prompt_join(int D, int64_t rows, int pieces, const float* __restrict__ part,
+                                                                    T* __restrict__ out) {
+  constexpr int kLanes = DP / 4;
+  using f32x4 = float __attribute__((ext_vector_type(4)));
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kPromptThreads + threadIdx.x) / kLanes;
+  const int d = 4 * (threadIdx.x % kLanes);
+  if (row >= rows || d >= D) return;
+  float top = -kInf;
+  for (int n = 0; n < pieces; ++n) top = fmaxf(top, part[(n * rows + row) * (DP + 4)]);
+  float sum = 0.f;
+  f32x4 y = {};
+  for (int n = 0; n < pieces; ++n) {
+    const float* const from = part + (n * rows + row) * (DP + 4);
+    const float keep = from[0] == -kInf ? 0.f : exp2_hw(from[0] - top);
+    sum += from[1] == from[1] ? from[1] * keep : from[1];
+    y += *reinterpret_cast<const f32x4*>(from + 4 + d) * keep;
+  }
+  union { T t[4]; uint2 u2; uint4 u4; } w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w.t[e] = static_cast<T>(part[row * (DP + 4) + 1] == -1.f ? 0.f : y[e] / sum);
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + row * D + d) = w.u2;
+  else *reinterpret_cast<uint4*>(out + row * D + d) = w.u4;
+}
+
+// A key head's query heads that one workgroup takes together, and the pieces of the longest history that the
+// table has room for: where rows do not fill the 256 CUs twice, pieces of at least 512 tokens do.
+struct PromptPlan {
+  int heads, unit, pieces, per;
+  int64_t tiles, blocks;
+};
+inline PromptPlan plan_prompt(int64_t T, int64_t B, int Hq, int Hk, int64_t most) {
+  PromptPlan p;
+  const int group = Hq / Hk;
+  p.heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  p.unit = p.heads == 4 ? 5 : p.heads == 2 ? 6 : 7;
+  p.tiles = tiles_of(T, B, p.unit);
+  const int64_t columns = static_cast<int64_t>(Hq) / p.heads, busy = ((T >> p.unit) + B) * columns;
+  p.pieces = 1;
+  while (busy * p.pieces < 512 && most / (2 * p.pieces) >= 512) p.pieces *= 2;
+  p.per = static_cast<int>(align_up(static_cast<size_t>(ceil_div(most, static_cast<int64_t>(p.pieces))), 64));
+  p.blocks = p.tiles * columns * p.pieces;
+  return p;
+}
+inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+template <typename T, typename C, int DP>
+int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
+  const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * (a.bias.maxd + 1) * 4 : 0);
+  GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(&paged_prompt<T, C, DP>), bytes));
+  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, p.per, part,
+                                                                                        static_cast<T*>(out));
+  GEO_LAUNCH_CHECK("paged_prompt");
+  if (p.pieces > 1) {
+    const int64_t rows = a.T * a.Hq, blocks = ceil_div(rows * (DP / 4), static_cast<int64_t>(kPromptThreads));
+    GEO_REQUIRE(grid_fits(blocks, kPromptThreads), "paged attention: too many workgroups");
+    paged_prompt_join<T, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kPromptThreads), 0, stream>>>(a.pool.D, rows, p.pieces, part,
+                                                                                                      static_cast<T*>(out));
+    GEO_LAUNCH_CHECK("paged_prompt_join");
+  }
+  return GEO_OK;
+}
+template <typename T, typename C>
+int choose_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
+  switch (prompt_padded(a.pool.D)) {
+    case 32: return launch_prompt<T, C, 32>(a, p, out, part, stream);
+    case 64: return launch_prompt<T, C, 64>(a, p, out, part, stream);
+    default: return launch_prompt<T, C, 128>(a, p, out, part, stream);
+  }
+}
+// One query type's kernels, each in a file of its own.
+template <typename T>
+int prompt_of(int stored, const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
+  if (stored == GEO_I8) return choose_prompt<T, I8>(a, p, out, part, stream);
+  return stored == GEO_E4M3 ? choose_prompt<T, E4>(a, p, out, part, stream) : choose_prompt<T, T>(a, p, out, part, stream);
+}
+
+}  // namespace paged
+}  // namespace geo

@@ -14,8 +14,6 @@
 namespace geo {
 namespace paged {
 
-using bf16x8 = attn::bf16x8;
-using f16x8 = attn::f16x8;
 using f32x4 = float __attribute__((ext_vector_type(4)));
 
 struct Step {
@@ -29,58 +27,12 @@ struct Step {
 };
 
 constexpr int kThreads = 256, kWaves = 4, kCols = 16;
-constexpr float kLazy = 8.f;  // how far scores (in units of log 2) may exceed the maximum that weights refer to
 
 // --- operands ---
 
-union Bytes16 {
-  uint4 u;
-  uint32_t w[4];
-  float f[4];
-  bf16x8 b;
-  f16x8 h;
-};
-
-// Eight codes (two words) as bf16, which holds them exactly.
-template <typename C>
-__device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
-  Bytes16 y;
-  if constexpr (__is_same(C, I8)) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const uint32_t x = n < 2 ? lo : hi;
-      const float a = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1))));
-      const float b = static_cast<float>(static_cast<int8_t>(x >> (16 * (n & 1) + 8)));
-      y.w[n] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // their upper halves
-    }
-  } else {
-    y.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
-    y.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
-    y.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
-    y.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
-  }
-  return y.b;
-}
 __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-
-// Eight float32 values as the sum of PARTS bf16 operands: 8, 16 or all 24 bits of them.  Codes are exact in
-// bf16, so products of 8-bit pools keep what the queries' type holds: one part for bfloat16, two for
-// float16, three for float32.
-template <int PARTS>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&y)[PARTS]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float r = x[e];
-#pragma unroll
-    for (int n = 0; n < PARTS; ++n) {
-      y[n][e] = static_cast<__bf16>(r);
-      if (n + 1 < PARTS) r -= static_cast<float>(y[n][e]);
-    }
-  }
-}
-template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1; }
 
 // The queries of a column in operand order: LOADS pieces of the 64 bytes of a pool row each.
 template <typename T, typename C, int LOADS>

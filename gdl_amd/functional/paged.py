@@ -23,7 +23,7 @@ import torch
 from torch import Tensor
 
 from gdl_amd import _native as _nat
-from gdl_amd.csrc import paged_attention_step_hip, paged_read_hip, paged_write_hip
+from gdl_amd.csrc import paged_attention_hip, paged_attention_step_hip, paged_read_hip, paged_write_hip
 from gdl_amd.functional.attention import _plan
 from gdl_amd.functional.relative_bias import check_buckets
 
@@ -68,6 +68,18 @@ def _step_op(q: Tensor, k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, 
 
 @_step_op.register_fake
 def _(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, bias, max_distance, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("geoembodied::paged_attention", mutates_args=())
+def _attention_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scale: Optional[Tensor], v_scale: Optional[Tensor], table: Tensor,
+                  ptr: Optional[Tensor], start: Optional[Tensor], bias: Optional[Tensor], max_distance: int,
+                  scale: float) -> Tensor:
+    return paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, scale, bias, _plan(bias, max_distance, False))
+
+
+@_attention_op.register_fake
+def _(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias, max_distance, scale):
     return q.new_empty(q.shape)
 
 
@@ -207,6 +219,49 @@ def _check_queries(name: str, q: Tensor, cache: PagedCache, bias: Optional[Tenso
     cache._token_dtype(name, q.dtype)
     if bias is not None and (bias.dim() != 2 or bias.shape[1] != q.shape[1]):
         raise ValueError(f"{name}: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
+
+
+def paged_attention(
+    q: Tensor,
+    cache: PagedCache,
+    table: Tensor,
+    ptr: Optional[Tensor] = None,
+    start: Optional[Tensor] = None,
+    *,
+    bias: Optional[Tensor] = None,
+    max_distance: int = 128,
+    scale: Optional[float] = None,
+) -> Tensor:
+    """Several new tokens of each stream: packed queries ``q [T, H, D]`` attend to all tokens of their streams up to
+    themselves, which the cache holds already (``PagedCache.write`` with the same ``table``, ``ptr`` and ``start``).
+
+    Args:
+        q: ``H`` a multiple of the cache's heads (query head ``h`` reads key head ``h // (H / Hk)``), of the
+            pool's type, or float32, bfloat16 or float16 over an 8-bit pool.
+        table: int32 [B, n], the streams' pages.
+        ptr: int64 [B + 1] offsets of the sequences in the T tokens; None: one sequence.
+        start: int64 [B], position of each sequence's first token in its stream; None: 0.
+        bias: [buckets, H], one-sided, as ``window_attention``'s.  The first call with a number of buckets and a
+            ``max_distance`` copies their table to the device and cannot be captured into a graph.
+        max_distance: where the bias's last bucket begins (at most 1024).
+        scale: of the scores; ``D ** -0.5`` by default.
+
+    Returns:
+        [T, H, D] of q's type: ``window_attention``'s rows with the window ``(-1, 0)``.  0 for tokens outside
+        ``ptr[0] .. ptr[B]`` and at negative positions, NaN for one of whose tokens has no page.  No gradients.
+    """
+    name = "paged_attention"
+    _check_queries(name, q, cache, bias)
+    _check_spans(name, table, ptr, start)
+    _no_grad(name, q, bias)
+    scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
+    pools = cache.k, cache.v, cache.k_scale, cache.v_scale
+    if _nat.plain_call(q, *pools, table, ptr, start, bias):
+        return paged_attention_hip(q, *pools, table, ptr, start, scale, bias, _plan(bias, int(max_distance), False))
+    _nat.no_tangents(name, q, bias)
+    if bias is not None:
+        check_buckets(bias.shape[0], int(max_distance), False)
+    return torch.ops.geoembodied.paged_attention(q, *pools, table, ptr, start, bias, int(max_distance), scale)
 
 
 def paged_attention_step(

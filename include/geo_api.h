@@ -740,6 +740,26 @@ int geo_paged_attention_step(const geo_paged_step_t* args, void* out, void* work
                              size_t workspace_bytes, void* stream);
 
 /*
+ * Several new tokens of each stream, which its pages hold already: queries of packed sequences, token t
+ * of sequence b at the position start[b] + t - ptr[b], attend to the stream's tokens 0 .. that position.
+ * NaN where one of these has no page; 0 for queries of no sequence or at negative positions.
+ */
+typedef struct {
+  geo_paged_t cache;
+  const void* q;                 /* [tokens, heads, head_dim] */
+  int64_t q_token, q_head;       /* strides in elements */
+  const int64_t *ptr, *start;    /* [batch + 1] or NULL: one sequence; [batch] or NULL: from 0 */
+  const void* bias;              /* [buckets, heads], or NULL */
+  const int32_t* bias_lut;
+  int64_t tokens, batch;
+  int32_t dtype, bias_dtype, heads, buckets, max_distance;
+  float scale;
+} geo_paged_prompt_t;
+size_t geo_paged_attention_workspace_bytes(const geo_paged_prompt_t* args);
+int geo_paged_attention(const geo_paged_prompt_t* args, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/*
  * Gated linear recurrence over packed sequences, in float32: with r = sigmoid(gate_a),
  * z = sigmoid(gate_x), log a = -rate softplus(decay) r, per channel
  *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) z_t x_t,
