@@ -60,6 +60,8 @@ union Bytes16 {
 template <typename C>
 __device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
   Bytes16 y;
+  // keeps the compiler from taking the bytes apart where they were loaded, an iteration earlier
+  asm("" : "+v"(lo), "+v"(hi));
   if constexpr (__is_same(C, I8)) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {

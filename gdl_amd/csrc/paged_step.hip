@@ -7,6 +7,9 @@
 // The rows of Sᵀ are dealt out so that a group's results are just its own tokens: weights become the second
 // product's operand without leaving their lane, and both operands from memory are read 16 bytes a lane,
 // straight into the registers that the instructions take.  Nothing goes through LDS but the join.
+#include <stdlib.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.hpp"
@@ -27,6 +30,14 @@ struct Step {
 };
 
 constexpr int kThreads = 256, kWaves = 4, kCols = 16;
+
+// Workgroups of the kernel on a CU, by the registers that it takes.
+constexpr int kMostWaves = 4;
+template <typename T, typename C, int DP>
+constexpr int step_waves() {
+  if (DP == 128) return 2;
+  return !Code<C>::kNarrow ? kMostWaves : sizeof(T) == 4 ? 2 : 3;
+}
 
 // --- operands ---
 
@@ -184,11 +195,34 @@ struct NewRow {
   }
 };
 
-// One workgroup: `per` tokens of one stream, for up to 16 query heads of one key head, a quarter of them
-// to each wave.  The new token is no part of that: the first piece's workgroup forms its row as the pool
-// keeps it, writes it, and adds it to the join, so that no read waits for the write.
+// How the work is dealt out.  A row is a stream, a key head and up to 16 of its query heads; its work is the
+// 64-token tiles that the stream holds, at least one.  The tiles of all rows, in a row, are cut into equal
+// shares, one for each of `groups` workgroups, which are as many as the card runs at a time: lengths are
+// read on the device, so streams of any ages fill it evenly.  A share of `least` tiles is worth a workgroup.
+// Without `parts` a workgroup takes a whole row.
+struct Deal {
+  int groups, least;
+  int4* desc;    // by workgroup: pieces of the row that begins in it and does not end in it (0: none), its heads, its output row
+  float* parts;  // by workgroup: what it adds to the row that it begins with, and to the one that it ends with
+};
+constexpr int kTile = 64;
+
+__device__ __forceinline__ int tiles_at(int64_t p, int room) {
+  return max(1, static_cast<int>((min(max(p, int64_t(0)), static_cast<int64_t>(room)) + kTile - 1) / kTile));
+}
+__device__ __forceinline__ int64_t scalar(int64_t x) { return static_cast<int64_t>(attn::uniform(static_cast<uint64_t>(x))); }
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+#pragma unroll
+  for (int n = 1; n < 64; n *= 2) x += __shfl_xor(x, n, 64);
+  return x;
+}
+
+// One workgroup: a share.  The part of a row goes to its four waves in quarters.  The new token is no part of
+// that: who has the row's beginning forms its row as the pool keeps it, writes it, and adds it to the join, so
+// that no read waits for the write.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces, int per, float* __restrict__ part, T* __restrict__ out) {
+__global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step(const Step a, const Deal deal, const int32_t* __restrict__ table,
+                                                                        const int64_t* __restrict__ positions, T* __restrict__ out) {
   constexpr bool kNarrow = Code<C>::kNarrow;
   constexpr int kSize = sizeof(C), kBlk = block_tokens<C>(), kOwn = kBlk / 4, kTiles = kBlk / 16;
   constexpr int kLoads = DP * kSize / 64, kRows = DP / 16, kLds = DP + 4;
@@ -196,54 +230,109 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
   using W = typename std::conditional<kNarrow, NarrowWeights<T, C>, Weights<T, C>>::type;
   __shared__ float sm[kWaves + 1][kCols], sl[kWaves + 1][kCols], fresh[DP];
   __shared__ __attribute__((aligned(16))) float so[kWaves][kCols][kLds];
+  extern __shared__ float sbias[];  // with a bias: [buckets][kCols], the row's heads; then the bucket of each distance back, a byte each
   const Pool& pool = a.pool;
-  const int D = pool.D, group = a.Hq / pool.Hk, chunks = (group + kCols - 1) / kCols;
-  uint32_t w = blockIdx.x;
-  const int piece = static_cast<int>(w % pieces); w /= pieces;
-  const int gc = static_cast<int>(w % chunks); w /= chunks;
-  const int hk = static_cast<int>(w % pool.Hk);
-  const int b = static_cast<int>(w / pool.Hk);
-  const int heads = min(kCols, group - gc * kCols), h0 = hk * group + gc * kCols;
-  const int64_t p = a.pos[b];
-  const int held = static_cast<int>(min(max(p, int64_t(0)), static_cast<int64_t>(pool.columns) * pool.page));  // tokens before the new one
-  const int s0 = piece * per, s1 = min(held, s0 + per);
-  if (piece > 0 && s0 >= s1) return;
-  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int D = pool.D, group = a.Hq / pool.Hk, chunks = (group + kCols - 1) / kCols, room = pool.columns * pool.page;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int share = ((s1 - s0 + kWaves - 1) / kWaves + kBlk - 1) / kBlk * kBlk;
-  const int w0 = s0 + wave * share, w1 = min(s1, w0 + share);
+  const int per_stream = pool.Hk * chunks;  // rows
+
+  uint8_t* const bucket = reinterpret_cast<uint8_t*>(sbias + a.bias.buckets * kCols);
+  if (a.bias.table)
+    for (int x = threadIdx.x; x <= a.bias.maxd; x += kThreads) bucket[x] = static_cast<uint8_t>(a.bias.lut[a.bias.maxd - x]);
+
+  // the share u .. end of all tiles, and where it begins: stream, row of the stream, tile
+  int b, r, t0;
+  int64_t u = 0, end, share = 0, before = 0;  // before: tiles ahead of the stream's
+  int64_t p;
+  if (deal.parts) {
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    for (int i = lane; i < a.B; i += 64) total += tiles_at(positions[i], room);
+    total = scalar(wave_sum64(total)) * per_stream;
+    share = max((total + deal.groups - 1) / deal.groups, static_cast<int64_t>(deal.least));
+    u = blockIdx.x * share;
+    end = min(u + share, total);
+    if (threadIdx.x == 0) deal.desc[blockIdx.x] = int4{0, 0, 0, 0};
+    if (u >= end) return;
+    int64_t at = u / per_stream;  // the stream is the one with this tile of all streams'
+    for (b = 0;; b += 64) {
+      const int i = b + lane, n = i < a.B ? tiles_at(positions[i], room) : 0;
+      int64_t upto = n;
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) {
+        const int64_t x = __shfl_up(upto, k, 64);
+        if (lane >= k) upto += x;
+      }
+      const uint64_t past = __ballot(before + upto > at);
+      if (past) {
+        const int k = __builtin_ctzll(past);
+        b += k;
+        before += scalar(__shfl(upto - n, k, 64));
+        break;
+      }
+      before += scalar(__shfl(upto, 63, 64));
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    p = positions[b];
+    const int64_t in = u - before * per_stream, n = tiles_at(p, room);
+    r = static_cast<int>(in / n);
+    t0 = static_cast<int>(in - r * n);
+  } else {
+    b = static_cast<int>(blockIdx.x / per_stream);
+    r = static_cast<int>(blockIdx.x % per_stream);
+    t0 = 0;
+    p = positions[b];
+    end = tiles_at(p, room);
+  }
+  for (bool again = false;; again = true) {
+  uint32_t thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // keeps what is formed from it in the row's part: ahead of them all it takes the registers
+  const int lane = thread & 63, g = lane >> 4, col = lane & 15;
+  const int tiles = tiles_at(p, room);
+  const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - u)));
+  const bool begins = t0 == 0, ends = t1 == tiles;
+  if (again) __syncthreads();  // the waves are done with the LDS of the row before
+  const int gc = r % chunks, hk = r / chunks;
+  const int heads = min(kCols, group - gc * kCols), h0 = hk * group + gc * kCols;
+  const int held = static_cast<int>(min(max(p, int64_t(0)), static_cast<int64_t>(room)));  // tokens before the new one
+  const int s0 = t0 * kTile, s1 = min(held, t1 * kTile);
+  const int quarter = ((s1 - s0 + kWaves - 1) / kWaves + kBlk - 1) / kBlk * kBlk;
+  const int w0 = s0 + wave * quarter, w1 = min(s1, w0 + quarter);
   const int head = h0 + min(col, heads - 1);
 
   Q q;
   q.load(static_cast<const T*>(a.q) + b * a.q_st + head * a.q_sh, g, D);
 
   // where the wave reads: a column of the table and a place in its page
-  const int32_t* const row = pool.table + b * pool.table_st;
+  const int32_t* const row = table + b * pool.table_st;
   int column = w0 / pool.page, off = w0 % pool.page;
   bool bad = false;
-  int at = 0;
-  auto page_here = [&]() {
-    at = w0 < w1 ? row[column] : 0;
+  int at = 0, next = 0;
+  auto entry = [&](int n) { return __builtin_amdgcn_readfirstlane(row[min(n, pool.columns - 1)]); };
+  auto page_here = [&]() {  // the entry behind it is on its way while this page is read
+    at = next;
+    next = entry(column + 1);
     if (static_cast<uint32_t>(at) >= static_cast<uint32_t>(pool.pages)) {
       bad = true;
       at = 0;
     }
-    at = __builtin_amdgcn_readfirstlane(at);
   };
-  page_here();
+  if (w0 < w1) {
+    next = entry(column);
+    page_here();
+  }
 
   // this lane's places in a block: row 4 g' + i of tile n is token g' kOwn + 4 n + i
-  uint32_t kat[kTiles][kLoads];
+  uint32_t kat[kLoads];
   bool idle[kLoads];
 #pragma unroll
   for (int c = 0; c < kLoads; ++c) {
-    const int d = (c * 64 + g * 16) / kSize;
-    idle[c] = d >= D;  // past the head: read the row's first values instead and count them as zeros
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n)
-      kat[n][c] = ((col >> 2) * kOwn + 4 * n + (col & 3)) * D * kSize + (idle[c] ? 0 : d * kSize);
+    idle[c] = (c * 64 + g * 16) / kSize >= D;  // past the head: read the row's first values instead and count them as zeros
+    kat[c] = ((col >> 2) * kOwn + (col & 3)) * D * kSize + (idle[c] ? 0 : c * 64 + g * 16);
   }
   const bool some_idle = D < DP;
+  // dimension 16 m + col of the values; past the head, rows that are not kept, any does
+  const uint32_t vat = col * 64 + g * 16, vat_edge = (col & 7) * 64 + g * 16;
   Bytes16 kx[kTiles][kLoads], vx[kRows];
   f32x4 ksx[kNarrow ? kTiles : 1], vsx[kNarrow ? kTiles : 1];
   auto load_k = [&](int page, int place) {
@@ -252,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int c = 0; c < kLoads; ++c) kx[n][c].u = *reinterpret_cast<const uint4*>(base + kat[n][c]);
+      for (int c = 0; c < kLoads; ++c) kx[n][c].u = *reinterpret_cast<const uint4*>(base + n * 4 * D * kSize + kat[c]);
     if constexpr (kNarrow) {
       const f32x4* const scales = reinterpret_cast<const f32x4*>(pool.ks + slot0 + g * kOwn);
 #pragma unroll
@@ -263,8 +352,8 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
     const int64_t slot0 = (static_cast<int64_t>(page) * pool.Hk + hk) * pool.page + place;
     const char* const base = pool.v + slot0 * D * kSize;
 #pragma unroll
-    for (int m = 0; m < kRows; ++m)  // rows past the head are not kept: any row does
-      vx[m].u = *reinterpret_cast<const uint4*>(base + min(16 * m + col, D - 1) * 64 + g * 16);
+    for (int m = 0; m < kRows; ++m)
+      vx[m].u = *reinterpret_cast<const uint4*>(base + (16 * m < D ? m * 1024 : 0) + (16 * m + 16 <= D ? vat : vat_edge));
     if constexpr (kNarrow) {
       const f32x4* const scales = reinterpret_cast<const f32x4*>(pool.vs + slot0 + g * kOwn);
 #pragma unroll
@@ -276,47 +365,12 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
     load_v(at, off);
   }
 
-  if (piece == 0 && p >= 0) {
-    const int cell = threadIdx.x >> 4, e = threadIdx.x & 15;  // 16 lanes to a head
-    NewRow<T, C, DP> nk, nv;
-    nk.load(static_cast<const T*>(a.k) + b * a.k_st + hk * a.k_sh, e, D);
-    nv.load(static_cast<const T*>(a.v) + b * a.v_st + hk * a.v_sh, e, D);
-    const T* const qr = static_cast<const T*>(a.q) + b * a.q_st + (h0 + min(cell, heads - 1)) * a.q_sh;
-    float s = 0.f;
-#pragma unroll
-    for (int n = 0; n < DP / 16; ++n) {
-      const int d = e + 16 * n;
-      if (d < D) s = fmaf(static_cast<float>(qr[d]), nk.value[n], s);
-    }
-    s = group_sum<16>(s) * (a.scale * kLog2e);
-    if (a.bias.table) s += bias_at(a.bias, a.Hq, h0 + min(cell, heads - 1), 0);
-    const int page = page_of(pool, b, p / pool.page), place = static_cast<int>(p % pool.page);
-    if (e == 0) {
-      sm[kWaves][cell] = s;
-      sl[kWaves][cell] = page < 0 ? __builtin_nanf("") : 1.f;
-    }
-    if (cell == 0) {
-      const int64_t slot0 = (static_cast<int64_t>(max(page, 0)) * pool.Hk + hk) * pool.page;
-      C* const kp = reinterpret_cast<C*>(pool.k) + (slot0 + place) * D;
-      C* const vp = reinterpret_cast<C*>(pool.v) + slot0 * D + place / kBlk * (kBlk * D) + place % kBlk;
-#pragma unroll
-      for (int n = 0; n < DP / 16; ++n) {
-        const int d = e + 16 * n;
-        fresh[d] = nv.value[n];
-        if (gc == 0 && page >= 0 && d < D) {
-          kp[d] = nk.code[n];
-          vp[d * kBlk] = nv.code[n];
-        }
-      }
-      if constexpr (kNarrow) {
-        if (gc == 0 && page >= 0 && e == 0) {
-          pool.ks[slot0 + place] = nk.scale;
-          pool.vs[slot0 + place] = nv.scale;
-        }
-      }
-    }
+  const bool near = a.bias.table && (t1 * kTile > p - a.bias.maxd || begins);  // distances with a bias of their own, the new token's
+  if (near) {
+    for (int x = thread; x < a.bias.buckets * kCols; x += kThreads)
+      sbias[x] = attn::bias_value(a.bias, static_cast<int64_t>(x / kCols) * a.Hq + h0 + min(x % kCols, heads - 1));
+    __syncthreads();
   }
-
   f32x4 o[kRows];
 #pragma unroll
   for (int m = 0; m < kRows; ++m) o[m] = f32x4{};
@@ -344,6 +398,7 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
         x[4 * n + i] = s[i] * scale2;
         if constexpr (kNarrow) x[4 * n + i] *= ksx[n][i];
       }
+      if constexpr (kNarrow) __builtin_amdgcn_sched_barrier(0);  // decode a tile at a time: all at once take the registers
     }
     // the next block's keys are on their way while this one's weights are formed
     const bool more = t + kBlk < w1;
@@ -359,7 +414,10 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
     if (a.bias.table) {
       if (p - (t + kBlk - 1) < a.bias.maxd) {
 #pragma unroll
-        for (int n = 0; n < kOwn; ++n) x[n] += bias_at(a.bias, a.Hq, head, max(p - (t + g * kOwn + n), int64_t(0)));
+        for (int n = 0; n < kOwn; ++n) {
+          const int back = static_cast<int>(min(max(p - (t + g * kOwn + n), int64_t(0)), static_cast<int64_t>(a.bias.maxd)));
+          x[n] += sbias[bucket[back] * kCols + col];
+        }
       } else {
 #pragma unroll
         for (int n = 0; n < kOwn; ++n) x[n] += far;
@@ -410,7 +468,10 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
     W weights;
     weights.from(x);
 #pragma unroll
-    for (int m = 0; m < kRows; ++m) o[m] = weights.times(vx[m], o[m]);
+    for (int m = 0; m < kRows; ++m) {
+      o[m] = weights.times(vx[m], o[m]);
+      if constexpr (kNarrow) __builtin_amdgcn_sched_barrier(0);
+    }
     if (more) load_v(at, off);
   }
 
@@ -422,9 +483,52 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
   }
 #pragma unroll
   for (int m = 0; m < kRows; ++m) *reinterpret_cast<f32x4*>(&so[wave][col][16 * m + 4 * g]) = o[m];
+
+  if (begins && p >= 0) {
+    const int cell = thread >> 4, e = thread & 15;  // 16 lanes to a head
+    NewRow<T, C, DP> nk, nv;
+    nk.load(static_cast<const T*>(a.k) + b * a.k_st + hk * a.k_sh, e, D);
+    nv.load(static_cast<const T*>(a.v) + b * a.v_st + hk * a.v_sh, e, D);
+    const T* const qr = static_cast<const T*>(a.q) + b * a.q_st + (h0 + min(cell, heads - 1)) * a.q_sh;
+    float s = 0.f;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+      const int d = e + 16 * n;
+      if (d < D) s = fmaf(static_cast<float>(qr[d]), nk.value[n], s);
+    }
+    s = group_sum<16>(s) * (a.scale * kLog2e);
+    if (a.bias.table) s += sbias[bucket[0] * kCols + cell];
+    const int page = page_of(pool, b, p / pool.page), place = static_cast<int>(p % pool.page);
+    if (e == 0) {
+      sm[kWaves][cell] = s;
+      sl[kWaves][cell] = page < 0 ? __builtin_nanf("") : 1.f;
+    }
+    if (cell == 0) {
+      const int64_t slot0 = (static_cast<int64_t>(max(page, 0)) * pool.Hk + hk) * pool.page;
+      C* const kp = reinterpret_cast<C*>(pool.k) + (slot0 + place) * D;
+      C* const vp = reinterpret_cast<C*>(pool.v) + slot0 * D + place / kBlk * (kBlk * D) + place % kBlk;
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        const int d = e + 16 * n;
+        fresh[d] = nv.value[n];
+        if (gc == 0 && page >= 0 && d < D) {
+          kp[d] = nk.code[n];
+          vp[d * kBlk] = nv.code[n];
+        }
+      }
+      if constexpr (kNarrow) {
+        if (gc == 0 && page >= 0 && e == 0) {
+          pool.ks[slot0 + place] = nk.scale;
+          pool.vs[slot0 + place] = nv.scale;
+        }
+      }
+    }
+  }
   __syncthreads();
-  const int sources = piece == 0 && p >= 0 ? kWaves + 1 : kWaves;
-  for (int x = threadIdx.x; x < heads * DP; x += kThreads) {
+  const int sources = begins && p >= 0 ? kWaves + 1 : kWaves;
+  const bool whole = begins && ends;
+  float* const part = whole ? nullptr : deal.parts + (2 * static_cast<int64_t>(blockIdx.x) + (begins ? 1 : 0)) * min(group, kCols) * (DP + 4);
+  for (int x = thread; x < heads * DP; x += kThreads) {
     const int c = x / DP, d = x % DP;
     float m = sm[0][c];
     for (int n = 1; n < sources; ++n) m = fmaxf(m, sm[n][c]);
@@ -435,39 +539,58 @@ __global__ __launch_bounds__(kThreads) void paged_step(const Step a, int pieces,
       l += sl[n][c] == sl[n][c] ? sl[n][c] * keep : sl[n][c];
       y += (n < kWaves ? so[n][c][d] : fresh[d]) * keep;
     }
-    if (pieces == 1) {
+    if (whole) {
       if (d < D) out[(static_cast<int64_t>(b) * a.Hq + h0 + c) * D + d] = static_cast<T>(p < 0 ? 0.f : y / l);
     } else {
-      float* const to = part + ((static_cast<int64_t>(b) * a.Hq + h0 + c) * pieces + piece) * (DP + 2);
-      to[2 + d] = y;
+      float* const to = part + c * (DP + 4);
+      to[4 + d] = y;
       if (d == 0) {
         to[0] = m;
         to[1] = l;
       }
     }
   }
+  if (begins && !ends && thread == 0) {  // whoever has a part of this row comes behind this workgroup
+    const int64_t last = (before * per_stream + static_cast<int64_t>(r + 1) * tiles - 1) / share;
+    const int64_t to = static_cast<int64_t>(b) * a.Hq + h0;
+    deal.desc[blockIdx.x] = int4{static_cast<int>(last - blockIdx.x + 1), heads, static_cast<int>(to), static_cast<int>(to >> 32)};
+  }
+  u += t1 - t0;
+  if (u >= end) return;
+  t0 = 0;
+  if (++r == per_stream) {
+    r = 0;
+    before += tiles;
+    p = positions[++b];
+  }
+  }
 }
 
-// One workgroup: the pieces of a stream and head.
-constexpr int kMostPieces = 1024;
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void paged_join(int D, int Hq, int pieces, int per, int most, const int64_t* __restrict__ pos,
-                                                       const float* __restrict__ part, T* __restrict__ out) {
-  constexpr int kRow = DP + 2, kSets = kThreads / DP;
-  __shared__ float weight[kMostPieces], wave_top[kWaves], wave_sum[kWaves], acc[kSets][DP];
-  const int64_t at = blockIdx.x, p = pos[at / Hq];
-  const int used = p < 0 ? 0 : max(1, static_cast<int>((min(p, static_cast<int64_t>(most)) + per - 1) / per));
-  const float* const row = part + at * pieces * kRow;
+// One workgroup: the pieces of one head of a row that several shares have parts of, four dimensions to a lane.
+constexpr int kMostGroups = 1024;
+template <typename T, int DP, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join(int D, int cells, const int4* __restrict__ desc, const float* __restrict__ parts,
+                                                      T* __restrict__ out) {
+  constexpr int kRow = DP + 4, kLanes = DP / 4, kSets = THREADS / kLanes, kW = THREADS / 64;
+  __shared__ float weight[kMostGroups], wave_top[kW], wave_sum[kW];
+  __shared__ f32x4 acc[kSets][kLanes];
+  const int4 what = desc[blockIdx.x];
+  const int used = what.x, cell = blockIdx.y;
+  if (cell >= what.y || used == 0) return;
+  const int64_t at = (static_cast<int64_t>(what.w) << 32 | static_cast<uint32_t>(what.z)) + cell;
+  // the first piece is the last one of its workgroup, the others are the first ones of theirs
+  auto row_of = [&](int n) { return parts + ((2 * static_cast<int64_t>(blockIdx.x + n) + (n == 0 ? 1 : 0)) * cells + cell) * kRow; };
   float top = -kInf;
-  for (int n = threadIdx.x; n < used; n += kThreads) top = fmaxf(top, row[n * kRow]);
+  for (int n = threadIdx.x; n < used; n += THREADS) top = fmaxf(top, row_of(n)[0]);
 #pragma unroll
   for (int n = 1; n < 64; n *= 2) top = fmaxf(top, __shfl_xor(top, n, 64));
   if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+#pragma unroll
+  for (int n = 0; n < kW; ++n) top = fmaxf(top, wave_top[n]);
   float sum = 0.f;
-  for (int n = threadIdx.x; n < used; n += kThreads) {
-    const float m = row[n * kRow], l = row[n * kRow + 1], keep = m == -kInf ? 0.f : exp2_hw(m - top);
+  for (int n = threadIdx.x; n < used; n += THREADS) {
+    const float m = row_of(n)[0], l = row_of(n)[1], keep = m == -kInf ? 0.f : exp2_hw(m - top);
     weight[n] = keep;
     sum += l == l ? l * keep : l;
   }
@@ -475,63 +598,87 @@ __global__ __launch_bounds__(kThreads) void paged_join(int D, int Hq, int pieces
   for (int n = 1; n < 64; n *= 2) sum += __shfl_xor(sum, n, 64);
   if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = sum;
   __syncthreads();
-  sum = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
-  const int d = threadIdx.x % DP, set = threadIdx.x / DP;
-  float y = 0.f;
-  for (int n = set; n < used; n += kSets) y = fmaf(row[n * kRow + 2 + d], weight[n], y);
-  acc[set][d] = y;
-  __syncthreads();
-  if (threadIdx.x < D) {
+  sum = 0.f;
 #pragma unroll
-    for (int n = 1; n < kSets; ++n) y += acc[n][d];
-    out[at * D + d] = static_cast<T>(p < 0 ? 0.f : y / sum);
+  for (int n = 0; n < kW; ++n) sum += wave_sum[n];
+  const int lane = threadIdx.x % kLanes, set = threadIdx.x / kLanes;
+  f32x4 y = {};
+#pragma unroll 4
+  for (int n = set; n < used; n += kSets) y += *reinterpret_cast<const f32x4*>(row_of(n) + 4 + 4 * lane) * weight[n];
+  acc[set][lane] = y;
+  __syncthreads();
+  if (set == 0 && 4 * lane < D) {
+#pragma unroll
+    for (int n = 1; n < kSets; ++n) y += acc[n][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[at * D + 4 * lane + e] = static_cast<T>(y[e] / sum);
   }
 }
 
-// How many tokens a workgroup takes, and how many workgroups that makes of the longest stream that the
-// table has room for (the lengths themselves are on the device): at least 256, more where the rows fill the
-// card anyway, and never more pieces than the join holds.
-struct Split { int per, pieces; };
-inline Split split_of(int64_t rows, int64_t most) {
-  int64_t per = 256;
-  while (per < most && (ceil_div(most, per) * rows > 4096 || ceil_div(most, per) > kMostPieces)) per *= 2;
-  return {static_cast<int>(per), static_cast<int>(ceil_div(most, per))};
-}
 inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64 ? 64 : 128; }
-inline Split split_for(const geo_paged_step_t* g) {
-  const int64_t chunks = ceil_div(static_cast<int64_t>(g->heads / g->cache.kv_heads), static_cast<int64_t>(kCols));
-  return split_of(g->batch * g->cache.kv_heads * chunks, g->cache.columns * g->cache.page);
+
+// Workgroups, the least share (in tiles) and the workspace of a call: whole rows where no stream can hold
+// more than `kWhole` tiles, else as many shares as run at a time.
+struct StepPlan {
+  int groups, least;
+  size_t bytes;
+};
+inline StepPlan plan_step(const geo_paged_step_t* g, int waves) {
+  static const int kWhole = getenv("PS_WHOLE") ? atoi(getenv("PS_WHOLE")) : 8, kLeast = getenv("PS_LEAST") ? atoi(getenv("PS_LEAST")) : 4;
+  const int group = g->heads / g->cache.kv_heads, cells = group < kCols ? group : kCols;
+  const int64_t most = ceil_div(g->cache.columns * g->cache.page, static_cast<int64_t>(kTile));
+  if (most <= kWhole) return {0, 0, 0};
+  const int64_t rows = g->batch * g->cache.kv_heads * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
+  int64_t groups = 256 * waves;
+  if (most < (int64_t(1) << 30) / rows) groups = std::min(groups, ceil_div(most * rows, static_cast<int64_t>(kLeast)));
+  const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
+  const size_t row = padded(g->cache.head_dim, narrow) + 4;
+  return {static_cast<int>(groups), kLeast, static_cast<size_t>(groups) * (sizeof(int4) + 2 * cells * row * sizeof(float))};
 }
 
 template <typename T, typename C, int DP>
-int launch_step(const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
-  const int64_t chunks = ceil_div(static_cast<int64_t>(a.Hq / a.pool.Hk), static_cast<int64_t>(kCols));
-  const int64_t blocks = static_cast<int64_t>(a.B) * a.pool.Hk * chunks * s.pieces;
-  GEO_REQUIRE(grid_fits(blocks, kThreads) && grid_fits(static_cast<int64_t>(a.B) * a.Hq, kThreads),
-              "paged attention step: too many workgroups");
-  paged_step<T, C, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, stream>>>(a, s.pieces, s.per, part, static_cast<T*>(out));
+int launch_step(const Step& a, const geo_paged_step_t* g, void* out, void* workspace, size_t bytes, hipStream_t stream) {
+  const int group = a.Hq / a.pool.Hk;
+  const StepPlan s = plan_step(g, step_waves<T, C, DP>());
+  if (s.bytes > bytes || (s.bytes && !workspace))
+    return set_error(GEO_ERR_WORKSPACE, "paged attention step: workspace of %zu bytes, %zu needed", workspace ? bytes : size_t(0), s.bytes);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.pool.Hk * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
+  const int64_t blocks = s.groups ? s.groups : rows;
+  GEO_REQUIRE(grid_fits(blocks, kThreads), "paged attention step: too many workgroups");
+  Deal deal{s.groups, s.least, nullptr, nullptr};
+  if (s.groups) {
+    deal.desc = static_cast<int4*>(workspace);
+    deal.parts = reinterpret_cast<float*>(deal.desc + s.groups);
+  }
+  const size_t lds = a.bias.table ? sizeof(float) * kCols * a.bias.buckets + align_up(a.bias.maxd + 1, 16) : 0;
+  paged_step<T, C, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), lds, stream>>>(a, deal, a.pool.table, a.pos, static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_step");
-  if (s.pieces > 1) {
-    paged_join<T, DP><<<dim3(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.Hq)), dim3(kThreads), 0, stream>>>(
-        a.pool.D, a.Hq, s.pieces, s.per, a.pool.columns * a.pool.page, a.pos, part, static_cast<T*>(out));
+  if (s.groups) {
+    const int cells = std::min(group, kCols);
+    // pieces of a row: many where there are few rows
+    const dim3 grid(static_cast<uint32_t>(s.groups), static_cast<uint32_t>(cells));
+    if (s.groups > 32 * rows)
+      paged_join<T, DP, 1024><<<grid, dim3(1024), 0, stream>>>(a.pool.D, cells, deal.desc, deal.parts, static_cast<T*>(out));
+    else
+      paged_join<T, DP, 128><<<grid, dim3(128), 0, stream>>>(a.pool.D, cells, deal.desc, deal.parts, static_cast<T*>(out));
     GEO_LAUNCH_CHECK("paged_join");
   }
   return GEO_OK;
 }
 template <typename T, typename C>
-int choose_head(const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
+int choose_head(const Step& a, const geo_paged_step_t* g, void* out, void* ws, size_t bytes, hipStream_t stream) {
   switch (padded(a.pool.D, Code<C>::kNarrow)) {
     case 32:
-      if constexpr (!Code<C>::kNarrow) return launch_step<T, C, 32>(a, s, out, part, stream);
+      if constexpr (!Code<C>::kNarrow) return launch_step<T, C, 32>(a, g, out, ws, bytes, stream);
       [[fallthrough]];
-    case 64: return launch_step<T, C, 64>(a, s, out, part, stream);
-    default: return launch_step<T, C, 128>(a, s, out, part, stream);
+    case 64: return launch_step<T, C, 64>(a, g, out, ws, bytes, stream);
+    default: return launch_step<T, C, 128>(a, g, out, ws, bytes, stream);
   }
 }
 template <typename T>
-int choose_stored(int stored, const Step& a, const Split& s, void* out, float* part, hipStream_t stream) {
-  if (stored == GEO_I8) return choose_head<T, I8>(a, s, out, part, stream);
-  return stored == GEO_E4M3 ? choose_head<T, E4>(a, s, out, part, stream) : choose_head<T, T>(a, s, out, part, stream);
+int choose_stored(int stored, const Step& a, const geo_paged_step_t* g, void* out, void* ws, size_t bytes, hipStream_t stream) {
+  if (stored == GEO_I8) return choose_head<T, I8>(a, g, out, ws, bytes, stream);
+  return stored == GEO_E4M3 ? choose_head<T, E4>(a, g, out, ws, bytes, stream) : choose_head<T, T>(a, g, out, ws, bytes, stream);
 }
 
 }  // namespace paged
@@ -540,9 +687,7 @@ int choose_stored(int stored, const Step& a, const Split& s, void* out, float* p
 extern "C" size_t geo_paged_attention_step_workspace_bytes(const geo_paged_step_t* g) {
   using namespace geo::paged;
   if (!g || g->batch < 1 || g->cache.kv_heads < 1 || g->heads < g->cache.kv_heads || g->cache.columns < 1 || g->cache.page < 1) return 0;
-  const Split s = split_for(g);
-  const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
-  return s.pieces == 1 ? 0 : static_cast<size_t>(g->batch) * g->heads * s.pieces * (padded(g->cache.head_dim, narrow) + 2) * sizeof(float);
+  return plan_step(g, kMostWaves).bytes;
 }
 
 extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, void* workspace, size_t workspace_bytes, void* stream) {
@@ -558,8 +703,8 @@ extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, vo
   if (g->bias) {
     GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16, "%s: bias dtype code %d", name,
                 static_cast<int>(g->bias_dtype));
-    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->max_distance >= 1 && g->max_distance <= 1024,
-                "%s: bias of %d buckets up to distance %d (at most 1024)", name, g->buckets, g->max_distance);
+    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->buckets <= 256 && g->max_distance >= 1 && g->max_distance <= 1024,
+                "%s: bias of %d buckets up to distance %d (at most 256 and 1024)", name, g->buckets, g->max_distance);
   }
   if (g->batch == 0) return GEO_OK;
   const int size = g->dtype == GEO_F32 ? 4 : 2;
@@ -570,18 +715,13 @@ extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, vo
                   in_pieces(g->v, g->v_stream, g->v_head),
               "%s: null q, k or v, or rows not on multiples of 16 bytes", name);
   GEO_REQUIRE(out && g->positions, "%s: null output or positions", name);
-  const size_t need = geo_paged_attention_step_workspace_bytes(g);
-  if (need && (!workspace || workspace_bytes < need))
-    return set_error(GEO_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace ? workspace_bytes : size_t(0), need);
   a.q = g->q, a.k = g->k, a.v = g->v;
   a.q_st = g->q_stream, a.q_sh = g->q_head, a.k_st = g->k_stream, a.k_sh = g->k_head, a.v_st = g->v_stream, a.v_sh = g->v_head;
   a.pos = g->positions;
   a.bias = {g->bias, g->bias_lut, g->bias_dtype, g->buckets, g->max_distance};
   a.B = static_cast<int>(g->batch), a.Hq = g->heads, a.scale = g->scale;
-  const paged::Split s = paged::split_for(g);
-  float* const part = static_cast<float*>(workspace);
   const hipStream_t on = as_stream(stream);
-  if (g->dtype == GEO_F32) return paged::choose_stored<float>(g->cache.stored, a, s, out, part, on);
-  if (g->dtype == GEO_BF16) return paged::choose_stored<__bf16>(g->cache.stored, a, s, out, part, on);
-  return paged::choose_stored<_Float16>(g->cache.stored, a, s, out, part, on);
+  if (g->dtype == GEO_F32) return paged::choose_stored<float>(g->cache.stored, a, g, out, workspace, workspace_bytes, on);
+  if (g->dtype == GEO_BF16) return paged::choose_stored<__bf16>(g->cache.stored, a, g, out, workspace, workspace_bytes, on);
+  return paged::choose_stored<_Float16>(g->cache.stored, a, g, out, workspace, workspace_bytes, on);
 }
