@@ -57,7 +57,8 @@ struct PromptLds {
 
 template <typename T, typename C, int DP>
 __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
-                                                                  float* __restrict__ part, T* __restrict__ out) {
+                                                                  const int32_t* __restrict__ table, float* __restrict__ part,
+                                                                  T* __restrict__ out) {
   using M = Meet<T, C>;
   using L = PromptLds<T, C, DP>;
   using TK = typename M::K;
@@ -167,11 +168,21 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
   }
   Bytes16 kx[kLoads], vx[kLoads];
   float ksx = 0.f, vsx = 0.f;
-  int at = -1;  // the fetched tile's page
-  auto fetch = [&](int t) {
-    const int column = t / pool.page, off = t - column * pool.page;
-    at = __builtin_amdgcn_readfirstlane(pool.table[s.b * pool.table_st + column]);
-    if (static_cast<uint32_t>(at) >= static_cast<uint32_t>(pool.pages)) at = -1;
+  // where the next fetch reads: a column of the table and a place in its page; the entry behind it is on its way
+  const int32_t* const entries = table + s.b * pool.table_st;
+  auto entry = [&](int n) { return __builtin_amdgcn_readfirstlane(entries[min(n, pool.columns - 1)]); };
+  int column = k0 / pool.page, place_in = k0 - column * pool.page, entry_now = 0, entry_next = 0;
+  if (k0 < k1) entry_now = entry(column), entry_next = entry(column + 1);
+  int at = -1, off = 0;  // the fetched tile's page, and its place there
+  auto fetch = [&]() {
+    at = static_cast<uint32_t>(entry_now) < static_cast<uint32_t>(pool.pages) ? entry_now : -1;
+    off = place_in;
+    place_in += kKeys;
+    if (place_in == pool.page) {
+      place_in = 0;
+      entry_now = entry_next;
+      entry_next = entry(++column + 1);
+    }
     const int64_t slot0 = (static_cast<int64_t>(max(at, 0)) * pool.Hk + hk) * pool.page + off;
     const char* const kb = pool.k + slot0 * D * kSize;
     const char* const vb = pool.v + (slot0 / kBlk * kBlk) * D * kSize + slot0 % kBlk * kSize;
@@ -195,32 +206,29 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
   // given back to those that do see them.
   auto store = [&](int t, char* to, uint32_t* note) {
     const bool edge = t + kKeys - 1 > first_query;
-    const int page = at;
-    int64_t slot0 = 0;
-    if constexpr (M::kNarrow && M::kFloat) {
-      const int column = t / pool.page;
-      slot0 = (static_cast<int64_t>(max(page, 0)) * pool.Hk + hk) * pool.page + (t - column * pool.page);
-    }
+    const int64_t slot0 = (static_cast<int64_t>(max(at, 0)) * pool.Hk + hk) * pool.page + off;
     char *const kt = to, *const vt = to + L::kK;
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
-      const int x = threadIdx.x + n * kPromptThreads;
-      if (x >= pieces_of_tile) break;
+      int x = threadIdx.x + n * kPromptThreads;
+      if (x >= pieces_of_tile) continue;
+      if (edge) asm volatile("" : "+v"(x));  // as below: not ahead of the loop
       const int key0 = x / (kCpb * D) * kSpan + x % kCpb * kPer;  // first of the values' tokens
       if constexpr (!M::kNarrow) {
         *reinterpret_cast<uint4*>(kt + kto[n]) = kx[n].u;
+        uint4 v = vx[n].u;
         if (edge) {
           union { uint4 u; C c[kPer]; } y;
-          y.u = vx[n].u;
+          y.u = v;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
             const bool in = t + key0 + e < end, fine = fabsf(static_cast<float>(y.c[e])) < kInf;
             if (in && !fine) atomicOr(&note[(key0 + e) >> 5], 1u << ((key0 + e) & 31));
             if (!in || !fine) y.c[e] = static_cast<C>(0.f);
           }
-          vx[n].u = y.u;
+          v = y.u;
         }
-        *reinterpret_cast<uint4*>(vt + vto[n]) = vx[n].u;
+        *reinterpret_cast<uint4*>(vt + vto[n]) = v;
       } else if constexpr (M::kFloat) {
         const float ks = pool.ks[slot0 + x / (D / kPer)];
         union { uint4 u; uint8_t c[16]; } y, z;
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
   if (a.bias.table) far = near[a.bias.maxd];
   int page_now = -1;
   if (k0 < k1) {
-    fetch(k0);
+    fetch();
     page_now = at;
     store(k0, lds, wild[0]);
   }
@@ -288,7 +296,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
     if (threadIdx.x < 2) wild[turn == 0 ? 2 : turn - 1][threadIdx.x] = 0;
     const char *const kt = lds + buf * L::kBuffer, *const vt = kt + L::kK;
     const bool more = t + kKeys < k1;
-    if (more) fetch(t + kKeys);
+    const int off_now = off;
+    if (more) fetch();
     const int page_next = at;
     if (t <= wave_last) {
       const bool whole = t + kKeys - 1 <= wave_first;
@@ -303,6 +312,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
         for (int c = 0; c < kKc; ++c)
           x[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], x[u]);
       }
+      if constexpr (!M::kFloat) attn::reads_ahead<kSub * kKc, 4, 1>();
       // register 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j
       if constexpr (M::kScaled) {
         const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 8 * half;
@@ -387,25 +397,31 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
             for (int n = 0; n < M::kParts; ++n) o[m] = Type<TV>::mma(v, w[n], o[m]);
           }
         }
+      if constexpr (!M::kFloat && M::kParts == 1) attn::reads_ahead<kSub * 2 * kMt, 4, 1>();
       for (int u = 0; u < kSub; ++u) {
         uint32_t rest = wild[turn][u];
         while (rest) {  // rare: the queries that see an infinity or NaN have one in its dimension
           const int key = 32 * u + __builtin_ctz(rest);
           rest &= rest - 1;
-          const int slot = (t % pool.page) + key;
+          const int slot = off_now + key;
           const int64_t slot0 = (static_cast<int64_t>(max(page_now, 0)) * pool.Hk + hk) * pool.page;
-          const C* const col = reinterpret_cast<const C*>(pool.v) + slot0 * D + static_cast<int64_t>(slot / kBlk) * kBlk * D + slot % kBlk;
+          const C* col = reinterpret_cast<const C*>(pool.v) + slot0 * D + static_cast<int64_t>(slot / kBlk) * kBlk * D + slot % kBlk;
+          int d0 = 4 * half;
+          asm volatile("" : "+v"(d0));  // nothing of this ahead of the loop: it would take the products' registers
+          float scale = 1.f;
+          if constexpr (M::kNarrow) scale = pool.vs[slot0 + slot];
 #pragma unroll
           for (int m = 0; m < kMt; ++m)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int d = 32 * m + 8 * (r >> 2) + 4 * half + (r & 3);
+              const int d = d0 + 32 * m + 8 * (r >> 2) + (r & 3);
               if (d < D && p >= t + key) {
                 float v;
-                if constexpr (M::kNarrow) v = Code<C>::value(col[d * kBlk].bits) * pool.vs[slot0 + slot];
+                if constexpr (M::kNarrow) v = Code<C>::value(col[d * kBlk].bits) * scale;
                 else v = static_cast<float>(col[d * kBlk]);
                 if (!(fabsf(v) < kInf)) o[m][r] = __builtin_nanf("");
               }
+              if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
       }
@@ -480,7 +496,7 @@ template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
   const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * (a.bias.maxd + 1) * 4 : 0);
   GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(&paged_prompt<T, C, DP>), bytes));
-  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, p.per, part,
+  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, p.per, a.pool.table, part,
                                                                                         static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_prompt");
   if (p.pieces > 1) {
