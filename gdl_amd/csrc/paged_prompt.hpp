@@ -10,6 +10,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "paged.hpp"
 
@@ -33,6 +34,7 @@ struct Prompt {
 };
 
 constexpr int kPromptThreads = 256;
+using Words = uint32_t __attribute__((ext_vector_type(4)));
 
 // How a pool of C meets queries of T: key tiles of type K, value tiles of type V.  Codes stay codes where a
 // 16-bit type holds them (float16 weights times a scale could leave its range, so those meet bf16 values in two
@@ -46,6 +48,29 @@ struct Meet {
   static constexpr int kParts = kScaled ? parts_of<T>() : 1;
   static constexpr int kKeys = kFloat ? 32 : 64;
 };
+
+// A word of values (two of 16 bits) of the tokens `key` on: zeros in the place of those from `limit` on and of
+// infinities and NaN, whose tokens are noted.  In words: as an array of elements they would go through memory.
+template <typename V>
+__device__ __forceinline__ uint32_t seen_and_finite(uint32_t w, int key, int limit, uint32_t* note) {
+  constexpr uint32_t kPower = sizeof(V) == 4 ? 0x7f800000u : __is_same(V, __bf16) ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int e = 0; e < 4 / static_cast<int>(sizeof(V)); ++e) {
+    const uint32_t power = kPower << (16 * e), all = sizeof(V) == 4 ? ~0u : 0xffffu << (16 * e);
+    const bool in = key + e < limit, wild = (w & power) == power;
+    if (in && wild) atomicOr(&note[(key + e) >> 5], 1u << ((key + e) & 31));
+    if (!in || wild) w &= ~all;
+  }
+  return w;
+}
+
+// x[r] times what lane r of the 16 holds.
+template <int... R>
+__device__ __forceinline__ void by_row_of(f32x16& x, float y, std::integer_sequence<int, R...>) {
+  constexpr int kRowBroadcast = 0x150;
+  ((x[R] *= __uint_as_float(dpp_u32<kRowBroadcast + R>(__float_as_uint(y)))), ...);
+}
+__device__ __forceinline__ void by_row(f32x16& x, float y) { by_row_of(x, y, std::make_integer_sequence<int, 16>()); }
 
 template <typename T, typename C, int DP>
 struct PromptLds {
@@ -131,15 +156,20 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
       const int d = 16 * c + 8 * half;
-      union { uint4 u[sizeof(T) / 2]; KFrag f; } x = {};
-      if (d < D) {
+      union { Words u[sizeof(T) / 2]; KFrag f; } x = {};
+      if (d < D && a.scale != 0.f) {
+        const uint32_t flip = a.scale < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
-        for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) x.u[n] = reinterpret_cast<const uint4*>(row + d)[n];
+        for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) {
+          x.u[n] = reinterpret_cast<const Words*>(row + d)[n];
+          x.u[n] ^= flip;
+        }
       }
       q[c] = x.f;
     }
   }
-  const float scale2 = a.scale * kLog2e;
+  // positive, so that the products' largest is the scores': the queries carry its sign, or are zeros
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   float far = 0.f;
   const float* const near = sbias + (wave % a.heads) * (a.bias.maxd + 1);
   if (a.bias.table) {
@@ -166,7 +196,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
     vfrom[n] = blk * 64 * D + d * 64 + at * 16;
     vto[n] = d * L::kVRow + (blk * kSpan + at * kPer) * static_cast<int>(sizeof(TV));
   }
-  Bytes16 kx[kLoads], vx[kLoads];
+  Words kx[kLoads], vx[kLoads];
   float ksx = 0.f, vsx = 0.f;
   // where the next fetch reads: a column of the table and a place in its page; the entry behind it is on its way
   const int32_t* const entries = table + s.b * pool.table_st;
@@ -190,8 +220,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
     for (int n = 0; n < kLoads; ++n) {
       const int x = threadIdx.x + n * kPromptThreads;
       if (x < pieces_of_tile) {
-        kx[n].u = *reinterpret_cast<const uint4*>(kb + x * 16);
-        vx[n].u = *reinterpret_cast<const uint4*>(vb + vfrom[n]);
+        kx[n] = *reinterpret_cast<const Words*>(kb + x * 16);
+        vx[n] = *reinterpret_cast<const Words*>(vb + vfrom[n]);
       }
     }
     if constexpr (M::kScaled) {
@@ -215,25 +245,21 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
       if (edge) asm volatile("" : "+v"(x));  // as below: not ahead of the loop
       const int key0 = x / (kCpb * D) * kSpan + x % kCpb * kPer;  // first of the values' tokens
       if constexpr (!M::kNarrow) {
-        *reinterpret_cast<uint4*>(kt + kto[n]) = kx[n].u;
-        uint4 v = vx[n].u;
+        *reinterpret_cast<Words*>(kt + kto[n]) = kx[n];
+        Words v = vx[n];
         if (edge) {
-          union { uint4 u; C c[kPer]; } y;
-          y.u = v;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const bool in = t + key0 + e < end, fine = fabsf(static_cast<float>(y.c[e])) < kInf;
-            if (in && !fine) atomicOr(&note[(key0 + e) >> 5], 1u << ((key0 + e) & 31));
-            if (!in || !fine) y.c[e] = static_cast<C>(0.f);
-          }
-          v = y.u;
+          constexpr int kWord = 4 / kSize;  // tokens of a word
+          v.x = seen_and_finite<TV>(v.x, key0, end - t, note);
+          v.y = seen_and_finite<TV>(v.y, key0 + kWord, end - t, note);
+          v.z = seen_and_finite<TV>(v.z, key0 + 2 * kWord, end - t, note);
+          v.w = seen_and_finite<TV>(v.w, key0 + 3 * kWord, end - t, note);
         }
-        *reinterpret_cast<uint4*>(vt + vto[n]) = v;
+        *reinterpret_cast<Words*>(vt + vto[n]) = v;
       } else if constexpr (M::kFloat) {
         const float ks = pool.ks[slot0 + x / (D / kPer)];
-        union { uint4 u; uint8_t c[16]; } y, z;
-        y.u = kx[n].u;
-        z.u = vx[n].u;
+        union { Words u; uint8_t c[16]; } y, z;
+        y.u = kx[n];
+        z.u = vx[n];
         float* const kr = reinterpret_cast<float*>(kt + kto[n]);
         float* const vr = reinterpret_cast<float*>(vt + vto[n]);
 #pragma unroll
@@ -250,18 +276,14 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if constexpr (__is_same(T, _Float16)) reinterpret_cast<f16x8*>(kt + kto[n])[h] = decode8_f16<C>(kx[n].w[2 * h], kx[n].w[2 * h + 1]);
-          else reinterpret_cast<bf16x8*>(kt + kto[n])[h] = decode8<C>(kx[n].w[2 * h], kx[n].w[2 * h + 1]);
+          const uint32_t klo = h ? kx[n].z : kx[n].x, khi = h ? kx[n].w : kx[n].y;
+          if constexpr (__is_same(T, _Float16)) reinterpret_cast<f16x8*>(kt + kto[n])[h] = decode8_f16<C>(klo, khi);
+          else reinterpret_cast<bf16x8*>(kt + kto[n])[h] = decode8<C>(klo, khi);
           Bytes16 v;
-          v.b = decode8<C>(vx[n].w[2 * h], vx[n].w[2 * h + 1]);
+          v.b = decode8<C>(h ? vx[n].z : vx[n].x, h ? vx[n].w : vx[n].y);
           if (edge) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int key = key0 + 8 * h + e;
-              const bool in = t + key < end, fine = fabsf(static_cast<float>(v.b[e])) < kInf;
-              if (in && !fine) atomicOr(&note[key >> 5], 1u << (key & 31));
-              if (!in || !fine) v.b[e] = static_cast<__bf16>(0.f);
-            }
+            for (int e = 0; e < 4; ++e) v.w[e] = seen_and_finite<__bf16>(v.w[e], key0 + 8 * h + 2 * e, end - t, note);
           }
           reinterpret_cast<bf16x8*>(vt + vto[n])[h] = v.b;
         }
@@ -314,28 +336,31 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
       }
       if constexpr (!M::kFloat) attn::reads_ahead<kSub * kKc, 4, 1>();
       // register 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j
-      if constexpr (M::kScaled) {
-        const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 8 * half;
+      float vs[kSub];
+      if constexpr (M::kScaled) {  // lane r of 16 holds the scale of the half's register r, and hands it round
+        const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 16 * (lane >> 3 & 1) + 8 * half + (lane & 7);
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] *= scales[32 * u + 16 * (r >> 3) + (r & 7)];
-      } else {
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) x[u] *= scale2;
+        for (int u = 0; u < kSub; ++u) {
+          by_row(x[u], scales[32 * u]);
+          vs[u] = scales[kKeys + 32 * u];
+        }
       }
       if (a.bias.table) {
+        const float by = M::kScaled ? 1.f : scale2;
         if (wave_first - (t + kKeys - 1) < a.bias.maxd) {
 #pragma unroll
           for (int u = 0; u < kSub; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              x[u][r] += near[min(max(p - (t + 32 * u + 16 * (r >> 3) + 8 * half + (r & 7)), 0), a.bias.maxd)];
+              x[u][r] = fmaf(x[u][r], by, near[min(max(p - (t + 32 * u + 16 * (r >> 3) + 8 * half + (r & 7)), 0), a.bias.maxd)]);
         } else {
 #pragma unroll
-          for (int u = 0; u < kSub; ++u) x[u] += far;
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[u][r] = fmaf(x[u][r], by, far);
         }
       }
+      const float by = M::kScaled || a.bias.table ? 1.f : scale2;  // what the scores still lack
       const int seen = p - t - 8 * half;  // a lane's tokens 32 u + 16 c + j up to this one
       if (!whole) {
 #pragma unroll
@@ -349,7 +374,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, x[u][r]);
-      most = halves_max(most);
+      most = halves_max(most) * by;
       const bool up = most > top + kLazy;
       if (__any(up)) {
         const float keep = up ? exp2_hw(top - most) : 1.f;
@@ -363,18 +388,19 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          x[u][r] = exp2_hw(x[u][r] - shift);
+          x[u][r] = exp2_hw(fmaf(x[u][r], by, -shift));
           sum += x[u][r];
         }
       if constexpr (M::kScaled) {
-        const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + kKeys + 8 * half;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+        for (int u = 0; u < kSub; ++u) {
+          by_row(x[u], vs[u]);
+          if (!whole) {  // an unseen scale may be NaN
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float y = x[u][r] * scales[32 * u + 16 * (r >> 3) + (r & 7)];
-            x[u][r] = whole || 32 * u + 16 * (r >> 3) + (r & 7) <= seen ? y : 0.f;  // an unseen scale may be NaN
+            for (int r = 0; r < 16; ++r)
+              if (32 * u + 16 * (r >> 3) + (r & 7) > seen) x[u][r] = 0.f;
           }
+        }
       }
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
