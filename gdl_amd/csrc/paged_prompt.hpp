@@ -66,11 +66,11 @@ __device__ __forceinline__ uint32_t seen_and_finite(uint32_t w, int key, int lim
 
 // x[r] times what lane r of the 16 holds.
 template <int... R>
-__device__ __forceinline__ void by_row_of(f32x16& x, float y, std::integer_sequence<int, R...>) {
+__device__ __forceinline__ void by_row_of(float* x, float y, std::integer_sequence<int, R...>) {
   constexpr int kRowBroadcast = 0x150;
-  ((x[R] *= __uint_as_float(dpp_u32<kRowBroadcast + R>(__float_as_uint(y)))), ...);
+  ((x[R] *= __uint_as_float(dpp0_u32<kRowBroadcast + R>(__float_as_uint(y)))), ...);
 }
-__device__ __forceinline__ void by_row(f32x16& x, float y) { by_row_of(x, y, std::make_integer_sequence<int, 16>()); }
+__device__ __forceinline__ void by_row(float (&x)[16], float y) { by_row_of(x, y, std::make_integer_sequence<int, 16>()); }
 
 template <typename T, typename C, int DP>
 struct PromptLds {
@@ -81,7 +81,7 @@ struct PromptLds {
 };
 
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
+__global__ __launch_bounds__(kPromptThreads, (DP == 128 ? 2 : 3)) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
                                                                   const int32_t* __restrict__ table, float* __restrict__ part,
                                                                   T* __restrict__ out) {
   using M = Meet<T, C>;
@@ -323,19 +323,25 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
     const int page_next = at;
     if (t <= wave_last) {
       const bool whole = t + kKeys - 1 <= wave_first;
-      f32x16 x[kSub];
+      f32x16 product[kSub];
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
-        x[u] = f32x16{};
+        product[u] = f32x16{};
         // row 16 c + 8 a + 4 h + i of the product is token 16 c + 8 h + 4 a + i
         const int r = lane & 31, key = 32 * u + ((r & 19) | (r >> 2 & 1) << 3 | (r >> 3 & 1) << 2);
         const char* const row = kt + key * L::kKRow + half * 8 * static_cast<int>(sizeof(TK));
 #pragma unroll
         for (int c = 0; c < kKc; ++c)
-          x[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], x[u]);
+          product[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], product[u]);
       }
       if constexpr (!M::kFloat) attn::reads_ahead<kSub * kKc, 4, 1>();
-      // register 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j
+      // number 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j; single registers, which branches may change
+      // without a copy of all sixteen
+      float x[kSub][16];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[u][r] = product[u][r];
       float vs[kSub];
       if constexpr (M::kScaled) {  // lane r of 16 holds the scale of the half's register r, and hands it round
         const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 16 * (lane >> 3 & 1) + 8 * half + (lane & 7);
@@ -413,7 +419,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void paged_prompt(const Prompt a
             for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
             split8<M::kParts>(y, w);
           } else {
-            w[0] = attn::frag_of<TV>(x[u], c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[0][e] = static_cast<TV>(x[u][8 * c + e]);
           }
           const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
 #pragma unroll

@@ -161,7 +161,7 @@ struct NarrowWeights {
 template <int... N>
 __device__ __forceinline__ void by_group_of(float* x, float y, std::integer_sequence<int, N...>) {
   constexpr int kRowBroadcast = 0x150;
-  ((x[N] *= __uint_as_float(dpp_u32<kRowBroadcast + N>(__float_as_uint(y)))), ...);
+  ((x[N] *= __uint_as_float(dpp0_u32<kRowBroadcast + N>(__float_as_uint(y)))), ...);
 }
 template <int N>
 __device__ __forceinline__ void by_group(float (&x)[N], float y) { by_group_of(x, y, std::make_integer_sequence<int, N>()); }
