@@ -7,7 +7,7 @@ extern template int prompt_of<float>(int, const Prompt&, const PromptPlan&, void
 extern template int prompt_of<_Float16>(int, const Prompt&, const PromptPlan&, void*, float*, hipStream_t);
 
 inline PromptPlan plan_for(const geo_paged_prompt_t* g) {
-  return plan_prompt(g->tokens, g->batch, g->heads, g->cache.kv_heads, g->cache.columns * g->cache.page);
+  return plan_prompt(g->tokens, g->batch, g->heads, g->cache.kv_heads, prompt_padded(g->cache.head_dim), g->cache.columns * g->cache.page);
 }
 }  // namespace paged
 }  // namespace geo

@@ -80,8 +80,11 @@ struct PromptLds {
   static constexpr int kBuffer = kK + kV + kS;
 };
 
+// Workgroups of the kernel on a CU, by the registers that it takes.
+constexpr int prompt_waves(int DP) { return DP == 128 ? 2 : 3; }
+
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kPromptThreads, (DP == 128 ? 2 : 3)) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
+__global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
                                                                   const int32_t* __restrict__ table, float* __restrict__ part,
                                                                   T* __restrict__ out) {
   using M = Meet<T, C>;
@@ -106,8 +109,9 @@ __global__ __launch_bounds__(kPromptThreads, (DP == 128 ? 2 : 3)) void paged_pro
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // one XCD works through one key head's sequences, so that their pages stay in its L2
-  int64_t w = xcd_block();
+  // One XCD works through one key head's sequences, so that their pages stay in its L2.  Pieces differ too much for
+  // that (late ones have only the last queries): they go to the XCDs in short runs.
+  int64_t w = pieces == 1 ? xcd_block() : xcd_block_runs(8);
   const int64_t tile = tiles - 1 - w % tiles;  // the longest first
   w /= tiles;
   const int piece = static_cast<int>(w % pieces);
@@ -478,39 +482,62 @@ __global__ __launch_bounds__(kPromptThreads, (DP == 128 ? 2 : 3)) void paged_pro
   }
 }
 
-// The pieces of a row joined: DP / 4 threads to a row.
-template <typename T, int DP>
+// The pieces of a row joined: DP / 4 lanes to a row, four dimensions each, SETS of them with a share of the pieces.
+template <typename T, int DP, int SETS>
 __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join(int D, int64_t rows, int pieces, const float* __restrict__ part,
                                                                     T* __restrict__ out) {
-  constexpr int kLanes = DP / 4;
+  constexpr int kLanes = DP / 4, kAtOnce = kPromptThreads / (kLanes * SETS), kRow = DP + 4;
   using f32x4 = float __attribute__((ext_vector_type(4)));
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kPromptThreads + threadIdx.x) / kLanes;
-  const int d = 4 * (threadIdx.x % kLanes);
-  if (row >= rows || d >= D) return;
-  float top = -kInf;
-  for (int n = 0; n < pieces; ++n) top = fmaxf(top, part[(n * rows + row) * (DP + 4)]);
-  float sum = 0.f;
-  f32x4 y = {};
-  for (int n = 0; n < pieces; ++n) {
-    const float* const from = part + (n * rows + row) * (DP + 4);
-    const float keep = from[0] == -kInf ? 0.f : exp2_hw(from[0] - top);
-    sum += from[1] == from[1] ? from[1] * keep : from[1];
-    y += *reinterpret_cast<const f32x4*>(from + 4 + d) * keep;
+  struct Part { float top, sum; f32x4 y; };
+  __shared__ float tops[SETS][kAtOnce], sums[SETS][kAtOnce];
+  __shared__ f32x4 acc[SETS][kAtOnce][kLanes];
+  const int lane = threadIdx.x % kLanes, set = threadIdx.x / kLanes % SETS, place = threadIdx.x / (kLanes * SETS);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kAtOnce + place;
+  if (SETS == 1 && row >= rows) return;
+  const float* const first = part + min(row, rows - 1) * kRow;
+  Part a{-kInf, 0.f, {}};
+  auto add = [&](float m, float l, const f32x4& v) {
+    const float most = fmaxf(a.top, m), before = a.top == -kInf ? 0.f : exp2_hw(a.top - most), keep = m == -kInf ? 0.f : exp2_hw(m - most);
+    a.sum = (a.sum == a.sum ? a.sum * before : a.sum) + (l == l ? l * keep : l);
+    a.y = a.y * before + v * keep;
+    a.top = most;
+  };
+#pragma unroll 4
+  for (int n = set; n < pieces; n += SETS) {
+    const float* const from = first + n * rows * kRow;
+    add(from[0], from[1], *reinterpret_cast<const f32x4*>(from + 4 + 4 * lane));
   }
+  if constexpr (SETS > 1) {
+    acc[set][place][lane] = a.y;
+    if (lane == 0) {
+      tops[set][place] = a.top;
+      sums[set][place] = a.sum;
+    }
+    __syncthreads();
+    if (set > 0 || row >= rows) return;
+    for (int n = 1; n < SETS; ++n) add(tops[n][place], sums[n][place], acc[n][place][lane]);
+  }
+  const int d = 4 * lane;
+  if (d >= D) return;
   union { T t[4]; uint2 u2; uint4 u4; } w;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w.t[e] = static_cast<T>(part[row * (DP + 4) + 1] == -1.f ? 0.f : y[e] / sum);
+  for (int e = 0; e < 4; ++e) w.t[e] = static_cast<T>(first[1] == -1.f ? 0.f : a.y[e] / a.sum);
   if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(out + row * D + d) = w.u2;
   else *reinterpret_cast<uint4*>(out + row * D + d) = w.u4;
 }
 
+inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
 // A key head's query heads that one workgroup takes together, and the pieces of the longest history that the
-// table has room for: where rows do not fill the 256 CUs twice, pieces of at least 512 tokens do.
+// table has room for.  Twice as many while they all run at a time: a workgroup alone on its CU waits most of
+// the time (1.8 us a tile), so there pieces of 256 tokens pay for the join; the more there are the longer they
+// have to be.  In us, whole | cut: 16 queries behind 3000 tokens 85 | 21 (4 heads to a
+// key head of 64, e4m3), 4 packets of 384 behind 20,000 330 | 131, 2 of 1000 behind 1000 (of 128, bfloat16) 58 | 66.
 struct PromptPlan {
   int heads, unit, pieces, per;
   int64_t tiles, blocks;
 };
-inline PromptPlan plan_prompt(int64_t T, int64_t B, int Hq, int Hk, int64_t most) {
+inline PromptPlan plan_prompt(int64_t T, int64_t B, int Hq, int Hk, int DP, int64_t most) {
   PromptPlan p;
   const int group = Hq / Hk;
   p.heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
@@ -518,12 +545,19 @@ inline PromptPlan plan_prompt(int64_t T, int64_t B, int Hq, int Hk, int64_t most
   p.tiles = tiles_of(T, B, p.unit);
   const int64_t columns = static_cast<int64_t>(Hq) / p.heads, busy = ((T >> p.unit) + B) * columns;
   p.pieces = 1;
-  while (busy * p.pieces < 512 && most / (2 * p.pieces) >= 512) p.pieces *= 2;
+  const int64_t at_once = 256 * prompt_waves(DP);
+  for (;;) {
+    const int64_t now = busy * p.pieces;
+    if (2 * now > at_once || most / (2 * p.pieces) < (4 * now <= at_once ? 256 : 8 * now < 3 * at_once ? 512 : 2048)) break;
+    p.pieces *= 2;
+  }
+  // Long prompts of few sequences end with their last queries' workgroups, which see twice the keys of the
+  // average: halves end sooner.  16 (4) heads of 128, bfloat16, whole | cut: 8000 tokens 419 | 398 us, 16,000 1554 | 1252.
+  if (p.pieces == 1 && 2 * T >= B * most && most >= 6144 && busy < 4 * at_once) p.pieces = 2;
   p.per = static_cast<int>(align_up(static_cast<size_t>(ceil_div(most, static_cast<int64_t>(p.pieces))), 64));
   p.blocks = p.tiles * columns * p.pieces;
   return p;
 }
-inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
@@ -533,10 +567,17 @@ int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, 
                                                                                         static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_prompt");
   if (p.pieces > 1) {
-    const int64_t rows = a.T * a.Hq, blocks = ceil_div(rows * (DP / 4), static_cast<int64_t>(kPromptThreads));
+    constexpr int kSets = 8;
+    const int64_t rows = a.T * a.Hq;
+    const bool many = p.pieces > 8;
+    const int64_t blocks = ceil_div(rows * (DP / 4) * (many ? kSets : 1), static_cast<int64_t>(kPromptThreads));
     GEO_REQUIRE(grid_fits(blocks, kPromptThreads), "paged attention: too many workgroups");
-    paged_prompt_join<T, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kPromptThreads), 0, stream>>>(a.pool.D, rows, p.pieces, part,
-                                                                                                      static_cast<T*>(out));
+    if (many)
+      paged_prompt_join<T, DP, kSets><<<dim3(static_cast<uint32_t>(blocks)), dim3(kPromptThreads), 0, stream>>>(a.pool.D, rows, p.pieces, part,
+                                                                                                           static_cast<T*>(out));
+    else
+      paged_prompt_join<T, DP, 1><<<dim3(static_cast<uint32_t>(blocks)), dim3(kPromptThreads), 0, stream>>>(a.pool.D, rows, p.pieces, part,
+                                                                                                       static_cast<T*>(out));
     GEO_LAUNCH_CHECK("paged_prompt_join");
   }
   return GEO_OK;
