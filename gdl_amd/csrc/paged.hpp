@@ -204,7 +204,7 @@ inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool) {
   GEO_REQUIRE(g->page >= 64 && g->page % 64 == 0 && g->page <= (1 << 20), "%s: pages of %d tokens (a multiple of 64 up to 2^20)",
               name, g->page);
   GEO_REQUIRE(g->pages >= 1 && g->pages < (int64_t(1) << 31), "%s: %lld pages", name, static_cast<long long>(g->pages));
-  GEO_REQUIRE(g->columns >= 1 && g->columns * g->page < (int64_t(1) << 30), "%s: a table of %lld columns of %d tokens (below 2^30)",
+  GEO_REQUIRE(g->columns >= 1 && g->columns < (int64_t(1) << 30) && g->columns * g->page < (int64_t(1) << 30), "%s: a table of %lld columns of %d tokens (below 2^30)",
               name, static_cast<long long>(g->columns), g->page);
   auto aligned = [](const void* p) { return p && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   GEO_REQUIRE(aligned(g->k) && aligned(g->v) && g->k != g->v, "%s: null pool, not on 16 bytes, or one for both", name);
@@ -214,6 +214,12 @@ inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool) {
   *pool = Pool{static_cast<char*>(g->k), static_cast<char*>(g->v), g->k_scale, g->v_scale, g->table, g->table_stream,
                static_cast<int>(g->pages), static_cast<int>(g->columns), g->page, g->kv_heads, g->head_dim};
   return GEO_OK;
+}
+// Numbers that a size can be formed of (the rest is checked where the call itself is).
+inline bool sizes_ok(const geo_paged_t& c, int64_t batch, int heads) {
+  return batch >= 1 && batch < (int64_t(1) << 31) && c.kv_heads >= 1 && c.kv_heads < (1 << 16) && heads >= c.kv_heads && heads < (1 << 20) &&
+         heads % c.kv_heads == 0 && c.page >= 64 && c.page <= (1 << 20) && c.columns >= 1 && c.columns < (int64_t(1) << 30) &&
+         c.columns * c.page < (int64_t(1) << 30);
 }
 inline bool type_ok(int dtype, int stored) {
   return (dtype == GEO_F32 || dtype == GEO_BF16 || dtype == GEO_F16) &&

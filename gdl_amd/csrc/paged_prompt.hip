@@ -14,9 +14,7 @@ inline PromptPlan plan_for(const geo_paged_prompt_t* g) {
 
 extern "C" size_t geo_paged_attention_workspace_bytes(const geo_paged_prompt_t* g) {
   using namespace geo::paged;
-  if (!g || g->tokens < 1 || g->batch < 1 || g->cache.kv_heads < 1 || g->heads < g->cache.kv_heads || g->cache.columns < 1 ||
-      g->cache.page < 1)
-    return 0;
+  if (!g || g->tokens < 1 || g->tokens >= (int64_t(1) << 31) || !sizes_ok(g->cache, g->batch, g->heads)) return 0;
   const PromptPlan p = plan_for(g);
   return p.pieces == 1 ? 0 : static_cast<size_t>(g->tokens) * g->heads * p.pieces * (prompt_padded(g->cache.head_dim) + 4) * sizeof(float);
 }
@@ -29,8 +27,8 @@ extern "C" int geo_paged_attention(const geo_paged_prompt_t* g, void* out, void*
   if (const int rc = paged::pool_args(name, &g->cache, &a.pool)) return rc;
   GEO_REQUIRE(paged::type_ok(g->dtype, g->cache.stored), "%s: queries of type code %d, a pool of %d", name,
               static_cast<int>(g->dtype), static_cast<int>(g->cache.stored));
-  GEO_REQUIRE(g->heads >= 1 && g->heads % g->cache.kv_heads == 0, "%s: %d heads are no multiple of %d key heads", name, g->heads,
-              g->cache.kv_heads);
+  GEO_REQUIRE(g->heads >= 1 && g->heads < (1 << 20) && g->heads % g->cache.kv_heads == 0,
+              "%s: %d heads are no multiple of %d key heads (below 2^20)", name, g->heads, g->cache.kv_heads);
   GEO_REQUIRE(g->tokens >= 0 && g->tokens < (int64_t(1) << 31) - 64 && g->batch >= 0 && g->batch < (int64_t(1) << 30) &&
                   (g->ptr || g->batch <= 1),
               "%s: %lld tokens of %lld sequences%s", name, static_cast<long long>(g->tokens), static_cast<long long>(g->batch),
@@ -38,8 +36,8 @@ extern "C" int geo_paged_attention(const geo_paged_prompt_t* g, void* out, void*
   if (g->bias) {
     GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16, "%s: bias dtype code %d", name,
                 static_cast<int>(g->bias_dtype));
-    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->max_distance >= 1 && g->max_distance <= 1024,
-                "%s: bias of %d buckets up to distance %d (at most 1024)", name, g->buckets, g->max_distance);
+    GEO_REQUIRE(g->bias_lut && g->buckets >= 1 && g->buckets <= 256 && g->max_distance >= 1 && g->max_distance <= 1024,
+                "%s: bias of %d buckets up to distance %d (at most 256 and 1024)", name, g->buckets, g->max_distance);
   }
   if (g->tokens == 0) return GEO_OK;
   GEO_REQUIRE(g->batch >= 1, "%s: tokens of no sequence", name);

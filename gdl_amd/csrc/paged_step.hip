@@ -760,7 +760,7 @@ int choose_stored(int stored, const Step& a, const geo_paged_step_t* g, void* ou
 
 extern "C" size_t geo_paged_attention_step_workspace_bytes(const geo_paged_step_t* g) {
   using namespace geo::paged;
-  if (!g || g->batch < 1 || g->cache.kv_heads < 1 || g->heads < g->cache.kv_heads || g->cache.columns < 1 || g->cache.page < 1) return 0;
+  if (!g || !sizes_ok(g->cache, g->batch, g->heads)) return 0;
   return plan_step(g, kMostWaves).bytes;
 }
 
@@ -772,8 +772,9 @@ extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, vo
   if (const int rc = paged::pool_args(name, &g->cache, &a.pool)) return rc;
   GEO_REQUIRE(paged::type_ok(g->dtype, g->cache.stored), "%s: tokens of type code %d, a pool of %d", name,
               static_cast<int>(g->dtype), static_cast<int>(g->cache.stored));
-  GEO_REQUIRE(g->batch >= 0 && g->batch < (int64_t(1) << 31) && g->heads >= 1 && g->heads % g->cache.kv_heads == 0,
-              "%s: %d heads are no multiple of %d key heads", name, g->heads, g->cache.kv_heads);
+  GEO_REQUIRE(g->batch >= 0 && g->batch < (int64_t(1) << 31) && g->heads >= 1 && g->heads < (1 << 20) &&
+                  g->heads % g->cache.kv_heads == 0,
+              "%s: %d heads are no multiple of %d key heads (below 2^20)", name, g->heads, g->cache.kv_heads);
   if (g->bias) {
     GEO_REQUIRE(g->bias_dtype == GEO_F32 || g->bias_dtype == GEO_BF16 || g->bias_dtype == GEO_F16, "%s: bias dtype code %d", name,
                 static_cast<int>(g->bias_dtype));

@@ -7,17 +7,22 @@
 
 The block mixes along the order twice: over the whole cloud by ``gated_recurrence``, near by
 ``window_attention`` with a relative position bias, each behind a norm and added to its input.
+``window=None`` attends to the whole stream; its cache keeps that in pages, in 8 bits if asked, and takes
+packets of points too:
+
+    cache = block.new_cache(B, torch.int8, tokens=100_000); y = block.extend(x, ptr, start, cache)
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 from torch import Tensor, nn
 
 from gdl_amd.functional.attention import WindowCache, window_attention, window_attention_step
+from gdl_amd.functional.paged import PagedCache, paged_attention, paged_attention_step
 from gdl_amd.functional.recurrence import gated_recurrence, gated_recurrence_step
 
 
@@ -45,10 +50,12 @@ def serial_order(pos: Tensor, ptr: Optional[Tensor] = None) -> Tensor:
 
 @dataclass
 class BlockCache:
-    """What a causal block keeps of its streams: recurrence states [B, C] and the attention's window."""
+    """What a causal block keeps of its streams: recurrence states [B, C], and the attention's window, or all
+    of the streams in pages and the ``table`` (int32 [B, n]) that says which are whose."""
 
     state: Tensor
-    window: WindowCache
+    window: Union[WindowCache, PagedCache]
+    table: Optional[Tensor] = None
 
 
 class PointSequenceBlock(nn.Module):
@@ -57,19 +64,21 @@ class PointSequenceBlock(nn.Module):
     Args:
         channels: width; ``channels / heads`` is the head size (a multiple of 8 up to 128 for ``step``).
         heads, kv_heads: query heads and the key heads that they share (all by default).
-        window: tokens seen before a token, and behind it unless ``causal``.
-        sinks: first tokens of a sequence that stay visible.
+        window: tokens seen before a token, and behind it unless ``causal``; None for all.
+        sinks: first tokens of a sequence that stay visible (of a window).
         buckets, max_distance: of the relative position bias.
         causal: tokens see earlier ones alone; else the recurrence runs both ways and its results are
             added.
     """
 
-    def __init__(self, channels: int, heads: int, window: int, *, kv_heads: Optional[int] = None, sinks: int = 0,
+    def __init__(self, channels: int, heads: int, window: Optional[int], *, kv_heads: Optional[int] = None, sinks: int = 0,
                  buckets: int = 32, max_distance: int = 128, causal: bool = True):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if channels % heads or heads % kv_heads:
             raise ValueError(f"PointSequenceBlock: {channels} channels, {heads} heads, {kv_heads} key heads do not divide")
+        if window is None and sinks:
+            raise ValueError(f"PointSequenceBlock: {sinks} first tokens of no window")
         self.channels, self.heads, self.kv_heads, self.head_dim = channels, heads, kv_heads, channels // heads
         self.window, self.sinks, self.max_distance, self.causal = window, sinks, max_distance, causal
         self.scan_norm, self.attend_norm = nn.LayerNorm(channels), nn.LayerNorm(channels)
@@ -99,15 +108,29 @@ class PointSequenceBlock(nn.Module):
         if not self.causal:
             h = h + gated_recurrence(*parts, self.decay, ptr=ptr, reverse=True)[0]
         x = x + self.scan_out(h)
-        out = window_attention(*self._split(x), (self.window, 0 if self.causal else self.window), sinks=self.sinks, ptr=ptr,
+        reach = -1 if self.window is None else self.window
+        out = window_attention(*self._split(x), (reach, 0 if self.causal else reach), sinks=self.sinks, ptr=ptr,
                                mask=mask, bias=self.bias, max_distance=self.max_distance)
         return x + self.attend_out(out.flatten(1))
 
-    def new_cache(self, batch: int, dtype: Optional[torch.dtype] = None) -> BlockCache:
-        """The cache of ``batch`` streams without tokens."""
+    def new_cache(self, batch: int, dtype: Optional[torch.dtype] = None, *, tokens: Optional[int] = None,
+                  page: int = 64) -> BlockCache:
+        """The cache of ``batch`` streams without tokens.  Without a window it has pages for ``tokens`` tokens of each
+        stream, of the block's type, torch.int8 or torch.float8_e4m3fn; to share a pool among streams of
+        unequal lengths, make a ``BlockCache`` of your own ``PagedCache`` and table."""
         if not self.causal:
             raise ValueError("PointSequenceBlock: only a causal block answers token by token")
         dev = self.decay.device
+        if self.window is None:
+            if tokens is None or tokens < 1 or batch < 1:
+                raise ValueError(f"PointSequenceBlock: a cache without a window is for a number of tokens, got {tokens} for {batch}")
+            each = -(-tokens // page)
+            pool = PagedCache.empty(batch * each, self.kv_heads, self.head_dim, page=page, dtype=dtype or self.attend_in.weight.dtype,
+                                    device=dev)
+            table = torch.arange(batch * each, dtype=torch.int32, device=dev).view(batch, each)
+            return BlockCache(torch.zeros(batch, self.channels, device=dev), pool, table)
+        if tokens is not None:
+            raise ValueError("PointSequenceBlock: a window's cache has no number of tokens")
         window = WindowCache.empty(batch, self.kv_heads, self.head_dim, self.window, sinks=self.sinks,
                                    dtype=dtype or self.attend_in.weight.dtype, device=dev)
         return BlockCache(torch.zeros(batch, self.channels, device=dev), window)
@@ -120,6 +143,30 @@ class PointSequenceBlock(nn.Module):
         parts = self.scan_in(self.scan_norm(x)).split(self.channels, 1)
         h, state = gated_recurrence_step(*parts, self.decay, cache.state, positions=positions)
         x = x + self.scan_out(h)
-        out = window_attention_step(*self._split(x), cache.window, positions, bias=self.bias, max_distance=self.max_distance)
+        near = dict(bias=self.bias, max_distance=self.max_distance)
+        if cache.table is None:
+            out = window_attention_step(*self._split(x), cache.window, positions, **near)
+        else:
+            out = paged_attention_step(*self._split(x), cache.window, cache.table, positions, **near)
         cache.state = state  # a call that is refused above leaves the cache as it was
+        return x + self.attend_out(out.flatten(1))
+
+    @torch.no_grad()
+    def extend(self, x: Tensor, ptr: Tensor, start: Tensor, cache: BlockCache) -> Tensor:
+        """New tokens x [T, channels] of the streams, packed (``ptr`` int64 [B + 1]), from the positions ``start``
+        (int64 [B]) on, which ``cache`` then holds; the forward's rows for them.  For a block without a window.
+        A stream whose tokens begin at position 0 begins anew; one without tokens is left alone."""
+        if cache.table is None:
+            raise ValueError("PointSequenceBlock: only a block without a window takes several tokens of a stream")
+        if ptr.shape != (cache.state.shape[0] + 1,) or start.shape != (cache.state.shape[0],):
+            raise ValueError(f"PointSequenceBlock: ptr and start of {cache.state.shape[0]} streams, got {tuple(ptr.shape)}, "
+                             f"{tuple(start.shape)}")
+        parts = self.scan_in(self.scan_norm(x)).split(self.channels, 1)
+        anew = (start == 0) & (ptr[1:] > ptr[:-1])
+        h, state = gated_recurrence(*parts, self.decay, ptr=ptr, state=cache.state.masked_fill(anew.unsqueeze(1), 0.0))
+        x = x + self.scan_out(h)
+        q, k, v = self._split(x)
+        cache.window.write(k, v, cache.table, ptr, start)
+        out = paged_attention(q, cache.window, cache.table, ptr, start, bias=self.bias, max_distance=self.max_distance)
+        cache.state = state
         return x + self.attend_out(out.flatten(1))
