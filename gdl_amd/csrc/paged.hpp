@@ -158,6 +158,10 @@ struct Span {
   int b, lo, hi;         // the sequence; the tile's places that have tokens, lo .. hi - 1 (none: lo >= hi)
   int64_t before;        // on a sequence's first tile: how many of its tokens have negative positions
 };
+// A start in a range in which nothing overflows; what lies as far out has no page either way.
+__device__ __forceinline__ int64_t start_of(const int64_t* start, int b) {
+  return start ? min(max(start[b], -(int64_t(1) << 60)), int64_t(1) << 60) : 0;
+}
 // Wave-wide: 64 sequences are looked at together.
 __device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile, int unit) {
   const int lane = threadIdx.x & 63;
@@ -174,7 +178,7 @@ __device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start
     lo = next;
   } while (len > 1);
   const int b = __builtin_amdgcn_readfirstlane(lo);
-  Span s{offset(b), start ? start[b] : 0, 0, b, 0, 0, 0};
+  Span s{offset(b), start_of(start, b), 0, b, 0, 0, 0};
   const int64_t n = offset(b + 1) - s.first, from = max(s.start, int64_t(0)), end = s.start + n;
   const int64_t turn = tile - ((s.first >> unit) + 2 * static_cast<int64_t>(b));
   s.tile0 = ((from >> unit) + turn) << unit;
