@@ -5,17 +5,13 @@ namespace geo {
 namespace paged {
 extern template int prompt_of<float>(int, const Prompt&, const PromptPlan&, void*, float*, hipStream_t);
 extern template int prompt_of<_Float16>(int, const Prompt&, const PromptPlan&, void*, float*, hipStream_t);
-
-inline PromptPlan plan_for(const geo_paged_prompt_t* g) {
-  return plan_prompt(g->tokens, g->batch, g->heads, g->cache.kv_heads, prompt_padded(g->cache.head_dim), g->cache.columns * g->cache.page);
-}
 }  // namespace paged
 }  // namespace geo
 
 extern "C" size_t geo_paged_attention_workspace_bytes(const geo_paged_prompt_t* g) {
   using namespace geo::paged;
   if (!g || g->tokens < 1 || g->tokens >= (int64_t(1) << 31) || !sizes_ok(g->cache, g->batch, g->heads)) return 0;
-  const PromptPlan p = plan_for(g);
+  const PromptPlan p = plan_prompt(g);
   return p.pieces == 1 ? 0 : static_cast<size_t>(g->tokens) * g->heads * p.pieces * (prompt_padded(g->cache.head_dim) + 4) * sizeof(float);
 }
 
@@ -44,7 +40,7 @@ extern "C" int geo_paged_attention(const geo_paged_prompt_t* g, void* out, void*
   const int size = g->dtype == GEO_F32 ? 4 : 2;
   GEO_REQUIRE(g->q && reinterpret_cast<uintptr_t>(g->q) % 16 == 0 && g->q_token * size % 16 == 0 && g->q_head * size % 16 == 0 && out,
               "%s: null q or output, or rows not on multiples of 16 bytes", name);
-  const paged::PromptPlan p = paged::plan_for(g);
+  const paged::PromptPlan p = paged::plan_prompt(g);
   GEO_REQUIRE(grid_fits(p.blocks, paged::kPromptThreads), "%s: too many workgroups", name);
   const size_t need = geo_paged_attention_workspace_bytes(g);
   if (need && (!workspace || workspace_bytes < need))

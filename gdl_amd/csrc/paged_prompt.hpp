@@ -9,6 +9,8 @@
 // weights of eight adjoining tokens.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -84,7 +86,7 @@ struct PromptLds {
 constexpr int prompt_waves(int DP) { return DP == 128 ? 2 : 3; }
 
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces, int per,
+__global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces,
                                                                   const int32_t* __restrict__ table, float* __restrict__ part,
                                                                   T* __restrict__ out) {
   using M = Meet<T, C>;
@@ -109,9 +111,10 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // One XCD works through one key head's sequences, so that their pages stay in its L2.  Pieces differ too much for
-  // that (late ones have only the last queries): they go to the XCDs in short runs.
-  int64_t w = pieces == 1 ? xcd_block() : xcd_block_runs(8);
+  // One XCD works through one key head's sequences, so that their pages stay in its L2; where the heads and pieces
+  // are not as many as to go round, in short runs (a prompt of 16,000 in 2 | 4 pieces of 2 heads: 496, 476 us in
+  // runs, 624, 451 us otherwise).
+  int64_t w = pieces == 1 || pieces * (a.Hq / a.heads) % 8 == 0 ? xcd_block() : xcd_block_runs(8);
   const int64_t tile = tiles - 1 - w % tiles;  // the longest first
   w /= tiles;
   const int piece = static_cast<int>(w % pieces);
@@ -149,7 +152,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   const int p = held(s.tile0 + place);                    // its position; `room`: beyond the table
   const int wave_first = held(s.tile0 + (wave / a.heads) * 32), wave_last = held(s.tile0 + (wave / a.heads) * 32 + 31);
   const int first_query = held(s.tile0 + s.lo), end = held(s.tile0 + s.hi);  // keys that someone here sees end there
-  const int k0 = piece * per, k1 = min(end, k0 + per);
+  const int per = ((end + pieces - 1) / pieces + 63) & ~63, k0 = piece * per, k1 = min(end, k0 + per);
   const int64_t token = s.first + s.tile0 - s.start + place;
   const bool real = place >= s.lo && place < s.hi;
 
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
       row[0] = top;
       row[1] = sum;
     }
-    attn::store_row<float>(row + 4, o, 1.f, DP);
+    if (k0 < k1) attn::store_row<float>(row + 4, o, 1.f, DP);
   }
 }
 
@@ -499,7 +502,7 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join(int D, int64
   auto add = [&](float m, float l, const f32x4& v) {
     const float most = fmaxf(a.top, m), before = a.top == -kInf ? 0.f : exp2_hw(a.top - most), keep = m == -kInf ? 0.f : exp2_hw(m - most);
     a.sum = (a.sum == a.sum ? a.sum * before : a.sum) + (l == l ? l * keep : l);
-    a.y = a.y * before + v * keep;
+    a.y = a.y * before + (m == -kInf && l == 0.f ? f32x4{} : v) * keep;  // a piece without tokens holds no values
     a.top = most;
   };
 #pragma unroll 4
@@ -528,33 +531,44 @@ __global__ __launch_bounds__(kPromptThreads) void paged_prompt_join(int D, int64
 
 inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
-// A key head's query heads that one workgroup takes together, and the pieces of the longest history that the
-// table has room for.  Twice as many while they all run at a time: a workgroup alone on its CU waits most of
-// the time (1.8 us a tile), so there pieces of 256 tokens pay for the join; the more there are the longer they
-// have to be.  In us, whole | cut: 16 queries behind 3000 tokens 85 | 21 (4 heads to a
-// key head of 64, e4m3), 4 packets of 384 behind 20,000 330 | 131, 2 of 1000 behind 1000 (of 128, bfloat16) 58 | 66.
+// A key head's query heads that one workgroup takes together, and the pieces into which it cuts a tile's keys.
 struct PromptPlan {
-  int heads, unit, pieces, per;
+  int heads, unit, pieces;
   int64_t tiles, blocks;
 };
-inline PromptPlan plan_prompt(int64_t T, int64_t B, int Hq, int Hk, int DP, int64_t most) {
+// The pieces are those of the least time by this estimate, in microseconds: a workgroup takes `tile` for 64 keys on a CU
+// that has all it can hold, two thirds of it on others (in float32, where two fill a CU's matrix units, when alone), and
+// 1.3 tiles to begin; full CUs end 0.38 of the longest workgroup apart; a join costs 6.3, 0.06 a piece and the
+// parts' way through memory at 6.6 TB/s.  Over 40 kinds of
+// calls, from prompts of 300 tokens to packets behind 60,000, the choice is within 2% of the best at the median, 11% at
+// most.  In us, whole | 2, 4, 8, 16 pieces: 8 (2) heads of 64 over e4m3, 16 packets of 100 behind 1000 41 | 31, 27, 31, 41,
+// 32 of up to 384 behind 4000 192 | 182, 178, 204, a prompt of 16,000 815 | 496, 451, 507, 667; 16 (4) heads of
+// 128, bfloat16, 2 of up to 2048 behind 8192 334 | 314, 294, 338.
+inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   PromptPlan p;
-  const int group = Hq / Hk;
+  const int Hq = g->heads, group = Hq / g->cache.kv_heads, DP = prompt_padded(g->cache.head_dim), waves = prompt_waves(DP);
+  const int64_t most = g->cache.columns * g->cache.page;
+  const double T = static_cast<double>(g->tokens), B = static_cast<double>(g->batch);
   p.heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   p.unit = p.heads == 4 ? 5 : p.heads == 2 ? 6 : 7;
-  p.tiles = tiles_of(T, B, p.unit);
-  const int64_t columns = static_cast<int64_t>(Hq) / p.heads, busy = ((T >> p.unit) + B) * columns;
+  p.tiles = tiles_of(g->tokens, g->batch, p.unit);
+  const int64_t columns = Hq / p.heads;
+  double tile = g->cache.stored == g->dtype ? 2.25 : g->dtype == GEO_BF16 ? 2.6 : 3.9;
+  if (DP == 128) tile *= 1.25;
+  if (g->dtype == GEO_F32) tile = DP == 32 ? 6.2 : 0.13 * DP;
+  const double rows = (std::floor(T / (1 << p.unit)) + 0.68 * B) * columns;            // tiles of queries that have any
+  const double longest = most / 64.0, all = rows * std::max(longest - T / (128 * B), longest / 2);  // in tiles of keys
+  double least = 0;
   p.pieces = 1;
-  const int64_t at_once = 256 * prompt_waves(DP);
-  for (;;) {
-    const int64_t now = busy * p.pieces;
-    if (2 * now > at_once || most / (2 * p.pieces) < (4 * now <= at_once ? 256 : 8 * now < 3 * at_once ? 512 : 2048)) break;
-    p.pieces *= 2;
+  for (int n = 1; most >= 64 * n; n *= 2) {
+    const double groups = rows * n, len = longest / n + 1.3;
+    double us = len * tile * (groups < 256 * (g->dtype == GEO_F32 ? 1 : waves - 1) ? 0.67 : 1);
+    if (groups > 256 * waves) us = std::max(us, tile * ((all + 1.3 * groups) / (256 * waves) + 0.38 * len));
+    if (n > 1) us += 6.3 + 0.06 * n + n * T * Hq * (DP + 4) * 8 / 6.6e6;
+    if (n > 1 && us >= least) continue;
+    least = us;
+    p.pieces = n;
   }
-  // Long prompts of few sequences end with their last queries' workgroups, which see twice the keys of the
-  // average: halves end sooner.  16 (4) heads of 128, bfloat16, whole | cut: 8000 tokens 419 | 398 us, 16,000 1554 | 1252.
-  if (p.pieces == 1 && 2 * T >= B * most && most >= 6144 && busy < 4 * at_once) p.pieces = 2;
-  p.per = static_cast<int>(align_up(static_cast<size_t>(ceil_div(most, static_cast<int64_t>(p.pieces))), 64));
   p.blocks = p.tiles * columns * p.pieces;
   return p;
 }
@@ -563,7 +577,7 @@ template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
   const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * (a.bias.maxd + 1) * 4 : 0);
   GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(&paged_prompt<T, C, DP>), bytes));
-  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, p.per, a.pool.table, part,
+  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, a.pool.table, part,
                                                                                         static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_prompt");
   if (p.pieces > 1) {

@@ -102,7 +102,7 @@ def test_two_graphs_and_eager_calls_in_turn(dev):
         with torch.cuda.graph(graphs[-1]):
             outs.append(call())
     for turn in range(4):
-        q.copy_(torch.randn(q.shape, generator=gen)), k1.copy_(torch.randn(k1.shape, generator=gen)), at.add_(3)
+        q.copy_(torch.randn(q.shape, generator=gen)), k1.copy_(torch.randn(k1.shape, generator=gen)), at.add_(1)
         for g in graphs:
             g.replay()
         torch.cuda.synchronize()
