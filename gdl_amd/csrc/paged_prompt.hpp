@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
       if (t < a.T && (t < first || t >= end)) nothing(t);
     }
   }
-  const Span s = span_of(a.ptr, a.start, a.B, a.T, tile, unit);
+  const Span s = span_of<kFromFirst>(a.ptr, a.start, a.B, a.T, tile, unit);
   for (int64_t r = lanes32; r < s.before; r += sets32) nothing(s.first + r);
   if (s.lo >= s.hi) return;
 
@@ -330,6 +330,8 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
     const int page_next = at;
     if (t <= wave_last) {
       const bool whole = t + kKeys - 1 <= wave_first;
+      // In float32 the products are what takes the time, and those past the head's size are left out (heads of 8: 193 | 163 us,
+      // of 80 646 | 496, of 128 664 | 674); in 16 bits the branches cost more (of 80 175 | 190 us, of 128 192 | 218).
       f32x16 product[kSub];
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
         const char* const row = kt + key * L::kKRow + half * 8 * static_cast<int>(sizeof(TK));
 #pragma unroll
         for (int c = 0; c < kKc; ++c)
-          product[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], product[u]);
+          if (!M::kFloat || 32 * c < DP || 16 * c < D) product[u] = Type<TK>::mma(*reinterpret_cast<const KLds*>(row + c * 16 * sizeof(TK)), q[c], product[u]);
       }
       if constexpr (!M::kFloat) attn::reads_ahead<kSub * kKc, 4, 1>();
       // number 8 c + j of x[u] is token t + 32 u + 16 c + 8 half + j; single registers, which branches may change
@@ -432,6 +434,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
           const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
 #pragma unroll
           for (int m = 0; m < kMt; ++m) {
+            if (M::kFloat && 64 * m >= DP && 32 * m >= D) continue;
             const VFrag v = *reinterpret_cast<const VLds*>(col + 32 * m * L::kVRow);
 #pragma unroll
             for (int n = 0; n < M::kParts; ++n) o[m] = Type<TV>::mma(v, w[n], o[m]);
@@ -551,12 +554,12 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   const double T = static_cast<double>(g->tokens), B = static_cast<double>(g->batch);
   p.heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   p.unit = p.heads == 4 ? 5 : p.heads == 2 ? 6 : 7;
-  p.tiles = tiles_of(g->tokens, g->batch, p.unit);
+  p.tiles = tiles_of<kFromFirst>(g->tokens, g->batch, p.unit);
   const int64_t columns = Hq / p.heads;
   double tile = g->cache.stored == g->dtype ? 2.25 : g->dtype == GEO_BF16 ? 2.6 : 3.9;
   if (DP == 128) tile *= 1.25;
   if (g->dtype == GEO_F32) tile = DP == 32 ? 6.2 : 0.13 * DP;
-  const double rows = (std::floor(T / (1 << p.unit)) + 0.68 * B) * columns;            // tiles of queries that have any
+  const double rows = (std::floor(T / (1 << p.unit)) + 0.5 * B) * columns;            // tiles of queries that have any
   const double longest = most / 64.0, all = rows * std::max(longest - T / (128 * B), longest / 2);  // in tiles of keys
   double least = 0;
   p.pieces = 1;
