@@ -148,12 +148,12 @@ struct Pool {
 template <typename C>
 constexpr int block_tokens() { return 64 / static_cast<int>(sizeof(C)); }
 
-// The packed sequences cut into tiles of U = 2^unit positions: at multiples of U (kCuts = 2), or from each sequence's
+// The packed sequences cut into tiles of U positions: at multiples of U (kCuts = 2), or from each sequence's
 // first on (kCuts = 1).  Sequence b has at most n / U + kCuts of them, so its tiles are numbered from
 // ptr[b] / U + kCuts b on; numbers without a tile are idle.
 constexpr int kAtMultiples = 2, kFromFirst = 1;
 template <int kCuts>
-inline int64_t tiles_of(int64_t tokens, int64_t batch, int unit) { return (tokens >> unit) + kCuts * batch; }
+inline int64_t tiles_of(int64_t tokens, int64_t batch, int U) { return tokens / U + kCuts * batch; }
 
 struct Span {
   int64_t first, start;  // row of the sequence's first token, and its position
@@ -167,14 +167,15 @@ __device__ __forceinline__ int64_t start_of(const int64_t* start, int b) {
 }
 // Wave-wide: 64 sequences are looked at together.
 template <int kCuts>
-__device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile, int unit) {
+__device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start, int B, int64_t T, int64_t tile, int U) {
   const int lane = threadIdx.x & 63;
   auto offset = [&](int b) { return ptr ? min(max(ptr[b], int64_t(0)), T) : b ? T : int64_t(0); };
+  auto tile_of = [&](int64_t first, int b) { return static_cast<uint32_t>(first) / static_cast<uint32_t>(U) + kCuts * static_cast<int64_t>(b); };
   int lo = 0, len = B;
   bool some = true;
   do {
     const int step = (len + 63) / 64, at = lo + lane * step;
-    const bool ok = at < lo + len && (offset(at) >> unit) + kCuts * static_cast<int64_t>(at) <= tile;
+    const bool ok = at < lo + len && tile_of(offset(at), at) <= tile;
     const int n = __popcll(__ballot(ok));
     some = some && n > 0;
     const int next = lo + max(n - 1, 0) * step;
@@ -184,12 +185,12 @@ __device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start
   const int b = __builtin_amdgcn_readfirstlane(lo);
   Span s{offset(b), start_of(start, b), 0, b, 0, 0, 0};
   const int64_t n = offset(b + 1) - s.first, from = max(s.start, int64_t(0)), end = s.start + n;
-  const int64_t turn = tile - ((s.first >> unit) + kCuts * static_cast<int64_t>(b));
-  s.tile0 = (kCuts == kAtMultiples ? from >> unit << unit : from) + (turn << unit);
+  const int64_t turn = tile - tile_of(s.first, b);
+  s.tile0 = (kCuts == kAtMultiples ? from / U * U : from) + turn * U;
   if (some && turn == 0 && s.start < 0 && n > 0) s.before = s.start < -n ? n : -s.start;
   if (!some || n <= 0 || s.tile0 >= end) return s;
   s.lo = static_cast<int>(max(from - s.tile0, int64_t(0)));
-  s.hi = static_cast<int>(min(end - s.tile0, int64_t(1) << unit));
+  s.hi = static_cast<int>(min(end - s.tile0, static_cast<int64_t>(U)));
   return s;
 }
 

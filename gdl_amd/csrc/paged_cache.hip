@@ -8,7 +8,7 @@
 namespace geo {
 namespace paged {
 
-constexpr int kUnit = 6, kTile = 1 << kUnit, kThreads = 256;
+constexpr int kTile = 64, kThreads = 256;
 
 // Eight values of a row of type T in float32.
 template <typename T>
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void paged_write(const Pool p, const T* _
   constexpr int kRow = lds_row<C, LW>(), kGroups = kThreads / LW, kBlk = block_tokens<C>(), kPer = 16 / sizeof(C);
   __shared__ __attribute__((aligned(16))) C turned[kTile * kRow];
   const int h = static_cast<int>(blockIdx.x % p.Hk);
-  const Span s = span_of<kAtMultiples>(ptr, start, B, T_all, blockIdx.x / p.Hk, kUnit);
+  const Span s = span_of<kAtMultiples>(ptr, start, B, T_all, blockIdx.x / p.Hk, kTile);
   if (s.lo >= s.hi) return;
   const int page = page_of(p, s.b, s.tile0 / p.page), off = static_cast<int>(s.tile0 % p.page);
   if (page < 0) return;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void paged_read(const Pool p, T* __restri
       if (t < T_all && (t < first || t >= end)) fill(t, 0.f);
     }
   }
-  const Span s = span_of<kAtMultiples>(ptr, start, B, T_all, tile, kUnit);
+  const Span s = span_of<kAtMultiples>(ptr, start, B, T_all, tile, kTile);
   const int64_t t0 = s.first + s.tile0 - s.start;
   for (int64_t r = g; r < s.before; r += kGroups) fill(s.first + r, __builtin_nanf(""));
   if (s.lo >= s.hi) return;
@@ -214,7 +214,7 @@ struct Move {  // arguments of either direction
 };
 template <typename T, typename C, int LW>
 int launch_move(const Pool& p, const Move& m, hipStream_t stream) {
-  const int64_t blocks = tiles_of<kAtMultiples>(m.T, m.B, kUnit) * p.Hk;
+  const int64_t blocks = tiles_of<kAtMultiples>(m.T, m.B, kTile) * p.Hk;
   GEO_REQUIRE(grid_fits(blocks, kThreads), "paged cache: too many workgroups");
   const dim3 grid(static_cast<uint32_t>(blocks));
   if (m.write)

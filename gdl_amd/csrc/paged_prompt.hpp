@@ -3,8 +3,9 @@
 //
 // Sᵀ = K Qᵀ and Oᵀ = Vᵀ Pᵀ on 32x32x16 products, a query to a lane (and its twin in the other half), as in the
 // window's attention.  Four waves of 32 queries share tiles of keys and values in LDS, which are filled
-// through registers one tile ahead: 8-bit codes are decoded once there, for four waves.  Query heads that
-// share a key head go to one workgroup where they can.  Values come in columns (one dimension's tokens
+// through registers one tile ahead: 8-bit codes are decoded once there, for four waves.  A workgroup's queries are
+// `heads` heads of one key head by up to 128 / heads tokens, token by token, so that the keys' way through memory and LDS is
+// shared and calls of few tokens fill their rows.  Values come in columns (one dimension's tokens
 // adjoin), as the second product takes them; the rows of Sᵀ are read in the order that leaves each lane the
 // weights of eight adjoining tokens.
 #pragma once
@@ -31,7 +32,8 @@ struct Prompt {
   const int64_t *ptr, *start;
   attn::Bias bias;
   int64_t T;
-  int B, Hq, heads;  // heads: of a key head's that a workgroup takes (1, 2 or 4), with 128 / heads tokens each
+  int B, Hq, heads, U;  // heads of a key head that a workgroup takes together, and how many tokens of each
+  int bias_row;          // floats of a head's biases in LDS
   float scale;
 };
 
@@ -86,7 +88,7 @@ struct PromptLds {
 constexpr int prompt_waves(int DP) { return DP == 128 ? 2 : 3; }
 
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int unit, int64_t tiles, int pieces,
+__global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int64_t tiles, int pieces,
                                                                   const int32_t* __restrict__ table, float* __restrict__ part,
                                                                   T* __restrict__ out) {
   using M = Meet<T, C>;
@@ -119,38 +121,37 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   w /= tiles;
   const int piece = static_cast<int>(w % pieces);
   w /= pieces;
-  const int set = static_cast<int>(w % sets), hk = static_cast<int>(w / sets);
-  const int head = hk * group + set * a.heads + wave % a.heads;
+  const int set = static_cast<int>(w % sets), hk = static_cast<int>(w / sets), head0 = hk * group + set * a.heads;
   const int64_t rows = a.T * a.Hq;  // of a piece's partial results
 
-  // rows that see nothing: outside all sequences, or at negative positions
+  // tokens that see nothing: outside all sequences, or at negative positions
   auto nothing = [&](int64_t t) {
+    const int64_t first = t * a.Hq + head0;
     if (pieces == 1) {
-      T* const row = out + (t * a.Hq + head) * D;
-      for (int d = lane & 31; d < D; d += 32) row[d] = static_cast<T>(0.f);
-    } else if ((lane & 31) == 0) {
-      float* const row = part + (piece * rows + t * a.Hq + head) * (DP + 4);
+      for (int x = threadIdx.x; x < a.heads * D; x += kPromptThreads) out[first * D + x] = static_cast<T>(0.f);
+    } else if (static_cast<int>(threadIdx.x) < a.heads) {
+      float* const row = part + (piece * rows + first + threadIdx.x) * (DP + 4);
       row[0] = -kInf;
       row[1] = -1.f;
     }
   };
-  const int lanes32 = (wave / a.heads) * 2 + half, sets32 = 8 / a.heads;  // half waves of this head
   if (a.ptr) {
-    const int64_t first = a.ptr[0], end = a.ptr[a.B];
-    for (int r = lanes32; r < 1 << unit; r += sets32) {
-      const int64_t t = (tile << unit) + r;
-      if (t < a.T && (t < first || t >= end)) nothing(t);
-    }
+    const int64_t first = a.ptr[0], end = a.ptr[a.B], from = tile * a.U, to = min(from + a.U, a.T);
+    for (int64_t t = from; t < min(first, to); ++t) nothing(t);
+    for (int64_t t = max(from, max(first, end)); t < to; ++t) nothing(t);
   }
-  const Span s = span_of<kFromFirst>(a.ptr, a.start, a.B, a.T, tile, unit);
-  for (int64_t r = lanes32; r < s.before; r += sets32) nothing(s.first + r);
+  const Span s = span_of<kFromFirst>(a.ptr, a.start, a.B, a.T, tile, a.U);
+  for (int64_t t = 0; t < s.before; ++t) nothing(s.first + t);
   if (s.lo >= s.hi) return;
 
   const int room = pool.columns * pool.page;  // tokens that the table has a place for
   auto held = [&](int64_t p) { return static_cast<int>(min(p, static_cast<int64_t>(room))); };
-  const int place = (wave / a.heads) * 32 + (lane & 31);  // the lane's query in the tile
+  const int row = 32 * wave + (lane & 31), place = row / a.heads;  // the lane's query in the workgroup, its token in the tile
+  const int head = head0 + row - place * a.heads;
   const int p = held(s.tile0 + place);                    // its position; `room`: beyond the table
-  const int wave_first = held(s.tile0 + (wave / a.heads) * 32), wave_last = held(s.tile0 + (wave / a.heads) * 32 + 31);
+  // the first and last positions of the wave's; of a wave without any, none
+  const int first_place = 32 * wave / a.heads, last_place = min((32 * wave + 31) / a.heads, s.hi - 1);
+  const int wave_first = held(s.tile0 + first_place), wave_last = first_place < s.hi ? held(s.tile0 + last_place) : -1;
   const int first_query = held(s.tile0 + s.lo), end = held(s.tile0 + s.hi);  // keys that someone here sees end there
   const int per = ((end + pieces - 1) / pieces + 63) & ~63, k0 = piece * per, k1 = min(end, k0 + per);
   const int64_t token = s.first + s.tile0 - s.start + place;
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   KFrag q[kKc];
   {
     const int64_t t = s.first + s.tile0 - s.start + min(max(place, s.lo), s.hi - 1);
-    const T* const row = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
+    const T* const from = static_cast<const T*>(a.q) + t * a.q_st + head * a.q_sh;
 #pragma unroll
     for (int c = 0; c < kKc; ++c) {
       const int d = 16 * c + 8 * half;
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
         const uint32_t flip = a.scale < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
         for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) {
-          x.u[n] = reinterpret_cast<const Words*>(row + d)[n];
+          x.u[n] = reinterpret_cast<const Words*>(from + d)[n];
           x.u[n] ^= flip;
         }
       }
@@ -178,11 +179,11 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   // positive, so that the products' largest is the scores': the queries carry its sign, or are zeros
   const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   float far = 0.f;
-  const float* const near = sbias + (wave % a.heads) * (a.bias.maxd + 1);
+  const float* const near = sbias + (head - head0) * a.bias_row;
   if (a.bias.table) {
     for (int x = threadIdx.x; x < a.heads * (a.bias.maxd + 1); x += kPromptThreads) {
       const int h = x / (a.bias.maxd + 1), back = x % (a.bias.maxd + 1);
-      sbias[x] = attn::bias_value(a.bias, static_cast<int64_t>(a.bias.lut[a.bias.maxd - back]) * a.Hq + hk * group + set * a.heads + h);
+      sbias[h * a.bias_row + back] = attn::bias_value(a.bias, static_cast<int64_t>(a.bias.lut[a.bias.maxd - back]) * a.Hq + head0 + h);
     }
   }
   if (threadIdx.x < 6) wild[threadIdx.x >> 1][threadIdx.x & 1] = 0;
@@ -479,12 +480,12 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   if (pieces == 1) {
     attn::store_row<T>(out + (token * a.Hq + head) * D, o, 1.f / sum, D);  // weights of nothing but -inf: 0 times infinity
   } else {
-    float* const row = part + (piece * rows + token * a.Hq + head) * (DP + 4);
+    float* const to = part + (piece * rows + token * a.Hq + head) * (DP + 4);
     if (half == 0) {
-      row[0] = top;
-      row[1] = sum;
+      to[0] = top;
+      to[1] = sum;
     }
-    if (k0 < k1) attn::store_row<float>(row + 4, o, 1.f, DP);
+    if (k0 < k1) attn::store_row<float>(to + 4, o, 1.f, DP);
   }
 }
 
@@ -536,7 +537,7 @@ inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // A key head's query heads that one workgroup takes together, and the pieces into which it cuts a tile's keys.
 struct PromptPlan {
-  int heads, unit, pieces;
+  int heads, U, bias_row, pieces;
   int64_t tiles, blocks;
 };
 // The pieces are those of the least time by this estimate, in microseconds: a workgroup takes `tile` for 64 keys on a CU
@@ -552,14 +553,22 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   const int Hq = g->heads, group = Hq / g->cache.kv_heads, DP = prompt_padded(g->cache.head_dim), waves = prompt_waves(DP);
   const int64_t most = g->cache.columns * g->cache.page;
   const double T = static_cast<double>(g->tokens), B = static_cast<double>(g->batch);
-  p.heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
-  p.unit = p.heads == 4 ? 5 : p.heads == 2 ? 6 : 7;
-  p.tiles = tiles_of<kFromFirst>(g->tokens, g->batch, p.unit);
+  // All heads of the key head, or the most that divide them and leave at most 13 of 128 rows empty, with biases of up to 10 KB
+  const int places = std::min(std::max(g->max_distance, 0), 1024) + 1;
+  p.heads = p.bias_row = 1;
+  for (int h = std::min(group, 128); h >= 1; --h) {
+    // a wave's heads begin in other banks
+    p.bias_row = g->bias ? places + (32 - places % 32 + (32 + h - 1) / h) % 32 : 0;
+    p.heads = h;
+    if (group % h == 0 && 128 / h * h >= 115 && (h <= 4 || h * p.bias_row <= 2560)) break;
+  }
+  p.U = 128 / p.heads;
+  p.tiles = tiles_of<kFromFirst>(g->tokens, g->batch, p.U);
   const int64_t columns = Hq / p.heads;
   double tile = g->cache.stored == g->dtype ? 2.25 : g->dtype == GEO_BF16 ? 2.6 : 3.9;
   if (DP == 128) tile *= 1.25;
   if (g->dtype == GEO_F32) tile = DP == 32 ? 6.2 : 0.13 * DP;
-  const double rows = (std::floor(T / (1 << p.unit)) + 0.5 * B) * columns;            // tiles of queries that have any
+  const double rows = (std::floor(T / p.U) + 0.5 * B) * columns;            // tiles of queries that have any
   const double longest = most / 64.0, all = rows * std::max(longest - T / (128 * B), longest / 2);  // in tiles of keys
   double least = 0;
   p.pieces = 1;
@@ -578,9 +587,9 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
 
 template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
-  const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * (a.bias.maxd + 1) * 4 : 0);
+  const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * a.bias_row * 4 : 0);
   GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(&paged_prompt<T, C, DP>), bytes));
-  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.unit, p.tiles, p.pieces, a.pool.table, part,
+  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.tiles, p.pieces, a.pool.table, part,
                                                                                         static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_prompt");
   if (p.pieces > 1) {
