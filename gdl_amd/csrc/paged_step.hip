@@ -367,6 +367,9 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
     next = entry(column);
     page_here();
   }
+  // the new token's place; `room`: beyond the table
+  const int pi = static_cast<int>(min(p, static_cast<int64_t>(room))), new_column = pi / pool.page, place = pi - new_column * pool.page;
+  int page = begins && p >= 0 && new_column < pool.columns ? entry(new_column) : -1;
 
   // this lane's places in a block: row 4 g' + i of tile n is token g' kOwn + 4 n + i
   uint32_t kat[kLoads];
@@ -526,8 +529,7 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
     for (int n = 0; n < DP / 16; ++n) s = fmaf(static_cast<float>(qraw.x[n]), nk.value[n], s);
     s = group_sum<16>(s) * scale2;
     if (a.bias.table) s += sbias[bucket[0] * kCols + cell];
-    const int pi = static_cast<int>(min(p, static_cast<int64_t>(room)));  // `room`: beyond the table
-    const int column = pi / pool.page, place = pi - column * pool.page, page = page_of(pool, b, column);
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(pool.pages)) page = -1;
     if (col == 0) {
       sm[kWaves][cell] = s;
       sl[kWaves][cell] = page < 0 ? __builtin_nanf("") : 1.f;
