@@ -31,6 +31,13 @@ template <> struct Code<I8> {
   }
   static __device__ __forceinline__ uint8_t bits(float y) { return static_cast<uint8_t>(static_cast<int>(y)); }
   static __device__ __forceinline__ float value(uint8_t b) { return static_cast<float>(static_cast<int8_t>(b)); }
+  // Four codes of such products: that sum's low byte is the code.
+  static __device__ __forceinline__ uint32_t four(const float* x, float rate) {
+    uint32_t y[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) y[n] = __float_as_uint(fmaf(x[n], rate, 12582912.f));
+    return __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u) | __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
+  }
 };
 template <> struct Code<E4> {
   static constexpr bool kNarrow = true;
@@ -38,13 +45,17 @@ template <> struct Code<E4> {
   // The same with steps of an eighth of the product's power of two, at least 2^-9.
   static __device__ __forceinline__ float round(float x, float rate) {
     const uint32_t power = max(__float_as_uint(x * rate) & 0x7f800000u, 0x3c800000u);
-    const float big = __uint_as_float((power + (20u << 23)) | 0x400000u);
+    const float big = __uint_as_float(power + ((20u << 23) | 0x400000u));
     return fmaf(x, rate, big) - big;
   }
   static __device__ __forceinline__ uint8_t bits(float y) {
     return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false));
   }
   static __device__ __forceinline__ float value(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8(b, 0); }
+  static __device__ __forceinline__ uint32_t four(const float* x, float rate) {
+    const uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(round(x[0], rate), round(x[1], rate), 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(round(x[2], rate), round(x[3], rate), lo, true);
+  }
 };
 
 using attn::bf16x8;

@@ -22,6 +22,23 @@ struct Eight {
 #pragma unroll
     for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) reinterpret_cast<uint4*>(p)[n] = u[n];
   }
+  // Bits of the largest magnitude in float32, NaN above all; 16-bit types in pairs.
+  __device__ __forceinline__ uint32_t most() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t y = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y = max(y, __float_as_uint(t[e]) & 0x7fffffffu);
+      return y;
+    } else {
+      using Pair = uint16_t __attribute__((ext_vector_type(2)));
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+      Pair y = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y = __builtin_elementwise_max(y, __builtin_bit_cast(Pair, w[e] & 0x7fff7fffu));
+      const uint16_t z = max(y.x, y.y);
+      return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, z))) & 0x7fffffffu;
+    }
+  }
 };
 template <typename T, typename C>
 struct Kept {  // eight values as the pool holds them
@@ -31,13 +48,14 @@ struct Kept {  // eight values as the pool holds them
   template <int LW>
   __device__ __forceinline__ void from(const Eight<T>& x) {
     if constexpr (Code<C>::kNarrow) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(static_cast<float>(x.t[e])) & 0x7fffffffu);
-      const RowScale s = row_scale<C>(group_most<LW>(most));
+      const RowScale s = row_scale<C>(group_most<LW>(x.most()));
       scale = s.scale;
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e].bits = Code<C>::bits(encode<C>(static_cast<float>(x.t[e]), s.rate));
+      for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(x.t[e]);
+      const uint32_t keep = s.rate > 0.f ? ~0u : 0u;
+      n.x = Code<C>::four(y, s.rate) & keep;
+      n.y = Code<C>::four(y + 4, s.rate) & keep;
     } else {
 #pragma unroll
       for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) w[n] = x.u[n];
