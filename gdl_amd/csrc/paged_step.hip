@@ -14,6 +14,7 @@
 // 252 us and 5 for the join, 5.6 TB/s; 128 in int8 with a bias 277 + 5 us, 5.2 TB/s (vector instructions in 46% of the cycles,
 // for codes to bfloat16, scales and weights); one of 131,072 tokens 16 + 7 us.  The least call takes 8 us.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -696,18 +697,20 @@ __global__ __launch_bounds__(1024) void paged_join_many(int D, int cells, const 
 
 inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64 ? 64 : 128; }
 
-// Workgroups, the least share (in tiles) and the workspace of a call: whole rows where no stream can hold
-// more than `kWhole` tiles, else as many shares as run at a time.
+// Workgroups, the least share (in tiles) and the workspace of a call: whole rows where no stream can hold many
+// tiles, more where there are more rows to fill the card; else as many shares as run at a time.  In us, shares | whole
+// rows: 4 rows of 1000 tokens (float32, heads of 32) 12.4 | 15.2, 16 (int8, of 64) 19.3 | 15.4, 1024 (bfloat16, of 128) 88 | 82;
+// 32 rows of 2000 (bfloat16) 18 | 27, 128 (int8) 24.6 | 21.7, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 32.
 struct StepPlan {
   int groups, least;
   size_t bytes;
 };
-constexpr int kWhole = 32, kLeast = 4;
+constexpr int kLeast = 4;
 inline StepPlan plan_step(const geo_paged_step_t* g, int waves) {
   const int group = g->heads / g->cache.kv_heads, cells = group < kCols ? group : kCols;
   const int64_t most = ceil_div(g->cache.columns * g->cache.page, static_cast<int64_t>(kTile));
-  if (most <= kWhole) return {0, 0, 0};
   const int64_t rows = g->batch * g->cache.kv_heads * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
+  if (most <= 64 && most <= 12 + 2 * std::sqrt(static_cast<double>(rows))) return {0, 0, 0};
   int64_t groups = 256 * waves;
   if (most < (int64_t(1) << 30) / rows) groups = std::min(groups, ceil_div(most * rows, static_cast<int64_t>(kLeast)));
   const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
