@@ -108,14 +108,14 @@ __device__ __forceinline__ f16x8 decode8_f16(uint32_t lo, uint32_t hi) {
 // Eight float32 values as the sum of PARTS bf16 operands: 8, 16 or all 24 bits of them.  Codes are exact in
 // bf16, so products of 8-bit pools keep what the queries' type holds: one part for bfloat16, two for
 // float16, three for float32.
-template <int PARTS>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&y)[PARTS]) {
+template <int PARTS, typename F>
+__device__ __forceinline__ void split8(const float (&x)[8], F (&y)[PARTS]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float r = x[e];
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) {
-      y[n][e] = static_cast<__bf16>(r);
+      y[n][e] = static_cast<std::remove_reference_t<decltype(y[n][0])>>(r);
       if (n + 1 < PARTS) r -= static_cast<float>(y[n][e]);
     }
   }

@@ -51,14 +51,14 @@ using Words = uint32_t __attribute__((ext_vector_type(4)));
 
 // How a pool of C meets queries of T: key tiles of type K, value tiles of type V.  Codes stay codes where a
 // 16-bit type holds them (float16 weights times a scale could leave its range, so those meet bf16 values in two
-// parts) and are multiplied out for float32.
-template <typename T, typename C>
+// parts) and are multiplied out for float32.  FINE: weights in two parts in any case.
+template <typename T, typename C, bool FINE = false>
 struct Meet {
   static constexpr bool kNarrow = Code<C>::kNarrow, kFloat = sizeof(T) == 4;
   static constexpr bool kScaled = kNarrow && !kFloat;  // scales meet scores and weights, not the tiles
   using K = T;
   using V = typename std::conditional<kScaled, __bf16, T>::type;
-  static constexpr int kParts = kScaled ? parts_of<T>() : 1;
+  static constexpr int kParts = kFloat ? 1 : FINE ? 2 : kScaled ? parts_of<T>() : 1;
   static constexpr int kKeys = kFloat ? 32 : 64;
 };
 
@@ -96,11 +96,11 @@ struct PromptLds {
 // Workgroups of the kernel on a CU, by the registers that it takes.
 constexpr int prompt_waves(int DP) { return DP == 128 ? 2 : 3; }
 
-template <typename T, typename C, int DP>
+template <typename T, typename C, int DP, bool FINE>
 __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prompt(const Prompt a, int64_t tiles, int pieces,
                                                                   const int32_t* __restrict__ table, float* __restrict__ part,
                                                                   T* __restrict__ out) {
-  using M = Meet<T, C>;
+  using M = Meet<T, C, FINE>;
   using L = PromptLds<T, C, DP>;
   using TK = typename M::K;
   using TV = typename M::V;
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           VFrag w[M::kParts];
-          if constexpr (M::kScaled) {
+          if constexpr (!M::kFloat) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
@@ -547,6 +547,7 @@ inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // A key head's query heads that one workgroup takes together, and the pieces into which it cuts a tile's keys.
 struct PromptPlan {
   int heads, U, bias_row, pieces;
+  bool fine;
   int64_t tiles, blocks;
 };
 // The pieces are those of the least time by this estimate, in microseconds: a workgroup takes `tile` for 64 keys on a CU
@@ -579,6 +580,10 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   if (g->dtype == GEO_F32) tile = DP == 32 ? 6.2 : 0.13 * DP;
   const double rows = (std::floor(T / p.U) + 0.5 * B) * columns;            // tiles of queries that have any
   const double longest = most / 64.0, all = rows * std::max(longest - T / (128 * B), longest / 2);  // in tiles of keys
+  // Weights rounded to the queries' type add an error as large as the output's own rounding: together 1.41 times it on the
+  // average of many rows and keys, more in a short call's few.  Two parts cost 20-27% of the products' time, which there is a
+  // small part (500 tokens, 8 (2) heads of 64: 15.1 | 15.4 us; 2000 31.5 | 36.0).
+  p.fine = all <= 1024;
   double least = 0;
   p.pieces = 1;
   for (int n = 1; most >= 64 * n; n *= 2) {
@@ -597,8 +602,10 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
 template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
   const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * a.bias_row * 4 : 0);
-  GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(&paged_prompt<T, C, DP>), bytes));
-  paged_prompt<T, C, DP><<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.tiles, p.pieces, a.pool.table, part,
+  constexpr bool kCanBeFine = sizeof(T) == 2 && Meet<T, C>::kParts == 1;
+  auto* const kernel = kCanBeFine && p.fine ? &paged_prompt<T, C, DP, kCanBeFine> : &paged_prompt<T, C, DP, false>;
+  GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(kernel), bytes));
+  kernel<<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.tiles, p.pieces, a.pool.table, part,
                                                                                         static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_prompt");
   if (p.pieces > 1) {

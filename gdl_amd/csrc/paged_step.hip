@@ -116,33 +116,39 @@ struct NarrowQuery {  // 8-bit pools
   }
 };
 
-// The weights of a group's tokens as the second product's operand.
+// The weights of a group's tokens as the second product's operand, 16-bit ones in two parts: rounded once they would add
+// an error as large as the output's own rounding, and the reading of the values leaves the time for it.
 template <typename T, typename C>
 struct Weights {
-  union { bf16x8 b; f16x8 h; float f[4]; } x;
-  __device__ __forceinline__ void from(const float* p) {
+  static constexpr int kParts = sizeof(T) == 4 ? 1 : 2;
+  using F = typename std::conditional<__is_same(T, __bf16), bf16x8, f16x8>::type;
+  float f[4];
+  F x[kParts];
+  __device__ __forceinline__ void from(const float (&p)[16 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) {
-      if constexpr (sizeof(T) == 4) x.f[e] = p[e];
-      else if constexpr (__is_same(T, __bf16)) x.b[e] = static_cast<__bf16>(p[e]);
-      else x.h[e] = static_cast<_Float16>(p[e]);
+      for (int e = 0; e < 4; ++e) f[e] = p[e];
+    } else {
+      split8<kParts>(p, x);
     }
   }
   __device__ __forceinline__ f32x4 times(const Bytes16& v, f32x4 o) const {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o = mma(v.f[e], x.f[e], o);
-    } else if constexpr (__is_same(T, __bf16)) {
-      o = mma(v.b, x.b, o);
+      for (int e = 0; e < 4; ++e) o = mma(v.f[e], f[e], o);
     } else {
-      o = mma(v.h, x.h, o);
+#pragma unroll
+      for (int n = 0; n < kParts; ++n) {
+        if constexpr (__is_same(T, __bf16)) o = mma(v.b, x[n], o);
+        else o = mma(v.h, x[n], o);
+      }
     }
     return o;
   }
 };
 template <typename T, typename C>
 struct NarrowWeights {
-  static constexpr int kParts = parts_of<T>();
+  static constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
   bf16x8 x[2][kParts];
   __device__ __forceinline__ void from(const float* p) {
 #pragma unroll
