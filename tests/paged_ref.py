@@ -88,11 +88,13 @@ def same(cache, want):
         assert not wrong.any(), (name, int(wrong.sum()), wrong.nonzero()[:5].tolist())
 
 
-def attend(q, K, V, first, pool_dtype, scale=None, table=None, maxd=128):
-    """(out, bound) [m, H, D] of queries q [m, H, D] at positions first .. over K, V float64 [n, Hk, D]."""
+def attend(q, K, V, first, pool_dtype, scale=None, table=None, maxd=128, unit=None):
+    """(out, bound) [m, H, D] of queries q [m, H, D] at positions first .. over K, V float64 [n, Hk, D].  unit: of the
+    weights' rounding, where it is another than above."""
     dtype, (m, H, D), (n, Hk, _) = q.dtype, q.shape, K.shape
     e, u_out, z = 2.0 ** -24, UNIT[q.dtype], SPACING[q.dtype] / 2
     u = u_out if pool_dtype not in MOST else {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16, torch.float32: e}[dtype]
+    u = u if unit is None else unit
     scale = 1 / math.sqrt(D) if scale is None else scale
     q = q.detach().cpu().double().transpose(0, 1)
     K, V = (x.transpose(0, 1).repeat_interleave(H // Hk, 0) for x in (K, V))
