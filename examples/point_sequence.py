@@ -4,7 +4,8 @@
 
 Clouds are sampled to equal coverage, brought into Morton order and run through two blocks of gated
 recurrence and window attention; the causal blocks then answer the same cloud token by token from
-their caches, which gives the same rows.
+their caches, which gives the same rows.  Blocks without a window, which see the whole past, answer clouds
+as a scanner delivers them: packets of unequal numbers of points, then single ones, over pages in 8 bits.
 """
 
 import argparse
@@ -55,6 +56,35 @@ class Classifier(nn.Module):
         return self.head(segment_reduce(x, *csr, ptr.numel() - 1, reduce="mean")), x
 
 
+def packets(dev, channels=64, streams=8, most=400):
+    """Two blocks without a window: rows of whole clouds against those of packets and single points over int8 pages."""
+    blocks = nn.ModuleList(PointSequenceBlock(channels, 4, None, kv_heads=2) for _ in range(2)).to(dev)
+    embed = nn.Linear(3, channels).to(dev)
+    pos, ptr, _ = clouds(streams, most, dev)
+    pos = pos[serial_order(pos, ptr)]
+    with torch.no_grad():
+        rows = x = embed(pos)
+        for block in blocks:
+            rows = block(rows, ptr)
+        got, caches = torch.full_like(rows, torch.nan), [block.new_cache(streams, torch.int8, tokens=most) for block in blocks]
+        sizes = (ptr[1:] - ptr[:-1]).cpu()
+        done = torch.zeros(streams, dtype=torch.int64)
+        while (sizes - done > 1).any():  # each stream's next packet, to one point before its end
+            new = torch.minimum(torch.randint(1, 90, (streams,)), sizes - done - 1)
+            at = torch.cat([torch.arange(int(n)) + int(first + d) for n, first, d in zip(new, ptr, done)]).to(dev)
+            y, offsets = x[at], torch.cat([new.new_zeros(1), new.cumsum(0)]).to(dev)
+            for block, cache in zip(blocks, caches):
+                y = block.extend(y, offsets, done.to(dev), cache)
+            got[at] = y
+            done += new
+        last = ptr[1:] - 1
+        y = x[last]
+        for block, cache in zip(blocks, caches):
+            y = block.step(y, (sizes - 1).to(dev), cache)
+        got[last] = y
+    return ((got - rows).norm() / rows.norm()).item()
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--steps", type=int, default=60)
@@ -87,6 +117,7 @@ def main():
                 x = block.step(x, torch.full((32,), t, device=dev), cache)
             worst = max(worst, (x - rows[ptr[:-1] + t]).abs().max().item())
     print(f"token by token: rows within {worst:.1e} of the forward's")
+    print(f"in packets over an 8-bit history: rows {packets(dev):.1e} from the forward's (2-norm)")
 
 
 if __name__ == "__main__":
