@@ -705,8 +705,9 @@ inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64
 
 // Workgroups, the least share (in tiles) and the workspace of a call: whole rows where no stream can hold many
 // tiles, more where there are more rows to fill the card; else as many shares as run at a time.  In us, shares | whole
-// rows: 4 rows of 1000 tokens (float32, heads of 32) 12.4 | 15.2, 16 (int8, of 64) 19.3 | 15.4, 1024 (bfloat16, of 128) 88 | 82;
-// 32 rows of 2000 (bfloat16) 18 | 27, 128 (int8) 24.6 | 21.7, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 32.
+// rows: 4 rows of 1000 tokens (float32, heads of 32) 12.4 | 15.2, but 20 | 16 with the host's time, of which the join's launch
+// and the workspace take 4; 16 (int8, of 64) 19.3 | 15.4, 1024 (bfloat16, of 128) 88 | 82; of 2000 tokens 4 (float32) 13 | 24,
+// 32 (bfloat16) 18 | 27, 128 (int8) 24.6 | 21.7, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 32.
 struct StepPlan {
   int groups, least;
   size_t bytes;
@@ -716,7 +717,7 @@ inline StepPlan plan_step(const geo_paged_step_t* g, int waves) {
   const int group = g->heads / g->cache.kv_heads, cells = group < kCols ? group : kCols;
   const int64_t most = ceil_div(g->cache.columns * g->cache.page, static_cast<int64_t>(kTile));
   const int64_t rows = g->batch * g->cache.kv_heads * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
-  if (most <= 64 && most <= 12 + 2 * std::sqrt(static_cast<double>(rows))) return {0, 0, 0};
+  if (most <= 24 || (most <= 64 && most <= 12 + 2 * std::sqrt(static_cast<double>(rows)))) return {0, 0, 0};
   int64_t groups = 256 * waves;
   if (most < (int64_t(1) << 30) / rows) groups = std::min(groups, ceil_div(most * rows, static_cast<int64_t>(kLeast)));
   const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
