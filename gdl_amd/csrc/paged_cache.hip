@@ -10,6 +10,8 @@
 // 16 streams read from int8 in 52 us (5.2 TB/s).  Small heads and packets are bound by the way to the rows (offsets, page,
 // rows, LDS, rows: 4 us for the least call) and e4m3 codes by vector instructions (64% of the cycles; codes in
 // fours 11.9 us, one by one 14.6, for 32 packets of up to 384 tokens, 8 heads of 64).
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace geo {
@@ -17,31 +19,46 @@ namespace paged {
 
 constexpr int kTile = 64, kThreads = 256;
 
-// Eight values of a row of type T in float32.
+// Eight values of a row of type T, as words: unions and arrays of elements would go through memory.
+using Words = uint32_t __attribute__((ext_vector_type(4)));
 template <typename T>
 struct Eight {
-  union { uint4 u[sizeof(T) / 2]; T t[8]; };
+  static constexpr int kWords = sizeof(T) / 2;
+  Words u[kWords];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) u[n] = reinterpret_cast<const uint4*>(p)[n];
+    for (int n = 0; n < kWords; ++n) u[n] = reinterpret_cast<const Words*>(p)[n];
   }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-    for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) reinterpret_cast<uint4*>(p)[n] = u[n];
+    for (int n = 0; n < kWords; ++n) reinterpret_cast<Words*>(p)[n] = u[n];
+  }
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[e / 4][e % 4]);
+    else return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(u[0][e / 2] >> (16 * (e % 2)))));
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e / 4][e % 4] = __float_as_uint(x[e]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        u[0][n] = __builtin_bit_cast(uint16_t, static_cast<T>(x[2 * n])) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<T>(x[2 * n + 1]))) << 16;
+    }
   }
   // Bits of the largest magnitude in float32, NaN above all; 16-bit types in pairs.
   __device__ __forceinline__ uint32_t most() const {
     if constexpr (sizeof(T) == 4) {
       uint32_t y = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y = max(y, __float_as_uint(t[e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; ++e) y = max(y, u[e / 4][e % 4] & 0x7fffffffu);
       return y;
     } else {
       using Pair = uint16_t __attribute__((ext_vector_type(2)));
-      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
       Pair y = {0, 0};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y = __builtin_elementwise_max(y, __builtin_bit_cast(Pair, w[e] & 0x7fff7fffu));
+      for (int e = 0; e < 4; ++e) y = __builtin_elementwise_max(y, __builtin_bit_cast(Pair, u[0][e] & 0x7fff7fffu));
       const uint16_t z = max(y.x, y.y);
       return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, z))) & 0x7fffffffu;
     }
@@ -49,51 +66,72 @@ struct Eight {
 };
 template <typename T, typename C>
 struct Kept {  // eight values as the pool holds them
-  union { uint4 w[sizeof(C) * 8 > 16 ? 2 : 1]; uint2 n; C c[8]; };
+  static constexpr bool kNarrow = Code<C>::kNarrow;
+  Eight<T> same;    // pools of the tokens' type
+  uint32_t n[2];    // codes
   float scale;
   // from the row's values, by the LW lanes that share the row
   template <int LW>
   __device__ __forceinline__ void from(const Eight<T>& x) {
-    if constexpr (Code<C>::kNarrow) {
+    if constexpr (kNarrow) {
       const RowScale s = row_scale<C>(group_most<LW>(x.most()));
       scale = s.scale;
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(x.t[e]);
+      for (int e = 0; e < 8; ++e) y[e] = x.at(e);
       const uint32_t keep = s.rate > 0.f ? ~0u : 0u;
-      n.x = Code<C>::four(y, s.rate) & keep;
-      n.y = Code<C>::four(y + 4, s.rate) & keep;
+      n[0] = Code<C>::four(y, s.rate) & keep;
+      n[1] = Code<C>::four(y + 4, s.rate) & keep;
     } else {
-#pragma unroll
-      for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) w[n] = x.u[n];
+      same = x;
     }
   }
   __device__ __forceinline__ void to(Eight<T>& x) const {
-    if constexpr (Code<C>::kNarrow) {
+    if constexpr (kNarrow) {
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x.t[e] = static_cast<T>(Code<C>::value(c[e].bits) * scale);
+      for (int e = 0; e < 8; ++e) y[e] = Code<C>::value(static_cast<uint8_t>(n[e / 4] >> (8 * (e % 4)))) * scale;
+      x.set(y);
     } else {
-#pragma unroll
-      for (int n = 0; n < static_cast<int>(sizeof(T) / 2); ++n) x.u[n] = w[n];
+      x = same;
     }
   }
   __device__ __forceinline__ void load(const C* p) {
-    if constexpr (sizeof(C) == 1) {
-      n = *reinterpret_cast<const uint2*>(p);
+    if constexpr (kNarrow) {
+      const uint2 y = *reinterpret_cast<const uint2*>(p);
+      n[0] = y.x;
+      n[1] = y.y;
     } else {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(C) / 2); ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+      same.load(reinterpret_cast<const T*>(p));
     }
   }
   __device__ __forceinline__ void store(C* p) const {
-    if constexpr (sizeof(C) == 1) {
-      *reinterpret_cast<uint2*>(p) = n;
-    } else {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(C) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
-    }
+    if constexpr (kNarrow) *reinterpret_cast<uint2*>(p) = uint2{n[0], n[1]};
+    else same.store(reinterpret_cast<T*>(p));
   }
 };
+
+// Sixteen bytes of adjoining values of C, from and to places STRIDE apart.
+template <typename C, int STRIDE>
+__device__ __forceinline__ Words gather(const C* p) {
+  Words y = {};
+#pragma unroll
+  for (int n = 0; n < static_cast<int>(16 / sizeof(C)); ++n) {
+    constexpr int kBits = 8 * sizeof(C);
+    using U = typename std::conditional<sizeof(C) == 4, uint32_t, typename std::conditional<sizeof(C) == 2, uint16_t, uint8_t>::type>::type;
+    y[n * kBits / 32] |= static_cast<uint32_t>(reinterpret_cast<const U*>(p)[n * STRIDE]) << (n * kBits % 32);
+  }
+  return y;
+}
+template <typename C, int STRIDE>
+__device__ __forceinline__ void scatter(C* p, const Words& y) {
+#pragma unroll
+  for (int n = 0; n < static_cast<int>(16 / sizeof(C)); ++n) {
+    constexpr int kBits = 8 * sizeof(C);
+    using U = typename std::conditional<sizeof(C) == 4, uint32_t, typename std::conditional<sizeof(C) == 2, uint16_t, uint8_t>::type>::type;
+    reinterpret_cast<U*>(p)[n * STRIDE] = static_cast<U>(y[n * kBits / 32] >> (n * kBits % 32));
+  }
+}
 
 // LDS rows of a tile's values: 16 bytes (8 of 8-bit types) more than the row, so that rows begin in other banks.
 template <typename C, int LW>
@@ -146,11 +184,8 @@ __global__ __launch_bounds__(kThreads) void paged_write(const Pool p, const T* _
   for (int x = threadIdx.x; x < pieces; x += kThreads) {
     const int row = x / (kBlk / kPer), e = row % p.D, r0 = row / p.D * kBlk + x % (kBlk / kPer) * kPer;
     if (r0 >= s.hi || r0 + kPer <= s.lo) continue;
-    union { uint4 u; C c[kPer]; } y;
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) y.c[n] = turned[(r0 + n) * kRow + e];
     if (r0 >= s.lo && r0 + kPer <= s.hi) {
-      reinterpret_cast<uint4*>(vp)[x] = y.u;
+      reinterpret_cast<Words*>(vp)[x] = gather<C, kRow>(turned + r0 * kRow + e);
     } else {
       for (int n = max(s.lo - r0, 0); n < min(s.hi - r0, kPer); ++n) vp[x * kPer + n] = turned[(r0 + n) * kRow + e];
     }
@@ -168,8 +203,7 @@ __global__ __launch_bounds__(kThreads) void paged_read(const Pool p, T* __restri
   const int lane = threadIdx.x % LW, g = threadIdx.x / LW, d = 8 * lane;
   auto fill = [&](int64_t t, float x) {
     Eight<T> y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y.t[e] = static_cast<T>(x);
+    y.set({x, x, x, x, x, x, x, x});
     if (d < p.D) {
       y.store(k + (t * p.Hk + h) * p.D + d);
       y.store(v + (t * p.Hk + h) * p.D + d);
@@ -208,10 +242,7 @@ __global__ __launch_bounds__(kThreads) void paged_read(const Pool p, T* __restri
   for (int x = threadIdx.x; x < pieces; x += kThreads) {
     const int row = x / (kBlk / kPer), e = row % p.D, r0 = row / p.D * kBlk + x % (kBlk / kPer) * kPer;
     if (r0 >= s.hi || r0 + kPer <= s.lo) continue;
-    union { uint4 u; C c[kPer]; } y;
-    y.u = reinterpret_cast<const uint4*>(vp)[x];
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) turned[(r0 + n) * kRow + e] = y.c[n];
+    scatter<C, kRow>(turned + r0 * kRow + e, reinterpret_cast<const Words*>(vp)[x]);
   }
   __syncthreads();
 #pragma unroll
