@@ -563,14 +563,15 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   const int Hq = g->heads, group = Hq / g->cache.kv_heads, DP = prompt_padded(g->cache.head_dim), waves = prompt_waves(DP);
   const int64_t most = g->cache.columns * g->cache.page;
   const double T = static_cast<double>(g->tokens), B = static_cast<double>(g->batch);
-  // All heads of the key head, or the most that divide them and leave at most 13 of 128 rows empty, with biases of up to 10 KB
+  // All heads of the key head, or the most that divide them and leave at most 13 of 128 rows empty, with biases that let two
+  // workgroups of the largest head size share a CU's LDS
   const int places = std::min(std::max(g->max_distance, 0), 1024) + 1;
   p.heads = p.bias_row = 1;
   for (int h = std::min(group, 128); h >= 1; --h) {
     // a wave's heads begin in other banks
     p.bias_row = g->bias ? places + (32 - places % 32 + (32 + h - 1) / h) % 32 : 0;
     p.heads = h;
-    if (group % h == 0 && 128 / h * h >= 115 && (h <= 4 || h * p.bias_row <= 2560)) break;
+    if (group % h == 0 && 128 / h * h >= 115 && h * p.bias_row <= 2240) break;
   }
   p.U = 128 / p.heads;
   p.tiles = tiles_of<kFromFirst>(g->tokens, g->batch, p.U);
@@ -586,7 +587,7 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   p.fine = all <= 1024;
   double least = 0;
   p.pieces = 1;
-  for (int n = 1; most >= 64 * n; n *= 2) {
+  for (int n = 1; n == 1 || (most >= 64 * n && rows * n <= 12 * 256 * waves); n *= 2) {  // tables may be far wider than streams are long
     const double groups = rows * n, len = longest / n + 1.3;
     double us = len * tile * (groups < 256 * (g->dtype == GEO_F32 ? 1 : waves - 1) ? 0.67 : 1);
     if (groups > 256 * waves) us = std::max(us, tile * ((all + 1.3 * groups) / (256 * waves) + 0.38 * len));
