@@ -656,17 +656,32 @@ def window_cache_fill_hip(k, v, k_cache, v_cache, sinks, ptr, start):
 
 
 def _paged_args(k, v, k_scale, v_scale, table):
-    """geo_paged_t of a pool (packed), and the table that it points into."""
-    if table.stride(1) != 1 and table.shape[1] > 1:
+    """geo_paged_t of a pool (packed), and the table that it points into.  Attributes of tensors cost a fifth of a
+    microsecond each, so these calls ask once."""
+    stream, step = table.stride()
+    columns = table.shape[1]
+    if step != 1 and columns > 1:
         table = table.contiguous()
+        stream = columns
     at = _nat.at
     pages, heads, page, d = k.shape
-    return _nat.pack_paged(k.data_ptr(), v.data_ptr(), at(k_scale), at(v_scale), table.data_ptr(), table.stride(0), pages,
-                           table.shape[1], _nat.PAGED_DTYPES[k.dtype], heads, d, page), table
+    return _nat.pack_paged(k.data_ptr(), v.data_ptr(), at(k_scale), at(v_scale), table.data_ptr(), stream, pages, columns,
+                           _nat.PAGED_DTYPES[k.dtype], heads, d, page), table
 
 
-def _paged_spans(dev, ptr, start):
-    return None if ptr is None else _i64(ptr, dev), None if start is None else _i64(start, dev)
+def _paged_rows(t: Tensor, d: int, size: int):
+    """(t, address, strides of tokens and heads) of [T, H, d] whose rows are contiguous, begin on multiples of 16
+    bytes and do not overlap: t itself where that holds."""
+    (st, sh, sd), at = t.stride(), t.data_ptr()
+    if sd != 1 or (at | st * size | sh * size) % 16 or not d <= st < 1 << 22:
+        t = t.clone(memory_format=torch.contiguous_format)
+        (st, sh, _), at = t.stride(), t.data_ptr()
+    return t, at, st, sh
+
+
+def _paged_int64(t: Optional[Tensor]):
+    """t, on the device already, as the kernels read it."""
+    return t if t is None or (t.dtype is torch.int64 and t.is_contiguous()) else t.to(torch.int64).contiguous()
 
 
 def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start):
@@ -674,34 +689,40 @@ def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
     name = "PagedCache.write"
     dev = _sequence_device(name, k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
     code = _sequence_code(name, k, v)
-    k, v = _in_pieces(k), _in_pieces(v)
-    ptr, start = _paged_spans(dev, ptr, start)
+    tokens, _, d = k.shape
+    size = k.element_size()
+    k, k_at, k_token, k_head = _paged_rows(k, d, size)
+    v, v_at, v_token, v_head = _paged_rows(v, d, size)
+    ptr, start = _paged_int64(ptr), _paged_int64(start)
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
+    at = _nat.at
     with _nat.on_device(dev):
-        _nat.check(_nat.lib().geo_paged_write(
-            cache, code, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _nat.ptr(ptr),
-            _nat.ptr(start), k.shape[0], table.shape[0], _nat.stream_of(dev)), "geo_paged_write")
+        _nat.check(_nat.lib().geo_paged_write(cache, code, k_at, v_at, k_token, k_head, v_token, v_head, at(ptr), at(start), tokens,
+                                              len(table), _nat.stream_of(dev)), "geo_paged_write")
 
 
 def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens, dtype):
     """(k, v) [tokens, Hk, D]: the values of packed sequences' tokens out of the pages."""
     dev = _sequence_device("PagedCache.read", k_pages, v_pages, k_scale, v_scale, table, ptr, start)
-    ptr, start = _paged_spans(dev, ptr, start)
+    ptr, start = _paged_int64(ptr), _paged_int64(start)
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
-    k, v = (torch.empty(tokens, k_pages.shape[1], k_pages.shape[3], dtype=dtype, device=dev) for _ in range(2))
+    _, heads, _, d = k_pages.shape
+    k = torch.empty(tokens, heads, d, dtype=dtype, device=dev)
+    v = _like(k)
+    at = _nat.at
     with _nat.on_device(dev):
-        _nat.check(_nat.lib().geo_paged_read(
-            cache, _nat.SEQUENCE_DTYPES[dtype], _nat.ptr(ptr), _nat.ptr(start), tokens, table.shape[0], k.data_ptr(),
-            v.data_ptr(), _nat.stream_of(dev)), "geo_paged_read")
+        _nat.check(_nat.lib().geo_paged_read(cache, _nat.SEQUENCE_DTYPES[dtype], at(ptr), at(start), tokens, len(table), k.data_ptr(),
+                                             v.data_ptr(), _nat.stream_of(dev)), "geo_paged_read")
     return k, v
 
 
 def _paged_bias(name, bias, plan):
-    """(bias, lut, type code, max_distance, buckets) as the packed structures take them."""
+    """(bias, address, lut's, type code, max_distance, buckets) as the packed structures take them."""
     if bias is None:
-        return None, None, 0, 0, 0
+        return None, 0, 0, 0, 0, 0
     lut, _, maxd = plan
-    return bias.contiguous(), lut, _sequence_code(f"{name} bias", bias), maxd, bias.shape[0]
+    bias = bias.contiguous()
+    return bias, bias.data_ptr(), lut.data_ptr(), _sequence_code(f"{name} bias", bias), maxd, len(bias)
 
 
 def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, scale, bias, plan):
@@ -709,15 +730,16 @@ def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table,
     name = "paged_attention_step"
     dev = _sequence_device(name, q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, bias)
     code = _sequence_code(name, q, k, v)
-    q, k, v = _in_pieces(q), _in_pieces(k), _in_pieces(v)
-    positions = _i64(positions, dev)
-    B, H, _ = q.shape
+    B, H, d = q.shape
+    size = q.element_size()
+    q, q_at, qs, qh = _paged_rows(q, d, size)
+    k, k_at, ks, kh = _paged_rows(k, d, size)
+    v, v_at, vs, vh = _paged_rows(v, d, size)
+    positions = _paged_int64(positions)
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
-    bias, lut, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
-    (qs, qh, _), (ks, kh, _), (vs, vh, _) = q.stride(), k.stride(), v.stride()
-    at = _nat.at
-    args = _nat.pack_paged_step(cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, qh, ks, kh, vs, vh, positions.data_ptr(),
-                                at(bias), at(lut), B, code, bias_code, H, buckets, maxd, scale)
+    bias, bias_at, lut_at, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
+    args = _nat.pack_paged_step(cache, q_at, k_at, v_at, qs, qh, ks, kh, vs, vh, positions.data_ptr(), bias_at, lut_at, B, code,
+                                bias_code, H, buckets, maxd, scale)
     out = _like(q)
     L = _nat.lib()
     with _nat.on_device(dev):
@@ -734,15 +756,14 @@ def paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start
     name = "paged_attention"
     dev = _sequence_device(name, q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias)
     code = _sequence_code(name, q)
-    q = _in_pieces(q)
-    ptr, start = _paged_spans(dev, ptr, start)
-    T, H, _ = q.shape
+    T, H, d = q.shape
+    q, q_at, qs, qh = _paged_rows(q, d, q.element_size())
+    ptr, start = _paged_int64(ptr), _paged_int64(start)
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
-    bias, lut, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
-    qs, qh, _ = q.stride()
+    bias, bias_at, lut_at, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
     at = _nat.at
-    args = _nat.pack_paged_prompt(cache, q.data_ptr(), qs, qh, at(ptr), at(start), at(bias), at(lut), T, table.shape[0], code,
-                                  bias_code, H, buckets, maxd, scale)
+    args = _nat.pack_paged_prompt(cache, q_at, qs, qh, at(ptr), at(start), bias_at, lut_at, T, len(table), code, bias_code, H, buckets,
+                                  maxd, scale)
     out = _like(q)
     L = _nat.lib()
     with _nat.on_device(dev):

@@ -86,8 +86,9 @@ def _(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias, max_distan
 def _check_table(name: str, table: Tensor, batch: int) -> None:
     if table.dtype is not torch.int32:
         raise TypeError(f"{name}: table must be int32, got {table.dtype}")
-    if table.dim() != 2 or table.shape[0] != batch or table.shape[1] < 1:
-        raise ValueError(f"{name}: table [{batch}, pages of a stream], got {tuple(table.shape)}")
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != batch or shape[1] < 1:
+        raise ValueError(f"{name}: table [{batch}, pages of a stream], got {tuple(shape)}")
 
 
 def _check_spans(name: str, table: Tensor, ptr: Optional[Tensor], start: Optional[Tensor]) -> None:
@@ -100,8 +101,10 @@ def _check_spans(name: str, table: Tensor, ptr: Optional[Tensor], start: Optiona
 
 
 def _no_grad(name: str, *tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward: call it under torch.no_grad()")
 
 
 class PagedCache:
@@ -166,8 +169,9 @@ class PagedCache:
         return cls(k, v, *scales)
 
     def _token_dtype(self, name: str, dtype: torch.dtype) -> None:
-        if dtype not in _nat.SEQUENCE_DTYPES or (self.k.dtype not in _NARROW and dtype is not self.k.dtype):
-            wanted = "float32, bfloat16 or float16" if self.k.dtype in _NARROW else f"{self.k.dtype} as the pool"
+        stored = self.k.dtype
+        if dtype not in _nat.SEQUENCE_DTYPES or (dtype is not stored and stored not in _NARROW):
+            wanted = "float32, bfloat16 or float16" if stored in _NARROW else f"{stored} as the pool"
             raise TypeError(f"{name}: tokens of {wanted}, got {dtype}")
 
     def write(self, k: Tensor, v: Tensor, table: Tensor, ptr: Optional[Tensor] = None, start: Optional[Tensor] = None) -> None:
@@ -181,7 +185,8 @@ class PagedCache:
             start: int64 [B], position of each sequence's first token in its stream; None: 0.  Tokens at
                 negative positions are left out.
         """
-        if k.dim() != 3 or v.shape != k.shape or k.shape[1:] != (self.kv_heads, self.head_dim):
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or shape[1:] != (self.kv_heads, self.head_dim):
             raise ValueError(f"PagedCache.write: k and v [T, {self.kv_heads}, {self.head_dim}], got {tuple(k.shape)}, "
                              f"{tuple(v.shape)}")
         _check_spans("PagedCache.write", table, ptr, start)
@@ -213,12 +218,15 @@ class PagedCache:
         return torch.ops.geoembodied.paged_read(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start, tokens, dtype)
 
 
-def _check_queries(name: str, q: Tensor, cache: PagedCache, bias: Optional[Tensor]) -> None:
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"{name}: q [N, H, {cache.head_dim}], H a multiple of {cache.kv_heads}, got {tuple(q.shape)}")
+def _check_queries(name: str, q: Tensor, cache: PagedCache, bias: Optional[Tensor]) -> int:
+    """The number of queries."""
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or shape[1] < 1 or shape[1] % cache.kv_heads:
+        raise ValueError(f"{name}: q [N, H, {cache.head_dim}], H a multiple of {cache.kv_heads}, got {tuple(shape)}")
     cache._token_dtype(name, q.dtype)
-    if bias is not None and (bias.dim() != 2 or bias.shape[1] != q.shape[1]):
-        raise ValueError(f"{name}: bias must be [buckets, {q.shape[1]}], got {tuple(bias.shape)}")
+    if bias is not None and (bias.dim() != 2 or bias.shape[1] != shape[1]):
+        raise ValueError(f"{name}: bias must be [buckets, {shape[1]}], got {tuple(bias.shape)}")
+    return shape[0]
 
 
 def paged_attention(
@@ -285,9 +293,9 @@ def paged_attention_step(
     No two streams may write to one slot.  No gradients.  ``bias`` is one-sided.
     """
     name, (hk, d) = "paged_attention_step", (cache.kv_heads, cache.head_dim)
-    _check_queries(name, q, cache, bias)
-    batch = q.shape[0]
-    if k.shape != (batch, hk, d) or v.shape != k.shape:
+    batch = _check_queries(name, q, cache, bias)
+    rows = batch, hk, d
+    if k.shape != rows or v.shape != rows:
         raise ValueError(f"{name}: k and v [{batch}, {hk}, {d}], got {tuple(k.shape)}, {tuple(v.shape)}")
     _check_table(name, table, batch)
     if positions.shape != (batch,) or positions.dtype.is_floating_point:
