@@ -35,7 +35,7 @@ struct Step {
   float scale;
 };
 
-constexpr int kThreads = 256, kWaves = 4, kCols = 16;
+constexpr int kCols = 16;
 
 // Workgroups of the kernel on a CU, by the registers that it takes.
 constexpr int kMostWaves = 4;
@@ -268,19 +268,20 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
   return x;
 }
 
-// One workgroup: a share.  The part of a row goes to its four waves in quarters.  The new token is no part of
+// One workgroup: a share.  The part of a row goes to its four or eight waves in equal pieces.  The new token is no part of
 // that: who has the row's beginning forms its row as the pool keeps it, writes it, and adds it to the join, so
 // that no read waits for the write.
-template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step(const Step a, const Deal deal, const int32_t* __restrict__ table,
+template <typename T, typename C, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 2)) void paged_step(const Step a, const Deal deal, const int32_t* __restrict__ table,
                                                                         const int64_t* __restrict__ positions, T* __restrict__ out) {
   constexpr bool kNarrow = Code<C>::kNarrow;
+  constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kCells = kCols * 4 / WAVES;  // heads that there is room to join
   constexpr int kSize = sizeof(C), kBlk = block_tokens<C>(), kOwn = kBlk / 4, kTiles = kBlk / 16;
   constexpr int kLoads = DP * kSize / 64, kRows = DP / 16, kLds = DP + 4;
   using Q = typename std::conditional<kNarrow, NarrowQuery<T, C, kLoads>, Query<T, C, kLoads>>::type;
   using W = typename std::conditional<kNarrow, NarrowWeights<T, C>, Weights<T, C>>::type;
-  __shared__ float sm[kWaves + 1][kCols], sl[kWaves + 1][kCols], fresh[DP];
-  __shared__ __attribute__((aligned(16))) float so[kWaves][kCols][kLds];
+  __shared__ float sm[kWaves + 1][kCells], sl[kWaves + 1][kCells], fresh[DP];
+  __shared__ __attribute__((aligned(16))) float so[kWaves][kCells][kLds];
   extern __shared__ float sbias[];  // with a bias: [buckets][kCols], the row's heads; then the bucket of each distance back, a byte each
   const Pool& pool = a.pool;
   const int D = pool.D, group = a.Hq / pool.Hk, chunks = (group + kCols - 1) / kCols, room = pool.columns * pool.page;
@@ -359,8 +360,8 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
   const bool ends = t1 == tiles;
   const int held = static_cast<int>(min(max(p, int64_t(0)), static_cast<int64_t>(room)));  // tokens before the new one
   const int s0 = t0 * kTile, s1 = min(held, t1 * kTile);
-  const int quarter = ((s1 - s0 + kWaves - 1) / kWaves + kBlk - 1) / kBlk * kBlk;
-  const int w0 = s0 + wave * quarter, w1 = min(s1, w0 + quarter);
+  const int piece = ((s1 - s0 + kWaves - 1) / kWaves + kBlk - 1) / kBlk * kBlk;
+  const int w0 = s0 + wave * piece, w1 = min(s1, w0 + piece);
 
   // where the wave reads: a column of the table and a place in its page
   const int32_t* const row = table + b * pool.table_st;
@@ -526,12 +527,14 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
 
   sum += __shfl_xor(sum, 16, 64);
   sum += __shfl_xor(sum, 32, 64);
-  if (g == 0) {
+  if (g == 0 && col < kCells) {
     sm[wave][col] = top;
     sl[wave][col] = bad ? __builtin_nanf("") : sum;
   }
+  if (col < kCells) {
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) *reinterpret_cast<f32x4*>(&so[wave][col][16 * m + 4 * g]) = o[m];
+    for (int m = 0; m < kRows; ++m) *reinterpret_cast<f32x4*>(&so[wave][col][16 * m + 4 * g]) = o[m];
+  }
 
   if (begins && p >= 0) {
     NewRow<T, C, DP> nk, nv;
@@ -541,9 +544,9 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) s = fmaf(static_cast<float>(qraw.x[n]), nk.value[n], s);
     s = group_sum<16>(s) * scale2;
-    if (a.bias.table) s += sbias[bucket[0] * kCols + cell];
+    if (a.bias.table) s += sbias[bucket[0] * kCols + min(cell, kCols - 1)];
     if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(pool.pages)) page = -1;
-    if (col == 0) {
+    if (col == 0 && cell < kCells) {
       sm[kWaves][cell] = s;
       sl[kWaves][cell] = page < 0 ? __builtin_nanf("") : 1.f;
     }
@@ -580,7 +583,9 @@ __global__ __launch_bounds__(kThreads, (step_waves<T, C, DP>())) void paged_step
       ls[n] = is ? sl[n][c] : 0.f;
       ys[n] = n < kWaves ? so[n % kWaves][c][d] : is ? fresh[d] : 0.f;
     }
-    const float m = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), ms[kWaves]);
+    float m = ms[kWaves];
+#pragma unroll
+    for (int n = 0; n < kWaves; ++n) m = fmaxf(m, ms[n]);
     float l = 0.f, y = 0.f;
 #pragma unroll
     for (int n = 0; n <= kWaves; ++n) {
@@ -709,7 +714,7 @@ inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64
 // and the workspace take 4; 16 (int8, of 64) 19.3 | 15.4, 1024 (bfloat16, of 128) 88 | 82; of 2000 tokens 4 (float32) 13 | 24,
 // 32 (bfloat16) 18 | 27, 128 (int8) 24.6 | 21.7, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 32.
 struct StepPlan {
-  int groups, least;
+  int groups, least, waves;
   size_t bytes;
 };
 constexpr int kLeast = 4;
@@ -717,12 +722,15 @@ inline StepPlan plan_step(const geo_paged_step_t* g, int waves) {
   const int group = g->heads / g->cache.kv_heads, cells = group < kCols ? group : kCols;
   const int64_t most = ceil_div(g->cache.columns * g->cache.page, static_cast<int64_t>(kTile));
   const int64_t rows = g->batch * g->cache.kv_heads * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
-  if (most <= 24 || (most <= 64 && most <= 12 + 2 * std::sqrt(static_cast<double>(rows)))) return {0, 0, 0};
+  // whole rows by eight waves where CUs have no more than one and joining heads takes no more LDS (four | eight: 1 stream of 1000
+  // tokens, 4 float32 heads of 32, 15.2 | 13.4 us, 64 of 2000 32 | 24; 16 of 2 int8 heads of 64, 1000 tokens 16.2 | 15.2)
+  const bool eight = group <= 8 && rows <= 256 && most > 4;
+  if (most <= 24 || (most <= 64 && most <= 12 + 2 * std::sqrt(static_cast<double>(rows)))) return {0, 0, eight ? 8 : 4, 0};
   int64_t groups = 256 * waves;
   if (most < (int64_t(1) << 30) / rows) groups = std::min(groups, ceil_div(most * rows, static_cast<int64_t>(kLeast)));
   const bool narrow = g->cache.stored == GEO_I8 || g->cache.stored == GEO_E4M3;
   const size_t row = padded(g->cache.head_dim, narrow) + 4;
-  return {static_cast<int>(groups), kLeast, static_cast<size_t>(std::min(groups, rows)) * sizeof(int4) + static_cast<size_t>(groups) * 2 * cells * row * sizeof(float)};
+  return {static_cast<int>(groups), kLeast, 4, static_cast<size_t>(std::min(groups, rows)) * sizeof(int4) + static_cast<size_t>(groups) * 2 * cells * row * sizeof(float)};
 }
 
 template <typename T, typename C, int DP>
@@ -733,7 +741,7 @@ int launch_step(const Step& a, const geo_paged_step_t* g, void* out, void* works
     return set_error(GEO_ERR_WORKSPACE, "paged attention step: workspace of %zu bytes, %zu needed", workspace ? bytes : size_t(0), s.bytes);
   const int64_t rows = static_cast<int64_t>(a.B) * a.pool.Hk * ceil_div(static_cast<int64_t>(group), static_cast<int64_t>(kCols));
   const int64_t blocks = s.groups ? s.groups : rows;
-  GEO_REQUIRE(grid_fits(blocks, kThreads), "paged attention step: too many workgroups");
+  GEO_REQUIRE(grid_fits(blocks, 64 * s.waves), "paged attention step: too many workgroups");
   Deal deal{s.groups, s.least, rows <= s.groups, nullptr, nullptr};
   const uint32_t places = static_cast<uint32_t>(std::min(rows, static_cast<int64_t>(s.groups)));
   if (s.groups) {
@@ -741,7 +749,8 @@ int launch_step(const Step& a, const geo_paged_step_t* g, void* out, void* works
     deal.parts = reinterpret_cast<float*>(deal.desc + places);
   }
   const size_t lds = a.bias.table ? sizeof(float) * kCols * a.bias.buckets + align_up(a.bias.maxd + 1, 16) : 0;
-  paged_step<T, C, DP><<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), lds, stream>>>(a, deal, a.pool.table, a.pos, static_cast<T*>(out));
+  auto* const kernel = s.waves == 8 ? &paged_step<T, C, DP, 8> : &paged_step<T, C, DP, 4>;
+  kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(64 * s.waves), lds, stream>>>(a, deal, a.pool.table, a.pos, static_cast<T*>(out));
   GEO_LAUNCH_CHECK("paged_step");
   if (s.groups) {
     const int cells = std::min(group, kCols);
