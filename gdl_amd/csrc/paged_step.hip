@@ -11,8 +11,8 @@
 // The work is the reading of the histories.  16 heads of 128 behind a key head of 16-bit values are 16 operations a byte,
 // far under what the matrix units do, and tiles of 16 columns cost the same for one head.  Shares are equal numbers of
 // 64-token tiles for as many workgroups as run at a time (two to four times as many were slower).  Of 6.3 TB/s that a kernel can read here: 64 streams to 16,384 tokens, 16 (4) heads of 128, bfloat16,
-// 252 us and 5 for the join, 5.6 TB/s; 128 in int8 with a bias 277 + 5 us, 5.2 TB/s (vector instructions in 46% of the cycles,
-// for codes to bfloat16, scales and weights); one of 131,072 tokens 16 + 7 us.  The least call takes 8 us.
+// 252 us and 5 for the join, 5.6 TB/s; 128 in int8 with a bias 277 + 5 us, 5.2 TB/s (vector instructions in 50% of the cycles,
+// for codes to bfloat16, scales and weights); one of 131,072 tokens 16 + 7 us.  The least call takes 7-8 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
