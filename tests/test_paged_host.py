@@ -71,7 +71,7 @@ def test_tensors_are_refused():
     with pytest.raises(ValueError):  # not on 16 bytes
         F.PagedCache(whole[1:2049].view(2, 1, 64, 16), v)
     with pytest.raises(ValueError):  # half shared
-        F.PagedCache(whole[:2048].view(2, 1, 64, 16), whole[1024:3072].view(2, 1, 4, 16, 16))
+        F.PagedCache(whole[:2048].view(2, 1, 64, 16), whole[1000:3048].view(2, 1, 4, 16, 16))
     k8, v8 = torch.zeros(2, 1, 64, 16, dtype=I8), torch.zeros(2, 1, 1, 16, 64, dtype=I8)
     F.PagedCache(k8, v8, s, s.clone())
     for bad in ((k8, v8), (k8, v8, s), (k8, v8, s, s), (k8, v8, s.half(), s.half().clone()), (k8, v8, s[:1], s)):
