@@ -280,6 +280,22 @@ def plain_call(x: torch.Tensor, *rest: torch.Tensor | None) -> bool:
     return plain_eager(x)
 
 
+def plain_device(x: torch.Tensor, *rest: torch.Tensor | None) -> torch.device | None:
+    """The GPU of an ordinary eager call's tensors (plain_call); None where the custom op takes the call, or says
+    what is wrong with the devices."""
+    if not plain_eager(x):
+        return None
+    index = x.get_device()
+    if index < 0:
+        return None
+    for t in rest:
+        if t is not None:
+            kind = type(t)
+            if (kind is not _Tensor and kind is not _Parameter) or t.get_device() != index:
+                return None
+    return x.device
+
+
 def no_tangents(name: str, *tensors: torch.Tensor | None) -> None:
     """Raises in forward-mode differentiation of one of the tensors: a custom op would drop its tangent
     without a word."""

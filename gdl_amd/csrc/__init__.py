@@ -684,10 +684,10 @@ def _paged_int64(t: Optional[Tensor]):
     return t if t is None or (t.dtype is torch.int64 and t.is_contiguous()) else t.to(torch.int64).contiguous()
 
 
-def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start):
+def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start, dev=None):
     """Tokens k, v [T, Hk, D] of packed sequences into the pages that ``table`` gives their streams."""
     name = "PagedCache.write"
-    dev = _sequence_device(name, k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
+    dev = dev or _sequence_device(name, k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
     code = _sequence_code(name, k, v)
     tokens, _, d = k.shape
     size = k.element_size()
@@ -701,9 +701,9 @@ def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start)
                                               len(table), _nat.stream_of(dev)), "geo_paged_write")
 
 
-def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens, dtype):
+def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens, dtype, dev=None):
     """(k, v) [tokens, Hk, D]: the values of packed sequences' tokens out of the pages."""
-    dev = _sequence_device("PagedCache.read", k_pages, v_pages, k_scale, v_scale, table, ptr, start)
+    dev = dev or _sequence_device("PagedCache.read", k_pages, v_pages, k_scale, v_scale, table, ptr, start)
     ptr, start = _paged_int64(ptr), _paged_int64(start)
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
     _, heads, _, d = k_pages.shape
@@ -725,10 +725,10 @@ def _paged_bias(name, bias, plan):
     return bias, bias.data_ptr(), lut.data_ptr(), _sequence_code(f"{name} bias", bias), maxd, len(bias)
 
 
-def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, scale, bias, plan):
+def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, scale, bias, plan, dev=None):
     """[B, H, D] of the tokens at ``positions``, whose k and v go into the streams' pages."""
     name = "paged_attention_step"
-    dev = _sequence_device(name, q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, bias)
+    dev = dev or _sequence_device(name, q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, bias)
     code = _sequence_code(name, q, k, v)
     B, H, d = q.shape
     size = q.element_size()
@@ -751,10 +751,10 @@ def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table,
     return out
 
 
-def paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, scale, bias, plan):
+def paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, scale, bias, plan, dev=None):
     """[T, H, D] of packed queries over the pages that ``table`` gives their streams."""
     name = "paged_attention"
-    dev = _sequence_device(name, q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias)
+    dev = dev or _sequence_device(name, q, k_pages, v_pages, k_scale, v_scale, table, ptr, start, bias)
     code = _sequence_code(name, q)
     T, H, d = q.shape
     q, q_at, qs, qh = _paged_rows(q, d, q.element_size())

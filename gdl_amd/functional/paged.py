@@ -192,8 +192,8 @@ class PagedCache:
         _check_spans("PagedCache.write", table, ptr, start)
         self._token_dtype("PagedCache.write", k.dtype)
         _no_grad("PagedCache.write", k, v)
-        if _nat.plain_call(k, v, self.k, self.v, self.k_scale, self.v_scale, table, ptr, start):
-            paged_write_hip(k, v, self.k, self.v, self.k_scale, self.v_scale, table, ptr, start)
+        if dev := _nat.plain_device(k, v, self.k, self.v, self.k_scale, self.v_scale, table, ptr, start):
+            paged_write_hip(k, v, self.k, self.v, self.k_scale, self.v_scale, table, ptr, start, dev)
         else:
             _nat.no_tangents("PagedCache.write", k, v)
             torch.ops.geoembodied.paged_write(k, v, self.k, self.v, self.k_scale, self.v_scale, table, ptr, start)
@@ -213,8 +213,8 @@ class PagedCache:
             dtype = torch.bfloat16 if self.k.dtype in _NARROW else self.k.dtype
         _check_spans("PagedCache.read", table, ptr, start)
         self._token_dtype("PagedCache.read", dtype)
-        if _nat.plain_call(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start):
-            return paged_read_hip(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start, tokens, dtype)
+        if dev := _nat.plain_device(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start):
+            return paged_read_hip(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start, tokens, dtype, dev)
         return torch.ops.geoembodied.paged_read(self.k, self.v, self.k_scale, self.v_scale, table, ptr, start, tokens, dtype)
 
 
@@ -264,8 +264,8 @@ def paged_attention(
     _no_grad(name, q, bias)
     scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
     pools = cache.k, cache.v, cache.k_scale, cache.v_scale
-    if _nat.plain_call(q, *pools, table, ptr, start, bias):
-        return paged_attention_hip(q, *pools, table, ptr, start, scale, bias, _plan(bias, int(max_distance), False))
+    if dev := _nat.plain_device(q, *pools, table, ptr, start, bias):
+        return paged_attention_hip(q, *pools, table, ptr, start, scale, bias, _plan(bias, int(max_distance), False), dev)
     _nat.no_tangents(name, q, bias)
     if bias is not None:
         check_buckets(bias.shape[0], int(max_distance), False)
@@ -303,8 +303,8 @@ def paged_attention_step(
     _no_grad(name, q, k, v, bias)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     pools = cache.k, cache.v, cache.k_scale, cache.v_scale
-    if _nat.plain_call(q, k, v, *pools, table, positions, bias):
-        return paged_attention_step_hip(q, k, v, *pools, table, positions, scale, bias, _plan(bias, int(max_distance), False))
+    if dev := _nat.plain_device(q, k, v, *pools, table, positions, bias):
+        return paged_attention_step_hip(q, k, v, *pools, table, positions, scale, bias, _plan(bias, int(max_distance), False), dev)
     _nat.no_tangents(name, q, k, v, bias)
     if bias is not None:
         check_buckets(bias.shape[0], int(max_distance), False)
