@@ -698,7 +698,7 @@ def paged_write_hip(k, v, k_pages, v_pages, k_scale, v_scale, table, ptr, start,
     at = _nat.at
     with _nat.on_device(dev):
         _nat.check(_nat.lib().geo_paged_write(cache, code, k_at, v_at, k_token, k_head, v_token, v_head, at(ptr), at(start), tokens,
-                                              len(table), _nat.stream_of(dev)), "geo_paged_write")
+                                              table.shape[0], _nat.stream_of(dev)), "geo_paged_write")
 
 
 def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens, dtype, dev=None):
@@ -711,7 +711,7 @@ def paged_read_hip(k_pages, v_pages, k_scale, v_scale, table, ptr, start, tokens
     v = _like(k)
     at = _nat.at
     with _nat.on_device(dev):
-        _nat.check(_nat.lib().geo_paged_read(cache, _nat.SEQUENCE_DTYPES[dtype], at(ptr), at(start), tokens, len(table), k.data_ptr(),
+        _nat.check(_nat.lib().geo_paged_read(cache, _nat.SEQUENCE_DTYPES[dtype], at(ptr), at(start), tokens, table.shape[0], k.data_ptr(),
                                              v.data_ptr(), _nat.stream_of(dev)), "geo_paged_read")
     return k, v
 
@@ -722,7 +722,7 @@ def _paged_bias(name, bias, plan):
         return None, 0, 0, 0, 0, 0
     lut, _, maxd = plan
     bias = bias.contiguous()
-    return bias, bias.data_ptr(), lut.data_ptr(), _sequence_code(f"{name} bias", bias), maxd, len(bias)
+    return bias, bias.data_ptr(), lut.data_ptr(), _sequence_code(f"{name} bias", bias), maxd, bias.shape[0]
 
 
 def paged_attention_step_hip(q, k, v, k_pages, v_pages, k_scale, v_scale, table, positions, scale, bias, plan, dev=None):
@@ -762,7 +762,7 @@ def paged_attention_hip(q, k_pages, v_pages, k_scale, v_scale, table, ptr, start
     cache, _held = _paged_args(k_pages, v_pages, k_scale, v_scale, table)
     bias, bias_at, lut_at, bias_code, maxd, buckets = _paged_bias(name, bias, plan)
     at = _nat.at
-    args = _nat.pack_paged_prompt(cache, q_at, qs, qh, at(ptr), at(start), bias_at, lut_at, T, len(table), code, bias_code, H, buckets,
+    args = _nat.pack_paged_prompt(cache, q_at, qs, qh, at(ptr), at(start), bias_at, lut_at, T, table.shape[0], code, bias_code, H, buckets,
                                   maxd, scale)
     out = _like(q)
     L = _nat.lib()
