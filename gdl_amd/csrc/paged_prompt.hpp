@@ -110,6 +110,8 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   typedef VFrag VLds __attribute__((aligned(16)));
   constexpr int kSize = sizeof(C), kKeys = M::kKeys, kBlk = block_tokens<C>(), kPer = 16 / kSize;
   constexpr int kSub = kKeys / 32, kKc = DP / 16, kMt = DP / 32;
+  constexpr bool kHalf = Faint<TV>::kHalf;
+  constexpr float kLift = Faint<TV>::kLift;
   constexpr int kLoads = (kKeys * DP * kSize + 16 * kPromptThreads - 1) / (16 * kPromptThreads);
   constexpr int kSpan = kKeys < kBlk ? kKeys : kBlk, kCpb = kSpan * kSize / 16;  // tokens and pieces of a dimension in a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   f32x16 o[kMt];
 #pragma unroll
   for (int m = 0; m < kMt; ++m) o[m] = f32x16{};
-  float top = -kInf, sum = 0.f;
+  float top = -kInf, sum = 0.f;  // what scores are taken less by: the largest, less kLift
   bool lost = p >= room;
 
   __syncthreads();  // zeros past the head, biases, notes
@@ -400,8 +402,9 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, x[u][r]);
       most = halves_max(most) * by;
-      const bool up = most > top + kLazy;
+      const bool up = most - top > kLazy + kLift;
       if (__any(up)) {
+        most -= kLift;
         const float keep = up ? exp2_hw(top - most) : 1.f;
         top = up ? most : top;
         sum *= keep;
@@ -427,6 +430,8 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
           }
         }
       }
+      using Half2 = _Float16 __attribute__((ext_vector_type(2)));
+      Half2 least = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -441,6 +446,10 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[0][e] = static_cast<TV>(x[u][8 * c + e]);
           }
+          if constexpr (kHalf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) least = __builtin_elementwise_minimum(least, Half2{w[0][2 * e], w[0][2 * e + 1]});
+          }
           const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
 #pragma unroll
           for (int m = 0; m < kMt; ++m) {
@@ -451,6 +460,35 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
           }
         }
       if constexpr (!M::kFloat && M::kParts == 1) attn::reads_ahead<kSub * 2 * kMt, 4, 1>();
+      if constexpr (kHalf) {
+        constexpr float kBelow = Faint<TV>::kBelow(M::kParts);
+        bool some = static_cast<float>(least.x) < kBelow || static_cast<float>(least.y) < kBelow;
+        if (!whole) {  // weights that the mask made 0 are none
+          some = false;
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) some |= x[u][r] > 0.f && x[u][r] < kBelow;
+        }
+        if (__any(some)) {
+#pragma unroll
+          for (int m = 0; m < kMt; ++m) o[m] *= Faint<TV>::kUp;
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
+              const VFrag w = faint8<M::kParts>(y);
+              const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
+#pragma unroll
+              for (int m = 0; m < kMt; ++m) o[m] = Type<TV>::mma(*reinterpret_cast<const VLds*>(col + 32 * m * L::kVRow), w, o[m]);
+            }
+#pragma unroll
+          for (int m = 0; m < kMt; ++m) o[m] *= Faint<TV>::kDown;
+        }
+      }
       for (int u = 0; u < kSub; ++u) {
         uint32_t rest = wild[turn][u];
         while (rest) {  // rare: the queries that see an infinity or NaN have one in its dimension

@@ -145,6 +145,16 @@ struct Weights {
     }
     return o;
   }
+  // what the parts leave of float16 weights (Faint)
+  static __device__ __forceinline__ bool some_faint(const float (&p)[16 / sizeof(T)]) {
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) some |= p[e] < Faint<T>::kBelow(kParts) && p[e] > 0.f;
+    return some;
+  }
+  static __device__ __forceinline__ f32x4 faint(const Bytes16& v, const f16x8& rest, f32x4 o) {
+    return mma(v.h, rest, o * Faint<T>::kUp) * Faint<T>::kDown;
+  }
 };
 template <typename T, typename C>
 struct NarrowWeights {
@@ -274,7 +284,8 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t x) {
 template <typename T, typename C, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 2)) void paged_step(const Step a, const Deal deal, const int32_t* __restrict__ table,
                                                                         const int64_t* __restrict__ positions, T* __restrict__ out) {
-  constexpr bool kNarrow = Code<C>::kNarrow;
+  constexpr bool kNarrow = Code<C>::kNarrow, kHalf = Faint<C>::kHalf;
+  constexpr float kLift = Faint<C>::kLift;
   constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kCells = kCols * 4 / WAVES;  // heads that there is room to join
   constexpr int kSize = sizeof(C), kBlk = block_tokens<C>(), kOwn = kBlk / 4, kTiles = kBlk / 16;
   constexpr int kLoads = DP * kSize / 64, kRows = DP / 16, kLds = DP + 4;
@@ -430,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
   f32x4 o[kRows];
 #pragma unroll
   for (int m = 0; m < kRows; ++m) o[m] = f32x4{};
-  float top = -kInf, sum = 0.f;
+  float top = -kInf, sum = 0.f;  // what scores are taken less by: the largest, less kLift
   const float scale2 = a.scale * kLog2e;
   const float far = a.bias.table ? bias_at(a.bias, a.Hq, head, a.bias.maxd) : 0.f;
 
@@ -497,9 +508,9 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
     float most = x[0];
 #pragma unroll
     for (int n = 1; n < kOwn; ++n) most = fmaxf(most, x[n]);
-    if (__any(most > top + kLazy)) {
+    if (__any(most - top > kLazy + kLift)) {
       most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(fmaxf(most, __shfl_xor(most, 32, 64)), top);
+      most = fmaxf(fmaxf(most, __shfl_xor(most, 32, 64)) - kLift, top);
       const float keep = top == -kInf ? 0.f : exp2_hw(top - most);
       if (top != -kInf) {
 #pragma unroll
@@ -521,6 +532,13 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
     for (int m = 0; m < kRows; ++m) {
       o[m] = weights.times(vx[m], o[m]);
       if constexpr (kNarrow) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kHalf) {
+      if (__any(W::some_faint(x))) {
+        const f16x8 rest = faint8<W::kParts>(x);
+#pragma unroll
+        for (int m = 0; m < kRows; ++m) o[m] = W::faint(vx[m], rest, o[m]);
+      }
     }
     if (more) load_v(at, off);
   }
