@@ -240,8 +240,8 @@ __device__ __forceinline__ int page_of(const Pool& p, int b, int64_t column) {
   return static_cast<uint32_t>(n) < static_cast<uint32_t>(p.pages) ? n : -1;
 }
 
-// Checks on the host; fills *pool.
-inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool) {
+// Checks on the host; fills *pool.  Without streams there is no table: a tensor without elements has no address.
+inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool, bool streams = true) {
   GEO_REQUIRE(g, "%s: null arguments", name);
   const bool narrow = g->stored == GEO_I8 || g->stored == GEO_E4M3;
   GEO_REQUIRE(narrow || g->stored == GEO_F32 || g->stored == GEO_BF16 || g->stored == GEO_F16, "%s: pool type code %d", name,
@@ -258,7 +258,7 @@ inline int pool_args(const char* name, const geo_paged_t* g, Pool* pool) {
   GEO_REQUIRE(aligned(g->k) && aligned(g->v) && g->k != g->v, "%s: null pool, not on 16 bytes, or one for both", name);
   GEO_REQUIRE(!narrow || (aligned(g->k_scale) && aligned(g->v_scale) && g->k_scale != g->v_scale),
               "%s: an 8-bit pool needs scales, on 16 bytes", name);
-  GEO_REQUIRE(g->table, "%s: null table", name);
+  GEO_REQUIRE(g->table || !streams, "%s: null table", name);
   *pool = Pool{static_cast<char*>(g->k), static_cast<char*>(g->v), g->k_scale, g->v_scale, g->table, g->table_stream,
                static_cast<int>(g->pages), static_cast<int>(g->columns), g->page, g->kv_heads, g->head_dim};
   return GEO_OK;

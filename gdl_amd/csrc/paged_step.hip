@@ -814,7 +814,7 @@ extern "C" int geo_paged_attention_step(const geo_paged_step_t* g, void* out, vo
   const char* const name = "paged attention step";
   GEO_REQUIRE(g, "%s: null arguments", name);
   paged::Step a;
-  if (const int rc = paged::pool_args(name, &g->cache, &a.pool)) return rc;
+  if (const int rc = paged::pool_args(name, &g->cache, &a.pool, g->batch != 0)) return rc;
   GEO_REQUIRE(paged::type_ok(g->dtype, g->cache.stored), "%s: tokens of type code %d, a pool of %d", name,
               static_cast<int>(g->dtype), static_cast<int>(g->cache.stored));
   GEO_REQUIRE(g->batch >= 0 && g->batch < (int64_t(1) << 31) && g->heads >= 1 && g->heads < (1 << 20) &&

@@ -722,7 +722,8 @@ int geo_paged_read(const geo_paged_t* cache, int dtype, const int64_t* ptr, cons
  * the stream's pages, and q attends to the tokens 0 .. positions[b] as the pool holds them, the new
  * one among them.  A negative position leaves the stream alone and gives 0.  NaN where one of these
  * tokens has no page (the new one is written where it has one).  bias by distance as above,
- * max_distance the last one with a place of its own.
+ * max_distance the last one with a place of its own.  No streams: nothing is done, and the table, the
+ * positions and the tokens may be NULL.
  */
 typedef struct {
   geo_paged_t cache;
