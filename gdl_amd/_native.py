@@ -169,6 +169,7 @@ _SIGNATURES = {
     "geo_paged_attention": (c_int, [c_bytes, c_vp, c_vp, c_size, c_vp]),
     "geo_recurrence_carry_size": (c_i64, [c_i64, c_i64]),
     "geo_recurrence_fwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_size, c_vp]),
+    "geo_recurrence_packets": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "geo_recurrence_bwd_workspace_bytes": (c_size, [c_i64, c_i64]),
     "geo_recurrence_bwd": (c_int, [c_bytes, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                    c_size, c_vp]),

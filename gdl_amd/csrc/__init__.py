@@ -851,6 +851,22 @@ def gated_recurrence_step_hip(x, gate_a, gate_x, decay, state, positions, rate):
     return h, new
 
 
+def recurrence_packets_hip(ptr, start, state):
+    """(offsets int64 [2 B], states float32 [2 B - 1, C]) of packets of B streams, as the scan's sequences: those
+    of even numbers are the streams' tokens from position 0 on."""
+    dev = _sequence_device("recurrence packets", ptr, start, state)
+    ptr, start = _paged_int64(ptr), _paged_int64(start)
+    if state.dtype is not torch.float32 or state.stride(1) != 1:
+        state = _nat.f32c(state)
+    B, C = state.shape
+    parts = torch.empty(2 * B, dtype=torch.int64, device=dev)
+    before = torch.empty(2 * B - 1, C, dtype=torch.float32, device=dev)
+    with _nat.on_device(dev):
+        _nat.check(_nat.lib().geo_recurrence_packets(ptr.data_ptr(), start.data_ptr(), state.data_ptr(), state.stride(0), B, C,
+                                                     parts.data_ptr(), before.data_ptr(), _nat.stream_of(dev)), "geo_recurrence_packets")
+    return parts, before
+
+
 def gather_weighted_sum_forward_hip(feat: Tensor, idx: Tensor, w: Tensor) -> Tensor:
     """out[n] = sum_k w[n, k] * feat[idx[n, k]] (idx < 0 or >= N_src contributes nothing)."""
     _require_gpu("gather_weighted_sum", feat, idx, w)
@@ -1225,7 +1241,7 @@ __all__ = [
     "window_attention_forward_hip", "window_attention_backward_hip", "window_attention_step_hip",
     "window_cache_fill_hip", "paged_write_hip", "paged_read_hip", "paged_attention_step_hip",
     "paged_attention_hip", "gated_recurrence_forward_hip", "gated_recurrence_backward_hip",
-    "gated_recurrence_step_hip",
+    "gated_recurrence_step_hip", "recurrence_packets_hip",
     "knn_available", "knn_cuda", "knn_self_cuda",
     "fps_available", "fps_cuda", "fps_uniform_hip",
 ]

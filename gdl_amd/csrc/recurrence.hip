@@ -702,6 +702,23 @@ __global__ __launch_bounds__(256) void scan_step(const Scan s, float* __restrict
   *reinterpret_cast<Raw*>(h + b * s.C + at) = pack<T, V>(H);
 }
 
+// Packets of streams as sequences of a scan: each stream's tokens from position 0 on, and between the streams those at
+// negative positions, whose states nobody takes.  The states ahead of the former are the streams', or 0 for
+// those whose position 0 is in the packet.
+__global__ __launch_bounds__(256) void scan_packets(const int64_t* __restrict__ ptr, const int64_t* __restrict__ start,
+                                                    const float* __restrict__ state, int64_t state_st, int64_t B, int64_t C,
+                                                    int64_t* __restrict__ parts, float* __restrict__ before) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < 2 * B) {
+    const int64_t b = i / 2, begin = ptr[b], end = ptr[b + 1], at = start[b];
+    parts[i] = i % 2 ? end : at >= 0 ? begin : at > begin - end ? begin - at : end;
+  }
+  if (i >= (2 * B - 1) * C) return;
+  const int64_t row = i / C, b = row / 2, at = start[b];
+  const bool goes_on = row % 2 == 0 && (at > 0 || at <= ptr[b] - ptr[b + 1]);
+  before[i] = goes_on ? state[b * state_st + i % C] : 0.f;
+}
+
 // ---------------------------------------------------------------------- host ---
 
 inline int64_t chunks_of(int64_t T) { return ceil_div(T, kChunk); }
@@ -827,6 +844,20 @@ int step(const Scan& s, float* state_out, void* h, hipStream_t stream) {
 }
 }  // namespace rec
 }  // namespace geo
+
+extern "C" int geo_recurrence_packets(const int64_t* ptr, const int64_t* start, const float* state, int64_t state_stream, int64_t streams,
+                                      int64_t channels, int64_t* parts, float* before, void* stream) {
+  using namespace geo;
+  GEO_REQUIRE(streams >= 1 && streams < (int64_t(1) << 30) && channels >= 0 && channels < (int64_t(1) << 31),
+              "gated recurrence packets: %lld streams of %lld channels", static_cast<long long>(streams), static_cast<long long>(channels));
+  GEO_REQUIRE(ptr && start && parts && (channels == 0 || (state && before)), "gated recurrence packets: null tensor");
+  const int64_t rows = 2 * streams - 1, blocks = ceil_div(rows * channels > 2 * streams ? rows * channels : 2 * streams, int64_t(256));
+  GEO_REQUIRE(grid_fits(blocks, 256), "gated recurrence packets: too many workgroups");
+  rec::scan_packets<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, as_stream(stream)>>>(ptr, start, state, state_stream, streams, channels,
+                                                                                             parts, before);
+  GEO_LAUNCH_CHECK("scan_packets");
+  return GEO_OK;
+}
 
 extern "C" int geo_recurrence_step(const geo_recurrence_t* g, float* state_out, void* h, void* stream) {
   geo::rec::Scan s;

@@ -26,6 +26,7 @@ from gdl_amd.csrc import (
     gated_recurrence_backward_hip,
     gated_recurrence_forward_hip,
     gated_recurrence_step_hip,
+    recurrence_packets_hip,
 )
 
 
@@ -92,6 +93,17 @@ def _step_op(x: Tensor, gate_a: Tensor, gate_x: Tensor, decay: Tensor, state: Te
 @_step_op.register_fake
 def _(x, gate_a, gate_x, decay, state, positions, rate):
     return x.new_empty(x.shape), state.new_empty(state.shape)
+
+
+@torch.library.custom_op("geoembodied::recurrence_packets", mutates_args=())
+def _packets_op(ptr: Tensor, start: Tensor, state: Tensor) -> Tuple[Tensor, Tensor]:
+    return recurrence_packets_hip(ptr, start, state)
+
+
+@_packets_op.register_fake
+def _(ptr, start, state):
+    B, C = state.shape
+    return ptr.new_empty(2 * B, dtype=torch.int64), state.new_empty((2 * B - 1, C), dtype=torch.float32)
 
 
 class _GatedRecurrence(torch.autograd.Function):
@@ -170,6 +182,20 @@ def gated_recurrence(
         return _GatedRecurrence.apply(*tensors, bool(reverse), rate)
     h, last, _ = gated_recurrence_forward_hip(x, gate_a, gate_x, decay, ptr, state, bool(reverse), rate, False)
     return h, last
+
+
+def packets_as_sequences(ptr: Tensor, start: Tensor, state: Tensor) -> Tuple[Tensor, Tensor]:
+    """Packets of streams, ``ptr`` [B + 1] from the positions ``start`` [B] on behind the states [B, C], as the
+    ``ptr`` [2 B] and ``state`` of 2 B - 1 sequences of ``gated_recurrence``: number 2 b holds stream b's tokens from
+    position 0 on and begins from 0 where that position is in the packet, those between hold tokens at
+    negative positions.  ``last[::2]`` are then the streams' states, which tokens at negative positions leave as they were."""
+    batch = start.numel()
+    if batch < 1 or start.dim() != 1 or ptr.shape != (batch + 1,) or state.dim() != 2 or len(state) != batch:
+        raise ValueError(f"packets_as_sequences: ptr [B + 1], start [B] and state [B, C] of one stream at least, got {tuple(ptr.shape)}, "
+                         f"{tuple(start.shape)}, {tuple(state.shape)}")
+    if _nat.plain_call(ptr, start, state):
+        return recurrence_packets_hip(ptr, start, state)
+    return torch.ops.geoembodied.recurrence_packets(ptr, start, state)
 
 
 def gated_recurrence_step(

@@ -23,7 +23,7 @@ from torch import Tensor, nn
 
 from gdl_amd.functional.attention import WindowCache, window_attention, window_attention_step
 from gdl_amd.functional.paged import PagedCache, paged_attention, paged_attention_step
-from gdl_amd.functional.recurrence import gated_recurrence, gated_recurrence_step
+from gdl_amd.functional.recurrence import gated_recurrence, gated_recurrence_step, packets_as_sequences
 
 
 def serial_order(pos: Tensor, ptr: Optional[Tensor] = None) -> Tensor:
@@ -155,18 +155,19 @@ class PointSequenceBlock(nn.Module):
     def extend(self, x: Tensor, ptr: Tensor, start: Tensor, cache: BlockCache) -> Tensor:
         """New tokens x [T, channels] of the streams, packed (``ptr`` int64 [B + 1]), from the positions ``start``
         (int64 [B]) on, which ``cache`` then holds; the forward's rows for them.  For a block without a window.
-        A stream whose tokens begin at position 0 begins anew; one without tokens is left alone."""
+        A stream begins anew with its token at position 0; one without tokens from there on is left alone.  Tokens at
+        negative positions are none, as in ``step``: the cache keeps nothing of them, and their rows mean nothing."""
         if cache.table is None:
             raise ValueError("PointSequenceBlock: only a block without a window takes several tokens of a stream")
         if ptr.shape != (cache.state.shape[0] + 1,) or start.shape != (cache.state.shape[0],):
             raise ValueError(f"PointSequenceBlock: ptr and start of {cache.state.shape[0]} streams, got {tuple(ptr.shape)}, "
                              f"{tuple(start.shape)}")
         parts = self.scan_in(self.scan_norm(x)).split(self.channels, 1)
-        anew = (start == 0) & (ptr[1:] > ptr[:-1])
-        h, state = gated_recurrence(*parts, self.decay, ptr=ptr, state=cache.state.masked_fill(anew.unsqueeze(1), 0.0))
+        pieces, before = packets_as_sequences(ptr, start, cache.state)
+        h, state = gated_recurrence(*parts, self.decay, ptr=pieces, state=before)
         x = x + self.scan_out(h)
         q, k, v = self._split(x)
         cache.window.write(k, v, cache.table, ptr, start)
         out = paged_attention(q, cache.window, cache.table, ptr, start, bias=self.bias, max_distance=self.max_distance)
-        cache.state = state
+        cache.state = state[::2]
         return x + self.attend_out(out.flatten(1))

@@ -794,6 +794,12 @@ int geo_recurrence_bwd(const geo_recurrence_t* args, const float* carry, const v
  * state_out written (they may be one tensor).  ptr holds the tokens' positions [streams], or is NULL: the
  * state ahead of position 0 is 0, and a stream at a negative position keeps its state and gives 0. */
 int geo_recurrence_step(const geo_recurrence_t* args, float* state_out, void* h, void* stream);
+/* Packets of `streams` streams, at ptr [streams + 1] and from the positions start [streams] on, as 2 streams - 1
+ * sequences of geo_recurrence_fwd with the offsets parts [2 streams]: number 2 b is stream b's tokens from position 0 on,
+ * those between are tokens at negative positions.  before [2 streams - 1, channels]: the states ahead of them, state
+ * [streams, channels] (rows state_stream apart), or 0 for a stream with its position 0 in the packet. */
+int geo_recurrence_packets(const int64_t* ptr, const int64_t* start, const float* state, int64_t state_stream,
+                           int64_t streams, int64_t channels, int64_t* parts, float* before, void* stream);
 
 #ifdef __cplusplus
 }
