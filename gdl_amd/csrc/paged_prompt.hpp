@@ -387,7 +387,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
             for (int r = 0; r < 16; ++r) x[u][r] = fmaf(x[u][r], by, far);
         }
       }
-      const float by = M::kScaled || a.bias.table ? 1.f : scale2;  // what the scores still lack
+      float by = M::kScaled || a.bias.table ? 1.f : scale2;  // what the scores still lack
       const int seen = p - t - 8 * half;  // a lane's tokens 32 u + 16 c + j up to this one
       if (!whole) {
 #pragma unroll
@@ -412,6 +412,19 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
         for (int m = 0; m < kMt; ++m) o[m] *= keep;
       }
       const float shift = top == -kInf ? 0.f : top;
+      if constexpr (!M::kScaled) {
+        // `top` is a product rounded once; taken from exact ones, far out, it would leave their step's half, and weights of
+        // more than the type holds
+        const bool far_out = fabsf(shift) > 0x1p20f;
+        if (__any(far_out)) {
+          const float rounded = far_out ? by : 1.f;
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[u][r] *= rounded;
+          by = far_out ? 1.f : by;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll

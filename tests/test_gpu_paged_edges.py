@@ -30,3 +30,35 @@ def test_no_streams(dev, dtype, stored):
     assert paged_attention(q, cache, table, ptr).shape == (0, 4, 32)
     assert all(x.shape == (0, 2, 32) for x in cache.read(table, ptr, 0, dtype=dtype))
     ref.same(cache, want)
+
+
+@pytest.mark.parametrize("dtype,stored", [(F32, F32), (BF16, BF16), (F16, F16), (F32, I8), (BF16, I8), (F16, E4)],
+                         ids=["f32", "bf16", "f16", "f32-i8", "bf16-i8", "f16-e4m3"])
+@pytest.mark.parametrize("d", [32, 128])
+@pytest.mark.parametrize("bias", [False, True])
+def test_scores_far_out(dev, dtype, stored, d, bias):
+    """Scores up to 2^37, where float32's steps are far above 1: which keys weigh most is up to the order of its sums (error
+    bound e (d + 8) S), and a row still is a mean of the values that it sees, weights above 0 and a sum of 1."""
+    from attention_ref import SPACING, UNIT
+    from gdl_amd.functional import PagedCache, paged_attention, paged_attention_step
+    gen = torch.Generator().manual_seed(d)
+    n, H, Hk = 300, 4, 2
+    cache = PagedCache.empty(5, Hk, d, dtype=stored, device=dev)
+    table = torch.tensor([[3, 1, 0, 4, 2]], dtype=torch.int32, device=dev)
+    q = (6e4 * (0.1 + 0.9 * torch.rand(n, H, 1, generator=gen))).expand(n, H, d).to(dtype).to(dev)
+    k = (6e4 * (0.1 + 0.9 * torch.rand(1, Hk, 1, generator=gen))).expand(n, Hk, d).to(dtype).to(dev)
+    v = torch.randn(n, Hk, d, generator=gen).to(dtype).to(dev)
+    cache.write(k, v, table)
+    kw = dict(bias=torch.full((8, H), 0.5, dtype=dtype, device=dev), max_distance=20) if bias else {}
+    V = ref.stored(v, stored).repeat_interleave(H // Hk, 1)
+    lo, hi = V.cummin(0).values, V.cummax(0).values
+
+    def check(out, lo, hi):
+        x, size = out.double().cpu(), torch.maximum(lo.abs(), hi.abs())
+        slack = SPACING[dtype] + (2 * UNIT[dtype] + (n + 8) * 2.0 ** -24) * size  # the weights' and the output's rounding
+        assert x.isfinite().all(), int((~x.isfinite()).sum())
+        assert (x >= lo - slack).all() and (x <= hi + slack).all()
+
+    check(paged_attention(q, cache, table, **kw), lo, hi)
+    at = torch.tensor([n - 1], device=dev)
+    check(paged_attention_step(q[-1:], k[-1:], v[-1:], cache, table, at, **kw), lo[-1:], hi[-1:])
