@@ -120,6 +120,19 @@ __device__ __forceinline__ void split8(const float (&x)[8], F (&y)[PARTS]) {
     }
   }
 }
+// The second of their parts alone.
+template <typename F>
+__device__ __forceinline__ F second8(const float (&x)[8]) {
+  F y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    using E = std::remove_reference_t<decltype(y[0])>;
+    float r = x[e];
+    asm volatile("" : "+v"(r));  // as in faint8
+    y[e] = static_cast<E>(r - static_cast<float>(static_cast<E>(r)));
+  }
+  return y;
+}
 template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1; }
 
 constexpr float kLazy = 8.f;  // how far scores (in units of log 2) may exceed the maximum that weights refer to
@@ -134,7 +147,7 @@ template <typename V>
 struct Faint {
   static constexpr bool kHalf = __is_same(V, _Float16);
   static constexpr float kLift = kHalf ? 7.f : 0.f, kUp = 0x1p38f, kDown = 0x1p-38f;
-  static constexpr float kBelow(int parts) { return parts > 1 ? 0x1p-9f : 0x1p-14f; }
+  static __host__ __device__ constexpr float below(int parts) { return parts > 1 ? 0x1p-9f : 0x1p-14f; }
 };
 // What PARTS float16 parts leave of eight weights, of those that are faint, 2^38 larger.
 template <int PARTS>
@@ -144,7 +157,7 @@ __device__ __forceinline__ f16x8 faint8(const float (&x)[8]) {
   for (int e = 0; e < 8; ++e) {
     float r = x[e];
     asm volatile("" : "+v"(r));  // formed again: the parts' remainders kept for this would take the registers
-    const bool small = r < Faint<_Float16>::kBelow(PARTS);
+    const bool small = r < Faint<_Float16>::below(PARTS);
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) r -= static_cast<float>(static_cast<_Float16>(r));
     y[e] = static_cast<_Float16>(small ? r * Faint<_Float16>::kUp : 0.f);
@@ -199,6 +212,7 @@ struct Span {
   int64_t tile0;         // the tile's first position
   int b, lo, hi;         // the sequence; the tile's places that have tokens, lo .. hi - 1 (none: lo >= hi)
   int64_t before;        // on a sequence's first tile: how many of its tokens have negative positions
+  int64_t middle;        // of a tile with tokens: the position halfway through the sequence's
 };
 // A start in a range in which nothing overflows; what lies as far out has no page either way.
 __device__ __forceinline__ int64_t start_of(const int64_t* start, int b) {
@@ -222,12 +236,13 @@ __device__ __forceinline__ Span span_of(const int64_t* ptr, const int64_t* start
     lo = next;
   } while (len > 1);
   const int b = __builtin_amdgcn_readfirstlane(lo);
-  Span s{offset(b), start_of(start, b), 0, b, 0, 0, 0};
+  Span s{offset(b), start_of(start, b), 0, b, 0, 0, 0, 0};
   const int64_t n = offset(b + 1) - s.first, from = max(s.start, int64_t(0)), end = s.start + n;
   const int64_t turn = tile - tile_of(s.first, b);
   s.tile0 = (kCuts == kAtMultiples ? from / U * U : from) + turn * U;
   if (some && turn == 0 && s.start < 0 && n > 0) s.before = s.start < -n ? n : -s.start;
   if (!some || n <= 0 || s.tile0 >= end) return s;
+  s.middle = (from + end) / 2;
   s.lo = static_cast<int>(max(from - s.tile0, int64_t(0)));
   s.hi = static_cast<int>(min(end - s.tile0, static_cast<int64_t>(U)));
   return s;

@@ -47,7 +47,7 @@ extern "C" int geo_paged_attention(const geo_paged_prompt_t* g, void* out, void*
     return set_error(GEO_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace ? workspace_bytes : size_t(0), need);
   a.q = g->q, a.q_st = g->q_token, a.q_sh = g->q_head, a.ptr = g->ptr, a.start = g->start;
   a.bias = {g->bias, g->bias_lut, g->bias_dtype, g->buckets, g->max_distance};
-  a.T = g->tokens, a.B = static_cast<int>(g->batch), a.Hq = g->heads, a.heads = p.heads, a.U = p.U, a.bias_row = p.bias_row, a.scale = g->scale;
+  a.T = g->tokens, a.B = static_cast<int>(g->batch), a.Hq = g->heads, a.heads = p.heads, a.U = p.U, a.bias_row = p.bias_row, a.fine = p.fine, a.scale = g->scale;
   float* const part = static_cast<float*>(workspace);
   const hipStream_t on = as_stream(stream);
   if (g->dtype == GEO_F32) return paged::prompt_of<float>(g->cache.stored, a, p, out, part, on);

@@ -43,6 +43,7 @@ struct Prompt {
   int64_t T;
   int B, Hq, heads, U;  // heads of a key head that a workgroup takes together, and how many tokens of each
   int bias_row;          // floats of a head's biases in LDS
+  int fine;              // sequences whose middle query sees at most so many keys have their weights in two parts
   float scale;
 };
 
@@ -51,14 +52,15 @@ using Words = uint32_t __attribute__((ext_vector_type(4)));
 
 // How a pool of C meets queries of T: key tiles of type K, value tiles of type V.  Codes stay codes where a
 // 16-bit type holds them (float16 weights times a scale could leave its range, so those meet bf16 values in two
-// parts) and are multiplied out for float32.  FINE: weights in two parts in any case.
+// parts) and are multiplied out for float32.  FINE: sequences that plan_prompt says so of have weights in two parts.
 template <typename T, typename C, bool FINE = false>
 struct Meet {
   static constexpr bool kNarrow = Code<C>::kNarrow, kFloat = sizeof(T) == 4;
   static constexpr bool kScaled = kNarrow && !kFloat;  // scales meet scores and weights, not the tiles
   using K = T;
   using V = typename std::conditional<kScaled, __bf16, T>::type;
-  static constexpr int kParts = kFloat ? 1 : FINE ? 2 : kScaled ? parts_of<T>() : 1;
+  static constexpr int kParts = kFloat ? 1 : kScaled ? parts_of<T>() : 1;
+  static constexpr bool kFine = FINE && !kFloat && kParts == 1;
   static constexpr int kKeys = kFloat ? 32 : 64;
 };
 
@@ -167,6 +169,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   const int per = ((end + pieces - 1) / pieces + 63) & ~63, k0 = piece * per, k1 = min(end, k0 + per);
   const int64_t token = s.first + s.tile0 - s.start + place;
   const bool real = place >= s.lo && place < s.hi;
+  const bool fine = M::kFine && __builtin_amdgcn_readfirstlane(s.middle <= a.fine);
 
   KFrag q[kKc];
   {
@@ -239,14 +242,16 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
     for (int n = 0; n < kLoads; ++n) {
       const int x = threadIdx.x + n * kPromptThreads;
       if (x < pieces_of_tile) {
-        kx[n] = *reinterpret_cast<const Words*>(kb + x * 16);
+        kx[n] = *reinterpret_cast<const Words*>(kb + static_cast<uint32_t>(x) * 16);
         vx[n] = *reinterpret_cast<const Words*>(vb + vfrom[n]);
       }
     }
     if constexpr (M::kScaled) {
       if (threadIdx.x < kKeys) {
-        ksx = pool.ks[slot0 + threadIdx.x];
-        vsx = pool.vs[slot0 + threadIdx.x];
+        uint32_t key = threadIdx.x;
+        asm volatile("" : "+v"(key));  // a scalar base and a lane's 32 bits: 64-bit sums of pool and lane would be kept, and spilled
+        ksx = (pool.ks + slot0)[key];
+        vsx = (pool.vs + slot0)[key];
       }
     }
   };
@@ -443,6 +448,24 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
           }
         }
       }
+      auto add = [&](auto part) {  // the product with a further part of the weights
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
+            const VFrag w = part(y);
+            const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
+#pragma unroll
+            for (int m = 0; m < kMt; ++m) o[m] = Type<TV>::mma(*reinterpret_cast<const VLds*>(col + 32 * m * L::kVRow), w, o[m]);
+          }
+      };
+      // ahead of the first part's product where scales and their mask end a block anyway: 2% less than behind it
+      if constexpr (M::kFine && M::kScaled) {
+        if (fine) add([](const float(&y)[8]) { return second8<VFrag>(y); });
+      }
       using Half2 = _Float16 __attribute__((ext_vector_type(2)));
       Half2 least = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
 #pragma unroll
@@ -473,31 +496,23 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
           }
         }
       if constexpr (!M::kFloat && M::kParts == 1) attn::reads_ahead<kSub * 2 * kMt, 4, 1>();
+      if constexpr (M::kFine && !M::kScaled) {
+        if (fine) add([](const float(&y)[8]) { return second8<VFrag>(y); });
+      }
       if constexpr (kHalf) {
-        constexpr float kBelow = Faint<TV>::kBelow(M::kParts);
-        bool some = static_cast<float>(least.x) < kBelow || static_cast<float>(least.y) < kBelow;
+        const float below = Faint<TV>::below(fine ? 2 : 1);
+        bool some = static_cast<float>(least.x) < below || static_cast<float>(least.y) < below;
         if (!whole) {  // weights that the mask made 0 are none
           some = false;
 #pragma unroll
           for (int u = 0; u < kSub; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) some |= x[u][r] > 0.f && x[u][r] < kBelow;
+            for (int r = 0; r < 16; ++r) some |= x[u][r] > 0.f && x[u][r] < below;
         }
         if (__any(some)) {
 #pragma unroll
           for (int m = 0; m < kMt; ++m) o[m] *= Faint<TV>::kUp;
-#pragma unroll
-          for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = x[u][8 * c + e];
-              const VFrag w = faint8<M::kParts>(y);
-              const char* const col = vt + (lane & 31) * L::kVRow + (32 * u + 16 * c + 8 * half) * static_cast<int>(sizeof(TV));
-#pragma unroll
-              for (int m = 0; m < kMt; ++m) o[m] = Type<TV>::mma(*reinterpret_cast<const VLds*>(col + 32 * m * L::kVRow), w, o[m]);
-            }
+          add([&](const float(&y)[8]) { return fine ? faint8<2>(y) : faint8<1>(y); });
 #pragma unroll
           for (int m = 0; m < kMt; ++m) o[m] *= Faint<TV>::kDown;
         }
@@ -597,8 +612,7 @@ inline int prompt_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // A key head's query heads that one workgroup takes together, and the pieces into which it cuts a tile's keys.
 struct PromptPlan {
-  int heads, U, bias_row, pieces;
-  bool fine;
+  int heads, U, bias_row, pieces, fine;
   int64_t tiles, blocks;
 };
 // The pieces are those of the least time by this estimate, in microseconds: a workgroup takes `tile` for 64 keys on a CU
@@ -633,9 +647,13 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
   const double rows = (std::floor(T / p.U) + 0.5 * B) * columns;            // tiles of queries that have any
   const double longest = most / 64.0, all = rows * std::max(longest - T / (128 * B), longest / 2);  // in tiles of keys
   // Weights rounded to the queries' type add an error as large as the output's own rounding: together 1.41 times it on the
-  // average of many rows and keys, more in a short call's few.  Two parts cost 20-27% of the products' time, which there is a
-  // small part (500 tokens, 8 (2) heads of 64: 15.1 | 15.4 us; 2000 31.5 | 36.0).
-  p.fine = all <= 1024;
+  // average of many rows and keys, more in a short call's few.  A second part costs 20-25% of the products' time.  It is taken
+  // where that is a small part: calls whose tiles of queries do not fill the card, and of those the sequences with which, were
+  // they all like it, the call would be of 1024 products at most, of a tile with 64 keys.  Their lengths are known on the device
+  // alone, and the table's width says nothing of them.  8 (2) heads of 64, bfloat16, one part | two: 500 tokens (250
+  // products) 15.0 | 15.5 us, 1000 (500) 21.3 | 22.6, 16 behind 60,000 (940) 25.8 | 28.9, 400 behind 4000 (1600) 28.6 | 30.7,
+  // 4 of 384 behind 20,000 (24,000) 109 | 137.  Where the kernel has to look, one part takes 1% longer, 4% over 8 bits.
+  p.fine = rows > 512 ? 0 : static_cast<int>(64 * 1024 / rows);
   double least = 0;
   p.pieces = 1;
   for (int n = 1; n == 1 || (most >= 64 * n && rows * n <= 12 * 256 * waves); n *= 2) {  // tables may be far wider than streams are long
@@ -654,7 +672,7 @@ inline PromptPlan plan_prompt(const geo_paged_prompt_t* g) {
 template <typename T, typename C, int DP>
 int launch_prompt(const Prompt& a, const PromptPlan& p, void* out, float* part, hipStream_t stream) {
   const size_t bytes = 2 * PromptLds<T, C, DP>::kBuffer + (a.bias.table ? static_cast<size_t>(a.heads) * a.bias_row * 4 : 0);
-  constexpr bool kCanBeFine = sizeof(T) == 2 && Meet<T, C>::kParts == 1;
+  constexpr bool kCanBeFine = Meet<T, C, true>::kFine;
   auto* const kernel = kCanBeFine && p.fine ? &paged_prompt<T, C, DP, kCanBeFine> : &paged_prompt<T, C, DP, false>;
   GEO_HIP_CHECK(attn::allow_lds(reinterpret_cast<const void*>(kernel), bytes));
   kernel<<<dim3(static_cast<uint32_t>(p.blocks)), dim3(kPromptThreads), bytes, stream>>>(a, p.tiles, p.pieces, a.pool.table, part,

@@ -149,7 +149,7 @@ struct Weights {
   static __device__ __forceinline__ bool some_faint(const float (&p)[16 / sizeof(T)]) {
     bool some = false;
 #pragma unroll
-    for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) some |= p[e] < Faint<T>::kBelow(kParts) && p[e] > 0.f;
+    for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) some |= p[e] < Faint<T>::below(kParts) && p[e] > 0.f;
     return some;
   }
   static __device__ __forceinline__ f32x4 faint(const Bytes16& v, const f16x8& rest, f32x4 o) {

@@ -62,3 +62,22 @@ def test_scores_far_out(dev, dtype, stored, d, bias):
     check(paged_attention(q, cache, table, **kw), lo, hi)
     at = torch.tensor([n - 1], device=dev)
     check(paged_attention_step(q[-1:], k[-1:], v[-1:], cache, table, at, **kw), lo[-1:], hi[-1:])
+
+
+@pytest.mark.parametrize("dtype,stored,unit", [(BF16, BF16, 2.0 ** -16), (F16, F16, 2.0 ** -22), (BF16, I8, 2.0 ** -16), (BF16, E4, 2.0 ** -16)],
+                         ids=["bf16", "f16", "bf16-i8", "bf16-e4m3"])
+@pytest.mark.parametrize("columns", [12, 300, 9000])
+@pytest.mark.parametrize("new", [5, 300])
+def test_weights_of_short_prompts_do_not_hang_on_the_table(dev, dtype, stored, unit, columns, new):
+    """Weights of a call of few queries over a short history are kept in two parts, however many tokens the table has room for."""
+    from gdl_amd.functional import PagedCache, paged_attention
+    gen = torch.Generator().manual_seed(new)
+    n, H, Hk, d = 700, 6, 2, 64
+    cache = PagedCache.empty(12, Hk, d, dtype=stored, device=dev)
+    table = torch.full((1, columns), -1, dtype=torch.int32)
+    table[0, :12] = torch.randperm(12, generator=gen).int()
+    table = table.to(dev)
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(dtype).to(dev) for h in (H, Hk, Hk))
+    cache.write(k, v, table)
+    out = paged_attention(q[-new:], cache, table, None, torch.tensor([n - new], device=dev))
+    ref.assert_near(out, *ref.attend(q[-new:], ref.stored(k, stored), ref.stored(v, stored), n - new, stored, unit=unit))
