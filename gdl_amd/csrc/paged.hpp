@@ -7,6 +7,9 @@
 // tokens, so a token block begins at the same offset in either.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "attention_args.hpp"
 
 namespace geo {
@@ -188,6 +191,15 @@ __device__ __forceinline__ uint32_t group_most(uint32_t x) {
   if constexpr (LW >= 16) x = max(x, dpp_u32<kDppMirror>(x));
   return x;
 }
+
+// x[n] times what lane n of the 16 holds.
+template <int... N>
+__device__ __forceinline__ void by_group_of(float* x, float y, std::integer_sequence<int, N...>) {
+  constexpr int kRowBroadcast = 0x150;
+  ((x[N] *= __uint_as_float(dpp0_u32<kRowBroadcast + N>(__float_as_uint(y)))), ...);
+}
+template <int N>
+__device__ __forceinline__ void by_group(float (&x)[N], float y) { by_group_of(x, y, std::make_integer_sequence<int, N>()); }
 
 struct Pool {
   char *k, *v;

@@ -79,14 +79,6 @@ __device__ __forceinline__ uint32_t seen_and_finite(uint32_t w, int key, int lim
   return w;
 }
 
-// x[r] times what lane r of the 16 holds.
-template <int... R>
-__device__ __forceinline__ void by_row_of(float* x, float y, std::integer_sequence<int, R...>) {
-  constexpr int kRowBroadcast = 0x150;
-  ((x[R] *= __uint_as_float(dpp0_u32<kRowBroadcast + R>(__float_as_uint(y)))), ...);
-}
-__device__ __forceinline__ void by_row(float (&x)[16], float y) { by_row_of(x, y, std::make_integer_sequence<int, 16>()); }
-
 template <typename T, typename C, int DP>
 struct PromptLds {
   using M = Meet<T, C>;
@@ -373,7 +365,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
         const float* const scales = reinterpret_cast<const float*>(kt + L::kK + L::kV) + 16 * (lane >> 3 & 1) + 8 * half + (lane & 7);
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          by_row(x[u], scales[32 * u]);
+          by_group(x[u], scales[32 * u]);
           vs[u] = scales[kKeys + 32 * u];
         }
       }
@@ -440,7 +432,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
       if constexpr (M::kScaled) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          by_row(x[u], vs[u]);
+          by_group(x[u], vs[u]);
           if (!whole) {  // an unseen scale may be NaN
 #pragma unroll
             for (int r = 0; r < 16; ++r)

@@ -180,22 +180,13 @@ struct NarrowWeights {
   }
 };
 
-// x[n] times what lane n of the 16 holds.
-template <int... N>
-__device__ __forceinline__ void by_group_of(float* x, float y, std::integer_sequence<int, N...>) {
-  constexpr int kRowBroadcast = 0x150;
-  ((x[N] *= __uint_as_float(dpp0_u32<kRowBroadcast + N>(__float_as_uint(y)))), ...);
-}
-template <int N>
-__device__ __forceinline__ void by_group(float (&x)[N], float y) { by_group_of(x, y, std::make_integer_sequence<int, N>()); }
-
 // x times log2 e for a key `back` tokens behind, of head h.
 __device__ __forceinline__ float bias_at(const attn::Bias& b, int Hq, int h, int64_t back) {
   const int n = static_cast<int>(min(back, static_cast<int64_t>(b.maxd)));
   return attn::bias_value(b, static_cast<int64_t>(b.lut[b.maxd - n]) * Hq + h);
 }
 
-template <int LW>
+// Over 16 lanes, in all of them.
 __device__ __forceinline__ float group_sum(float x) {
   x += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(x)));
   x += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(x)));
@@ -561,7 +552,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
     float s = 0.f;
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) s = fmaf(static_cast<float>(qraw.x[n]), nk.value[n], s);
-    s = group_sum<16>(s) * scale2;
+    s = group_sum(s) * scale2;
     if (a.bias.table) s += sbias[bucket[0] * kCols + min(cell, kCols - 1)];
     if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(pool.pages)) page = -1;
     if (col == 0 && cell < kCells) {
