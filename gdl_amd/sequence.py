@@ -122,8 +122,9 @@ class PointSequenceBlock(nn.Module):
             raise ValueError("PointSequenceBlock: only a causal block answers token by token")
         dev = self.decay.device
         if self.window is None:
-            if tokens is None or tokens < 1 or batch < 1:
-                raise ValueError(f"PointSequenceBlock: a cache without a window is for a number of tokens, got {tokens} for {batch}")
+            if tokens is None or tokens < 1 or batch < 1 or page < 1:
+                raise ValueError("PointSequenceBlock: a cache without a window is for a number of tokens, got "
+                                 f"{tokens} for {batch} streams in pages of {page}")
             each = -(-tokens // page)
             pool = PagedCache.empty(batch * each, self.kv_heads, self.head_dim, page=page, dtype=dtype or self.attend_in.weight.dtype,
                                     device=dev)

@@ -49,3 +49,11 @@ def test_packets_of_other_shapes_are_refused():
             packets_as_sequences(*bad)
     with pytest.raises(RuntimeError, match="GPU only"):
         packets_as_sequences(ptr, start, state)
+
+
+@pytest.mark.parametrize("kw", [dict(page=0), dict(page=-64), dict(page=32), dict(page=100), dict(tokens=0), dict(tokens=None), dict(batch=0)])
+def test_caches_of_a_block_are_refused(kw):
+    from gdl_amd.sequence import PointSequenceBlock
+    args = {"batch": 2, "dtype": torch.int8, "tokens": 10, **kw}
+    with pytest.raises(ValueError):
+        PointSequenceBlock(32, 2, None).new_cache(args.pop("batch"), args.pop("dtype"), **args)
