@@ -138,19 +138,21 @@ __device__ __forceinline__ F second8(const float (&x)[8]) {
 }
 template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1; }
 
-constexpr float kLazy = 8.f;  // how far scores (in units of log 2) may exceed the maximum that weights refer to
-
-// Weights as float16 operands.  Many keys 2^20 and more below one whose value is small are what a row consists of, and
-// float16 has no digits for weights that small.  They are formed 2^7 larger than those of other types, up to 2^15
-// then; of those that are still below 2^-14 (2^-9 where two parts are to keep 16 bits), what the parts leave is
-// taken 2^38 larger, as a further operand whose products join sums brought up as far.  These are powers of
-// two, so other rows' sums come back as they were.  Looking for such weights costs prompts 3-7% (8 pieces of up to 1024 behind
-// 2048, 16 (4) heads of 64: 106 | 113 us; 32 packets of up to 384 behind 4000 150 | 154), steps nothing.
+// Weights of operands of type V: kLazy is how far (in units of log 2) scores may exceed the maximum that weights refer to.
+// Many keys 2^20 and more below one whose value is small are what a row consists of, and float16 has no digits for weights
+// that small.  Its weights are formed 2^11 larger than those of other types, up to 2^15 then; of those that are still below
+// 2^-14 (2^-9 where two parts are to keep 16 bits), what the parts leave is taken 2^38 larger, as a further
+// operand whose products join sums brought up as far.  These are powers of two, so other rows' sums come back as they
+// were.  Looking for such weights costs prompts 3-7% (8 pieces of up to 1024 behind 2048, 16 (4) heads of 64: 106 | 113 us; 32
+// packets of up to 384 behind 4000 150 | 154), steps nothing.  Where scores spread so far that most tiles hold some, a deviation of 4,
+// prompts take 1.4 to 1.5 times as long (heads of 128: 215 | 300 us; of 2 215 | 215, where weights 2^7 larger, and scores 8 above the maximum, took 237), steps 3%.
 template <typename V>
 struct Faint {
   static constexpr bool kHalf = __is_same(V, _Float16);
-  static constexpr float kLift = kHalf ? 7.f : 0.f, kUp = 0x1p38f, kDown = 0x1p-38f;
+  static constexpr float kLift = kHalf ? 11.f : 0.f, kLazy = kHalf ? 4.f : 8.f, kUp = 0x1p38f, kDown = 0x1p-38f;
   static __host__ __device__ constexpr float below(int parts) { return parts > 1 ? 0x1p-9f : 0x1p-14f; }
+  // What scores are taken less by, of the largest: itself where the difference would be rounded up past what V holds.
+  static __device__ __forceinline__ float lifted(float most) { return kHalf && fabsf(most) < 0x1p20f ? most - kLift : most; }
 };
 // What PARTS float16 parts leave of eight weights, of those that are faint, 2^38 larger.
 template <int PARTS>

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   constexpr int kSize = sizeof(C), kKeys = M::kKeys, kBlk = block_tokens<C>(), kPer = 16 / kSize;
   constexpr int kSub = kKeys / 32, kKc = DP / 16, kMt = DP / 32;
   constexpr bool kHalf = Faint<TV>::kHalf;
-  constexpr float kLift = Faint<TV>::kLift;
+  constexpr float kLift = Faint<TV>::kLift, kLazy = Faint<TV>::kLazy;
   constexpr int kLoads = (kKeys * DP * kSize + 16 * kPromptThreads - 1) / (16 * kPromptThreads);
   constexpr int kSpan = kKeys < kBlk ? kKeys : kBlk, kCpb = kSpan * kSize / 16;  // tokens and pieces of a dimension in a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
   f32x16 o[kMt];
 #pragma unroll
   for (int m = 0; m < kMt; ++m) o[m] = f32x16{};
-  float top = -kInf, sum = 0.f;  // what scores are taken less by: the largest, less kLift
+  float top = -kInf, sum = 0.f;  // what scores are taken less by (Faint)
   bool lost = p >= room;
 
   __syncthreads();  // zeros past the head, biases, notes
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(kPromptThreads, (prompt_waves(DP))) void paged_prom
       most = halves_max(most) * by;
       const bool up = most - top > kLazy + kLift;
       if (__any(up)) {
-        most -= kLift;
+        most = Faint<TV>::lifted(most);
         const float keep = up ? exp2_hw(top - most) : 1.f;
         top = up ? most : top;
         sum *= keep;

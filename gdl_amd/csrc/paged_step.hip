@@ -276,7 +276,7 @@ template <typename T, typename C, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 2)) void paged_step(const Step a, const Deal deal, const int32_t* __restrict__ table,
                                                                         const int64_t* __restrict__ positions, T* __restrict__ out) {
   constexpr bool kNarrow = Code<C>::kNarrow, kHalf = Faint<C>::kHalf;
-  constexpr float kLift = Faint<C>::kLift;
+  constexpr float kLift = Faint<C>::kLift, kLazy = Faint<C>::kLazy;
   constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kCells = kCols * 4 / WAVES;  // heads that there is room to join
   constexpr int kSize = sizeof(C), kBlk = block_tokens<C>(), kOwn = kBlk / 4, kTiles = kBlk / 16;
   constexpr int kLoads = DP * kSize / 64, kRows = DP / 16, kLds = DP + 4;
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
   f32x4 o[kRows];
 #pragma unroll
   for (int m = 0; m < kRows; ++m) o[m] = f32x4{};
-  float top = -kInf, sum = 0.f;  // what scores are taken less by: the largest, less kLift
+  float top = -kInf, sum = 0.f;  // what scores are taken less by (Faint)
   const float scale2 = a.scale * kLog2e;
   const float far = a.bias.table ? bias_at(a.bias, a.Hq, head, a.bias.maxd) : 0.f;
 
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 4 ? step_waves<T, C, DP>() : 
     for (int n = 1; n < kOwn; ++n) most = fmaxf(most, x[n]);
     if (__any(most - top > kLazy + kLift)) {
       most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(fmaxf(most, __shfl_xor(most, 32, 64)) - kLift, top);
+      most = fmaxf(Faint<C>::lifted(fmaxf(most, __shfl_xor(most, 32, 64))), top);
       const float keep = top == -kInf ? 0.f : exp2_hw(top - most);
       if (top != -kInf) {
 #pragma unroll

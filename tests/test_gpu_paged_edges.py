@@ -81,3 +81,29 @@ def test_weights_of_short_prompts_do_not_hang_on_the_table(dev, dtype, stored, u
     cache.write(k, v, table)
     out = paged_attention(q[-new:], cache, table, None, torch.tensor([n - new], device=dev))
     ref.assert_near(out, *ref.attend(q[-new:], ref.stored(k, stored), ref.stored(v, stored), n - new, stored, unit=unit))
+
+
+@pytest.mark.parametrize("dtype,stored", [(F32, F32), (BF16, BF16), (F16, F16), (F16, I8)], ids=["f32", "bf16", "f16", "f16-i8"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_every_size(dev, dtype, stored, sign):
+    """Scores from 2^14 to 2^40 and their negatives, several in each power of two: rows are means of what they see."""
+    from attention_ref import SPACING, UNIT
+    from gdl_amd.functional import PagedCache, paged_attention, paged_attention_step
+    gen = torch.Generator().manual_seed(3)
+    n, H, d = 200, 8, 32
+    cache = PagedCache.empty(4, 1, d, dtype=stored, device=dev)
+    table = torch.tensor([[3, 1, 0, 2]], dtype=torch.int32, device=dev)
+    q = (0.5 + 0.5 * torch.rand(n, H, 1, generator=gen)).expand(n, H, d).to(dtype).to(dev)
+    k, v = torch.ones(n, 1, d, dtype=dtype, device=dev), torch.randn(n, 1, d, generator=gen).to(dtype).to(dev)
+    cache.write(k, v, table)
+    V = ref.stored(v, stored).expand(n, H, d)
+    lo, hi = V.cummin(0).values, V.cummax(0).values
+    slack = SPACING[dtype] + (2 * UNIT[dtype] + (n + 8) * 2.0 ** -24) * torch.maximum(lo.abs(), hi.abs())
+    at = torch.tensor([n - 1], device=dev)
+    for e in range(14, 41):
+        scale = sign * 2.0 ** e / d
+        x = paged_attention(q, cache, table, scale=scale).double().cpu()
+        assert x.isfinite().all(), (e, int((~x.isfinite()).sum()))
+        assert (x >= lo - slack).all() and (x <= hi + slack).all(), e
+        x = paged_attention_step(q[-1:], k[-1:], v[-1:], cache, table, at, scale=scale).double().cpu()
+        assert x.isfinite().all() and (x >= lo[-1:] - slack[-1:]).all() and (x <= hi[-1:] + slack[-1:]).all(), e
