@@ -13,10 +13,10 @@
 // weights of eight adjoining tokens.
 //
 // A wave's scores, exponentials and product with V follow one another, and two (to head size 64 three) waves a SIMD cover for
-// each other: 8 pieces of up to 2048 tokens behind 8192, 16 (4) heads of 128, bfloat16, 970 us, 820 TFLOP/s, matrix instructions
-// in 39% of the cycles, vector instructions in 41%; int8 1.11 ms, float32 100 TFLOP/s (matrix instructions 79%).
+// each other: 8 pieces of up to 2048 tokens behind 8192, 16 (4) heads of 128, bfloat16, 966 us, 823 TFLOP/s, matrix instructions
+// in 39% of the cycles, vector instructions in 40%; int8 1.08 ms, float32 100 TFLOP/s (matrix instructions 77%).
 // Codes cost a conversion each and their scales two products a score: 32 packets of up to 384 behind 4000 e4m3
-// tokens, 8 (2) heads of 64, 157 us and 12 for the join, vector instructions in 63% of the cycles.
+// tokens, 8 (2) heads of 64, 151 us with the join, vector instructions in 63% of the cycles.
 #pragma once
 
 #include <algorithm>

@@ -719,9 +719,9 @@ inline int padded(int D, bool narrow) { return D <= 32 && !narrow ? 32 : D <= 64
 
 // Workgroups, the least share (in tiles) and the workspace of a call: whole rows where no stream can hold many
 // tiles, more where there are more rows to fill the card; else as many shares as run at a time.  In us, shares | whole
-// rows: 4 rows of 1000 tokens (float32, heads of 32) 12.4 | 15.2, but 20 | 16 with the host's time, of which the join's launch
-// and the workspace take 4; 16 (int8, of 64) 19.3 | 15.4, 1024 (bfloat16, of 128) 88 | 82; of 2000 tokens 4 (float32) 13 | 24,
-// 32 (bfloat16) 18 | 27, 128 (int8) 24.6 | 21.7, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 32.
+// rows: 4 rows of 1000 tokens (float32, heads of 32) 11.9 | 12.8, but 16.5 | 12.0 a call with the host's time, of which the join's
+// launch and the workspace take 4; 16 of up to 1000 (int8, of 64) 15.7 | 11.2, 1024 (bfloat16, of 128) 87 | 81; of up to 2000
+// tokens 4 (float32) 12.4 | 19.8, 32 (bfloat16) 18 | 26, 128 (int8) 21.2 | 16.2, 256 (bfloat16) 40 | 36, 256 (float32) 27 | 24.
 struct StepPlan {
   int groups, least, waves;
   size_t bytes;

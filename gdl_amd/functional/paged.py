@@ -290,7 +290,7 @@ def paged_attention_step(
     Over a pool of the tokens' type the result is ``window_attention``'s with the window ``(-1, 0)`` for the
     last token of such streams.  A stream at a negative position is left alone (its row is 0); one with a
     token that has no page (an entry of ``table`` [B, n] outside the pool, a position beyond it) gives NaN.
-    No two streams may write to one slot.  No gradients.  ``bias`` is one-sided.
+    No two streams may write to one slot.  No gradients.  ``bias`` is one-sided.  No streams: an empty result.
     """
     name, (hk, d) = "paged_attention_step", (cache.kv_heads, cache.head_dim)
     batch = _check_queries(name, q, cache, bias)
