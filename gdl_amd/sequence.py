@@ -170,5 +170,5 @@ class PointSequenceBlock(nn.Module):
         q, k, v = self._split(x)
         cache.window.write(k, v, cache.table, ptr, start)
         out = paged_attention(q, cache.window, cache.table, ptr, start, bias=self.bias, max_distance=self.max_distance)
-        cache.state = state[::2]
+        cache.state = state[::2].contiguous()  # as a caller may view it
         return x + self.attend_out(out.flatten(1))

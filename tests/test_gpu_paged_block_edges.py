@@ -68,6 +68,7 @@ def test_packets_and_steps_agree_at_negative_positions(dev):
         if start + t >= 0:
             assert (y - rows[:, t]).abs().max() <= 2e-5 * max(1.0, y.abs().max().item()), t
     assert (a.state - b.state).abs().max() <= 2e-5
+    assert a.state.is_contiguous() and b.state.is_contiguous()
 
 
 @pytest.mark.parametrize("B,C", [(1, 1), (1, 64), (3, 5), (70, 33)])
